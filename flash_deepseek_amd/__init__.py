@@ -16,6 +16,8 @@ for this path, over the C ABI of libfdm.so (include/fdm.h):
   layer_forward MoE branch      :1878-1922 moe_layer
   expert streaming (flash)      :1478-1602 stream_layer / moe_layer_streamed
   mla_forward                   :766-903   attn_upload / attn_forward
+    (its parts for several          -      rope / kv_write / kv_read / mla_attend
+     sequences and drafted tokens)
   layer_forward dense branch    :1852-1868 dense_ffn (weights: upload_dense /
                                            attach_dense / load_dense_gguf)
 
@@ -35,7 +37,8 @@ __all__ = [
     "attach_layer", "upload_layer", "release_layer", "layer_info", "moe_forward",
     "moe_forward_host", "moe_layer", "f32_to_f16", "upload_dense", "attach_dense", "load_dense_gguf",
     "release_dense", "dense_info", "dense_ffn", "DENSE_FFN", "stream_layer", "moe_layer_streamed",
-    "stream_stats", "attn_upload", "attn_load_gguf", "attn_forward", "attn_reset", "attn_len", "attn_release", "set_batch_kernel", "BATCH_AUTO", "BATCH_DOT4", "BATCH_MFMA", "prof_enable", "prof_reset", "prof_read", "synth_q4k", "synth_q6k", "synth_normal", "FdmError",
+    "stream_stats", "rope_table", "rope", "KvCache", "kv_cache", "kv_write", "kv_read", "mla_workspace", "mla_attend",
+    "attn_upload", "attn_load_gguf", "attn_forward", "attn_reset", "attn_len", "attn_release", "set_batch_kernel", "BATCH_AUTO", "BATCH_DOT4", "BATCH_MFMA", "prof_enable", "prof_reset", "prof_read", "synth_q4k", "synth_q6k", "synth_normal", "FdmError",
     "QK_K", "Q4K_BLOCK_SIZE", "Q6K_BLOCK_SIZE", "HIDDEN", "MOE_FFN", "N_EXPERTS", "MAX_K",
     "MAX_LAYERS", "MAX_TOKENS", "EXPERT_Q4K_BYTES", "EXPERT_Q6K_BYTES",
 ]
@@ -70,7 +73,9 @@ def _stream(stream=None):
 def init(device=0):
     """Select the device and allocate the workspace (metal_init).  Raises
     FdmError when no gfx950 device is usable."""
+    global _device
     call("fdm_init", int(device))
+    _device = int(device)
 
 
 def shutdown():
@@ -311,6 +316,224 @@ def attn_release(L):
     call("fdm_attn_release", L)
 
 
+# ---- rotary positions, the paged latent cache and its attention ------------------------
+# These take whole tensors: sizes, strides and types are theirs, and what does not
+# fit is refused (FdmError, FDM_E_INVAL) before anything is launched.
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+KV_FORMATS = {"f16": _lib.KV_F16, "bf16": _lib.KV_BF16, "fp8": _lib.KV_FP8}
+_device = None  # of init()
+_types = {}     # torch dtype -> element type (filled at first use: torch is imported lazily)
+
+
+def _refuse(fn, why):
+    raise FdmError(_lib.FDM_E_INVAL, fn, why)
+
+
+def _elem(fn, name, dtype):
+    if not _types:
+        import torch
+        _types.update({torch.float32: _lib.GGML_F32, torch.float16: _lib.GGML_F16, torch.bfloat16: _lib.GGML_BF16})
+    t = _types.get(dtype)
+    if t is None:
+        _refuse(fn, f"{name}: {dtype} is none of float32, float16, bfloat16")
+    return t
+
+
+def _on_device(fn, **tensors):
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or (_device is not None and t.get_device() != _device)):
+            _refuse(fn, f"{name} is on {t.device}, the library on device {_device}")
+
+
+def _ints(fn, name, t, n, dtype="torch.int32"):
+    """A contiguous vector (or matrix) of n int32."""
+    if str(t.dtype) != dtype or t.numel() != n or not t.is_contiguous():
+        _refuse(fn, f"{name}: {n} contiguous values of {dtype} are wanted, got {tuple(t.shape)} of {t.dtype}")
+
+
+def _call_stream(stream):
+    """The stream handle of a call: the given one, or torch's current one on the library's device."""
+    if stream is not None or _device is None:
+        return _stream(stream)
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return torch.cuda.current_stream(_device).cuda_stream if raw is None else raw(_device)
+
+
+def rope_table(dim, base=10000.0, layout="interleaved", scaling="none", factor=1.0, orig_ctx=4096, beta_fast=32.0,
+               beta_slow=1.0, mul=1.0):
+    """The angles of rotary positions over `dim` values (fdm_rope_table_init):
+    layout "interleaved" (pairs 2i, 2i + 1) or "half" (i, i + dim / 2), scaling
+    "none", "linear" or "yarn" by `factor`; rotated values are multiplied by mul."""
+    for name, value, known in (("layout", layout, ROPE_LAYOUTS), ("scaling", scaling, ROPE_SCALINGS)):
+        if value not in known:
+            _refuse("rope_table", f"{name} {value!r}: one of {', '.join(known)}")
+    if mul == 0.0:
+        _refuse("rope_table", "mul 0 would clear what is rotated")
+    p = _lib.RopeParams(dim, ROPE_LAYOUTS[layout], ROPE_SCALINGS[scaling], orig_ctx, base, factor, beta_fast, beta_slow, mul)
+    t = _lib.RopeTable()
+    call("fdm_rope_table_init", ctypes.byref(p), ctypes.byref(t))
+    return t
+
+
+def rope(table, x, pos, out, offset=0, stream=None):
+    """out = x [T, H, D] with the table's dim values from `offset` of every head
+    turned by the token's position (pos [T] int32).  Any token and head
+    strides; float32, float16 or bfloat16 on either side.  out may be x."""
+    T, H, D = x.shape if x.dim() == 3 else _refuse("rope", f"x: [T, H, D] is wanted, got {tuple(x.shape)}")
+    if out.shape != x.shape:
+        _refuse("rope", f"out: {tuple(x.shape)} is wanted, got {tuple(out.shape)}")
+    if (x.stride(2) != 1 or out.stride(2) != 1) and D > 1:
+        _refuse("rope", "the values of a head must be contiguous")
+    _on_device("rope", x=x, pos=pos, out=out)
+    _ints("rope", "pos", pos, T)
+    call("fdm_rope", ctypes.byref(table), pos.data_ptr(), T, H, D, offset, x.data_ptr(), _elem("rope", "x", x.dtype),
+         x.stride(0), x.stride(1), out.data_ptr(), _elem("rope", "out", out.dtype), out.stride(0), out.stride(1),
+         _call_stream(stream))
+
+
+class KvCache:
+    """The planes of a paged latent cache (tensors of the caller, kept alive
+    here): latent [n_pages, page_size, 512] and rope [n_pages, page_size, 64] in
+    float16 or bfloat16; or, for FP8 rows, latent in float8_e4m3fn, rope in
+    bfloat16 and scale [n_pages, page_size, 4] in float8_e8m0fnu (or uint8)."""
+
+    def __init__(self, latent, rope, scale=None):
+        fmt = {"torch.float16": "f16", "torch.bfloat16": "bf16", "torch.float8_e4m3fn": "fp8"}.get(str(latent.dtype))
+        if fmt is None:
+            _refuse("KvCache", f"latent: {latent.dtype} is none of float16, bfloat16, float8_e4m3fn")
+        if latent.dim() != 3 or latent.shape[2] != _lib.KV_LATENT:
+            _refuse("KvCache", f"latent: [pages, page_size, {_lib.KV_LATENT}] is wanted, got {tuple(latent.shape)}")
+        lead = tuple(latent.shape[:2])
+        if tuple(rope.shape) != lead + (_lib.KV_ROPE,) or str(rope.dtype) != ("torch.float16" if fmt == "f16" else "torch.bfloat16"):
+            _refuse("KvCache", f"rope: {lead + (_lib.KV_ROPE,)} in the cache's 16-bit type is wanted, got {tuple(rope.shape)} of {rope.dtype}")
+        if (scale is None) == (fmt == "fp8"):
+            _refuse("KvCache", "scale: FP8 rows have one, the others none")
+        if scale is not None and (tuple(scale.shape) != lead + (4,) or scale.element_size() != 1):
+            _refuse("KvCache", f"scale: {lead + (4,)} bytes are wanted, got {tuple(scale.shape)} of {scale.dtype}")
+        for name, t in (("latent", latent), ("rope", rope), ("scale", scale)):
+            if t is not None and not t.is_contiguous():
+                _refuse("KvCache", f"{name}: not contiguous")
+        if lead[1] < 1 or lead[1] & (lead[1] - 1):
+            _refuse("KvCache", f"page_size {lead[1]}: a power of two")
+        _on_device("KvCache", latent=latent, rope=rope, scale=scale)
+        self.latent, self.rope, self.scale, self.format = latent, rope, scale, fmt
+        self.n_pages, self.page_size = lead
+        self.desc = _lib.KvCacheDesc(latent.data_ptr(), rope.data_ptr(), _p(scale), KV_FORMATS[fmt], *lead)
+
+
+def kv_cache(format, n_pages, page_size=64):
+    """A KvCache of fresh zeroed planes; format "f16", "bf16" or "fp8"."""
+    import torch
+    if format not in KV_FORMATS:
+        _refuse("kv_cache", f"format {format!r}: one of {', '.join(KV_FORMATS)}")
+    dev = torch.device("cuda", torch.cuda.current_device() if _device is None else _device)
+    half = torch.float16 if format == "f16" else torch.bfloat16
+    lead = (n_pages, page_size)
+    rope_plane = torch.zeros(*lead, _lib.KV_ROPE, dtype=half, device=dev)
+    if format != "fp8":
+        return KvCache(torch.zeros(*lead, _lib.KV_LATENT, dtype=half, device=dev), rope_plane)
+    codes = torch.zeros(*lead, _lib.KV_LATENT, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    return KvCache(codes, rope_plane, torch.zeros(*lead, 4, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu))
+
+
+def _rows(fn, name, t, T):
+    if t.dim() != 2 or t.shape[0] != T or t.shape[1] != _lib.KV_LATENT + _lib.KV_ROPE or t.stride(1) != 1:
+        _refuse(fn, f"{name}: [{T}, {_lib.KV_LATENT + _lib.KV_ROPE}] with contiguous rows is wanted, got {tuple(t.shape)}")
+
+
+def kv_write(cache, kv, slots, norm_w=None, table=None, pos=None, stream=None):
+    """Rows kv [T, 576] into the cache at slots [T] int32 (page * page_size + place;
+    negative: nowhere): the latent 512 normed by norm_w (float32 [512]; None: as
+    they are), the last 64 turned by table at pos [T] (None: as they are),
+    quantised to the cache's format."""
+    T = slots.numel()
+    _rows("kv_write", "kv", kv, T)
+    _on_device("kv_write", kv=kv, slots=slots, norm_w=norm_w, pos=pos, cache=cache.latent)
+    _ints("kv_write", "slots", slots, T)
+    if norm_w is not None:
+        _ints("kv_write", "norm_w", norm_w, _lib.KV_LATENT, "torch.float32")
+    if table is not None:
+        if pos is None:
+            _refuse("kv_write", "a rotation needs positions")
+        _ints("kv_write", "pos", pos, T)
+    call("fdm_kv_write", ctypes.byref(cache.desc), kv.data_ptr(), _elem("kv_write", "kv", kv.dtype), kv.stride(0),
+         _p(norm_w), None if table is None else ctypes.byref(table), _p(pos), slots.data_ptr(), T, _call_stream(stream))
+
+
+def kv_read(cache, slots, out, stream=None):
+    """out [T, 576] = the rows at slots [T] int32, widened; a negative slot leaves its row as it was."""
+    T = slots.numel()
+    _rows("kv_read", "out", out, T)
+    _on_device("kv_read", slots=slots, out=out, cache=cache.latent)
+    _ints("kv_read", "slots", slots, T)
+    call("fdm_kv_read", ctypes.byref(cache.desc), slots.data_ptr(), T, out.data_ptr(), _elem("kv_read", "out", out.dtype),
+         out.stride(0), _call_stream(stream))
+
+
+def mla_workspace(N, H):
+    """A workspace for mla_attend calls of up to N query tokens and H heads that run one after the other."""
+    import torch
+    n = ctypes.c_size_t()
+    call("fdm_mla_workspace", N, H, ctypes.byref(n))
+    return torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", _device or 0))
+
+
+def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=None, lse=None, workspace=None, max_kv=0,
+               stream=None):
+    """Latent attention of B sequences' query tokens over the paged cache.
+
+    q_lat [N, H, 512] (the absorbed queries) and q_rope [N, H, 64]; sequence b has
+    the tokens q_start[b] .. q_start[b + 1] - 1 and kv_len[b] cached positions, its
+    own tokens the last of them, in the pages pages[b] (int32 [B, P]).  Each
+    token sees what stands before its sequence's tokens, and among these the ones
+    of its mask (int64 [N, words], bit d: the sequence's token d) or, without
+    one, those up to itself.  out [N, H, 512] = sum of softmax(scale q k) latent;
+    lse (float32 [N, H]) the log of the sums.  workspace: mla_workspace's (None:
+    allocated for the call).  max_kv: the longest kv_len to expect, if known."""
+    fn = "mla_attend"
+    if q_lat.dim() != 3 or q_lat.shape[2] != _lib.KV_LATENT:
+        _refuse(fn, f"q_lat: [N, H, {_lib.KV_LATENT}] is wanted, got {tuple(q_lat.shape)}")
+    N, H, _ = q_lat.shape
+    if tuple(q_rope.shape) != (N, H, _lib.KV_ROPE) or out.shape != q_lat.shape:
+        _refuse(fn, f"q_rope, out: {(N, H, _lib.KV_ROPE)} and {tuple(q_lat.shape)} are wanted, got {tuple(q_rope.shape)} and {tuple(out.shape)}")
+    half = cache.rope.dtype
+    if q_lat.dtype != half or q_rope.dtype != half or out.dtype != half:
+        _refuse(fn, f"q_lat, q_rope and out are {half} with this cache, got {q_lat.dtype}, {q_rope.dtype}, {out.dtype}")
+    if q_lat.stride(2) != 1 or q_rope.stride(2) != 1 or out.stride(2) != 1:
+        _refuse(fn, "the values of a head must be contiguous")
+    B = kv_len.numel()
+    if pages.dim() != 2 or pages.shape[0] != B:
+        _refuse(fn, f"pages: [{B}, P] is wanted, got {tuple(pages.shape)}")
+    _on_device(fn, cache=cache.latent, q_lat=q_lat, q_rope=q_rope, q_start=q_start, kv_len=kv_len, pages=pages, out=out,
+               mask=mask, lse=lse, workspace=workspace)
+    _ints(fn, "q_start", q_start, B + 1)
+    _ints(fn, "kv_len", kv_len, B)
+    _ints(fn, "pages", pages, pages.numel())
+    words = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != N:
+            _refuse(fn, f"mask: [{N}, words] is wanted, got {tuple(mask.shape)}")
+        words = mask.shape[1]
+        _ints(fn, "mask", mask, N * words, "torch.int64")
+    if lse is not None:
+        if tuple(lse.shape) != (N, H):
+            _refuse(fn, f"lse: {(N, H)} is wanted, got {tuple(lse.shape)}")
+        _ints(fn, "lse", lse, N * H, "torch.float32")
+    handle = _call_stream(stream)
+    if workspace is None:  # torch's allocator keeps it for the stream that it is made on
+        import torch
+        with torch.cuda.stream(torch.cuda.current_stream(q_lat.device) if stream is None
+                               else torch.cuda.ExternalStream(handle, device=q_lat.device)):
+            workspace = mla_workspace(N, H)
+    batch = _lib.MlaBatch(B, N, H, q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), pages.shape[1], max_kv,
+                          _p(mask), words)
+    call("fdm_mla_attend", ctypes.byref(cache.desc), ctypes.byref(batch), q_lat.data_ptr(), q_lat.stride(0),
+         q_lat.stride(1), q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1), scale, out.data_ptr(), out.stride(0),
+         out.stride(1), _p(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), handle)
+
+
 # ---- dense FFN layers (layer_forward's branch for L < 3) ------------------------------
 def f32_to_f16(src, dst, n=None, stream=None):
     """(__fp16) cast of f32_to_f16_alloc on the device: fp32 -> F16 bits."""
@@ -357,7 +580,8 @@ def dense_ffn(L, h_post, h_in, hidden, stream=None):
 PHASES = {"router": _lib.PROF_ROUTER, "gateup": _lib.PROF_GATEUP, "down": _lib.PROF_DOWN,
           "xdigits": _lib.PROF_XDIGITS, "matvec": _lib.PROF_MATVEC, "layer": _lib.PROF_LAYER,
           "batch": _lib.PROF_BATCH, "prefill": _lib.PROF_PREFILL, "dense": _lib.PROF_DENSE,
-          "attn": _lib.PROF_ATTN, "ceiling": _lib.PROF_CEILING}
+          "attn": _lib.PROF_ATTN, "ceiling": _lib.PROF_CEILING, "rope": _lib.PROF_ROPE, "kv": _lib.PROF_KV,
+          "mla": _lib.PROF_MLA}
 
 
 def prof_enable(on=True):

@@ -20,7 +20,7 @@ FDM_E_IO = -7
 FDM_E_FORMAT = -8
 
 (PROF_ROUTER, PROF_GATEUP, PROF_DOWN, PROF_XDIGITS, PROF_MATVEC, PROF_LAYER, PROF_BATCH,
- PROF_PREFILL, PROF_DENSE, PROF_ATTN, PROF_CEILING) = range(11)
+ PROF_PREFILL, PROF_DENSE, PROF_ATTN, PROF_CEILING, PROF_ROPE, PROF_KV, PROF_MLA) = range(14)
 
 QK_K = 256
 Q4K_BLOCK_SIZE = 144
@@ -39,6 +39,39 @@ class AttnWeights(ctypes.Structure):
     """struct fdm_attn_weights (host pointers)."""
     _fields_ = [(n, ctypes.c_void_p) for n in
                 ("attn_norm", "q_a", "q_a_norm", "q_b", "kv_a", "kv_a_norm", "k_b", "v_b", "o_proj")]
+
+
+ROPE_MAX_DIM = 256
+GGML_F32, GGML_F16, GGML_BF16 = 0, 1, 30  # element types
+KV_LATENT, KV_ROPE = 512, 64
+KV_F16, KV_BF16, KV_FP8 = range(3)
+
+
+class RopeParams(ctypes.Structure):
+    """struct fdm_rope_params."""
+    _fields_ = [(n, ctypes.c_int) for n in ("dim", "layout", "scaling", "orig_ctx")] + [
+        (n, ctypes.c_double) for n in ("base", "factor", "beta_fast", "beta_slow", "mul")]
+
+
+class RopeTable(ctypes.Structure):
+    """struct fdm_rope_table."""
+    _fields_ = [("dim", ctypes.c_int), ("layout", ctypes.c_int), ("mul", ctypes.c_float), ("spare", ctypes.c_int),
+                ("turns", ctypes.c_uint64 * (ROPE_MAX_DIM // 2))]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """struct fdm_kv_cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("latent", "rope", "scale")] + [
+        (n, ctypes.c_int) for n in ("format", "n_pages", "page_size")]
+
+
+class MlaBatch(ctypes.Structure):
+    """struct fdm_mla_batch."""
+    _fields_ = [("B", ctypes.c_int), ("N", ctypes.c_int), ("H", ctypes.c_int), ("q_start", ctypes.c_void_p),
+                ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("pages_stride", ctypes.c_int),
+                ("max_kv", ctypes.c_int), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_int)]
+
+
 EXPERT_Q4K_BYTES = 24772608
 EXPERT_Q6K_BYTES = 28557312
 
@@ -48,6 +81,7 @@ _sz = ctypes.c_size_t
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 _f = ctypes.c_float
+_i64 = ctypes.c_int64
 
 # name -> argtypes (all functions return int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -102,6 +136,13 @@ SIGNATURES = {
     "fdm_moe_forward_batched_noalloc": [_i, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp],
     "fdm_rms_norm": [_vp, _vp, _vp, _i, _i, _vp],
     "fdm_moe_prefill": [_vp, _i, _vp, _i, _i, _vp, _vp, _vp],
+    "fdm_rope_table_init": [ctypes.POINTER(RopeParams), ctypes.POINTER(RopeTable)],
+    "fdm_rope": [ctypes.POINTER(RopeTable), _vp, _i, _i, _i, _i, _vp, _i, _i64, _i64, _vp, _i, _i64, _i64, _vp],
+    "fdm_kv_write": [ctypes.POINTER(KvCacheDesc), _vp, _i, _i64, _vp, ctypes.POINTER(RopeTable), _vp, _vp, _i, _vp],
+    "fdm_kv_read": [ctypes.POINTER(KvCacheDesc), _vp, _i, _vp, _i, _i64, _vp],
+    "fdm_mla_workspace": [_i, _i, ctypes.POINTER(_sz)],
+    "fdm_mla_attend": [ctypes.POINTER(KvCacheDesc), ctypes.POINTER(MlaBatch), _vp, _i64, _i64, _vp, _i64, _i64, _f,
+                       _vp, _i64, _i64, _vp, _vp, _sz, _vp],
     "fdm_prof_enable": [_i],
     "fdm_prof_reset": [],
     "fdm_prof_read": [_i, ctypes.POINTER(_i), ctypes.POINTER(ctypes.c_double),

@@ -33,6 +33,9 @@ SOURCES = [
     "dense_kernels.hip",
     "expert_stream.hip",
     "attn_kernels.hip",
+    "rope_kernels.hip",
+    "kvcache_kernels.hip",
+    "mla_tree_kernels.hip",
     "gguf_host.hip",
     "capi.hip",
 ]

@@ -9,6 +9,7 @@
 #include <sys/stat.h>
 #include <unistd.h>
 
+#include <algorithm>
 #include <atomic>
 #include <initializer_list>
 #include <math.h>
@@ -2309,6 +2310,285 @@ int fdm_dense_ffn(int L, const float* d_h_post, const float* d_h_in, float* d_hi
   a.inter = d.inter;
   a.n_cus = g_num_cus;
   FDM_HIP(launch_dense_ffn(a, s));
+  return FDM_OK;
+}
+
+// ---- rotary positions, the paged latent cache and its attention -------------------------
+// Arguments are checked before anything of the device is needed.
+static_assert(sizeof(RopeTable) == sizeof(fdm_rope_table) && kRopeMaxDim == FDM_ROPE_MAX_DIM, "one table");
+static_assert(kKvF16 == FDM_KV_F16 && kKvBf16 == FDM_KV_BF16 && kKvFp8 == FDM_KV_FP8, "formats");
+
+// The calling thread's device is the library's while this lives.
+struct OnDevice {
+  int prev = -1;
+  OnDevice() {
+    int now = -1;
+    if (hipGetDevice(&now) == hipSuccess && now != g.device && hipSetDevice(g.device) == hipSuccess) prev = now;
+  }
+  ~OnDevice() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
+static int elem_type(int ggml, ElemType* out, const char* what) {
+  switch (ggml) {
+    case FDM_GGML_F32: *out = ElemType::f32; return FDM_OK;
+    case FDM_GGML_F16: *out = ElemType::f16; return FDM_OK;
+    case FDM_GGML_BF16: *out = ElemType::bf16; return FDM_OK;
+  }
+  return fail(FDM_E_INVAL, "%s: type %d is none of F32, F16, BF16", what, ggml);
+}
+
+static size_t elem_size(ElemType t) { return t == ElemType::f32 ? 4 : 2; }
+
+// Whether n x m rows of `width` elements at strides a and b do not fall on each other.
+static bool rows_apart(int64_t a, int n, int64_t b, int m, int64_t width) {
+  a = llabs(a);
+  b = llabs(b);
+  if ((n > 1 && a < width) || (m > 1 && b < width)) return false;
+  if (n < 2 || m < 2) return true;
+  return a <= b ? (n - 1) * a + width <= b : (m - 1) * b + width <= a;
+}
+
+static int check_table(const fdm_rope_table* t) {
+  if (t->dim < 2 || t->dim > FDM_ROPE_MAX_DIM || t->dim % 2 || (t->layout != FDM_ROPE_INTERLEAVED && t->layout != FDM_ROPE_HALF))
+    return fail(FDM_E_INVAL, "rope table: dim %d layout %d", t->dim, t->layout);
+  return FDM_OK;
+}
+
+int fdm_rope_table_init(const fdm_rope_params* p, fdm_rope_table* out) {
+  if (!p || !out) return fail(FDM_E_INVAL, "null pointer");
+  if (p->dim < 2 || p->dim > FDM_ROPE_MAX_DIM || p->dim % 2)
+    return fail(FDM_E_INVAL, "rope dim %d: even, 2 .. %d", p->dim, FDM_ROPE_MAX_DIM);
+  if (p->layout != FDM_ROPE_INTERLEAVED && p->layout != FDM_ROPE_HALF) return fail(FDM_E_INVAL, "rope layout %d", p->layout);
+  if (p->scaling != FDM_ROPE_PLAIN && p->scaling != FDM_ROPE_LINEAR && p->scaling != FDM_ROPE_YARN)
+    return fail(FDM_E_INVAL, "rope scaling %d", p->scaling);
+  if (!(p->base > 1.0) || !isfinite(p->base)) return fail(FDM_E_INVAL, "rope base %g: above 1", p->base);
+  if (!isfinite(p->mul)) return fail(FDM_E_INVAL, "rope mul %g", p->mul);
+  if (p->scaling != FDM_ROPE_PLAIN && (!(p->factor >= 1.0) || !isfinite(p->factor)))
+    return fail(FDM_E_INVAL, "rope factor %g: at least 1", p->factor);
+  const int half = p->dim / 2;
+  long double lo = 0, hi = 1;
+  if (p->scaling == FDM_ROPE_YARN) {
+    if (p->orig_ctx < 1 || !(p->beta_slow > 0.0) || !(p->beta_fast > 0.0) || !isfinite(p->beta_slow) || !isfinite(p->beta_fast))
+      return fail(FDM_E_INVAL, "rope: orig_ctx %d, beta_fast %g, beta_slow %g", p->orig_ctx, p->beta_fast, p->beta_slow);
+    // in double, as the definition: floor and ceil may turn on the last bit
+    auto c = [&](double turns) { return p->dim * log(p->orig_ctx / (2.0 * M_PI * turns)) / (2.0 * log(p->base)); };
+    lo = fmax(floor(c(p->beta_fast)), 0.0);
+    hi = fmin(ceil(c(p->beta_slow)), (double)(half - 1));
+    if (hi < lo + 1) hi = lo + 1;
+  }
+  memset(out, 0, sizeof *out);
+  out->dim = p->dim;
+  out->layout = p->layout;
+  out->mul = p->mul == 0.0 ? 1.0f : (float)p->mul;
+  for (int i = 0; i < half; ++i) {
+    long double f = powl((long double)p->base, -2.0L * i / p->dim);
+    if (p->scaling == FDM_ROPE_LINEAR) f /= p->factor;
+    if (p->scaling == FDM_ROPE_YARN) {
+      long double ramp = (i - lo) / (hi - lo);
+      ramp = ramp < 0 ? 0 : ramp > 1 ? 1 : ramp;
+      f = f * ramp / p->factor + f * (1 - ramp);
+    }
+    out->turns[i] = (uint64_t)(f / (2.0L * 3.14159265358979323846264338327950288L) * 18446744073709551616.0L);
+  }
+  return FDM_OK;
+}
+
+int fdm_rope(const fdm_rope_table* table, const int32_t* d_pos, int T, int H, int D, int offset, const void* d_x,
+             int x_type, int64_t x_token_stride, int64_t x_head_stride, void* d_y, int y_type, int64_t y_token_stride,
+             int64_t y_head_stride, void* stream) {
+  if (!table) return fail(FDM_E_INVAL, "null rope table");
+  if (int rc = check_table(table)) return rc;
+  RopeArgs a{};
+  if (int rc = elem_type(x_type, &a.x_type, "x")) return rc;
+  if (int rc = elem_type(y_type, &a.y_type, "y")) return rc;
+  if (T < 0 || H < 1 || H > 4096 || D < 1 || D > 4096) return fail(FDM_E_INVAL, "T=%d H=%d D=%d (H, D <= 4096)", T, H, D);
+  if (offset < 0 || offset > D - table->dim) return fail(FDM_E_INVAL, "offset %d + dim %d past the head's %d", offset, table->dim, D);
+  if (T == 0) return check_ready();
+  if (!d_pos || !d_x || !d_y) return fail(FDM_E_INVAL, "null pointer");
+  const size_t xs = elem_size(a.x_type), ys = elem_size(a.y_type);
+  if (!aligned(d_x, xs) || !aligned(d_y, ys) || !aligned(d_pos, 4)) return fail(FDM_E_INVAL, "misaligned pointer");
+  const bool in_place = d_x == d_y;
+  if (in_place && (a.x_type != a.y_type || x_token_stride != y_token_stride || x_head_stride != y_head_stride))
+    return fail(FDM_E_INVAL, "in place: x and y must have one type and the same strides");
+  if (!rows_apart(y_head_stride, H, y_token_stride, T, in_place ? table->dim : D))
+    return fail(FDM_E_INVAL, "y: heads overlap (token stride %lld, head stride %lld)", (long long)y_token_stride,
+                (long long)y_head_stride);
+  if (int rc = check_ready()) return rc;
+  memcpy(&a.table, table, sizeof a.table);
+  a.pos = d_pos;
+  a.x = d_x;
+  a.y = d_y;
+  a.x_token = x_token_stride;
+  a.x_head = x_head_stride;
+  a.y_token = y_token_stride;
+  a.y_head = y_head_stride;
+  a.T = T;
+  a.H = H;
+  a.D = D;
+  a.offset = offset;
+  a.pass = !in_place;
+  const bool place = offset % 8 == 0 && (table->layout == FDM_ROPE_INTERLEAVED || table->dim % 16 == 0);
+  a.vec_x = place && aligned(d_x, 16) && x_token_stride % 8 == 0 && x_head_stride % 8 == 0;
+  a.vec_y = place && aligned(d_y, 16) && y_token_stride % 8 == 0 && y_head_stride % 8 == 0;
+  a.vec_behind = table->dim % 8 == 0;
+  OnDevice dev;
+  ProfScope prof(FDM_PROF_ROPE, as_stream(stream));
+  FDM_HIP(launch_rope(a, as_stream(stream)));
+  return FDM_OK;
+}
+
+static int check_cache(const fdm_kv_cache* c) {
+  if (!c) return fail(FDM_E_INVAL, "null cache");
+  if (c->format != FDM_KV_F16 && c->format != FDM_KV_BF16 && c->format != FDM_KV_FP8)
+    return fail(FDM_E_INVAL, "cache format %d", c->format);
+  if (c->page_size < 1 || (c->page_size & (c->page_size - 1)) || c->n_pages < 1 ||
+      (int64_t)c->n_pages * c->page_size > INT32_MAX)
+    return fail(FDM_E_INVAL, "%d pages of %d rows: a power of two each, below 2^31 in all", c->n_pages, c->page_size);
+  if (!c->d_latent || !c->d_rope || !aligned(c->d_latent, 16) || !aligned(c->d_rope, 16))
+    return fail(FDM_E_INVAL, "cache planes must be 16-byte aligned pointers");
+  if (c->format == FDM_KV_FP8 && (!c->d_scale || !aligned(c->d_scale, 4)))
+    return fail(FDM_E_INVAL, "an FP8 cache needs a 4-byte aligned scale plane");
+  return FDM_OK;
+}
+
+int fdm_kv_write(const fdm_kv_cache* c, const void* d_x, int x_type, int64_t x_stride, const float* d_norm_w,
+                 const fdm_rope_table* table, const int32_t* d_pos, const int32_t* d_slots, int T, void* stream) {
+  if (int rc = check_cache(c)) return rc;
+  KvWriteArgs a{};
+  ElemType t;
+  if (int rc = elem_type(x_type, &t, "x")) return rc;
+  if (T < 0) return fail(FDM_E_INVAL, "T=%d", T);
+  if (table) {
+    if (int rc = check_table(table)) return rc;
+    if (table->dim != FDM_KV_ROPE) return fail(FDM_E_INVAL, "rope table of dim %d: the cache's rows have %d", table->dim, FDM_KV_ROPE);
+  }
+  if (T == 0) return check_ready();
+  if (!d_x || !d_slots) return fail(FDM_E_INVAL, "null pointer");
+  if (table && !d_pos) return fail(FDM_E_INVAL, "a rotation needs positions");
+  const size_t es = elem_size(t);
+  if (!aligned(d_x, es) || !aligned(d_norm_w, 4) || !aligned(d_slots, 4) || !aligned(d_pos, 4))
+    return fail(FDM_E_INVAL, "misaligned pointer");
+  if (int rc = check_ready()) return rc;
+  if (table) memcpy(&a.table, table, sizeof a.table);
+  a.rotate = table != nullptr;
+  a.pos = d_pos;
+  a.x = d_x;
+  a.x_stride = x_stride;
+  a.vec_x = aligned(d_x, 16) && x_stride % 8 == 0;
+  a.vec_w = aligned(d_norm_w, 16);
+  a.norm_w = d_norm_w;
+  a.slots = d_slots;
+  a.T = T;
+  a.rows = c->n_pages * c->page_size;
+  a.latent = c->d_latent;
+  a.rope = c->d_rope;
+  a.scale = static_cast<uint8_t*>(c->d_scale);
+  OnDevice dev;
+  ProfScope prof(FDM_PROF_KV, as_stream(stream));
+  FDM_HIP(launch_kv_write(a, c->format, t, as_stream(stream)));
+  return FDM_OK;
+}
+
+int fdm_kv_read(const fdm_kv_cache* c, const int32_t* d_slots, int T, void* d_y, int y_type, int64_t y_stride,
+                void* stream) {
+  if (int rc = check_cache(c)) return rc;
+  ElemType t;
+  if (int rc = elem_type(y_type, &t, "y")) return rc;
+  if (T < 0) return fail(FDM_E_INVAL, "T=%d", T);
+  if (T == 0) return check_ready();
+  if (!d_y || !d_slots) return fail(FDM_E_INVAL, "null pointer");
+  if (!aligned(d_y, elem_size(t)) || !aligned(d_slots, 4)) return fail(FDM_E_INVAL, "misaligned pointer");
+  if (T > 1 && llabs(y_stride) < FDM_KV_LATENT + FDM_KV_ROPE)
+    return fail(FDM_E_INVAL, "y: rows of %d overlap at stride %lld", FDM_KV_LATENT + FDM_KV_ROPE, (long long)y_stride);
+  if (int rc = check_ready()) return rc;
+  KvReadArgs a{};
+  a.latent = c->d_latent;
+  a.rope = c->d_rope;
+  a.scale = static_cast<const uint8_t*>(c->d_scale);
+  a.slots = d_slots;
+  a.T = T;
+  a.rows = c->n_pages * c->page_size;
+  a.y = d_y;
+  a.y_stride = y_stride;
+  a.vec_y = aligned(d_y, 16) && y_stride % 8 == 0;
+  OnDevice dev;
+  ProfScope prof(FDM_PROF_KV, as_stream(stream));
+  FDM_HIP(launch_kv_read(a, c->format, t, as_stream(stream)));
+  return FDM_OK;
+}
+
+static int check_mla_shape(int N, int H) {
+  if (N < 0 || H < 1 || H > FDM_MLA_MAX_HEADS) return fail(FDM_E_INVAL, "N=%d H=%d (1 .. %d heads)", N, H, FDM_MLA_MAX_HEADS);
+  return FDM_OK;
+}
+
+int fdm_mla_workspace(int N, int H, size_t* bytes) {
+  if (int rc = check_mla_shape(N, H)) return rc;
+  if (!bytes) return fail(FDM_E_INVAL, "null pointer");
+  if (int rc = check_ready()) return rc;
+  *bytes = mla_tree_workspace(N, H);
+  return FDM_OK;
+}
+
+int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_q_lat, int64_t q_lat_token,
+                   int64_t q_lat_head, const void* d_q_rope, int64_t q_rope_token, int64_t q_rope_head, float scale,
+                   void* d_out, int64_t out_token, int64_t out_head, float* d_lse, void* d_workspace,
+                   size_t workspace_bytes, void* stream) {
+  if (int rc = check_cache(c)) return rc;
+  if (!b) return fail(FDM_E_INVAL, "null batch");
+  if (int rc = check_mla_shape(b->N, b->H)) return rc;
+  if (b->B < 1 || b->B > FDM_MLA_MAX_SEQS) return fail(FDM_E_INVAL, "%d sequences: 1 .. %d", b->B, FDM_MLA_MAX_SEQS);
+  if (b->pages_stride < 1) return fail(FDM_E_INVAL, "pages_stride %d", b->pages_stride);
+  if (b->max_kv < 0) return fail(FDM_E_INVAL, "max_kv %d", b->max_kv);
+  if (b->d_mask ? b->mask_words < 1 : b->mask_words != 0) return fail(FDM_E_INVAL, "mask_words %d", b->mask_words);
+  if (!isfinite(scale)) return fail(FDM_E_INVAL, "scale %g", (double)scale);
+  if (b->N == 0) return check_ready();
+  if (!b->d_q_start || !b->d_kv_len || !b->d_pages || !d_q_lat || !d_q_rope || !d_out || !d_workspace)
+    return fail(FDM_E_INVAL, "null pointer");
+  if (!aligned(b->d_q_start, 4) || !aligned(b->d_kv_len, 4) || !aligned(b->d_pages, 4) || !aligned(b->d_mask, 8) ||
+      !aligned(d_lse, 4) || !aligned(d_workspace, 256) || !aligned(d_q_lat, 16) || !aligned(d_q_rope, 16) ||
+      !aligned(d_out, 16))
+    return fail(FDM_E_INVAL, "misaligned pointer (q_lat, q_rope, out: 16 bytes, workspace: 256)");
+  for (int64_t s : {q_lat_token, q_lat_head, q_rope_token, q_rope_head, out_token, out_head})
+    if (s % 8) return fail(FDM_E_INVAL, "stride %lld: a multiple of 8 elements", (long long)s);
+  if (!rows_apart(out_head, b->H, out_token, b->N, FDM_KV_LATENT))
+    return fail(FDM_E_INVAL, "out: rows of %d overlap", FDM_KV_LATENT);
+  if (int rc = check_ready()) return rc;
+  if (workspace_bytes < mla_tree_workspace(b->N, b->H))
+    return fail(FDM_E_INVAL, "workspace of %zu bytes: %zu are needed", workspace_bytes, mla_tree_workspace(b->N, b->H));
+  MlaTreeArgs a{};
+  a.latent = c->d_latent;
+  a.rope = c->d_rope;
+  a.scale = static_cast<const uint8_t*>(c->d_scale);
+  a.n_pages = c->n_pages;
+  a.page_shift = __builtin_ctz(c->page_size);
+  a.pages = b->d_pages;
+  a.pages_stride = b->pages_stride;
+  a.max_len = (int)std::min<int64_t>((int64_t)b->pages_stride * c->page_size, INT32_MAX - 4096);
+  a.q_start = b->d_q_start;
+  a.kv_len = b->d_kv_len;
+  a.B = b->B;
+  a.N = b->N;
+  a.H = b->H;
+  a.mask = b->d_mask;
+  a.mask_words = b->mask_words;
+  a.q_lat = d_q_lat;
+  a.q_rope = d_q_rope;
+  a.ql_token = q_lat_token;
+  a.ql_head = q_lat_head;
+  a.qr_token = q_rope_token;
+  a.qr_head = q_rope_head;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.out = d_out;
+  a.out_token = out_token;
+  a.out_head = out_head;
+  a.lse = d_lse;
+  a.workspace = d_workspace;
+  OnDevice dev;
+  ProfScope prof(FDM_PROF_MLA, as_stream(stream));
+  FDM_HIP(launch_mla_tree(a, c->format, as_stream(stream)));
   return FDM_OK;
 }
 

@@ -355,6 +355,78 @@ class ExpertStream {
 // frees the pinned read buffers shared by all streamed layers
 void release_stream_pool();
 
+// the operators around the paged latent cache (rope_kernels.hip,
+// kvcache_kernels.hip, mla_tree_kernels.hip)
+enum class ElemType { f32, f16, bf16 };
+constexpr int kKvF16 = 0, kKvBf16 = 1, kKvFp8 = 2;  // FDM_KV_*
+constexpr int kRopeMaxDim = 256;
+struct RopeTable {  // fdm_rope_table
+  int dim, layout;
+  float mul;
+  int spare;
+  uint64_t turns[kRopeMaxDim / 2];  // frequency / 2 pi, in 2^-64 of a turn
+};
+struct RopeArgs {
+  RopeTable table;
+  const int* pos;             // [T]
+  const void* x;
+  void* y;
+  int64_t x_token, x_head, y_token, y_head;  // strides in elements
+  ElemType x_type, y_type;
+  int T, H, D, offset;
+  bool pass;                  // the values that are not rotated are copied (y is not x)
+  bool vec_x, vec_y;          // every run of eight rotated or leading values is 16-byte aligned
+  bool vec_behind;            // so are those behind the rotated part
+  int tpw;                    // tokens of a workgroup (set by the launcher)
+};
+hipError_t launch_rope(RopeArgs a, hipStream_t s);
+
+struct KvWriteArgs {
+  RopeTable table;
+  bool rotate;
+  const int* pos;             // [T], if rotate
+  const void* x;              // [T][576]
+  int64_t x_stride;
+  bool vec_x, vec_w;
+  const float* norm_w;        // [512] or null
+  const int* slots;           // [T]
+  int T, rows;                // rows of the cache
+  void *latent, *rope;
+  uint8_t* scale;
+};
+hipError_t launch_kv_write(const KvWriteArgs& a, int fmt, ElemType x, hipStream_t s);
+struct KvReadArgs {
+  const void *latent, *rope;
+  const uint8_t* scale;
+  const int* slots;
+  int T, rows;
+  void* y;                    // [T][576]
+  int64_t y_stride;
+  bool vec_y;
+};
+hipError_t launch_kv_read(const KvReadArgs& a, int fmt, ElemType y, hipStream_t s);
+
+struct MlaTreeArgs {
+  const void *latent, *rope;  // the cache's planes
+  const uint8_t* scale;
+  int n_pages, page_shift;
+  const int* pages;           // [B][pages_stride]
+  int pages_stride, max_len;  // max_len: positions a row of the table covers
+  const int *q_start, *kv_len;
+  int B, N, H;
+  const uint64_t* mask;       // [N][mask_words] or null: in order
+  int mask_words;
+  const void *q_lat, *q_rope;
+  int64_t ql_token, ql_head, qr_token, qr_head;
+  float scale_log2;           // score scale x log2(e)
+  void* out;
+  int64_t out_token, out_head;
+  float* lse;                 // [N][H] or null
+  void* workspace;
+};
+size_t mla_tree_workspace(int N, int H);
+hipError_t launch_mla_tree(const MlaTreeArgs& a, int fmt, hipStream_t s);
+
 // synth_kernels.hip
 hipError_t launch_synth_q4k(uint8_t* dst, size_t n_blocks, uint64_t seed, hipStream_t s);
 hipError_t launch_synth_q6k(uint8_t* dst, size_t n_blocks, uint64_t seed, hipStream_t s);

@@ -425,6 +425,134 @@ int fdm_attn_reset(int L);
 int fdm_attn_len(int L, int *len);
 int fdm_attn_release(int L);
 
+/* ---- rotary positions (no counterpart as a call of its own in the reference,
+ * whose mla_forward rotates in place for one token, infer.m:586-655).  Of each
+ * head's D values the `dim` from `offset` on are turned in pairs:
+ *   (u, v) -> mul * (u cos a - v sin a, u sin a + v cos a),  a = pos * f_i,
+ * pairs (2i, 2i + 1) (FDM_ROPE_INTERLEAVED) or (i, i + dim / 2) (FDM_ROPE_HALF),
+ * f_i = base^(-2i / dim), for longer contexts scaled:
+ *   FDM_ROPE_LINEAR  f_i / factor
+ *   FDM_ROPE_YARN    f_i ((1 - m) / factor + m), m = 1 - clamp((i - lo) / (hi - lo), 0, 1),
+ *     lo = max(floor(c(beta_fast)), 0), hi = min(ceil(c(beta_slow)), dim / 2 - 1), at least lo + 1,
+ *     c(b) = dim ln(orig_ctx / (2 pi b)) / (2 ln base)   (infer.m:586-624)
+ * fdm_rope_table_init fills a table on the host (no fdm_init needed): dim even,
+ * 2 .. FDM_ROPE_MAX_DIM, base > 1, factor >= 1, mul finite (0: 1).  A table is
+ * plain data and may be copied.  Its frequencies are fractions of a turn in
+ * 64-bit fixed point, so that angles are exact at every 32-bit position.
+ *
+ * fdm_rope: T tokens of H heads; d_pos [T] int32.  Types are FDM_GGML_F32,
+ * _F16 or _BF16; strides in elements; element e of head h of token t lies at
+ * t * token_stride + h * head_stride + e.  The arithmetic is fp32, rounded once
+ * to y_type.  In place (d_y = d_x, same type and strides) only the rotated
+ * values are written; otherwise all D are, and the two must not overlap.
+ * Aligned data (16-byte rows, offset and dim / 2 multiples of 8) moves by
+ * 16-byte accesses, any other element by element. */
+#define FDM_ROPE_INTERLEAVED 0
+#define FDM_ROPE_HALF 1
+#define FDM_ROPE_PLAIN 0
+#define FDM_ROPE_LINEAR 1
+#define FDM_ROPE_YARN 2
+#define FDM_ROPE_MAX_DIM 256
+typedef struct fdm_rope_params {
+  int dim, layout, scaling;
+  int orig_ctx;                /* YaRN: the context the model was trained on */
+  double base, factor;
+  double beta_fast, beta_slow; /* YaRN: 32 and 1 in R1                        */
+  double mul;
+} fdm_rope_params;
+typedef struct fdm_rope_table {
+  int dim, layout;
+  float mul;
+  int spare;
+  uint64_t turns[FDM_ROPE_MAX_DIM / 2];
+} fdm_rope_table;
+int fdm_rope_table_init(const fdm_rope_params *p, fdm_rope_table *out);
+int fdm_rope(const fdm_rope_table *table, const int32_t *d_pos, int T, int H, int D, int offset, const void *d_x,
+             int x_type, int64_t x_token_stride, int64_t x_head_stride, void *d_y, int y_type,
+             int64_t y_token_stride, int64_t y_head_stride, void *stream);
+
+/* ---- the paged latent cache of several sequences (MLACache, infer.m:663-669,
+ * holds one sequence in fp32).  A row is FDM_KV_LATENT latent values (keys and
+ * values) and FDM_KV_ROPE rotary ones (keys).  The planes are the caller's
+ * device memory, [n_pages][page_size][..]:
+ *   FDM_KV_F16, FDM_KV_BF16  latent [512] and rope [64] in that type, no scales
+ *   FDM_KV_FP8               latent [512] bytes e4m3, rope [64] BF16, scale [4] bytes:
+ *     byte e + 127 of each 128 latent values, which stand for code * 2^e; 255:
+ *     the group held an infinity or a NaN and reads back as NaN
+ * A row's slot is page * page_size + place, below 2^31.  page_size is a power
+ * of two.  latent and rope are 16-byte aligned, scale 4-byte.
+ *
+ * fdm_kv_write: rows x [T][576] (x_type F32, F16 or BF16, row stride in
+ * elements) into slots d_slots [T]:
+ *   latent = x[:512] / sqrt(mean(x[:512]^2) + 1e-6) * norm_w  (norm_w fp32 [512];
+ *            NULL: x[:512]), rope = x[512:] turned by table at d_pos [T]
+ *            (table NULL: x[512:]; table->dim is 64),
+ * in fp32, rounded once.  FP8: e is the smallest exponent with max |latent| <=
+ * 448 * 2^e, in -100 .. 119.  A slot that is negative or past the cache writes
+ * nothing (a padded batch).  The slots of one call must differ: a slot named
+ * twice holds one of its rows or a mix of them.
+ * fdm_kv_read: the rows widened into y [T][576]; a slot that is none leaves its
+ * row of y as it was. */
+#define FDM_KV_LATENT 512
+#define FDM_KV_ROPE 64
+#define FDM_KV_F16 0
+#define FDM_KV_BF16 1
+#define FDM_KV_FP8 2
+typedef struct fdm_kv_cache {
+  void *d_latent, *d_rope, *d_scale;
+  int format, n_pages, page_size;
+} fdm_kv_cache;
+int fdm_kv_write(const fdm_kv_cache *cache, const void *d_x, int x_type, int64_t x_stride, const float *d_norm_w,
+                 const fdm_rope_table *table, const int32_t *d_pos, const int32_t *d_slots, int T, void *stream);
+int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *d_y, int y_type, int64_t y_stride,
+                void *stream);
+
+/* ---- latent attention of several sequences' query tokens over the paged cache
+ * (infer.m:829-873 for one token of one sequence, between the absorbed query
+ * and v_b): for token i of sequence b and head h
+ *   s_j = scale (q_lat . latent_j + q_rope . rope_j)  over the positions j it sees,
+ *   out = sum_j softmax(s)_j latent_j,  lse = ln sum_j e^s_j.
+ * Sequence b has the query tokens q_start[b] .. q_start[b + 1] - 1 (n_b of
+ * them) and kv_len[b] cached positions, its own tokens (written before) the
+ * last n_b of these; position j lies in row j % page_size of page
+ * pages[b][j / page_size].  A token sees every position before its sequence's
+ * tokens, and of these the ones whose bit is set in its mask: bit d of the
+ * 64-bit words mask[token][mask_words] for the sequence's token d (bits past the
+ * words are clear: a tree of drafted tokens sets those of its branch, its own
+ * among them).  mask NULL: the tokens are in order, each sees those up to
+ * itself.  A token that sees nothing gets out = 0, lse = -infinity.  Values of
+ * positions that no token sees are not used, whatever they are; a page number
+ * outside the cache makes its positions unseen.  kv_len is cut to 0 .. pages_stride *
+ * page_size, q_start to 0 .. N.  Rows of out and lse outside every sequence
+ * are left as they were; sequences must not share tokens.
+ * q_lat [N][H][512], q_rope [N][H][64], out [N][H][512]: F16 for an F16 cache,
+ * else BF16; strides in elements, multiples of 8, 16-byte aligned.  lse
+ * (optional) fp32 [N][H].  Products of the 16-bit values accumulate in fp32 and
+ * softmax weights round to 16 bits before the second product.  1 <= H <=
+ * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS.  max_kv: the longest kv_len the
+ * caller expects (0: unknown); it only chooses among kernels.
+ * d_workspace: at least fdm_mla_workspace(N, H) bytes, 256-byte aligned, used
+ * by the call alone until it has run on its stream: calls that may overlap, and
+ * graphs that may run at once, need one each.  The call allocates nothing and
+ * may be captured.  The same arguments give the same bits. */
+#define FDM_MLA_MAX_HEADS 128
+#define FDM_MLA_MAX_SEQS 1024
+typedef struct fdm_mla_batch {
+  int B, N, H;
+  const int32_t *d_q_start;  /* [B + 1]          */
+  const int32_t *d_kv_len;   /* [B]              */
+  const int32_t *d_pages;    /* [B][pages_stride] */
+  int pages_stride;
+  int max_kv;
+  const uint64_t *d_mask;    /* [N][mask_words], or NULL */
+  int mask_words;
+} fdm_mla_batch;
+int fdm_mla_workspace(int N, int H, size_t *bytes);
+int fdm_mla_attend(const fdm_kv_cache *cache, const fdm_mla_batch *batch, const void *d_q_lat, int64_t q_lat_token,
+                   int64_t q_lat_head, const void *d_q_rope, int64_t q_rope_token, int64_t q_rope_head, float scale,
+                   void *d_out, int64_t out_token, int64_t out_head, float *d_lse, void *d_workspace,
+                   size_t workspace_bytes, void *stream);
+
 /* ---- dense FFN layers (the layers before the first MoE layer, L < 3 in
  * R1): replaces the dense branch of layer_forward (infer.m:1852-1868),
  *   hidden = h_in + W_down . (silu(W_gate . h_post) * (W_up . h_post)),
@@ -468,7 +596,10 @@ int fdm_dense_ffn(int L, const float *d_h_post, const float *d_h_in, float *d_hi
 #define FDM_PROF_DENSE 8    /* fdm_dense_ffn: both launches             */
 #define FDM_PROF_ATTN 9     /* fdm_attn_forward: the whole token        */
 #define FDM_PROF_CEILING 10 /* fdm_layer_read_ceiling                   */
-#define FDM_PROF_PHASES 11
+#define FDM_PROF_ROPE 11    /* fdm_rope                                 */
+#define FDM_PROF_KV 12      /* fdm_kv_write / fdm_kv_read               */
+#define FDM_PROF_MLA 13     /* fdm_mla_attend: both launches            */
+#define FDM_PROF_PHASES 14
 int fdm_prof_enable(int on);
 int fdm_prof_reset(void);
 int fdm_prof_read(int phase, int *count, double *total_ms, double *min_ms, double *max_ms);
