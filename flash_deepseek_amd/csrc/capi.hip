@@ -2317,6 +2317,7 @@ int fdm_dense_ffn(int L, const float* d_h_post, const float* d_h_in, float* d_hi
 // Arguments are checked before anything of the device is needed.
 static_assert(sizeof(RopeTable) == sizeof(fdm_rope_table) && kRopeMaxDim == FDM_ROPE_MAX_DIM, "one table");
 static_assert(kKvF16 == FDM_KV_F16 && kKvBf16 == FDM_KV_BF16 && kKvFp8 == FDM_KV_FP8, "formats");
+static_assert(kMlaMaxSeqs == FDM_MLA_MAX_SEQS, "sequences");
 
 // The calling thread's device is the library's while this lives.
 struct OnDevice {
@@ -2543,7 +2544,7 @@ int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_
   if (b->pages_stride < 1) return fail(FDM_E_INVAL, "pages_stride %d", b->pages_stride);
   if (b->max_kv < 0) return fail(FDM_E_INVAL, "max_kv %d", b->max_kv);
   if (b->d_mask ? b->mask_words < 1 : b->mask_words != 0) return fail(FDM_E_INVAL, "mask_words %d", b->mask_words);
-  if (!isfinite(scale)) return fail(FDM_E_INVAL, "scale %g", (double)scale);
+  if (!(scale > 0.0f) || !isfinite(scale)) return fail(FDM_E_INVAL, "scale %g: above 0", (double)scale);
   if (b->N == 0) return check_ready();
   if (!b->d_q_start || !b->d_kv_len || !b->d_pages || !d_q_lat || !d_q_rope || !d_out || !d_workspace)
     return fail(FDM_E_INVAL, "null pointer");

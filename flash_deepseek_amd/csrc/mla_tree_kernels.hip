@@ -6,117 +6,674 @@
 // stands before the tokens (j < len - n), or if bit j - (len - n) of the
 // token's mask is set; without a mask, if it does not stand behind token i's
 // own place len - n + i.
+//
+// The heads of a token share its sequence's rows, so (token, head) pairs are
+// the rows of two matrix products with the cached rows, 1088 products a pair
+// and position: 242 flops a byte of a BF16 cache with 128 heads, about what
+// separates the matrix cores from HBM.  A workgroup takes 128 such rows (one
+// token of 128 heads, eight of 16) and walks a range of positions, 32 at a time.
 #include "latent_device.h"
 
 namespace fdm {
 
 namespace {
 
-__device__ __forceinline__ bool tree_sees(const MlaTreeArgs& a, int token, int place, int64_t prefix, int64_t j) {
-  const int64_t d = j - prefix;
-  if (d < 0) return true;
-  if (!a.mask) return d <= place;
-  if (d >= 64 * (int64_t)a.mask_words) return false;
-  return (a.mask[(size_t)token * a.mask_words + (d >> 6)] >> (d & 63)) & 1;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kTileRows = 128;  // (token, head) rows of a workgroup
+constexpr int kTilePos = 32;    // positions of a step
+constexpr int kRing = 3;        // steps in LDS: one's values, one's keys, one landing
+constexpr int kLatBytes = kTilePos * kLatDim * 2, kRotBytes = kTilePos * kRotDim * 2;
+constexpr int kStepBytes = kLatBytes + kRotBytes;
+constexpr int kPBytes = kTileRows * kTilePos * 2;
+constexpr size_t kPartFloats = (size_t)kTileRows * kLatDim;
+constexpr float kGrow = 8.0f;  // a row's maximum (log2) is moved when it grew by more
+
+// A tile that several workgroups share is put together from their parts; the
+// workgroup that has its first part says so.
+struct JoinDesc {
+  int b, tile, parts, spare;
+};
+
+// workspace: JoinDesc [groups], row statistics [2 groups][128] (max, sum),
+// parts [2 groups][128][512]
+struct Space {
+  JoinDesc* desc;
+  float2* stat;
+  float* part;
+};
+__host__ __device__ size_t space_stat_at(int groups) { return ((size_t)groups * sizeof(JoinDesc) + 255) / 256 * 256; }
+__host__ __device__ size_t space_part_at(int groups) { return space_stat_at(groups) + (size_t)2 * groups * kTileRows * sizeof(float2); }
+__device__ Space space_of(void* p, int groups) {
+  char* c = static_cast<char*>(p);
+  return {reinterpret_cast<JoinDesc*>(c), reinterpret_cast<float2*>(c + space_stat_at(groups)),
+          reinterpret_cast<float*>(c + space_part_at(groups))};
 }
 
 template <int FMT>
-__device__ __forceinline__ float cache_value(const MlaTreeArgs& a, int64_t slot, int d) {
-  if constexpr (FMT == kKvFp8) {
-    const float s = scale_value(a.scale[slot * 4 + d / kLatGroup]);
-    return __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(a.latent)[slot * kLatDim + d], 0) * s;
-  } else if constexpr (FMT == kKvF16) {
-    return (float)static_cast<const _Float16*>(a.latent)[slot * kLatDim + d];
+struct Half {
+  typedef std::conditional_t<FMT == kKvF16, _Float16, __bf16> T;
+  typedef std::conditional_t<FMT == kKvF16, f16x4, bf16x4> x4;
+  typedef std::conditional_t<FMT == kKvF16, f16x8, bf16x8> x8;
+};
+// The matrix products in assembly: the 256 accumulation registers hold the
+// output all along and the scores' sums are in VGPRs, which the compiler does
+// not do by itself (it moves the output between the two files in every turn,
+// and spills).  It knows nothing of a product in assembly, so the waits that it
+// would insert are here: two states before one (an operand that an ALU
+// instruction has just written), and 20 behind the last one before its result
+// is read (8 passes and 3 more).  Products that add to one sum need none
+// between them.
+#define FDM_MFMA_OF(FMT, form, ...)                               \
+  if constexpr (FMT == kKvF16) {                                  \
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 " form : __VA_ARGS__); \
+  } else {                                                        \
+    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 " form : __VA_ARGS__); \
+  }
+template <int FMT, bool FIRST, bool LAST>
+__device__ __forceinline__ void mfma_score(f32x16& c, i32x4 a, i32x4 b) {
+  if constexpr (FIRST) {
+    FDM_MFMA_OF(FMT, "%0, %1, %2, 0", "=&v"(c) : "v"(a), "v"(b))
+  } else if constexpr (LAST) {
+    FDM_MFMA_OF(FMT, "%0, %1, %2, %0\n\ts_nop 15\n\ts_nop 3", "+v"(c) : "v"(a), "v"(b))
   } else {
-    return (float)static_cast<const __bf16*>(a.latent)[slot * kLatDim + d];
+    FDM_MFMA_OF(FMT, "%0, %1, %2, %0", "+v"(c) : "v"(a), "v"(b))
   }
 }
+template <int FMT>
+__device__ __forceinline__ void mfma_out(f32x16& o, i32x4 a, i32x4 b) {
+  FDM_MFMA_OF(FMT, "%0, %1, %2, %0", "+a"(o) : "v"(a), "v"(b))
+}
+#undef FDM_MFMA_OF
+// Between the two files, one register at a time, so that no sum is ever a
+// tuple of VGPRs to the compiler.
+__device__ __forceinline__ float acc_get(float a) {
+  float v;
+  asm("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(a));
+  return v;
+}
+__device__ __forceinline__ float acc_put(float v) {
+  float a;
+  asm("v_accvgpr_write_b32 %0, %1" : "=a"(a) : "v"(v));
+  return a;
+}
+// before the output's registers are read
+__device__ __forceinline__ void mfma_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+#define FDM_LDS __attribute__((address_space(3)))
+// four rows x 16 columns of 16-bit values, lane i of 16 pointing at four
+// columns of row i / 4: lane i gets column i of the four rows
+__device__ __forceinline__ f16x4 read_turned(const char* p, f16x4) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((FDM_LDS s16x4*)p));
+}
+__device__ __forceinline__ bf16x4 read_turned(const char* p, bf16x4) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((FDM_LDS bf16x4*)p);
+}
+
+// the row's place of its 16-byte piece g is g ^ row_swap(row): 16 rows' same
+// piece lie in 16 bank groups, and four rows' same four pieces in four
+__device__ __forceinline__ int row_swap(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+
+// a value that is the same in every lane, in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)(((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+}
+
+// A value that the compiler computes where it stands: it would otherwise
+// keep dozens of addresses that differ by constants over the whole loop.
+__device__ __forceinline__ int here(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// the value of lane ^ 32, combined
+template <typename F>
+__device__ __forceinline__ float across_halves(float v, F f) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+__device__ __attribute__((aligned(16))) uint32_t zero_row[kLatDim * 2 / 4];  // stands for a row that is none
 
 }  // namespace
 
-// One workgroup a (token, head): 256 positions at a time, a score a thread,
-// then two latent dims a thread over the chunk's positions.
-template <int FMT>
-__global__ __launch_bounds__(256) void k_mla_tree_plain(MlaTreeArgs a) {
-  typedef std::conditional_t<FMT == kKvF16, _Float16, __bf16> T;
-  __shared__ float q[kLatDim + kRotDim], red[4], ps[256];
-  __shared__ int slots[256];
-  const int token = blockIdx.x, h = blockIdx.y, tid = threadIdx.x;
-  int b = -1;
-  for (int k = 0; k < a.B; ++k)
-    if (token >= a.q_start[k] && token < a.q_start[k + 1]) {
-      b = k;
-      break;
-    }
-  if (b < 0) return;
-  const int place = token - a.q_start[b];
-  const int64_t len = min(max(a.kv_len[b], 0), a.max_len);
-  const int64_t prefix = len - (a.q_start[b + 1] - a.q_start[b]);
-  const T* ql = static_cast<const T*>(a.q_lat) + token * a.ql_token + h * a.ql_head;
-  const T* qr = static_cast<const T*>(a.q_rope) + token * a.qr_token + h * a.qr_head;
-  for (int d = tid; d < kLatDim; d += 256) q[d] = (float)ql[d];
-  if (tid < kRotDim) q[kLatDim + tid] = (float)qr[tid];
-  float m = -__builtin_inff(), was = m, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int64_t j0 = 0; j0 < len; j0 += 256) {
-    __syncthreads();
-    const int64_t j = j0 + tid;
-    int slot = -1;
-    if (j < len && tree_sees(a, token, place, prefix, j)) {
-      const int page = a.pages[(size_t)b * a.pages_stride + (j >> a.page_shift)];
-      if (page >= 0 && page < a.n_pages) slot = (page << a.page_shift) + (int)(j & ((1 << a.page_shift) - 1));
-    }
-    float s = -__builtin_inff();
-    if (slot >= 0) {
-      s = 0.0f;
-      for (int d = 0; d < kLatDim; ++d) s = fmaf(q[d], cache_value<FMT>(a, slot, d), s);
-      const T* r = static_cast<const T*>(a.rope) + (size_t)slot * kRotDim;
-      for (int d = 0; d < kRotDim; ++d) s = fmaf(q[kLatDim + d], (float)r[d], s);
-      s *= a.scale_log2;
-    }
-    slots[tid] = slot;
-    float c = s;
-#pragma unroll
-    for (int k = 32; k >= 1; k >>= 1) c = fmaxf(c, __shfl_xor(c, k));
-    if ((tid & 63) == 0) red[tid >> 6] = c;
-    __syncthreads();
-    c = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    m = fmaxf(m, c);
-    const float top = m == -__builtin_inff() ? 0.0f : m;  // nothing but -infinity or NaN so far
-    const float keep = exp2f(was - top);
-    ps[tid] = slot >= 0 ? exp2f(s - top) : 0.0f;
-    __syncthreads();
-    was = m;
-    l *= keep;
-    o0 *= keep;
-    o1 *= keep;
-    for (int k = 0; k < 256; ++k) {
-      if (slots[k] < 0) continue;
-      const float p = ps[k];
-      l += p;
-      o0 = fmaf(p, cache_value<FMT>(a, slots[k], tid), o0);
-      o1 = fmaf(p, cache_value<FMT>(a, slots[k], tid + 256), o1);
-    }
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(a.out) + token * a.out_token + h * a.out_head;
-  out[tid] = (T)(o0 * inv);
-  out[tid + 256] = (T)(o1 * inv);
-  if (a.lse && tid == 0)
-    a.lse[(size_t)token * a.H + h] = l == 0.0f ? -__builtin_inff() : (m + log2f(l)) * 0.6931471805599453f;
+// ---- the work: tiles of rows, steps of positions --------------------------------------
+// A tile is g = 128 / H tokens of one sequence; it has a step for every 32
+// positions that its last token may see (one at least, so that rows that see
+// nothing are written).  All steps of all tiles in order (sequence, tile,
+// step) are cut into equal ranges, one a workgroup.
+struct SeqWork {
+  int n, len, t0;  // tokens, positions, first token
+};
+__device__ __forceinline__ SeqWork seq_work(const MlaTreeArgs& a, int b) {
+  SeqWork s;
+  s.t0 = min(max(a.q_start[b], 0), a.N);
+  s.n = max(min(a.q_start[b + 1], a.N) - s.t0, 0);
+  s.len = min(max(a.kv_len[b], 0), a.max_len);
+  return s;
+}
+__device__ __forceinline__ int tile_steps(const SeqWork& s, int tile, int g, bool in_order) {
+  const int64_t seen = in_order ? (int64_t)s.len - s.n + min((tile + 1) * g, s.n) : s.len;
+  return max(1, (int)((seen + kTilePos - 1) / kTilePos));
+}
+// ceil(1 / 32) + .. + ceil(x / 32)
+__device__ __forceinline__ int64_t step_sum(int64_t x) {
+  const int64_t q = x / kTilePos, r = x % kTilePos;
+  return kTilePos * q * (q + 1) / 2 + r * (q + 1);
+}
+// steps of the sequence's tiles 0 .. tiles - 1
+__device__ int64_t steps_before(const SeqWork& s, int tiles, int g, bool in_order) {
+  if (!in_order || s.n == 1) return (int64_t)tiles * tile_steps(s, 0, s.n, in_order);
+  if (g == 1 && s.len >= s.n) return step_sum(s.len - s.n + tiles) - step_sum(s.len - s.n);
+  int64_t sum = 0;
+  for (int i = 0; i < tiles; ++i) sum += tile_steps(s, i, g, in_order);
+  return sum;
 }
 
-size_t mla_tree_workspace(int N, int H) {
-  (void)N;
-  (void)H;
-  return 256;
+template <int FMT>
+__global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
+  typedef typename Half<FMT>::T T;
+  typedef typename Half<FMT>::x4 x4;
+  typedef typename Half<FMT>::x8 x8;
+  __shared__ __attribute__((aligned(256))) char ring[kRing * kStepBytes];
+  __shared__ __attribute__((aligned(256))) char pbuf[2 * kPBytes];  // weights [2][step of 16][32 rows][lane] x 8
+  __shared__ float scale_by[2][kTileRows];                          // what the rows' sums so far are scaled by
+  __shared__ int moved[2][4];                                       // whether a wave's rows are
+  __shared__ uint32_t live[kRing];                                  // bytes: which rows of the step exist
+  __shared__ int64_t before[kMlaMaxSeqs + 1];                 // steps before each sequence
+  __shared__ int64_t wave_total[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, h = lane >> 5;
+  const int g = kTileRows / a.H;
+  const bool in_order = a.mask == nullptr;
+
+  // steps before each sequence: four sequences a thread
+  {
+    int64_t mine[4], sum = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      mine[k] = sum;
+      const int b = 4 * tid + k;
+      if (b < a.B) {
+        const SeqWork s = seq_work(a, b);
+        sum += steps_before(s, (s.n + g - 1) / g, g, in_order);
+      }
+    }
+    int64_t upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t v = __shfl_up(upto, d);
+      if (lane >= d) upto += v;
+    }
+    if (lane == 63) wave_total[wave] = upto;
+    __syncthreads();
+    int64_t base = upto - sum;
+    for (int w = 0; w < wave; ++w) base += wave_total[w];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (4 * tid + k <= a.B) before[4 * tid + k] = base + mine[k];
+    if (tid == 255 && a.B == 1024) before[1024] = base + sum;
+    __syncthreads();
+  }
+  const int64_t total = uniform(before[a.B]);
+  const int groups = gridDim.x;
+  // neighbours in the list on one XCD (workgroups go round the eight in turn)
+  const int group = groups % 8 ? blockIdx.x : (blockIdx.x % 8) * (groups / 8) + blockIdx.x / 8;
+  const int64_t per = uniform((total + groups - 1) / groups);
+  int64_t u = group * per;
+  const int64_t u_end = min(u + per, total);
+  const Space space = space_of(a.workspace, groups);
+  JoinDesc desc = {0, 0, 0, 0};
+
+  int b = 0;
+  if (u < u_end) {  // the last sequence that starts at or before u
+    int hi = a.B - 1;
+    while (b < hi) {
+      const int mid = (b + hi + 1) / 2;
+      if (uniform(before[mid]) <= u) b = mid;
+      else hi = mid - 1;
+    }
+  }
+  while (u < u_end) {
+    while (uniform(before[b + 1]) <= u) ++b;
+    SeqWork s = seq_work(a, b);
+    s = {uniform(s.n), uniform(s.len), uniform(s.t0)};
+    const int64_t seq_u = uniform(before[b]);
+    int tile = 0;
+    {  // the last tile that starts at or before u
+      int hi = (s.n + g - 1) / g - 1;
+      while (tile < hi) {
+        const int mid = (tile + hi + 1) / 2;
+        if (seq_u + steps_before(s, mid, g, in_order) <= u) tile = mid;
+        else hi = mid - 1;
+      }
+    }
+    const int64_t tile_u = seq_u + steps_before(s, tile, g, in_order);
+    const int steps = tile_steps(s, tile, g, in_order);
+    const int from = (int)(u - tile_u);
+    const int to = (int)min((int64_t)steps, u_end - tile_u);
+    const int n = s.n, len = s.len;
+    u = tile_u + to;
+    const int prefix = len - n;                // may be negative
+    const int first = s.t0 + tile * g;         // the tile's first token
+    const int rows = min(g, n - tile * g) * a.H;
+
+    // the row of this lane's scores, and its query as the products' B operand
+    const int row = 32 * wave + l32;
+    const bool row_is = row < rows;
+    const int tok = row_is ? row / a.H : 0, head = row_is ? row - tok * a.H : 0;
+    x8 q[36];
+    {
+      const T* ql = static_cast<const T*>(a.q_lat) + (int64_t)(first + tok) * a.ql_token + head * a.ql_head + 8 * h;
+      const T* qr = static_cast<const T*>(a.q_rope) + (int64_t)(first + tok) * a.qr_token + head * a.qr_head + 8 * h;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) q[k] = *reinterpret_cast<const x8*>(ql + 16 * k);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[32 + k] = *reinterpret_cast<const x8*>(qr + 16 * k);
+    }
+
+    // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7
+    const int my_row = 8 * wave + (lane >> 3);
+    auto page_of = [&](int step) -> int {  // the page of this lane's row; -1: none
+      const int64_t j = (int64_t)step * kTilePos + my_row;
+      if (step >= to || j >= len) return -1;
+      return a.pages[(size_t)b * a.pages_stride + (j >> a.page_shift)];
+    };
+    auto slot_of = [&](int step, int page) -> int {
+      if ((unsigned)page >= (unsigned)a.n_pages) return -1;
+      return (page << a.page_shift) + ((step * kTilePos + my_row) & ((1 << a.page_shift) - 1));
+    };
+    u32x4 code[4];
+    uint8_t code_scale[4];
+    auto bring = [&](int step, int page) {  // into ring place step % 3
+      char* at = ring + (step % kRing) * kStepBytes;
+      const int slot = slot_of(step, page);
+      const uint64_t is = __ballot(slot >= 0);
+      uint32_t byte = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) byte |= (uint32_t)((is >> (8 * k)) & 1) << k;
+      if (lane == 0) reinterpret_cast<uint8_t*>(&live[step % kRing])[wave] = (uint8_t)byte;
+      const int rope_piece = (lane & 7) ^ ((my_row >> 1) & 7);
+      const char* rp = slot >= 0 ? static_cast<const char*>(a.rope) + (size_t)slot * (kRotDim * 2) + 16 * rope_piece
+                                 : reinterpret_cast<const char*>(zero_row);
+      __builtin_amdgcn_global_load_lds(rp, (FDM_LDS uint32_t*)(at + kLatBytes + wave * 1024), 16, 0, 0);
+      if constexpr (FMT == kKvFp8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int sl = __shfl(slot, 8 * (2 * k + h));
+          const char* p = sl >= 0 ? static_cast<const char*>(a.latent) + (size_t)sl * kLatDim + 16 * l32
+                                  : reinterpret_cast<const char*>(zero_row);
+          code[k] = *reinterpret_cast<const u32x4*>(p);
+          const uint8_t* sp = sl >= 0 ? a.scale + (size_t)sl * 4 + (l32 >> 3) : reinterpret_cast<const uint8_t*>(zero_row);
+          code_scale[k] = *sp;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int sl = __builtin_amdgcn_readlane(slot, 8 * k);
+          const int r = 8 * wave + k;
+          const char* p = sl >= 0 ? static_cast<const char*>(a.latent) + (size_t)sl * (kLatDim * 2)
+                                  : reinterpret_cast<const char*>(zero_row);
+          __builtin_amdgcn_global_load_lds(p + ((lane ^ row_swap(r)) << 4), (FDM_LDS uint32_t*)(at + r * 1024), 16, 0, 0);
+        }
+      }
+    };
+    // FP8: the codes that bring() has in flight -> 16-bit values in LDS (exact)
+    auto widen = [&](int step) {
+      if constexpr (FMT == kKvFp8) {
+        char* at = ring + (step % kRing) * kStepBytes;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 8 * wave + 2 * k + h;
+          const float sc = scale_value(code_scale[k]);
+          u32x4 v[2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            v[i >> 1][2 * (i & 1)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, false));
+            v[i >> 1][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, true));
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<u32x4*>(at + r * 1024 + (((2 * l32 + i) ^ row_swap(r)) << 4)) = v[i];
+        }
+      }
+    };
+
+    // ---- the products
+    f32x16 o[8][2];  // [32 dims][32 rows]: dims 256 (wave & 1) + 32 i, rows 64 (wave >> 1) + 32 k
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][k][e] = acc_put(0.0f);
+    float m = -__builtin_inff(), l = 0.0f;
+    const int rh = wave >> 1, dh = wave & 1;
+
+    // scores of 32 positions x this wave's 32 rows: D row = position, column = query row
+    auto scores = [&](int step) {
+      const char* at = ring + (step % kRing) * kStepBytes;
+      const int key = here(l32 * 1024 + ((row_swap(l32) ^ h) << 4));
+      const int rot = here(kLatBytes + l32 * 128 + ((((l32 >> 1) & 7) ^ h) << 4));
+      f32x16 c;
+      auto product = [&](auto first, auto last, const char* p, const x8& qk) {
+        mfma_score<FMT, decltype(first)::value, decltype(last)::value>(c, *reinterpret_cast<const i32x4*>(p),
+                                                                      __builtin_bit_cast(i32x4, qk));
+      };
+      constexpr std::true_type yes{};
+      constexpr std::false_type no{};
+      product(yes, no, at + key, q[0]);
+#pragma unroll
+      for (int k = 1; k < 32; ++k) {
+        product(no, no, at + (key ^ ((k & 7) << 5)) + (k >> 3) * 256, q[k]);
+        if (k % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) product(no, no, at + (rot ^ (k << 5)), q[32 + k]);
+      product(no, yes, at + (rot ^ (3 << 5)), q[35]);
+      return c;
+    };
+    // the step's weights from its scores, into pbuf
+    auto weigh = [&](int step, f32x16 c, uint32_t see) {
+      if (__any(see != ~0u)) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (!((see >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1)) c[e] = -__builtin_inff();
+      }
+      float top = c[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, c[e]);
+      top = across_halves(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
+      const bool need = top > m + kGrow;
+      const bool any = __any(need);
+      if (any) {
+        const float keep = need ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+        if (need) m = top;
+        l *= keep;
+        if (lane < 32) scale_by[step & 1][row] = keep;
+      }
+      if (lane == 0) moved[step & 1][wave] = any;
+      const float off = m == -__builtin_inff() ? 0.0f : m;
+      float p[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(c[e], a.scale_log2, -off));
+        l += p[e];
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (T)p[8 * ks + e];
+        *reinterpret_cast<x8*>(pbuf + (step & 1) * kPBytes + ((ks * 4 + wave) * 64 + lane) * 16) = v;
+      }
+    };
+    // the rows' sums so far follow a moved maximum
+    auto follow = [&](int step) {
+      const int mv = moved[step & 1][2 * rh] | moved[step & 1][2 * rh + 1];
+      if (__builtin_amdgcn_readfirstlane(mv)) {
+        mfma_done();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float f = moved[step & 1][2 * rh + k] ? scale_by[step & 1][64 * rh + 32 * k + l32] : 1.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][k][e] = acc_put(acc_get(o[i][k][e]) * f);
+            __builtin_amdgcn_sched_barrier(0);  // 16 of them in VGPRs at a time
+          }
+        }
+      }
+    };
+    auto values = [&](int step) {
+      const char* at = ring + (step % kRing) * kStepBytes;
+      const int i16 = lane & 15, u4 = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+      const int vrow = 4 * h + (i16 >> 2);
+      const int v0 = here(vrow * 1024 + (((i16 >> 2) << 6) | ((u4 ^ h) << 4)) + 8 * (i16 & 1) + 512 * dh);
+      const int pl = here(2 * rh * 1024 + lane * 16);
+      const int v1 = (v0 + 8 * 1024) ^ 32;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x4 p[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          p[k] = *reinterpret_cast<const i32x4*>(pbuf + (step & 1) * kPBytes + (ks * 4 + k) * 1024 + pl);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int off = ks * 16384 + (i >> 2) * 256;
+          const x4 lo = read_turned(at + (v0 ^ ((i & 3) << 6)) + off, x4{});
+          const x4 hi = read_turned(at + (v1 ^ ((i & 3) << 6)) + off, x4{});
+          x8 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) mfma_out<FMT>(o[i][k], __builtin_bit_cast(i32x4, v), p[k]);
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    };
+    // values that are no numbers count for the tokens that see them through
+    // their score; a weight of 0 must not meet them
+    auto clean = [&](int step) {
+      char* at = ring + (step % kRing) * kStepBytes + 8 * wave * 1024 + 16 * lane;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        x8 v = *reinterpret_cast<x8*>(at + r * 1024);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!(__builtin_fabsf((float)v[e]) < __builtin_inff())) v[e] = (T)0.0f;
+        *reinterpret_cast<x8*>(at + r * 1024) = v;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // which positions of the step the lane's row sees
+    auto seen = [&](int step, uint32_t exists) -> uint32_t {
+      const int64_t d0 = (int64_t)step * kTilePos - prefix;  // the token place of the step's first position
+      uint32_t see = d0 >= 0 ? 0u : d0 <= -32 ? ~0u : (1u << -d0) - 1;
+      if (d0 > -32) {
+        if (in_order) {
+          const int64_t last = tile * g + tok - d0;  // of the step's positions
+          see = last >= 31 ? ~0u : last < 0 ? see : (see | ((2u << last) - 1));
+        } else {
+          // bits d0 .. d0 + 31 of the mask
+          const uint64_t* mask = a.mask + (size_t)(first + tok) * a.mask_words;
+          const int64_t at = d0 >= 0 ? d0 : 0;
+          const int64_t w = at >> 6;
+          uint64_t bits = w < a.mask_words ? mask[w] >> (at & 63) : 0;
+          if ((at & 63) && w + 1 < a.mask_words) bits |= mask[w + 1] << (64 - (at & 63));
+          see |= d0 >= 0 ? (uint32_t)bits : (uint32_t)bits << -d0;
+        }
+      }
+      return see & exists;
+    };
+
+    // Step j's keys and step j - 1's values are multiplied in one turn, so that
+    // the weights of one are computed beside the products of the other.
+    __syncthreads();  // the tile before has left LDS
+    int page = page_of(from);
+    bring(from, page);
+    page = page_of(from + 1);
+    widen(from);
+    bool dirty = false;
+    f32x16 c;
+    uint32_t see = 0;
+    auto landed = [&] {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __syncthreads();
+    };
+    auto ask = [&](int j) {  // what the rows see of step j, and its scores
+      const uint32_t exists = __builtin_amdgcn_readfirstlane(live[j % kRing]);
+      dirty = (int64_t)(j + 1) * kTilePos > prefix;
+      see = dirty ? seen(j, exists) : exists;
+      c = scores(j);
+    };
+    auto next = [&](int j) {
+      if (j < to) {
+        bring(j, page);
+        page = page_of(j + 1);
+      }
+    };
+    landed();
+    next(from + 1);
+    ask(from);
+    weigh(from, c, see);
+    if (from + 1 < to) widen(from + 1);
+#pragma nounroll
+    for (int j = from + 1; j <= to; ++j) {
+      landed();
+      if (dirty) {
+        clean(j - 1);
+        __syncthreads();
+      }
+      next(j + 1);
+      follow(j - 1);
+      if (j < to)
+        ask(j);
+      else
+        see = 0;  // no step: nothing is weighed
+      values(j - 1);
+      weigh(j, c, see);
+      if (j + 1 < to) widen(j + 1);
+    }
+
+    // ---- the tile's results, or a part of them
+    mfma_done();
+    l = across_halves(l, [](float x, float y) { return x + y; });
+    __syncthreads();
+    float* stat = reinterpret_cast<float*>(pbuf);  // [128] max, [128] sum
+    if (lane < 32) {
+      stat[row] = m;
+      stat[kTileRows + row] = l;
+    }
+    __syncthreads();
+    if (from == 0 && to == steps) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int r = 64 * rh + 32 * k + l32;
+        if (r < rows) {
+          const int t = r / a.H, hd = r - t * a.H;
+          const float sum = stat[kTileRows + r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+          T* out = static_cast<T*>(a.out) + (int64_t)(first + t) * a.out_token + hd * a.out_head + 256 * dh + 4 * h;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x4 v;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) v[c] = (T)(acc_get(o[i][k][4 * e + c]) * inv);
+              *reinterpret_cast<x4*>(out + 32 * i + 8 * e) = v;
+              __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+      }
+      if (a.lse && lane < 32 && row_is)
+        a.lse[(size_t)(first + tok) * a.H + head] =
+            l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    } else {
+      // the range's first tile may have begun in the workgroup before; its last goes on in the next
+      const int part = 2 * group + (from == 0 ? 1 : 0);
+      if (from == 0) desc = {b, tile, (int)((tile_u + steps - 1) / per) - group + 1, 0};
+      if (tid < kTileRows) space.stat[(size_t)part * kTileRows + tid] = make_float2(stat[tid], stat[kTileRows + tid]);
+      f32x4* to_part = reinterpret_cast<f32x4*>(space.part + (size_t)part * kPartFloats) + wave * 4096 + lane;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            to_part[((i * 2 + k) * 4 + e) * 64] =
+                f32x4{acc_get(o[i][k][4 * e]), acc_get(o[i][k][4 * e + 1]), acc_get(o[i][k][4 * e + 2]),
+                      acc_get(o[i][k][4 * e + 3])};
+            __builtin_amdgcn_sched_barrier(0);
+          }
+    }
+  }
+  if (tid == 0) space.desc[group] = desc;
+}
+
+// A tile's parts put together: M = max m, out = sum 2^(m - M) part / sum 2^(m - M) l.
+// Workgroup (group, w, i): the 32 dims x 64 rows that wave w holds as its
+// o[i]; thread: four dims of a row, twice.
+template <int FMT>
+__global__ __launch_bounds__(256) void k_mla_tree_join(MlaTreeArgs a, int groups) {
+  typedef typename Half<FMT>::T T;
+  typedef typename Half<FMT>::x4 x4;
+  const Space space = space_of(a.workspace, groups);
+  const int group = blockIdx.x;
+  const JoinDesc d = space.desc[group];
+  if (!d.parts) return;
+  const int w = blockIdx.y >> 3, i = blockIdx.y & 7;
+  const int lane = threadIdx.x & 63, e = threadIdx.x >> 6, l32 = lane & 31, h = lane >> 5;
+  const int g = kTileRows / a.H;
+  const SeqWork s = seq_work(a, d.b);
+  const int first = s.t0 + d.tile * g, rows = min(g, s.n - d.tile * g) * a.H;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int r = 64 * (w >> 1) + 32 * k + l32;
+    if (r >= rows) continue;
+    const f32x4* from = reinterpret_cast<const f32x4*>(space.part) + w * 4096 + ((i * 2 + k) * 4 + e) * 64 + lane;
+    auto part_of = [&](int p) { return p ? 2 * (group + p) : 2 * group + 1; };
+    float top = -__builtin_inff();
+    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, space.stat[(size_t)part_of(p) * kTileRows + r].x);
+    const float off = top == -__builtin_inff() ? 0.0f : top;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+    for (int p = 0; p < d.parts; ++p) {
+      const float2 st = space.stat[(size_t)part_of(p) * kTileRows + r];
+      const float f = __builtin_amdgcn_exp2f(st.x - off);
+      const f32x4 v = from[(size_t)part_of(p) * (kPartFloats / 4)];
+      l = fmaf(f, st.y, l);
+      // a part without any weight holds zeros
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] = fmaf(f, v[c], sum[c]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int t = r / a.H, hd = r - t * a.H;
+    T* out = static_cast<T*>(a.out) + (int64_t)(first + t) * a.out_token + hd * a.out_head;
+    x4 v;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = (T)(sum[c] * inv);
+    *reinterpret_cast<x4*>(out + 256 * (w & 1) + 32 * i + 8 * e + 4 * h) = v;
+    if (a.lse && (w & 1) == 0 && i == 0 && e == 0 && h == 0)
+      a.lse[(size_t)(first + t) * a.H + hd] =
+          l == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+  }
+}
+
+static int mla_tree_groups() { return max(1, g_num_cus); }
+
+size_t mla_tree_workspace(int, int) {
+  const int groups = mla_tree_groups();
+  return space_part_at(groups) + (size_t)2 * groups * kPartFloats * sizeof(float);
 }
 
 hipError_t launch_mla_tree(const MlaTreeArgs& a, int fmt, hipStream_t s) {
-  const dim3 grid(a.N, a.H);
+  const int groups = mla_tree_groups();
+  const dim3 join(groups, 32);
   switch (fmt) {
-    case kKvF16: k_mla_tree_plain<kKvF16><<<grid, 256, 0, s>>>(a); break;
-    case kKvBf16: k_mla_tree_plain<kKvBf16><<<grid, 256, 0, s>>>(a); break;
-    default: k_mla_tree_plain<kKvFp8><<<grid, 256, 0, s>>>(a);
+    case kKvF16:
+      k_mla_tree<kKvF16><<<groups, 256, 0, s>>>(a);
+      k_mla_tree_join<kKvF16><<<join, 256, 0, s>>>(a, groups);
+      break;
+    case kKvBf16:
+      k_mla_tree<kKvBf16><<<groups, 256, 0, s>>>(a);
+      k_mla_tree_join<kKvBf16><<<join, 256, 0, s>>>(a, groups);
+      break;
+    default:
+      k_mla_tree<kKvFp8><<<groups, 256, 0, s>>>(a);
+      k_mla_tree_join<kKvFp8><<<join, 256, 0, s>>>(a, groups);
   }
   return hipGetLastError();
 }

@@ -510,7 +510,7 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
 /* ---- latent attention of several sequences' query tokens over the paged cache
  * (infer.m:829-873 for one token of one sequence, between the absorbed query
  * and v_b): for token i of sequence b and head h
- *   s_j = scale (q_lat . latent_j + q_rope . rope_j)  over the positions j it sees,
+ *   s_j = scale (q_lat . latent_j + q_rope . rope_j)  over the positions j it sees (scale > 0),
  *   out = sum_j softmax(s)_j latent_j,  lse = ln sum_j e^s_j.
  * Sequence b has the query tokens q_start[b] .. q_start[b + 1] - 1 (n_b of
  * them) and kv_len[b] cached positions, its own tokens (written before) the

@@ -104,7 +104,7 @@ def attend(c=None, **kw):
                                  dict(q_start=None), dict(kv_len=None), dict(pages=None), dict(ql=None), dict(qr=None), dict(out=None),
                                  dict(ws=None), dict(ws=P + 128), dict(ql=P + 8), dict(qr=P + 8), dict(out=P + 8), dict(ql0=2052),
                                  dict(ql1=516), dict(qr0=260), dict(qr1=4), dict(o0=2044), dict(o1=511), dict(o1=504), dict(o0=512),
-                                 dict(scale=math.nan), dict(scale=math.inf), dict(lse=P + 2)])
+                                 dict(scale=math.nan), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(lse=P + 2)])
 def test_attend_refusals(bad):
     assert attend(**bad) == INVAL
 
