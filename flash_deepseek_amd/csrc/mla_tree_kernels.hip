@@ -76,12 +76,10 @@ struct Half {
   } else {                                                        \
     asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 " form : __VA_ARGS__); \
   }
-template <int FMT, bool FIRST, bool LAST>
+template <int FMT, bool FIRST>
 __device__ __forceinline__ void mfma_score(f32x16& c, i32x4 a, i32x4 b) {
   if constexpr (FIRST) {
     FDM_MFMA_OF(FMT, "%0, %1, %2, 0", "=&v"(c) : "v"(a), "v"(b))
-  } else if constexpr (LAST) {
-    FDM_MFMA_OF(FMT, "%0, %1, %2, %0\n\ts_nop 15\n\ts_nop 3", "+v"(c) : "v"(a), "v"(b))
   } else {
     FDM_MFMA_OF(FMT, "%0, %1, %2, %0", "+v"(c) : "v"(a), "v"(b))
   }
@@ -110,6 +108,19 @@ __device__ __forceinline__ void mfma_done() {
   __builtin_amdgcn_sched_barrier(0);
 }
 #define FDM_LDS __attribute__((address_space(3)))
+// 16 bytes a lane from memory straight into LDS: lane i's land at `to` + 16 i.
+// In assembly, because the compiler lets no LDS read start while a direct load
+// that it knows of is in flight, whichever part of LDS that fills; there is no
+// result register, and landed() waits for these loads.
+__device__ __forceinline__ void lds_load16(const char* from, char* to) {
+  const int at = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(FDM_LDS char*)to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+}
+// the same from `base` (in scalar registers) + `off`
+__device__ __forceinline__ void lds_load16(const char* base, int off, char* to) {
+  const int at = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(FDM_LDS char*)to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
+}
 // four rows x 16 columns of 16-bit values, lane i of 16 pointing at four
 // columns of row i / 4: lane i gets column i of the four rows
 __device__ __forceinline__ f16x4 read_turned(const char* p, f16x4) {
@@ -286,7 +297,8 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 
     // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7
     const int my_row = 8 * wave + (lane >> 3);
-    auto page_of = [&](int step) -> int {  // the page of this lane's row; -1: none
+    int page = -1;  // of this lane's row in the step that comes next; -1: none
+    auto page_of = [&](int step) -> int {
       const int64_t j = (int64_t)step * kTilePos + my_row;
       if (step >= to || j >= len) return -1;
       return a.pages[(size_t)b * a.pages_stride + (j >> a.page_shift)];
@@ -295,59 +307,59 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       if ((unsigned)page >= (unsigned)a.n_pages) return -1;
       return (page << a.page_shift) + ((step * kTilePos + my_row) & ((1 << a.page_shift) - 1));
     };
+    // Eight pieces of work (0 .. 7) that bring a step into ring place step % 3: 16-bit
+    // rows straight into LDS, FP8 codes into registers, from where widen() puts
+    // their 16-bit values (exact) into LDS in four.  A row that is none reads zeros.
     u32x4 code[4];
-    uint8_t code_scale[4];
-    auto bring = [&](int step, int page) {  // into ring place step % 3
+    uint32_t code_scale = 0;
+    int slot = -1;
+    auto bring = [&](int step, int piece) {
       char* at = ring + (step % kRing) * kStepBytes;
-      const int slot = slot_of(step, page);
-      const uint64_t is = __ballot(slot >= 0);
-      uint32_t byte = 0;
+      if (piece == 0) {
+        slot = slot_of(step, page);
+        const uint64_t is = __ballot(slot >= 0);
+        uint32_t byte = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) byte |= (uint32_t)((is >> (8 * k)) & 1) << k;
-      if (lane == 0) reinterpret_cast<uint8_t*>(&live[step % kRing])[wave] = (uint8_t)byte;
-      const int rope_piece = (lane & 7) ^ ((my_row >> 1) & 7);
-      const char* rp = slot >= 0 ? static_cast<const char*>(a.rope) + (size_t)slot * (kRotDim * 2) + 16 * rope_piece
-                                 : reinterpret_cast<const char*>(zero_row);
-      __builtin_amdgcn_global_load_lds(rp, (FDM_LDS uint32_t*)(at + kLatBytes + wave * 1024), 16, 0, 0);
+        for (int k = 0; k < 8; ++k) byte |= (uint32_t)((is >> (8 * k)) & 1) << k;
+        if (lane == 0) reinterpret_cast<uint8_t*>(&live[step % kRing])[wave] = (uint8_t)byte;
+        const int rope_piece = (lane & 7) ^ ((my_row >> 1) & 7);
+        const char* rp = static_cast<const char*>(a.rope) + (size_t)max(slot, 0) * (kRotDim * 2) + here(16 * rope_piece);
+        rp = slot >= 0 ? rp : reinterpret_cast<const char*>(zero_row);
+        lds_load16(rp, at + kLatBytes + wave * 1024);
+        page = page_of(step + 1);
+      }
       if constexpr (FMT == kKvFp8) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int sl = __shfl(slot, 8 * (2 * k + h));
-          const char* p = sl >= 0 ? static_cast<const char*>(a.latent) + (size_t)sl * kLatDim + 16 * l32
-                                  : reinterpret_cast<const char*>(zero_row);
-          code[k] = *reinterpret_cast<const u32x4*>(p);
-          const uint8_t* sp = sl >= 0 ? a.scale + (size_t)sl * 4 + (l32 >> 3) : reinterpret_cast<const uint8_t*>(zero_row);
-          code_scale[k] = *sp;
-        }
+        // eight lanes a row, 16 codes of each of its four groups a lane
+        if (piece & 1) return;
+        const int k = piece >> 1;
+        const char* p = static_cast<const char*>(a.latent) + (size_t)max(slot, 0) * kLatDim + here(16 * (lane & 7));
+        p = slot >= 0 ? p : reinterpret_cast<const char*>(zero_row);
+        code[k] = *reinterpret_cast<const u32x4*>(p + 128 * k);
+        if (k == 0)
+          code_scale = *reinterpret_cast<const uint32_t*>(
+              slot >= 0 ? reinterpret_cast<const char*>(a.scale) + (size_t)slot * 4 : reinterpret_cast<const char*>(zero_row));
       } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int sl = __builtin_amdgcn_readlane(slot, 8 * k);
-          const int r = 8 * wave + k;
-          const char* p = sl >= 0 ? static_cast<const char*>(a.latent) + (size_t)sl * (kLatDim * 2)
-                                  : reinterpret_cast<const char*>(zero_row);
-          __builtin_amdgcn_global_load_lds(p + ((lane ^ row_swap(r)) << 4), (FDM_LDS uint32_t*)(at + r * 1024), 16, 0, 0);
-        }
+        const int sl = __builtin_amdgcn_readlane(slot, 8 * piece);
+        const int r = 8 * wave + piece;
+        const char* p = static_cast<const char*>(a.latent) + (size_t)max(sl, 0) * (kLatDim * 2);
+        p = sl >= 0 ? p : reinterpret_cast<const char*>(zero_row);
+        lds_load16(p, here((lane ^ ((2 * wave + (piece >> 2)) & 3)) << 4) ^ ((piece & 3) << 6), at + r * 1024);
       }
     };
-    // FP8: the codes that bring() has in flight -> 16-bit values in LDS (exact)
-    auto widen = [&](int step) {
+    auto widen = [&](int step, int k) {
       if constexpr (FMT == kKvFp8) {
         char* at = ring + (step % kRing) * kStepBytes;
+        const int widen_at = here(my_row * 1024 + (((2 * (lane & 7)) ^ row_swap(my_row)) << 4));
+        const float sc = scale_value((int)((code_scale >> (8 * k)) & 0xFF));
+        u32x4 v[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 8 * wave + 2 * k + h;
-          const float sc = scale_value(code_scale[k]);
-          u32x4 v[2];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            v[i >> 1][2 * (i & 1)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, false));
-            v[i >> 1][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, true));
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            *reinterpret_cast<u32x4*>(at + r * 1024 + (((2 * l32 + i) ^ row_swap(r)) << 4)) = v[i];
+        for (int i = 0; i < 4; ++i) {
+          v[i >> 1][2 * (i & 1)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, false));
+          v[i >> 1][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, true));
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<u32x4*>(at + (widen_at ^ (16 * i)) + 256 * k) = v[i];
       }
     };
 
@@ -362,62 +374,92 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     float m = -__builtin_inff(), l = 0.0f;
     const int rh = wave >> 1, dh = wave & 1;
 
-    // scores of 32 positions x this wave's 32 rows: D row = position, column = query row
-    auto scores = [&](int step) {
-      const char* at = ring + (step % kRing) * kStepBytes;
-      const int key = here(l32 * 1024 + ((row_swap(l32) ^ h) << 4));
-      const int rot = here(kLatBytes + l32 * 128 + ((((l32 >> 1) & 7) ^ h) << 4));
-      f32x16 c;
-      auto product = [&](auto first, auto last, const char* p, const x8& qk) {
-        mfma_score<FMT, decltype(first)::value, decltype(last)::value>(c, *reinterpret_cast<const i32x4*>(p),
-                                                                      __builtin_bit_cast(i32x4, qk));
-      };
-      constexpr std::true_type yes{};
-      constexpr std::false_type no{};
-      product(yes, no, at + key, q[0]);
-#pragma unroll
-      for (int k = 1; k < 32; ++k) {
-        product(no, no, at + (key ^ ((k & 7) << 5)) + (k >> 3) * 256, q[k]);
-        if (k % 8 == 7) __builtin_amdgcn_sched_barrier(0);
-      }
-#pragma unroll
-      for (int k = 0; k < 3; ++k) product(no, no, at + (rot ^ (k << 5)), q[32 + k]);
-      product(no, yes, at + (rot ^ (3 << 5)), q[35]);
-      return c;
+    // Operands come out of LDS kAhead reads before the product that wants them:
+    // 36 of keys (position = l32, 8 dims at 16 k + 8 h), then 16 of values (dim =
+    // l32 of a block of 32; positions 16 s + 4 h + {0 .. 3, 8 .. 11}, the ones
+    // whose weights the lane has).
+    constexpr int kKeys = 36, kVals = 16, kAhead = 6;
+    i32x4 f[kAhead];
+    int key_at, rot_at, v0_at, v1_at;  // this lane's addresses
+    auto key_place = [&](int step) {
+      const int at = (step % kRing) * kStepBytes;
+      key_at = here(at + l32 * 1024 + ((row_swap(l32) ^ h) << 4));
+      rot_at = here(at + kLatBytes + l32 * 128 + ((((l32 >> 1) & 7) ^ h) << 4));
     };
-    // the step's weights from its scores, into pbuf
-    auto weigh = [&](int step, f32x16 c, uint32_t see) {
-      if (__any(see != ~0u)) {
+    auto val_place = [&](int step) {
+      const int i16 = lane & 15, u4 = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
+      v0_at = here((step % kRing) * kStepBytes + (4 * h + (i16 >> 2)) * 1024 + (((i16 >> 2) << 6) | ((u4 ^ h) << 4)) +
+                   8 * (i16 & 1) + 512 * dh);
+      v1_at = here((v0_at + 8 * 1024) ^ 32);
+    };
+    auto fetch_key = [&](int k) {
+      f[k % kAhead] = k < 32 ? *reinterpret_cast<const i32x4*>(ring + (key_at ^ ((k & 7) << 5)) + (k >> 3) * 256)
+                             : *reinterpret_cast<const i32x4*>(ring + (rot_at ^ ((k & 3) << 5)));
+    };
+    auto fetch_val = [&](int i, int place) {  // block i & 7 of 32 dims, positions 16 (i >> 3) ..
+      const int off = (i >> 3) * 16384 + ((i >> 2) & 1) * 256;
+      const x4 lo = read_turned(ring + (v0_at ^ ((i & 3) << 6)) + off, x4{});
+      const x4 hi = read_turned(ring + (v1_at ^ ((i & 3) << 6)) + off, x4{});
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+      f[place % kAhead] = i32x4{(int)x[0], (int)x[1], (int)y[0], (int)y[1]};
+    };
+    i32x4 w[2][2];  // the weights of step j - 1: [16 positions][32 rows]
+    auto fetch_weights = [&](int step) {
+      const int at = here((step & 1) * kPBytes + 2 * rh * 1024 + lane * 16);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (!((see >> (8 * (e >> 2) + 4 * h + (e & 3))) & 1)) c[e] = -__builtin_inff();
-      }
-      float top = c[0];
+      for (int i = 0; i < 4; ++i) w[i >> 1][i & 1] = *reinterpret_cast<const i32x4*>(pbuf + at + (i >> 1) * 4096 + (i & 1) * 1024);
+    };
+    f32x16 c;  // scores of 32 positions x this wave's 32 rows: D row = position, column = query row
+    auto key_product = [&](int k) {
+      const i32x4 b = __builtin_bit_cast(i32x4, q[k]);
+      if (k == 0) mfma_score<FMT, true>(c, f[0], b);
+      else mfma_score<FMT, false>(c, f[k % kAhead], b);
+    };
+    auto val_product = [&](int i, int place) {
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, c[e]);
-      top = across_halves(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
-      const bool need = top > m + kGrow;
-      const bool any = __any(need);
-      if (any) {
+      for (int k = 0; k < 2; ++k) mfma_out<FMT>(o[i & 7][k], f[place % kAhead], w[i >> 3][k]);
+    };
+
+    // The step's weights from its scores, in kWeigh pieces; the last puts them into pbuf.
+    constexpr int kWeigh = 7;
+    float off = 0.0f;
+    auto hide = [&](uint32_t see) {
+      const uint32_t mine = see >> (4 * h);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!((mine >> (8 * (e >> 2) + (e & 3))) & 1)) c[e] = -__builtin_inff();
+    };
+    i32x4 p8[2];
+    auto weigh = [&](int step, int piece) {
+      if (piece == 0) {
+        float top = c[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, c[e]);
+        top = across_halves(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
+        const bool need = top > m + kGrow;
         const float keep = need ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-        if (need) m = top;
+        m = need ? top : m;
         l *= keep;
-        if (lane < 32) scale_by[step & 1][row] = keep;
-      }
-      if (lane == 0) moved[step & 1][wave] = any;
-      const float off = m == -__builtin_inff() ? 0.0f : m;
-      float p[16];
+        if (lane < 32) scale_by[step & 1][here(row)] = keep;
+        const uint64_t any = __ballot(need);
+        if (lane == 0) moved[step & 1][wave] = any != 0;
+        off = m == -__builtin_inff() ? 0.0f : m;
+      } else if (piece < 5) {
+        float p[4];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(fmaf(c[e], a.scale_log2, -off));
-        l += p[e];
-      }
+        for (int e = 0; e < 4; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(fmaf(c[4 * (piece - 1) + e], a.scale_log2, -off));
+          l += p[e];
+        }
+        x4 v;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        x8 v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (T)p[8 * ks + e];
-        *reinterpret_cast<x8*>(pbuf + (step & 1) * kPBytes + ((ks * 4 + wave) * 64 + lane) * 16) = v;
+        for (int e = 0; e < 4; ++e) v[e] = (T)p[e];
+        const u32x2 u = __builtin_bit_cast(u32x2, v);
+        p8[(piece - 1) >> 1][2 * ((piece - 1) & 1)] = (int)u[0];
+        p8[(piece - 1) >> 1][2 * ((piece - 1) & 1) + 1] = (int)u[1];
+      } else {
+        const int ks = piece - 5;
+        *reinterpret_cast<i32x4*>(pbuf + (step & 1) * kPBytes + ((ks * 4 + wave) * 64 + lane) * 16) = p8[ks];
       }
     };
     // the rows' sums so far follow a moved maximum
@@ -434,33 +476,6 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
             for (int e = 0; e < 16; ++e) o[i][k][e] = acc_put(acc_get(o[i][k][e]) * f);
             __builtin_amdgcn_sched_barrier(0);  // 16 of them in VGPRs at a time
           }
-        }
-      }
-    };
-    auto values = [&](int step) {
-      const char* at = ring + (step % kRing) * kStepBytes;
-      const int i16 = lane & 15, u4 = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-      const int vrow = 4 * h + (i16 >> 2);
-      const int v0 = here(vrow * 1024 + (((i16 >> 2) << 6) | ((u4 ^ h) << 4)) + 8 * (i16 & 1) + 512 * dh);
-      const int pl = here(2 * rh * 1024 + lane * 16);
-      const int v1 = (v0 + 8 * 1024) ^ 32;
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        i32x4 p[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          p[k] = *reinterpret_cast<const i32x4*>(pbuf + (step & 1) * kPBytes + (ks * 4 + k) * 1024 + pl);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int off = ks * 16384 + (i >> 2) * 256;
-          const x4 lo = read_turned(at + (v0 ^ ((i & 3) << 6)) + off, x4{});
-          const x4 hi = read_turned(at + (v1 ^ ((i & 3) << 6)) + off, x4{});
-          x8 v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
-#pragma unroll
-          for (int k = 0; k < 2; ++k) mfma_out<FMT>(o[i][k], __builtin_bit_cast(i32x4, v), p[k]);
-          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
       }
     };
@@ -499,53 +514,95 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       return see & exists;
     };
 
-    // Step j's keys and step j - 1's values are multiplied in one turn, so that
-    // the weights of one are computed beside the products of the other.
-    __syncthreads();  // the tile before has left LDS
-    int page = page_of(from);
-    bring(from, page);
-    page = page_of(from + 1);
-    widen(from);
-    bool dirty = false;
-    f32x16 c;
-    uint32_t see = 0;
+    // In one turn step j's keys and then step j - 1's values are multiplied;
+    // beside the keys step j + 1 is brought, beside the values step j's weights
+    // are computed.  The order of issue is the source's: a piece of that work
+    // behind each product, a product's operand requested six products ahead.
     auto landed = [&] {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
     };
-    auto ask = [&](int j) {  // what the rows see of step j, and its scores
-      const uint32_t exists = __builtin_amdgcn_readfirstlane(live[j % kRing]);
+    uint32_t see = 0;
+    bool dirty = false;
+    auto look = [&](int j) {  // what the rows see of step j
+      const uint32_t exists = uniform((int)live[j % kRing]);
       dirty = (int64_t)(j + 1) * kTilePos > prefix;
       see = dirty ? seen(j, exists) : exists;
-      c = scores(j);
     };
-    auto next = [&](int j) {
-      if (j < to) {
-        bring(j, page);
-        page = page_of(j + 1);
+    auto turn = [&](int j, auto with_values) {
+      constexpr bool VALUES = decltype(with_values)::value;
+      key_place(j);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) fetch_key(k);
+      if (VALUES) val_place(j - 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k) {
+        key_product(k);
+        if (k + kAhead < kKeys) fetch_key(k + kAhead);
+        else if (VALUES) fetch_val(k + kAhead - kKeys, k + kAhead);
+        if (VALUES && k == kKeys - 3) fetch_weights(j - 1);
+        if (k % 3 == 1 && k < 24) bring(j + 1, k / 3);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (VALUES) {
+        val_product(0, kKeys);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");  // the scores may be read
+      __builtin_amdgcn_sched_barrier(0);
+      if (__any(see != ~0u)) hide(see);
+      if constexpr (VALUES) {
+#pragma unroll
+        for (int i = 0; i < kVals; ++i) {
+          if (i) val_product(i, kKeys + i);
+          if (i + kAhead < kVals) fetch_val(i + kAhead, kKeys + i + kAhead);
+          if (i < kWeigh) weigh(j, i);
+          else if (i >= kVals - 4) widen(j + 1, i - (kVals - 4));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kWeigh; ++i) weigh(j, i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) widen(j + 1, i);
       }
     };
-    landed();
-    next(from + 1);
-    ask(from);
-    weigh(from, c, see);
-    if (from + 1 < to) widen(from + 1);
-#pragma nounroll
-    for (int j = from + 1; j <= to; ++j) {
-      landed();
+    auto clear_of = [&](int j) {  // step j's values and sums made ready for its weights
       if (dirty) {
-        clean(j - 1);
+        clean(j);
         __syncthreads();
       }
-      next(j + 1);
-      follow(j - 1);
-      if (j < to)
-        ask(j);
-      else
-        see = 0;  // no step: nothing is weighed
-      values(j - 1);
-      weigh(j, c, see);
-      if (j + 1 < to) widen(j + 1);
+      if (j > from) follow(j);  // the first step's sums are zeros
+    };
+    __syncthreads();  // the tile before has left LDS
+    page = page_of(from);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) bring(from, k);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) widen(from, k);
+    landed();
+    look(from);
+    turn(from, std::false_type{});
+#pragma nounroll
+    for (int j = from + 1; j < to; ++j) {
+      landed();
+      clear_of(j - 1);
+      look(j);
+      turn(j, std::true_type{});
+    }
+    landed();
+    clear_of(to - 1);
+    val_place(to - 1);
+    fetch_weights(to - 1);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch_val(i, i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kVals; ++i) {
+      val_product(i, i);
+      if (i + kAhead < kVals) fetch_val(i + kAhead, i + kAhead);
+      __builtin_amdgcn_sched_barrier(0);
     }
 
     // ---- the tile's results, or a part of them
