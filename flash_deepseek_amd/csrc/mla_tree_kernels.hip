@@ -65,16 +65,18 @@ struct Half {
 // The matrix products in assembly: the 256 accumulation registers hold the
 // output all along and the scores' sums are in VGPRs, which the compiler does
 // not do by itself (it moves the output between the two files in every turn,
-// and spills).  It knows nothing of a product in assembly, so the waits that it
-// would insert are here: two states before one (an operand that an ALU
-// instruction has just written), and 20 behind the last one before its result
-// is read (8 passes and 3 more).  Products that add to one sum need none
-// between them.
+// and spills).  It knows nothing of a product in assembly and inserts no waits
+// for one, so the source sees to them:
+//  - an operand that an ALU instruction wrote needs two states before the
+//    product: every operand here was loaded, from LDS or memory;
+//  - a result needs 11 states (8 passes and 3) before an ALU instruction reads
+//    it: products_done() stands before such reads;
+//  - products that add to one sum need none between them.
 #define FDM_MFMA_OF(FMT, form, ...)                               \
   if constexpr (FMT == kKvF16) {                                  \
-    asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 " form : __VA_ARGS__); \
+    asm("v_mfma_f32_32x32x16_f16 " form : __VA_ARGS__); \
   } else {                                                        \
-    asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 " form : __VA_ARGS__); \
+    asm("v_mfma_f32_32x32x16_bf16 " form : __VA_ARGS__); \
   }
 template <int FMT, bool FIRST>
 __device__ __forceinline__ void mfma_score(f32x16& c, i32x4 a, i32x4 b) {
@@ -101,24 +103,24 @@ __device__ __forceinline__ float acc_put(float v) {
   asm("v_accvgpr_write_b32 %0, %1" : "=a"(a) : "v"(v));
   return a;
 }
-// before the output's registers are read
-__device__ __forceinline__ void mfma_done() {
+// before an ALU instruction reads what products have written
+__device__ __forceinline__ void products_done() {
   __builtin_amdgcn_sched_barrier(0);
-  asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+  asm volatile("s_nop 11" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
 #define FDM_LDS __attribute__((address_space(3)))
 // 16 bytes a lane from memory straight into LDS: lane i's land at `to` + 16 i.
 // In assembly, because the compiler lets no LDS read start while a direct load
 // that it knows of is in flight, whichever part of LDS that fills; there is no
-// result register, and landed() waits for these loads.
+// result register, and landed() waits for these loads.  With a scalar base
+// that v_readlane wrote, five states must lie between that and this.
 __device__ __forceinline__ void lds_load16(const char* from, char* to) {
-  const int at = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(FDM_LDS char*)to);
+  const int at = (int)(uintptr_t)(FDM_LDS char*)to;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
 }
-// the same from `base` (in scalar registers) + `off`
-__device__ __forceinline__ void lds_load16(const char* base, int off, char* to) {
-  const int at = __builtin_amdgcn_readfirstlane((int)(uintptr_t)(FDM_LDS char*)to);
+__device__ __forceinline__ void lds_load16(uint64_t base, int off, char* to) {
+  const int at = (int)(uintptr_t)(FDM_LDS char*)to;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
 }
 // four rows x 16 columns of 16-bit values, lane i of 16 pointing at four
@@ -201,8 +203,8 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   __shared__ __attribute__((aligned(256))) char ring[kRing * kStepBytes];
   __shared__ __attribute__((aligned(256))) char pbuf[2 * kPBytes];  // weights [2][step of 16][32 rows][lane] x 8
   __shared__ float scale_by[2][kTileRows];                          // what the rows' sums so far are scaled by
-  __shared__ int moved[2][4];                                       // whether a wave's rows are
-  __shared__ uint32_t live[kRing];                                  // bytes: which rows of the step exist
+  __shared__ int moved[2][4];                                       // the step at which a wave's rows last were
+  __shared__ int live[kRing];                                       // bytes: which rows of the step exist
   __shared__ int64_t before[kMlaMaxSeqs + 1];                 // steps before each sequence
   __shared__ int64_t wave_total[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -295,60 +297,64 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       for (int k = 0; k < 4; ++k) q[32 + k] = *reinterpret_cast<const x8*>(qr + 16 * k);
     }
 
-    // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7
+    // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7, eight lanes
+    // each.  kBring pieces of work: 16-bit rows go straight into LDS, one a piece;
+    // FP8 codes into registers, from where widen() puts their 16-bit values
+    // (exact) into LDS in four pieces.  A row that is none reads zeros.
+    constexpr int kBring = 9;
     const int my_row = 8 * wave + (lane >> 3);
-    int page = -1;  // of this lane's row in the step that comes next; -1: none
-    auto page_of = [&](int step) -> int {
-      const int64_t j = (int64_t)step * kTilePos + my_row;
-      if (step >= to || j >= len) return -1;
-      return a.pages[(size_t)b * a.pages_stride + (j >> a.page_shift)];
+    const int* pages = a.pages + (size_t)b * a.pages_stride;
+    int page;          // of this lane's row in the step that comes next
+    const char* mine;  // this lane's row in the step that is brought
+    uint64_t base;     // the row that the next piece brings
+    auto page_of = [&](int step) { return pages[min(step * kTilePos + my_row, max(len - 1, 0)) >> a.page_shift]; };
+    auto base_of = [&](int k) {
+      return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uintptr_t)mine, 8 * k) |
+             (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)((uintptr_t)mine >> 32), 8 * k) << 32;
     };
-    auto slot_of = [&](int step, int page) -> int {
-      if ((unsigned)page >= (unsigned)a.n_pages) return -1;
-      return (page << a.page_shift) + ((step * kTilePos + my_row) & ((1 << a.page_shift) - 1));
-    };
-    // Eight pieces of work (0 .. 7) that bring a step into ring place step % 3: 16-bit
-    // rows straight into LDS, FP8 codes into registers, from where widen() puts
-    // their 16-bit values (exact) into LDS in four.  A row that is none reads zeros.
     u32x4 code[4];
     uint32_t code_scale = 0;
-    int slot = -1;
-    auto bring = [&](int step, int piece) {
-      char* at = ring + (step % kRing) * kStepBytes;
+    auto bring = [&](int step, int piece, int ring_at) {
+      char* at = ring + ring_at;
       if (piece == 0) {
-        slot = slot_of(step, page);
-        const uint64_t is = __ballot(slot >= 0);
-        uint32_t byte = 0;
+        const int j = step * kTilePos + my_row;
+        const bool is = (unsigned)page < (unsigned)a.n_pages && j < len && step < to;
+        const int slot = is ? (page << a.page_shift) + (j & ((1 << a.page_shift) - 1)) : 0;
+        const uint64_t all = __ballot(is);
+        uint32_t byte = 0xFF;
+        if (all != ~0ull) {
+          byte = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) byte |= (uint32_t)((is >> (8 * k)) & 1) << k;
-        if (lane == 0) reinterpret_cast<uint8_t*>(&live[step % kRing])[wave] = (uint8_t)byte;
-        const int rope_piece = (lane & 7) ^ ((my_row >> 1) & 7);
-        const char* rp = static_cast<const char*>(a.rope) + (size_t)max(slot, 0) * (kRotDim * 2) + here(16 * rope_piece);
-        rp = slot >= 0 ? rp : reinterpret_cast<const char*>(zero_row);
-        lds_load16(rp, at + kLatBytes + wave * 1024);
+          for (int k = 0; k < 8; ++k) byte |= (uint32_t)((all >> (8 * k)) & 1) << k;
+        }
+        reinterpret_cast<uint8_t*>(&live[step % kRing])[wave] = (uint8_t)byte;
+        const char* rp = static_cast<const char*>(a.rope) + (size_t)slot * (kRotDim * 2) + here(16 * ((lane & 7) ^ ((my_row >> 1) & 7)));
+        mine = static_cast<const char*>(a.latent) + (size_t)slot * (FMT == kKvFp8 ? kLatDim : kLatDim * 2);
+        const char* none = reinterpret_cast<const char*>(zero_row);
+        mine = is ? mine : none;
+        lds_load16(is ? rp : none, at + kLatBytes + wave * 1024);
+        if constexpr (FMT == kKvFp8) {
+          mine += here(16 * (lane & 7));
+          code_scale = *reinterpret_cast<const uint32_t*>(is ? reinterpret_cast<const char*>(a.scale) + (size_t)slot * 4 : none);
+        } else {
+          base = base_of(0);
+        }
         page = page_of(step + 1);
+        return;
       }
+      const int k = piece - 1;
       if constexpr (FMT == kKvFp8) {
-        // eight lanes a row, 16 codes of each of its four groups a lane
-        if (piece & 1) return;
-        const int k = piece >> 1;
-        const char* p = static_cast<const char*>(a.latent) + (size_t)max(slot, 0) * kLatDim + here(16 * (lane & 7));
-        p = slot >= 0 ? p : reinterpret_cast<const char*>(zero_row);
-        code[k] = *reinterpret_cast<const u32x4*>(p + 128 * k);
-        if (k == 0)
-          code_scale = *reinterpret_cast<const uint32_t*>(
-              slot >= 0 ? reinterpret_cast<const char*>(a.scale) + (size_t)slot * 4 : reinterpret_cast<const char*>(zero_row));
+        // 16 codes of each of the row's four groups a lane
+        if (k < 4) code[k] = *reinterpret_cast<const u32x4*>(mine + 128 * k);
       } else {
-        const int sl = __builtin_amdgcn_readlane(slot, 8 * piece);
-        const int r = 8 * wave + piece;
-        const char* p = static_cast<const char*>(a.latent) + (size_t)max(sl, 0) * (kLatDim * 2);
-        p = sl >= 0 ? p : reinterpret_cast<const char*>(zero_row);
-        lds_load16(p, here((lane ^ ((2 * wave + (piece >> 2)) & 3)) << 4) ^ ((piece & 3) << 6), at + r * 1024);
+        const int r = 8 * wave + k;
+        lds_load16(base, here((lane ^ ((2 * wave) & 3)) << 4) ^ (((k >> 2) << 4) | ((k & 3) << 6)), at + r * 1024);
+        if (k < 7) base = base_of(k + 1);
       }
     };
-    auto widen = [&](int step, int k) {
+    auto widen = [&](int k, int ring_at) {
       if constexpr (FMT == kKvFp8) {
-        char* at = ring + (step % kRing) * kStepBytes;
+        char* at = ring + ring_at;
         const int widen_at = here(my_row * 1024 + (((2 * (lane & 7)) ^ row_swap(my_row)) << 4));
         const float sc = scale_value((int)((code_scale >> (8 * k)) & 0xFF));
         u32x4 v[2];
@@ -381,14 +387,13 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     constexpr int kKeys = 36, kVals = 16, kAhead = 6;
     i32x4 f[kAhead];
     int key_at, rot_at, v0_at, v1_at;  // this lane's addresses
-    auto key_place = [&](int step) {
-      const int at = (step % kRing) * kStepBytes;
+    auto key_place = [&](int at) {
       key_at = here(at + l32 * 1024 + ((row_swap(l32) ^ h) << 4));
       rot_at = here(at + kLatBytes + l32 * 128 + ((((l32 >> 1) & 7) ^ h) << 4));
     };
-    auto val_place = [&](int step) {
+    auto val_place = [&](int at) {
       const int i16 = lane & 15, u4 = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-      v0_at = here((step % kRing) * kStepBytes + (4 * h + (i16 >> 2)) * 1024 + (((i16 >> 2) << 6) | ((u4 ^ h) << 4)) +
+      v0_at = here(at + (4 * h + (i16 >> 2)) * 1024 + (((i16 >> 2) << 6) | ((u4 ^ h) << 4)) +
                    8 * (i16 & 1) + 512 * dh);
       v1_at = here((v0_at + 8 * 1024) ^ 32);
     };
@@ -420,9 +425,9 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       for (int k = 0; k < 2; ++k) mfma_out<FMT>(o[i & 7][k], f[place % kAhead], w[i >> 3][k]);
     };
 
-    // The step's weights from its scores, in kWeigh pieces; the last puts them into pbuf.
-    constexpr int kWeigh = 7;
-    float off = 0.0f;
+    // The step's weights from its scores, in kWeigh pieces; the last two put them into pbuf.
+    constexpr int kWeigh = 8;
+    float top = 0.0f, off = 0.0f;
     auto hide = [&](uint32_t see) {
       const uint32_t mine = see >> (4 * h);
 #pragma unroll
@@ -432,57 +437,57 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     i32x4 p8[2];
     auto weigh = [&](int step, int piece) {
       if (piece == 0) {
-        float top = c[0];
+        top = c[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, c[e]);
+      } else if (piece == 1) {
         top = across_halves(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
         const bool need = top > m + kGrow;
-        const float keep = need ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-        m = need ? top : m;
-        l *= keep;
-        if (lane < 32) scale_by[step & 1][here(row)] = keep;
-        const uint64_t any = __ballot(need);
-        if (lane == 0) moved[step & 1][wave] = any != 0;
+        if (__any(need)) {
+          const float keep = need ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
+          m = need ? top : m;
+          l *= keep;
+          scale_by[step & 1][row] = keep;  // both halves of the wave have it
+          moved[step & 1][wave] = step;
+        }
         off = m == -__builtin_inff() ? 0.0f : m;
-      } else if (piece < 5) {
+      } else if (piece < 6) {
+        const int i = piece - 2;
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(fmaf(c[4 * (piece - 1) + e], a.scale_log2, -off));
+          p[e] = __builtin_amdgcn_exp2f(fmaf(c[4 * i + e], a.scale_log2, -off));
           l += p[e];
         }
         x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = (T)p[e];
         const u32x2 u = __builtin_bit_cast(u32x2, v);
-        p8[(piece - 1) >> 1][2 * ((piece - 1) & 1)] = (int)u[0];
-        p8[(piece - 1) >> 1][2 * ((piece - 1) & 1) + 1] = (int)u[1];
+        p8[i >> 1][2 * (i & 1)] = (int)u[0];
+        p8[i >> 1][2 * (i & 1) + 1] = (int)u[1];
       } else {
-        const int ks = piece - 5;
-        *reinterpret_cast<i32x4*>(pbuf + (step & 1) * kPBytes + ((ks * 4 + wave) * 64 + lane) * 16) = p8[ks];
+        const int ks = piece - 6;
+        *reinterpret_cast<i32x4*>(pbuf + (step & 1) * kPBytes + here((wave * 64 + lane) * 16) + ks * 4096) = p8[ks];
       }
     };
     // the rows' sums so far follow a moved maximum
-    auto follow = [&](int step) {
-      const int mv = moved[step & 1][2 * rh] | moved[step & 1][2 * rh + 1];
-      if (__builtin_amdgcn_readfirstlane(mv)) {
-        mfma_done();
+    auto follow = [&](int step, int mv0, int mv1) {
+      products_done();
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float f = moved[step & 1][2 * rh + k] ? scale_by[step & 1][64 * rh + 32 * k + l32] : 1.0f;
+      for (int k = 0; k < 2; ++k) {
+        const float f = (k ? mv1 : mv0) == step ? scale_by[step & 1][64 * rh + 32 * k + l32] : 1.0f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; ++i) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][k][e] = acc_put(acc_get(o[i][k][e]) * f);
-            __builtin_amdgcn_sched_barrier(0);  // 16 of them in VGPRs at a time
-          }
+          for (int e = 0; e < 16; ++e) o[i][k][e] = acc_put(acc_get(o[i][k][e]) * f);
+          __builtin_amdgcn_sched_barrier(0);  // 16 of them in VGPRs at a time
         }
       }
     };
     // values that are no numbers count for the tokens that see them through
     // their score; a weight of 0 must not meet them
-    auto clean = [&](int step) {
-      char* at = ring + (step % kRing) * kStepBytes + 8 * wave * 1024 + 16 * lane;
+    auto clean = [&](int ring_at) {
+      char* at = ring + ring_at + 8 * wave * 1024 + 16 * lane;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         x8 v = *reinterpret_cast<x8*>(at + r * 1024);
@@ -522,19 +527,36 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
     };
+    // Ring places of the steps before, at and after the turn's.
+    int at_prev = 0, at_now = 0, at_next = kStepBytes;
     uint32_t see = 0;
     bool dirty = false;
-    auto look = [&](int j) {  // what the rows see of step j
-      const uint32_t exists = uniform((int)live[j % kRing]);
-      dirty = (int64_t)(j + 1) * kTilePos > prefix;
-      see = dirty ? seen(j, exists) : exists;
+    int mv0 = -1, mv1 = -1;
+    auto begin = [&](int j, bool first) {  // the turn's first operands and what it has to know
+      key_place(at_now);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) fetch_key(k);
+      const int exists = live[j % kRing];
+      if (!first) {
+        mv0 = moved[(j - 1) & 1][2 * rh];
+        mv1 = moved[(j - 1) & 1][2 * rh + 1];
+      }
+      see = (uint32_t)uniform(exists);
+    };
+    auto clear_of = [&](int j) {  // step j's values and sums made ready for its weights
+      if (dirty) {
+        clean(at_prev);
+        __syncthreads();
+      }
+      mv0 = uniform(mv0);
+      mv1 = uniform(mv1);
+      if ((mv0 == j || mv1 == j) && j > from) follow(j, mv0, mv1);  // the first step's sums are zeros
     };
     auto turn = [&](int j, auto with_values) {
       constexpr bool VALUES = decltype(with_values)::value;
-      key_place(j);
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) fetch_key(k);
-      if (VALUES) val_place(j - 1);
+      dirty = (int64_t)(j + 1) * kTilePos > prefix;
+      if (dirty) see = seen(j, see);
+      if (VALUES) val_place(at_prev);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < kKeys; ++k) {
@@ -542,15 +564,11 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
         if (k + kAhead < kKeys) fetch_key(k + kAhead);
         else if (VALUES) fetch_val(k + kAhead - kKeys, k + kAhead);
         if (VALUES && k == kKeys - 3) fetch_weights(j - 1);
-        if (k % 3 == 1 && k < 24) bring(j + 1, k / 3);
+        if (k % 3 == 1 && k / 3 < kBring) bring(j + 1, k / 3, at_next);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (VALUES) {
-        val_product(0, kKeys);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");  // the scores may be read
-      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (VALUES) val_product(0, kKeys);
+      products_done();
       if (__any(see != ~0u)) hide(see);
       if constexpr (VALUES) {
 #pragma unroll
@@ -558,42 +576,46 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           if (i) val_product(i, kKeys + i);
           if (i + kAhead < kVals) fetch_val(i + kAhead, kKeys + i + kAhead);
           if (i < kWeigh) weigh(j, i);
-          else if (i >= kVals - 4) widen(j + 1, i - (kVals - 4));
+          else if (i >= kVals - 4) widen(i - (kVals - 4), at_next);
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < kWeigh; ++i) weigh(j, i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) widen(j + 1, i);
+        for (int i = 0; i < 4; ++i) widen(i, at_next);
       }
+      at_prev = at_now;
+      at_now = at_next;
+      at_next = at_next == 2 * kStepBytes ? 0 : at_next + kStepBytes;
     };
-    auto clear_of = [&](int j) {  // step j's values and sums made ready for its weights
-      if (dirty) {
-        clean(j);
-        __syncthreads();
-      }
-      if (j > from) follow(j);  // the first step's sums are zeros
-    };
-    __syncthreads();  // the tile before has left LDS
     page = page_of(from);
+    __syncthreads();  // the tile before has left LDS
+    if (tid < 8) moved[tid >> 2][tid & 3] = -1;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) bring(from, k);
+    for (int k = 0; k < kBring; ++k) {
+      bring(from, k, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_nop 4" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) widen(from, k);
+    for (int k = 0; k < 4; ++k) widen(k, 0);
     landed();
-    look(from);
+    begin(from, true);
     turn(from, std::false_type{});
 #pragma nounroll
     for (int j = from + 1; j < to; ++j) {
       landed();
+      begin(j, false);
       clear_of(j - 1);
-      look(j);
       turn(j, std::true_type{});
     }
     landed();
+    mv0 = moved[(to - 1) & 1][2 * rh];
+    mv1 = moved[(to - 1) & 1][2 * rh + 1];
     clear_of(to - 1);
-    val_place(to - 1);
+    val_place(at_prev);
     fetch_weights(to - 1);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch_val(i, i);
@@ -606,7 +628,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     }
 
     // ---- the tile's results, or a part of them
-    mfma_done();
+    products_done();
     l = across_halves(l, [](float x, float y) { return x + y; });
     __syncthreads();
     float* stat = reinterpret_cast<float*>(pbuf);  // [128] max, [128] sum
