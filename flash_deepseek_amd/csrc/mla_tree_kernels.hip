@@ -33,6 +33,7 @@ constexpr int kLatBytes = kTilePos * kLatDim * 2, kRotBytes = kTilePos * kRotDim
 constexpr int kStepBytes = kLatBytes + kRotBytes;
 constexpr int kPBytes = kTileRows * kTilePos * 2;
 constexpr size_t kPartFloats = (size_t)kTileRows * kLatDim;
+constexpr int kMaxGroups = 256;  // workgroups that share the work
 constexpr float kGrow = 8.0f;  // a row's maximum (log2) is moved when it grew by more
 
 // A tile that several workgroups share is put together from their parts; the
@@ -683,76 +684,142 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 }
 
 // A tile's parts put together: M = max m, out = sum 2^(m - M) part / sum 2^(m - M) l.
-// Workgroup (group, w, i): the 32 dims x 64 rows that wave w holds as its
-// o[i]; thread: four dims of a row, twice.
-template <int FMT>
-__global__ __launch_bounds__(256) void k_mla_tree_join(MlaTreeArgs a, int groups) {
+// Workgroup (x, y): of the x-th tile that has parts, 32 rows and I blocks of 32
+// dims; 256 threads of four dims each, S times over for every S-th part.  Few
+// tiles of many parts are bound by latency (I = 1, S = 4: one token over 1024
+// positions, 32 parts, 9.6 us), many of few by memory and by the dependent
+// reads before the first part (I = 8, S = 1).
+template <int FMT, int S, int I>
+__global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int groups) {
   typedef typename Half<FMT>::T T;
   typedef typename Half<FMT>::x4 x4;
+  constexpr int kSlots = 8 * S;  // parts side by side in the statistics
+  __shared__ float weight[kMaxGroups][32];
+  __shared__ float red[kSlots][32];
+  __shared__ int owner;
+  __shared__ f32x4 sums[S > 1 ? S - 1 : 1][256];
   const Space space = space_of(a.workspace, groups);
-  const int group = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // the x-th group that has the first part of a tile
+  if (wave == 0) {
+    int before = 0, found = -1;
+    for (int at = 0; at < groups && found < 0; at += 64) {
+      const uint64_t has = __ballot(at + lane < groups && space.desc[at + lane].parts != 0);
+      const int n = __popcll(has);
+      const int mine = before + __popcll(has & ((1ull << lane) - 1));
+      const uint64_t hit = __ballot(((has >> lane) & 1) && mine == (int)blockIdx.x);
+      if (hit) found = at + __builtin_ctzll(hit);
+      before += n;
+    }
+    if (lane == 0) owner = found;
+  }
+  __syncthreads();
+  const int group = owner;
+  if (group < 0) return;
   const JoinDesc d = space.desc[group];
-  if (!d.parts) return;
-  const int w = blockIdx.y >> 3, i = blockIdx.y & 7;
-  const int lane = threadIdx.x & 63, e = threadIdx.x >> 6, l32 = lane & 31, h = lane >> 5;
+  const int dim0 = (int)blockIdx.y / 4 * I;  // blocks of 32 dims, of 16
+  const int rh = ((int)blockIdx.y >> 1) & 1, k = blockIdx.y & 1, w = 2 * rh + dim0 / 8;
+  const int row0 = 64 * rh + 32 * k;
   const int g = kTileRows / a.H;
   const SeqWork s = seq_work(a, d.b);
   const int first = s.t0 + d.tile * g, rows = min(g, s.n - d.tile * g) * a.H;
+  if (row0 >= rows) return;
+  auto part_of = [&](int p) { return (size_t)(p ? 2 * (group + p) : 2 * group + 1); };
+  // the rows' weights of each part
+  const int srow = tid & 31, slot = tid >> 5;
+  float top = -__builtin_inff();
+  for (int p = slot; p < d.parts; p += kSlots) top = fmaxf(top, space.stat[part_of(p) * kTileRows + row0 + srow].x);
+  red[slot][srow] = top;
+  __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int r = 64 * (w >> 1) + 32 * k + l32;
-    if (r >= rows) continue;
-    const f32x4* from = reinterpret_cast<const f32x4*>(space.part) + w * 4096 + ((i * 2 + k) * 4 + e) * 64 + lane;
-    auto part_of = [&](int p) { return p ? 2 * (group + p) : 2 * group + 1; };
-    float top = -__builtin_inff();
-    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, space.stat[(size_t)part_of(p) * kTileRows + r].x);
-    const float off = top == -__builtin_inff() ? 0.0f : top;
+  for (int t = 0; t < kSlots; ++t) top = fmaxf(top, red[t][srow]);
+  __syncthreads();
+  const float off = top == -__builtin_inff() ? 0.0f : top;
+  float l = 0.0f;
+  for (int p = slot; p < d.parts; p += kSlots) {
+    const float2 st = space.stat[part_of(p) * kTileRows + row0 + srow];
+    const float f = __builtin_amdgcn_exp2f(st.x - off);
+    weight[p][srow] = f;
+    l = fmaf(f, st.y, l);
+  }
+  red[slot][srow] = l;
+  __syncthreads();
+  const int id = tid & 255, ps = tid >> 8, e = id >> 6, l32 = lane & 31, h = lane >> 5;
+  const int r = row0 + l32;
+  l = 0.0f;
+#pragma unroll
+  for (int t = 0; t < kSlots; ++t) l += red[t][l32];
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int t = r / a.H, hd = r - t * a.H;
+  T* out = static_cast<T*>(a.out) + (int64_t)(first + t) * a.out_token + hd * a.out_head + 32 * dim0 + 8 * e + 4 * h;
+  constexpr int kFlight = I > 1 ? 4 : 8;
+#pragma unroll 2
+  for (int i = 0; i < I; ++i) {
+    const f32x4* from = reinterpret_cast<const f32x4*>(space.part) + w * 4096 + (((dim0 % 8 + i) * 2 + k) * 4 + e) * 64 + lane;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-    for (int p = 0; p < d.parts; ++p) {
-      const float2 st = space.stat[(size_t)part_of(p) * kTileRows + r];
-      const float f = __builtin_amdgcn_exp2f(st.x - off);
-      const f32x4 v = from[(size_t)part_of(p) * (kPartFloats / 4)];
-      l = fmaf(f, st.y, l);
-      // a part without any weight holds zeros
+    for (int p0 = ps; p0 < d.parts; p0 += kFlight * S) {
+      f32x4 v[kFlight];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) sum[c] = fmaf(f, v[c], sum[c]);
+      for (int t = 0; t < kFlight; ++t)
+        if (p0 + t * S < d.parts) v[t] = from[part_of(p0 + t * S) * (kPartFloats / 4)];
+#pragma unroll
+      for (int t = 0; t < kFlight; ++t)
+        if (p0 + t * S < d.parts) {
+          const float f = weight[p0 + t * S][l32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[c] = fmaf(f, v[t][c], sum[c]);
+        }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int t = r / a.H, hd = r - t * a.H;
-    T* out = static_cast<T*>(a.out) + (int64_t)(first + t) * a.out_token + hd * a.out_head;
-    x4 v;
+    if constexpr (S > 1) {
+      static_assert(I == 1, "one block of dims where parts are shared out");
+      if (ps) sums[ps - 1][id] = sum;
+      __syncthreads();
+      if (ps) return;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) v[c] = (T)(sum[c] * inv);
-    *reinterpret_cast<x4*>(out + 256 * (w & 1) + 32 * i + 8 * e + 4 * h) = v;
-    if (a.lse && (w & 1) == 0 && i == 0 && e == 0 && h == 0)
-      a.lse[(size_t)(first + t) * a.H + hd] =
-          l == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+      for (int t = 0; t < S - 1; ++t) sum += sums[t][id];
+    }
+    if (r < rows) {
+      x4 v;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = (T)(sum[c] * inv);
+      *reinterpret_cast<x4*>(out + 32 * i) = v;
+    }
+  }
+  if (a.lse && r < rows && dim0 == 0 && e == 0 && h == 0) {
+    top = -__builtin_inff();
+    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, space.stat[part_of(p) * kTileRows + r].x);
+    a.lse[(size_t)(first + t) * a.H + hd] =
+        l == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
   }
 }
 
-static int mla_tree_groups() { return max(1, g_num_cus); }
+static int mla_tree_groups() { return min(max(1, g_num_cus), kMaxGroups); }
 
 size_t mla_tree_workspace(int, int) {
   const int groups = mla_tree_groups();
   return space_part_at(groups) + (size_t)2 * groups * kPartFloats * sizeof(float);
 }
 
-hipError_t launch_mla_tree(const MlaTreeArgs& a, int fmt, hipStream_t s) {
+namespace {
+template <int FMT>
+void launch_fmt(const MlaTreeArgs& a, hipStream_t s) {
   const int groups = mla_tree_groups();
-  const dim3 join(groups, 32);
+  k_mla_tree<FMT><<<groups, 256, 0, s>>>(a);
+  // no more tiles than these, whatever the sequences' sizes
+  const int g = kTileRows / a.H;
+  const int tiles = min(groups, min(a.N, a.N / g + a.B));
+  if (tiles * 16 <= groups)  // 16 parts a tile, if all workgroups have work
+    k_mla_tree_join<FMT, 4, 1><<<dim3(tiles, 64), 1024, 0, s>>>(a, groups);
+  else
+    k_mla_tree_join<FMT, 1, 8><<<dim3(tiles, 8), 256, 0, s>>>(a, groups);
+}
+}  // namespace
+
+hipError_t launch_mla_tree(const MlaTreeArgs& a, int fmt, hipStream_t s) {
   switch (fmt) {
-    case kKvF16:
-      k_mla_tree<kKvF16><<<groups, 256, 0, s>>>(a);
-      k_mla_tree_join<kKvF16><<<join, 256, 0, s>>>(a, groups);
-      break;
-    case kKvBf16:
-      k_mla_tree<kKvBf16><<<groups, 256, 0, s>>>(a);
-      k_mla_tree_join<kKvBf16><<<join, 256, 0, s>>>(a, groups);
-      break;
-    default:
-      k_mla_tree<kKvFp8><<<groups, 256, 0, s>>>(a);
-      k_mla_tree_join<kKvFp8><<<join, 256, 0, s>>>(a, groups);
+    case kKvF16: launch_fmt<kKvF16>(a, s); break;
+    case kKvBf16: launch_fmt<kKvBf16>(a, s); break;
+    default: launch_fmt<kKvFp8>(a, s);
   }
   return hipGetLastError();
 }
