@@ -406,7 +406,7 @@ struct KvReadArgs {
 };
 hipError_t launch_kv_read(const KvReadArgs& a, int fmt, ElemType y, hipStream_t s);
 
-constexpr int kMlaMaxSeqs = 1024;  // FDM_MLA_MAX_SEQS
+constexpr int kMlaMaxSeqs = 512;  // FDM_MLA_MAX_SEQS
 struct MlaTreeArgs {
   const void *latent, *rope;  // the cache's planes
   const uint8_t* scale;

@@ -28,11 +28,13 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTileRows = 128;  // (token, head) rows of a workgroup
 constexpr int kTilePos = 32;    // positions of a step
-constexpr int kRing = 3;        // steps in LDS: one's values, one's keys, one landing
 constexpr int kLatBytes = kTilePos * kLatDim * 2, kRotBytes = kTilePos * kRotDim * 2;
-constexpr int kStepBytes = kLatBytes + kRotBytes;
 constexpr int kPBytes = kTileRows * kTilePos * 2;
+// LDS: four steps' latent rows (one's values, one's keys, one landed, one landing),
+// three steps' rotary parts, the weights of two steps
+constexpr int kRotAt = 4 * kLatBytes, kPAt = kRotAt + 3 * kRotBytes, kStepLds = kPAt + 2 * kPBytes;
 constexpr size_t kPartFloats = (size_t)kTileRows * kLatDim;
+constexpr uint32_t kMaxSteps = 0x7FFFFFFFu;
 constexpr int kMaxGroups = 256;  // workgroups that share the work
 constexpr float kGrow = 8.0f;  // a row's maximum (log2) is moved when it grew by more
 
@@ -201,47 +203,49 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   typedef typename Half<FMT>::T T;
   typedef typename Half<FMT>::x4 x4;
   typedef typename Half<FMT>::x8 x8;
-  __shared__ __attribute__((aligned(256))) char ring[kRing * kStepBytes];
-  __shared__ __attribute__((aligned(256))) char pbuf[2 * kPBytes];  // weights [2][step of 16][32 rows][lane] x 8
-  __shared__ float scale_by[2][kTileRows];                          // what the rows' sums so far are scaled by
-  __shared__ int moved[2][4];                                       // the step at which a wave's rows last were
-  __shared__ int live[kRing];                                       // bytes: which rows of the step exist
-  __shared__ int64_t before[kMlaMaxSeqs + 1];                 // steps before each sequence
-  __shared__ int64_t wave_total[4];
+  __shared__ __attribute__((aligned(256))) char lds[kStepLds];
+  __shared__ float scale_by[2][kTileRows];   // what the rows' sums so far are scaled by
+  __shared__ int moved[2][4];                // the step at which a wave's rows last were
+  __shared__ int live[4];                    // bytes: which rows of a step exist
+  __shared__ uint32_t before[kMlaMaxSeqs + 1];  // steps before each sequence
+  __shared__ uint32_t wave_total[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, h = lane >> 5;
   const int g = kTileRows / a.H;
   const bool in_order = a.mask == nullptr;
 
-  // steps before each sequence: four sequences a thread
+  // steps before each sequence, two sequences a thread.  A call's steps are
+  // below 2^31; starts that make them more (sequences that share tokens) are cut.
   {
-    int64_t mine[4], sum = 0;
+    uint32_t mine[2], sum = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
       mine[k] = sum;
-      const int b = 4 * tid + k;
+      const int b = 2 * tid + k;
       if (b < a.B) {
         const SeqWork s = seq_work(a, b);
-        sum += steps_before(s, (s.n + g - 1) / g, g, in_order);
+        sum = (uint32_t)min((int64_t)sum + steps_before(s, (s.n + g - 1) / g, g, in_order), (int64_t)kMaxSteps);
       }
     }
-    int64_t upto = sum;
+    uint32_t upto = sum;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
+      const uint32_t v = __shfl_up(upto, d);
+      if (lane >= d) upto = min(upto + v, kMaxSteps);
     }
     if (lane == 63) wave_total[wave] = upto;
+    const uint32_t inside = __shfl_up(upto, 1);
     __syncthreads();
-    int64_t base = upto - sum;
-    for (int w = 0; w < wave; ++w) base += wave_total[w];
+    uint32_t base = 0;
+    for (int w = 0; w < wave; ++w) base = min(base + wave_total[w], kMaxSteps);
+    base = min(base + (lane ? inside : 0), kMaxSteps);
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (4 * tid + k <= a.B) before[4 * tid + k] = base + mine[k];
-    if (tid == 255 && a.B == 1024) before[1024] = base + sum;
+    for (int k = 0; k < 2; ++k)
+      if (2 * tid + k <= a.B) before[2 * tid + k] = min(base + mine[k], kMaxSteps);
+    if (tid == 255 && a.B == kMlaMaxSeqs) before[kMlaMaxSeqs] = min(base + sum, kMaxSteps);
     __syncthreads();
   }
-  const int64_t total = uniform(before[a.B]);
+  const int64_t total = (uint32_t)uniform((int)before[a.B]);
   const int groups = gridDim.x;
   // neighbours in the list on one XCD (workgroups go round the eight in turn)
   const int group = groups % 8 ? blockIdx.x : (blockIdx.x % 8) * (groups / 8) + blockIdx.x / 8;
@@ -256,15 +260,15 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     int hi = a.B - 1;
     while (b < hi) {
       const int mid = (b + hi + 1) / 2;
-      if (uniform(before[mid]) <= u) b = mid;
+      if ((uint32_t)uniform((int)before[mid]) <= u) b = mid;
       else hi = mid - 1;
     }
   }
   while (u < u_end) {
-    while (uniform(before[b + 1]) <= u) ++b;
+    while ((uint32_t)uniform((int)before[b + 1]) <= u) ++b;
     SeqWork s = seq_work(a, b);
     s = {uniform(s.n), uniform(s.len), uniform(s.t0)};
-    const int64_t seq_u = uniform(before[b]);
+    const int64_t seq_u = (uint32_t)uniform((int)before[b]);
     int tile = 0;
     {  // the last tile that starts at or before u
       int hi = (s.n + g - 1) / g - 1;
@@ -299,65 +303,55 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     }
 
     // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7, eight lanes
-    // each.  kBring pieces of work: 16-bit rows go straight into LDS, one a piece;
-    // FP8 codes into registers, from where widen() puts their 16-bit values
-    // (exact) into LDS in four pieces.  A row that is none reads zeros.
+    // each, in kBring pieces of work.  16-bit rows go straight into LDS, one a
+    // piece.  FP8 codes go into registers, and from there in the same turn as 16-bit
+    // values (exact) into LDS.  A row that is none reads zeros.
+    constexpr bool kCodes = FMT == kKvFp8;
     constexpr int kBring = 9;
     const int my_row = 8 * wave + (lane >> 3);
     const int* pages = a.pages + (size_t)b * a.pages_stride;
-    int page;          // of this lane's row in the step that comes next
-    const char* mine;  // this lane's row in the step that is brought
-    uint64_t base;     // the row that the next piece brings
+    const char* none = reinterpret_cast<const char*>(zero_row);
+    int page;                // of this lane's row in the step that is placed next
+    int slot = 0;            // this lane's row in the step placed last; -1: none
+    const char* mine;        // 16 bits: that row
+    uint64_t base;           //   the row that the next piece brings
+    u32x4 code[4];           // FP8: that row's codes (16 of each group) and scales
+    uint32_t code_scale = 0;
     auto page_of = [&](int step) { return pages[min(step * kTilePos + my_row, max(len - 1, 0)) >> a.page_shift]; };
+    auto place = [&](int step) {
+      const int j = step * kTilePos + my_row;
+      const bool is = (unsigned)page < (unsigned)a.n_pages && j < len && step < to;
+      slot = is ? (page << a.page_shift) + (j & ((1 << a.page_shift) - 1)) : -1;
+      page = page_of(step + 1);
+    };
+    auto announce = [&](int step, int rot_at) {  // which rows exist, and their rotary parts
+      const uint64_t all = __ballot(slot >= 0);
+      uint32_t byte = 0xFF;
+      if (all != ~0ull) {
+        byte = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) byte |= (uint32_t)((all >> (8 * k)) & 1) << k;
+      }
+      reinterpret_cast<uint8_t*>(&live[step & 3])[wave] = (uint8_t)byte;
+      const char* rp = static_cast<const char*>(a.rope) + (size_t)max(slot, 0) * (kRotDim * 2) + here(16 * ((lane & 7) ^ ((my_row >> 1) & 7)));
+      lds_load16(slot >= 0 ? rp : none, lds + rot_at + wave * 1024);
+    };
     auto base_of = [&](int k) {
       return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uintptr_t)mine, 8 * k) |
              (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)((uintptr_t)mine >> 32), 8 * k) << 32;
     };
-    u32x4 code[4];
-    uint32_t code_scale = 0;
-    auto bring = [&](int step, int piece, int ring_at) {
-      char* at = ring + ring_at;
-      if (piece == 0) {
-        const int j = step * kTilePos + my_row;
-        const bool is = (unsigned)page < (unsigned)a.n_pages && j < len && step < to;
-        const int slot = is ? (page << a.page_shift) + (j & ((1 << a.page_shift) - 1)) : 0;
-        const uint64_t all = __ballot(is);
-        uint32_t byte = 0xFF;
-        if (all != ~0ull) {
-          byte = 0;
-#pragma unroll
-          for (int k = 0; k < 8; ++k) byte |= (uint32_t)((all >> (8 * k)) & 1) << k;
-        }
-        reinterpret_cast<uint8_t*>(&live[step % kRing])[wave] = (uint8_t)byte;
-        const char* rp = static_cast<const char*>(a.rope) + (size_t)slot * (kRotDim * 2) + here(16 * ((lane & 7) ^ ((my_row >> 1) & 7)));
-        mine = static_cast<const char*>(a.latent) + (size_t)slot * (FMT == kKvFp8 ? kLatDim : kLatDim * 2);
-        const char* none = reinterpret_cast<const char*>(zero_row);
-        mine = is ? mine : none;
-        lds_load16(is ? rp : none, at + kLatBytes + wave * 1024);
-        if constexpr (FMT == kKvFp8) {
-          mine += here(16 * (lane & 7));
-          code_scale = *reinterpret_cast<const uint32_t*>(is ? reinterpret_cast<const char*>(a.scale) + (size_t)slot * 4 : none);
-        } else {
-          base = base_of(0);
-        }
-        page = page_of(step + 1);
-        return;
-      }
-      const int k = piece - 1;
-      if constexpr (FMT == kKvFp8) {
-        // 16 codes of each of the row's four groups a lane
-        if (k < 4) code[k] = *reinterpret_cast<const u32x4*>(mine + 128 * k);
-      } else {
-        const int r = 8 * wave + k;
-        lds_load16(base, here((lane ^ ((2 * wave) & 3)) << 4) ^ (((k >> 2) << 4) | ((k & 3) << 6)), at + r * 1024);
-        if (k < 7) base = base_of(k + 1);
-      }
+    auto load_codes = [&](int k) {
+      const char* p = static_cast<const char*>(a.latent) + (size_t)max(slot, 0) * kLatDim + here(16 * (lane & 7));
+      p = slot >= 0 ? p : none;
+      if (k == 0)
+        code_scale = *reinterpret_cast<const uint32_t*>(slot >= 0 ? reinterpret_cast<const char*>(a.scale) + (size_t)slot * 4 : none);
+      code[k] = *reinterpret_cast<const u32x4*>(p + 128 * k);
     };
-    auto widen = [&](int k, int ring_at) {
-      if constexpr (FMT == kKvFp8) {
-        char* at = ring + ring_at;
-        const int widen_at = here(my_row * 1024 + (((2 * (lane & 7)) ^ row_swap(my_row)) << 4));
-        const float sc = scale_value((int)((code_scale >> (8 * k)) & 0xFF));
+    auto widen = [&](int step, int k) {
+      char* at = lds + (step & 3) * kLatBytes;
+      const int widen_at = here(my_row * 1024 + (((2 * (lane & 7)) ^ row_swap(my_row)) << 4));
+      const float sc = scale_value((int)((code_scale >> (8 * k)) & 0xFF));
+      if constexpr (kCodes) {
         u32x4 v[2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -365,8 +359,23 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           v[i >> 1][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, true));
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<u32x4*>(at + (widen_at ^ (16 * i)) + 256 * k) = v[i];
+        for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4*>(at + (widen_at ^ (16 * i)) + 256 * k) = v[i];
+      }
+    };
+    auto bring = [&](int step, int piece, int rot_at) {
+      if constexpr (kCodes) {
+        if (piece == 0) place(step), announce(step, rot_at);
+        else if (piece < 5) load_codes(piece - 1);
+      } else if (piece == 0) {
+        place(step);
+        announce(step, rot_at);
+        mine = slot >= 0 ? static_cast<const char*>(a.latent) + (size_t)slot * (kLatDim * 2) : none;
+        base = base_of(0);
+      } else {
+        const int k = piece - 1, r = 8 * wave + k;
+        lds_load16(base, here((lane ^ ((2 * wave) & 3)) << 4) ^ (((k >> 2) << 4) | ((k & 3) << 6)),
+                   lds + (step & 3) * kLatBytes + r * 1024);
+        if (k < 7) base = base_of(k + 1);
       }
     };
 
@@ -385,35 +394,36 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     // 36 of keys (position = l32, 8 dims at 16 k + 8 h), then 16 of values (dim =
     // l32 of a block of 32; positions 16 s + 4 h + {0 .. 3, 8 .. 11}, the ones
     // whose weights the lane has).
-    constexpr int kKeys = 36, kVals = 16, kAhead = 6;
+    constexpr int kKeys = 36, kVals = 16, kAhead = kCodes ? 6 : 6;
+    static_assert(kKeys % kAhead == 0, "keys and values take the registers in turn");
     i32x4 f[kAhead];
     int key_at, rot_at, v0_at, v1_at;  // this lane's addresses
-    auto key_place = [&](int at) {
-      key_at = here(at + l32 * 1024 + ((row_swap(l32) ^ h) << 4));
-      rot_at = here(at + kLatBytes + l32 * 128 + ((((l32 >> 1) & 7) ^ h) << 4));
+    auto key_place = [&](int step, int rot) {
+      key_at = here((step & 3) * kLatBytes + l32 * 1024 + ((row_swap(l32) ^ h) << 4));
+      rot_at = here(rot + l32 * 128 + ((((l32 >> 1) & 7) ^ h) << 4));
     };
-    auto val_place = [&](int at) {
+    auto val_place = [&](int step) {
       const int i16 = lane & 15, u4 = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);
-      v0_at = here(at + (4 * h + (i16 >> 2)) * 1024 + (((i16 >> 2) << 6) | ((u4 ^ h) << 4)) +
+      v0_at = here((step & 3) * kLatBytes + (4 * h + (i16 >> 2)) * 1024 + (((i16 >> 2) << 6) | ((u4 ^ h) << 4)) +
                    8 * (i16 & 1) + 512 * dh);
       v1_at = here((v0_at + 8 * 1024) ^ 32);
     };
     auto fetch_key = [&](int k) {
-      f[k % kAhead] = k < 32 ? *reinterpret_cast<const i32x4*>(ring + (key_at ^ ((k & 7) << 5)) + (k >> 3) * 256)
-                             : *reinterpret_cast<const i32x4*>(ring + (rot_at ^ ((k & 3) << 5)));
+      f[k % kAhead] = k < 32 ? *reinterpret_cast<const i32x4*>(lds + (key_at ^ ((k & 7) << 5)) + (k >> 3) * 256)
+                             : *reinterpret_cast<const i32x4*>(lds + (rot_at ^ ((k & 3) << 5)));
     };
     auto fetch_val = [&](int i, int place) {  // block i & 7 of 32 dims, positions 16 (i >> 3) ..
       const int off = (i >> 3) * 16384 + ((i >> 2) & 1) * 256;
-      const x4 lo = read_turned(ring + (v0_at ^ ((i & 3) << 6)) + off, x4{});
-      const x4 hi = read_turned(ring + (v1_at ^ ((i & 3) << 6)) + off, x4{});
+      const x4 lo = read_turned(lds + (v0_at ^ ((i & 3) << 6)) + off, x4{});
+      const x4 hi = read_turned(lds + (v1_at ^ ((i & 3) << 6)) + off, x4{});
       const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
       f[place % kAhead] = i32x4{(int)x[0], (int)x[1], (int)y[0], (int)y[1]};
     };
     i32x4 w[2][2];  // the weights of step j - 1: [16 positions][32 rows]
-    auto fetch_weights = [&](int step) {
+    auto fetch_weights = [&](int step, int s) {
       const int at = here((step & 1) * kPBytes + 2 * rh * 1024 + lane * 16);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i >> 1][i & 1] = *reinterpret_cast<const i32x4*>(pbuf + at + (i >> 1) * 4096 + (i & 1) * 1024);
+      for (int i = 0; i < 2; ++i) w[s][i] = *reinterpret_cast<const i32x4*>(lds + kPAt + at + s * 4096 + i * 1024);
     };
     f32x16 c;  // scores of 32 positions x this wave's 32 rows: D row = position, column = query row
     auto key_product = [&](int k) {
@@ -426,8 +436,8 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       for (int k = 0; k < 2; ++k) mfma_out<FMT>(o[i & 7][k], f[place % kAhead], w[i >> 3][k]);
     };
 
-    // The step's weights from its scores, in kWeigh pieces; the last two put them into pbuf.
-    constexpr int kWeigh = 8;
+    // The step's weights from its scores, in kWeigh pieces; the last two put them into LDS.
+    constexpr int kWeigh = 12;
     float top = 0.0f, off = 0.0f;
     auto hide = [&](uint32_t see) {
       const uint32_t mine = see >> (4 * h);
@@ -452,23 +462,17 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           moved[step & 1][wave] = step;
         }
         off = m == -__builtin_inff() ? 0.0f : m;
-      } else if (piece < 6) {
+      } else if (piece < 10) {
         const int i = piece - 2;
-        float p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(fmaf(c[4 * i + e], a.scale_log2, -off));
-          l += p[e];
-        }
-        x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)p[e];
-        const u32x2 u = __builtin_bit_cast(u32x2, v);
-        p8[i >> 1][2 * (i & 1)] = (int)u[0];
-        p8[i >> 1][2 * (i & 1) + 1] = (int)u[1];
+        typedef T x2 __attribute__((ext_vector_type(2)));
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(c[2 * i], a.scale_log2, -off));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(c[2 * i + 1], a.scale_log2, -off));
+        l += p0;
+        l += p1;
+        p8[i >> 2][i & 3] = __builtin_bit_cast(int, x2{(T)p0, (T)p1});
       } else {
-        const int ks = piece - 6;
-        *reinterpret_cast<i32x4*>(pbuf + (step & 1) * kPBytes + here((wave * 64 + lane) * 16) + ks * 4096) = p8[ks];
+        const int ks = piece - 10;
+        *reinterpret_cast<i32x4*>(lds + kPAt + (step & 1) * kPBytes + here((wave * 64 + lane) * 16) + ks * 4096) = p8[ks];
       }
     };
     // the rows' sums so far follow a moved maximum
@@ -487,8 +491,8 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     };
     // values that are no numbers count for the tokens that see them through
     // their score; a weight of 0 must not meet them
-    auto clean = [&](int ring_at) {
-      char* at = ring + ring_at + 8 * wave * 1024 + 16 * lane;
+    auto clean = [&](int step) {
+      char* at = lds + (step & 3) * kLatBytes + 8 * wave * 1024 + 16 * lane;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         x8 v = *reinterpret_cast<x8*>(at + r * 1024);
@@ -520,104 +524,123 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       return see & exists;
     };
 
-    // In one turn step j's keys and then step j - 1's values are multiplied;
-    // beside the keys step j + 1 is brought, beside the values step j's weights
-    // are computed.  The order of issue is the source's: a piece of that work
-    // behind each product, a product's operand requested six products ahead.
+    // In one turn step j's keys and then step j - 1's values are multiplied.
+    // Step j + 1 is in LDS already, so its first keys are requested before the
+    // turn ends, and the barrier stands among the keys' products: behind it the
+    // weights of step j - 1 are whole, step j + 2 may be brought where step j - 2
+    // was, and what was brought in the turn before has landed.  Beside the values
+    // step j's weights are computed.  The order of issue is the source's: a piece
+    // of that work behind each product, its operand requested six products ahead.
+    constexpr int kBarrier = 6;  // after so many of the keys' products
+    constexpr int kApart = kCodes ? 5 : 6;  // products between two pieces of what is brought
+    static_assert(kBarrier + 2 + 4 * kApart < kKeys, "five pieces have a place beside the keys");
+    int rot_now = kRotAt, rot_next = kRotAt + kRotBytes, rot_then = kRotAt + 2 * kRotBytes;
     auto landed = [&] {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
     };
-    // Ring places of the steps before, at and after the turn's.
-    int at_prev = 0, at_now = 0, at_next = kStepBytes;
-    uint32_t see = 0;
-    bool dirty = false;
+    bool dirty = false;   // step j - 1 has rows that not all tokens see
     int mv0 = -1, mv1 = -1;
-    auto begin = [&](int j, bool first) {  // the turn's first operands and what it has to know
-      key_place(at_now);
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) fetch_key(k);
-      const int exists = live[j % kRing];
-      if (!first) {
-        mv0 = moved[(j - 1) & 1][2 * rh];
-        mv1 = moved[(j - 1) & 1][2 * rh + 1];
-      }
-      see = (uint32_t)uniform(exists);
+    auto moves = [&](int j) {
+      mv0 = moved[j & 1][2 * rh];
+      mv1 = moved[j & 1][2 * rh + 1];
     };
-    auto clear_of = [&](int j) {  // step j's values and sums made ready for its weights
+    auto clear_of = [&](int j) {  // step j's values and the sums made ready for its weights
       if (dirty) {
-        clean(at_prev);
+        clean(j);
         __syncthreads();
       }
       mv0 = uniform(mv0);
       mv1 = uniform(mv1);
       if ((mv0 == j || mv1 == j) && j > from) follow(j, mv0, mv1);  // the first step's sums are zeros
     };
+    auto apart = [&] {  // v_readlane's scalar and the load that it is the address of
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_nop 4" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
     auto turn = [&](int j, auto with_values) {
       constexpr bool VALUES = decltype(with_values)::value;
-      dirty = (int64_t)(j + 1) * kTilePos > prefix;
-      if (dirty) see = seen(j, see);
-      if (VALUES) val_place(at_prev);
-      __builtin_amdgcn_sched_barrier(0);
+      const int exists = live[j & 3];
 #pragma unroll
       for (int k = 0; k < kKeys; ++k) {
         key_product(k);
         if (k + kAhead < kKeys) fetch_key(k + kAhead);
         else if (VALUES) fetch_val(k + kAhead - kKeys, k + kAhead);
-        if (VALUES && k == kKeys - 3) fetch_weights(j - 1);
-        if (k % 3 == 1 && k / 3 < kBring) bring(j + 1, k / 3, at_next);
+        if (k == kBarrier - 1) {
+          landed();
+          if (VALUES) moves(j - 1);
+        }
+        if (VALUES && k == kBarrier + 1) clear_of(j - 1);
+        if (VALUES && k == kBarrier + 2) val_place(j - 1);
+        if (VALUES && k == kKeys - 4) fetch_weights(j - 1, 0);
+        if (k >= kBarrier + 2 && (k - kBarrier - 2) % kApart == 0 && (k - kBarrier - 2) / kApart < 5)
+          bring(j + 2, (k - kBarrier - 2) / kApart, rot_then);
         __builtin_amdgcn_sched_barrier(0);
       }
+      const bool edge = (int64_t)(j + 1) * kTilePos > prefix;
+      uint32_t see = (uint32_t)uniform(exists);
+      if (edge) see = seen(j, see);
+      dirty = edge;
       if constexpr (VALUES) val_product(0, kKeys);
       products_done();
       if (__any(see != ~0u)) hide(see);
+      key_place(j + 1, rot_next);
       if constexpr (VALUES) {
 #pragma unroll
         for (int i = 0; i < kVals; ++i) {
           if (i) val_product(i, kKeys + i);
           if (i + kAhead < kVals) fetch_val(i + kAhead, kKeys + i + kAhead);
+          else fetch_key((kKeys + i) % kAhead);  // the register that this product has left
+          if (i == 4) fetch_weights(j - 1, 1);
           if (i < kWeigh) weigh(j, i);
-          else if (i >= kVals - 4) widen(i - (kVals - 4), at_next);
+          else widen(j + 2, i - kWeigh);
+          if (!kCodes && i % 4 == 1) bring(j + 2, 5 + i / 4, rot_then);
           __builtin_amdgcn_sched_barrier(0);
         }
+        static_assert(kWeigh + 4 == kVals, "all pieces have a place");
       } else {
 #pragma unroll
         for (int i = 0; i < kWeigh; ++i) weigh(j, i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) widen(i, at_next);
+        for (int i = 0; i < 4; ++i) {
+          widen(j + 2, i);
+          if (!kCodes) bring(j + 2, 5 + i, rot_then), apart();
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) fetch_key(k);
       }
-      at_prev = at_now;
-      at_now = at_next;
-      at_next = at_next == 2 * kStepBytes ? 0 : at_next + kStepBytes;
+      const int r = rot_now;
+      rot_now = rot_next;
+      rot_next = rot_then;
+      rot_then = r;
     };
     page = page_of(from);
     __syncthreads();  // the tile before has left LDS
     if (tid < 8) moved[tid >> 2][tid & 3] = -1;
 #pragma unroll
-    for (int k = 0; k < kBring; ++k) {
-      bring(from, k, 0);
-      __builtin_amdgcn_sched_barrier(0);
-      asm volatile("s_nop 4" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) widen(k, 0);
+      for (int k = 0; k < kBring; ++k) {
+        bring(from + t, k, t ? rot_next : rot_now);
+        if constexpr (!kCodes) apart();
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) widen(from + t, k);
+    }
     landed();
-    begin(from, true);
+    key_place(from, rot_now);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch_key(k);
     turn(from, std::false_type{});
 #pragma nounroll
-    for (int j = from + 1; j < to; ++j) {
-      landed();
-      begin(j, false);
-      clear_of(j - 1);
-      turn(j, std::true_type{});
-    }
+    for (int j = from + 1; j < to; ++j) turn(j, std::true_type{});
     landed();
-    mv0 = moved[(to - 1) & 1][2 * rh];
-    mv1 = moved[(to - 1) & 1][2 * rh + 1];
+    moves(to - 1);
     clear_of(to - 1);
-    val_place(at_prev);
-    fetch_weights(to - 1);
+    val_place(to - 1);
+    fetch_weights(to - 1, 0);
+    fetch_weights(to - 1, 1);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch_val(i, i);
     __builtin_amdgcn_sched_barrier(0);
@@ -632,7 +655,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     products_done();
     l = across_halves(l, [](float x, float y) { return x + y; });
     __syncthreads();
-    float* stat = reinterpret_cast<float*>(pbuf);  // [128] max, [128] sum
+    float* stat = reinterpret_cast<float*>(lds + kPAt);  // [128] max, [128] sum
     if (lane < 32) {
       stat[row] = m;
       stat[kTileRows + row] = l;

@@ -536,7 +536,7 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
  * graphs that may run at once, need one each.  The call allocates nothing and
  * may be captured.  The same arguments give the same bits. */
 #define FDM_MLA_MAX_HEADS 128
-#define FDM_MLA_MAX_SEQS 1024
+#define FDM_MLA_MAX_SEQS 512
 typedef struct fdm_mla_batch {
   int B, N, H;
   const int32_t *d_q_start;  /* [B + 1]          */

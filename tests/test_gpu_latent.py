@@ -307,6 +307,37 @@ def test_attend_long_and_split(fdm, fmt):
     run_attend(fdm, cache, rows, page, *q, start, lens, pages)
 
 
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "fp8"])
+@pytest.mark.parametrize("H,B,L,most,kind", [(128, 24, 1500, 4, "tree"), (16, 400, 260, 3, "order"), (96, 5, 700, 70, "order"), (64, 512, 150, 1, "order")])
+def test_attend_many_steps_a_workgroup(fdm, fmt, H, B, L, most, kind):
+    """Enough work that every workgroup walks many steps of one tile, and several tiles; a
+    sample of the sequences is checked."""
+    g = rng(B)
+    page = 32
+    per = -(-L // page)
+    cache, rows = filled(fdm, fmt, B * per, page, g)
+    pages = torch.randperm(B * per, generator=g).reshape(B, per)
+    counts = torch.randint(1, most + 1, (B,), generator=g).tolist()
+    lens = torch.randint(L // 3, L + 1, (B,), generator=g).tolist()
+    lens[B // 2], counts[B // 3] = L, most
+    start = [0] + np.cumsum(counts).tolist()
+    mask = None if kind == "order" else tree(g, counts)
+    q = queries(g, fmt, start[-1], H)
+    out = torch.full((start[-1], H, 512), 7.0, dtype=q[0].dtype, device="cuda")
+    lse = torch.full((start[-1], H), 7.0, device="cuda")
+    i32 = lambda v: torch.as_tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    say(f"mla_attend {fmt} H={H} B={B} L={L} up to {most} {kind}")
+    fdm.mla_attend(cache, q[0].cuda(), q[1].cuda(), i32(start), i32(lens), pages.to(torch.int32).cuda(), SCALE, out,
+                   mask=None if mask is None else mask.cuda(), lse=lse)
+    out, lse = out.cpu(), lse.cpu()
+    for b in sorted({0, 1, B // 3, B // 2, B - 1, *torch.randint(0, B, (6,), generator=g).tolist()}):
+        t0, t1 = start[b], start[b + 1]
+        want = C.attend(rows, page, q[0][t0:t1], q[1][t0:t1], [0, t1 - t0], [lens[b]], [pages[b].tolist()], SCALE,
+                        None if mask is None else mask[t0:t1])
+        C.check(out[t0:t1], want[0], want[2], f"out of {b}")
+        C.check(lse[t0:t1], want[1], want[3], f"lse of {b}")
+
+
 def test_attend_empty_rows_and_unseen_values(fdm):
     """A mask that leaves a row nothing, a sequence without positions, more tokens than
     positions, no tokens at all; NaN and infinity where no token looks, or only others do."""
