@@ -323,33 +323,42 @@ ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 KV_FORMATS = {"f16": _lib.KV_F16, "bf16": _lib.KV_BF16, "fp8": _lib.KV_FP8}
 _device = None  # of init()
-_types = {}     # torch dtype -> element type (filled at first use: torch is imported lazily)
+_types = {}     # torch dtype -> element type
+_i32 = _i64 = _f32 = None  # torch's (imported lazily)
 
 
 def _refuse(fn, why):
     raise FdmError(_lib.FDM_E_INVAL, fn, why)
 
 
+def _load_types():
+    global _i32, _i64, _f32
+    import torch
+    _i32, _i64, _f32 = torch.int32, torch.int64, torch.float32
+    _types.update({torch.float32: _lib.GGML_F32, torch.float16: _lib.GGML_F16, torch.bfloat16: _lib.GGML_BF16})
+
+
 def _elem(fn, name, dtype):
-    if not _types:
-        import torch
-        _types.update({torch.float32: _lib.GGML_F32, torch.float16: _lib.GGML_F16, torch.bfloat16: _lib.GGML_BF16})
     t = _types.get(dtype)
     if t is None:
         _refuse(fn, f"{name}: {dtype} is none of float32, float16, bfloat16")
     return t
 
 
-def _on_device(fn, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or (_device is not None and t.get_device() != _device)):
-            _refuse(fn, f"{name} is on {t.device}, the library on device {_device}")
+def _on_device(fn, *tensors):
+    """Every tensor is on the library's device (a call without one to go by: on a GPU)."""
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()  # -1: not on a GPU
+            if d != _device and (d < 0 or _device is not None):
+                _refuse(fn, f"a tensor is on {t.device}, the library on device {_device}")
 
 
-def _ints(fn, name, t, n, dtype="torch.int32"):
-    """A contiguous vector (or matrix) of n int32."""
-    if str(t.dtype) != dtype or t.numel() != n or not t.is_contiguous():
+def _vector(fn, name, t, n, dtype):
+    """n contiguous values; returns their address."""
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
         _refuse(fn, f"{name}: {n} contiguous values of {dtype} are wanted, got {tuple(t.shape)} of {t.dtype}")
+    return t.data_ptr()
 
 
 def _call_stream(stream):
@@ -381,15 +390,18 @@ def rope(table, x, pos, out, offset=0, stream=None):
     """out = x [T, H, D] with the table's dim values from `offset` of every head
     turned by the token's position (pos [T] int32).  Any token and head
     strides; float32, float16 or bfloat16 on either side.  out may be x."""
-    T, H, D = x.shape if x.dim() == 3 else _refuse("rope", f"x: [T, H, D] is wanted, got {tuple(x.shape)}")
-    if out.shape != x.shape:
-        _refuse("rope", f"out: {tuple(x.shape)} is wanted, got {tuple(out.shape)}")
-    if (x.stride(2) != 1 or out.stride(2) != 1) and D > 1:
+    if x.dim() != 3 or out.shape != x.shape:
+        _refuse("rope", f"x and out: [T, H, D] are wanted, got {tuple(x.shape)} and {tuple(out.shape)}")
+    T, H, D = x.shape
+    xt, xh, xe = x.stride()
+    yt, yh, ye = out.stride()
+    if (xe != 1 or ye != 1) and D > 1:
         _refuse("rope", "the values of a head must be contiguous")
-    _on_device("rope", x=x, pos=pos, out=out)
-    _ints("rope", "pos", pos, T)
-    call("fdm_rope", ctypes.byref(table), pos.data_ptr(), T, H, D, offset, x.data_ptr(), _elem("rope", "x", x.dtype),
-         x.stride(0), x.stride(1), out.data_ptr(), _elem("rope", "out", out.dtype), out.stride(0), out.stride(1),
+    if not _types:
+        _load_types()
+    _on_device("rope", x, pos, out)
+    call("fdm_rope", ctypes.byref(table), _vector("rope", "pos", pos, T, _i32), T, H, D, offset, x.data_ptr(),
+         _elem("rope", "x", x.dtype), xt, xh, out.data_ptr(), _elem("rope", "out", out.dtype), yt, yh,
          _call_stream(stream))
 
 
@@ -417,10 +429,11 @@ class KvCache:
                 _refuse("KvCache", f"{name}: not contiguous")
         if lead[1] < 1 or lead[1] & (lead[1] - 1):
             _refuse("KvCache", f"page_size {lead[1]}: a power of two")
-        _on_device("KvCache", latent=latent, rope=rope, scale=scale)
+        _on_device("KvCache", latent, rope, scale)
         self.latent, self.rope, self.scale, self.format = latent, rope, scale, fmt
         self.n_pages, self.page_size = lead
         self.desc = _lib.KvCacheDesc(latent.data_ptr(), rope.data_ptr(), _p(scale), KV_FORMATS[fmt], *lead)
+        self.device, self.half = latent.get_device(), rope.dtype
 
 
 def kv_cache(format, n_pages, page_size=64):
@@ -439,7 +452,7 @@ def kv_cache(format, n_pages, page_size=64):
 
 
 def _rows(fn, name, t, T):
-    if t.dim() != 2 or t.shape[0] != T or t.shape[1] != _lib.KV_LATENT + _lib.KV_ROPE or t.stride(1) != 1:
+    if t.shape != (T, _lib.KV_LATENT + _lib.KV_ROPE) or t.stride(1) != 1:
         _refuse(fn, f"{name}: [{T}, {_lib.KV_LATENT + _lib.KV_ROPE}] with contiguous rows is wanted, got {tuple(t.shape)}")
 
 
@@ -450,26 +463,28 @@ def kv_write(cache, kv, slots, norm_w=None, table=None, pos=None, stream=None):
     quantised to the cache's format."""
     T = slots.numel()
     _rows("kv_write", "kv", kv, T)
-    _on_device("kv_write", kv=kv, slots=slots, norm_w=norm_w, pos=pos, cache=cache.latent)
-    _ints("kv_write", "slots", slots, T)
-    if norm_w is not None:
-        _ints("kv_write", "norm_w", norm_w, _lib.KV_LATENT, "torch.float32")
-    if table is not None:
-        if pos is None:
-            _refuse("kv_write", "a rotation needs positions")
-        _ints("kv_write", "pos", pos, T)
+    if not _types:
+        _load_types()
+    if table is None:
+        pos = None
+    elif pos is None:
+        _refuse("kv_write", "a rotation needs positions")
+    _on_device("kv_write", kv, slots, norm_w, pos)
     call("fdm_kv_write", ctypes.byref(cache.desc), kv.data_ptr(), _elem("kv_write", "kv", kv.dtype), kv.stride(0),
-         _p(norm_w), None if table is None else ctypes.byref(table), _p(pos), slots.data_ptr(), T, _call_stream(stream))
+         None if norm_w is None else _vector("kv_write", "norm_w", norm_w, _lib.KV_LATENT, _f32),
+         None if table is None else ctypes.byref(table), None if pos is None else _vector("kv_write", "pos", pos, T, _i32),
+         _vector("kv_write", "slots", slots, T, _i32), T, _call_stream(stream))
 
 
 def kv_read(cache, slots, out, stream=None):
     """out [T, 576] = the rows at slots [T] int32, widened; a negative slot leaves its row as it was."""
     T = slots.numel()
     _rows("kv_read", "out", out, T)
-    _on_device("kv_read", slots=slots, out=out, cache=cache.latent)
-    _ints("kv_read", "slots", slots, T)
-    call("fdm_kv_read", ctypes.byref(cache.desc), slots.data_ptr(), T, out.data_ptr(), _elem("kv_read", "out", out.dtype),
-         out.stride(0), _call_stream(stream))
+    if not _types:
+        _load_types()
+    _on_device("kv_read", slots, out)
+    call("fdm_kv_read", ctypes.byref(cache.desc), _vector("kv_read", "slots", slots, T, _i32), T, out.data_ptr(),
+         _elem("kv_read", "out", out.dtype), out.stride(0), _call_stream(stream))
 
 
 def mla_workspace(N, H):
@@ -496,42 +511,41 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
     if q_lat.dim() != 3 or q_lat.shape[2] != _lib.KV_LATENT:
         _refuse(fn, f"q_lat: [N, H, {_lib.KV_LATENT}] is wanted, got {tuple(q_lat.shape)}")
     N, H, _ = q_lat.shape
-    if tuple(q_rope.shape) != (N, H, _lib.KV_ROPE) or out.shape != q_lat.shape:
+    if q_rope.shape != (N, H, _lib.KV_ROPE) or out.shape != q_lat.shape:
         _refuse(fn, f"q_rope, out: {(N, H, _lib.KV_ROPE)} and {tuple(q_lat.shape)} are wanted, got {tuple(q_rope.shape)} and {tuple(out.shape)}")
-    half = cache.rope.dtype
-    if q_lat.dtype != half or q_rope.dtype != half or out.dtype != half:
-        _refuse(fn, f"q_lat, q_rope and out are {half} with this cache, got {q_lat.dtype}, {q_rope.dtype}, {out.dtype}")
-    if q_lat.stride(2) != 1 or q_rope.stride(2) != 1 or out.stride(2) != 1:
+    if q_lat.dtype is not cache.half or q_rope.dtype is not cache.half or out.dtype is not cache.half:
+        _refuse(fn, f"q_lat, q_rope and out are {cache.half} with this cache, got {q_lat.dtype}, {q_rope.dtype}, {out.dtype}")
+    lt, lh, le = q_lat.stride()
+    rt, rh, re = q_rope.stride()
+    ot, oh, oe = out.stride()
+    if le != 1 or re != 1 or oe != 1:
         _refuse(fn, "the values of a head must be contiguous")
     B = kv_len.numel()
     if pages.dim() != 2 or pages.shape[0] != B:
         _refuse(fn, f"pages: [{B}, P] is wanted, got {tuple(pages.shape)}")
-    _on_device(fn, cache=cache.latent, q_lat=q_lat, q_rope=q_rope, q_start=q_start, kv_len=kv_len, pages=pages, out=out,
-               mask=mask, lse=lse, workspace=workspace)
-    _ints(fn, "q_start", q_start, B + 1)
-    _ints(fn, "kv_len", kv_len, B)
-    _ints(fn, "pages", pages, pages.numel())
+    if not _types:
+        _load_types()
+    _on_device(fn, q_lat, q_rope, q_start, kv_len, pages, out, mask, lse, workspace)
     words = 0
     if mask is not None:
         if mask.dim() != 2 or mask.shape[0] != N:
             _refuse(fn, f"mask: [{N}, words] is wanted, got {tuple(mask.shape)}")
         words = mask.shape[1]
-        _ints(fn, "mask", mask, N * words, "torch.int64")
+        mask = _vector(fn, "mask", mask, N * words, _i64)
     if lse is not None:
-        if tuple(lse.shape) != (N, H):
+        if lse.shape != (N, H):
             _refuse(fn, f"lse: {(N, H)} is wanted, got {tuple(lse.shape)}")
-        _ints(fn, "lse", lse, N * H, "torch.float32")
+        lse = _vector(fn, "lse", lse, N * H, _f32)
+    batch = _lib.MlaBatch(B, N, H, _vector(fn, "q_start", q_start, B + 1, _i32), _vector(fn, "kv_len", kv_len, B, _i32),
+                          _vector(fn, "pages", pages, pages.numel(), _i32), pages.shape[1], max_kv, mask, words)
     handle = _call_stream(stream)
     if workspace is None:  # torch's allocator keeps it for the stream that it is made on
         import torch
         with torch.cuda.stream(torch.cuda.current_stream(q_lat.device) if stream is None
                                else torch.cuda.ExternalStream(handle, device=q_lat.device)):
             workspace = mla_workspace(N, H)
-    batch = _lib.MlaBatch(B, N, H, q_start.data_ptr(), kv_len.data_ptr(), pages.data_ptr(), pages.shape[1], max_kv,
-                          _p(mask), words)
-    call("fdm_mla_attend", ctypes.byref(cache.desc), ctypes.byref(batch), q_lat.data_ptr(), q_lat.stride(0),
-         q_lat.stride(1), q_rope.data_ptr(), q_rope.stride(0), q_rope.stride(1), scale, out.data_ptr(), out.stride(0),
-         out.stride(1), _p(lse), workspace.data_ptr(), workspace.numel() * workspace.element_size(), handle)
+    call("fdm_mla_attend", ctypes.byref(cache.desc), ctypes.byref(batch), q_lat.data_ptr(), lt, lh, q_rope.data_ptr(), rt,
+         rh, scale, out.data_ptr(), ot, oh, lse, workspace.data_ptr(), workspace.numel() * workspace.element_size(), handle)
 
 
 # ---- dense FFN layers (layer_forward's branch for L < 3) ------------------------------

@@ -202,7 +202,9 @@ class _LazyLib:
     def __getattr__(self, name):
         if _LazyLib._handle is None:
             _LazyLib._handle = _load()
-        return getattr(_LazyLib._handle, name)
+        fn = getattr(_LazyLib._handle, name)
+        setattr(self, name, fn)  # the next call finds it without coming here
+        return fn
 
 
 lib = _LazyLib()

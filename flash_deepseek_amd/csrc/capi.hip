@@ -2417,7 +2417,6 @@ int fdm_rope(const fdm_rope_table* table, const int32_t* d_pos, int T, int H, in
     return fail(FDM_E_INVAL, "y: heads overlap (token stride %lld, head stride %lld)", (long long)y_token_stride,
                 (long long)y_head_stride);
   if (int rc = check_ready()) return rc;
-  memcpy(&a.table, table, sizeof a.table);
   a.pos = d_pos;
   a.x = d_x;
   a.y = d_y;
@@ -2436,7 +2435,9 @@ int fdm_rope(const fdm_rope_table* table, const int32_t* d_pos, int T, int H, in
   a.vec_behind = table->dim % 8 == 0;
   OnDevice dev;
   ProfScope prof(FDM_PROF_ROPE, as_stream(stream));
-  FDM_HIP(launch_rope(a, as_stream(stream)));
+  RopeTable t;
+  memcpy(&t, table, sizeof t);
+  FDM_HIP(launch_rope(a, t, as_stream(stream)));
   return FDM_OK;
 }
 
@@ -2472,7 +2473,12 @@ int fdm_kv_write(const fdm_kv_cache* c, const void* d_x, int x_type, int64_t x_s
   if (!aligned(d_x, es) || !aligned(d_norm_w, 4) || !aligned(d_slots, 4) || !aligned(d_pos, 4))
     return fail(FDM_E_INVAL, "misaligned pointer");
   if (int rc = check_ready()) return rc;
-  if (table) memcpy(&a.table, table, sizeof a.table);
+  if (table) {
+    a.table.dim = table->dim;
+    a.table.layout = table->layout;
+    a.table.mul = table->mul;
+    memcpy(a.table.turns, table->turns, sizeof a.table.turns);
+  }
   a.rotate = table != nullptr;
   a.pos = d_pos;
   a.x = d_x;

@@ -366,8 +366,15 @@ struct RopeTable {  // fdm_rope_table
   int spare;
   uint64_t turns[kRopeMaxDim / 2];  // frequency / 2 pi, in 2^-64 of a turn
 };
+// The same as a kernel argument, for up to N pairs (launching with 1 KB of
+// arguments where 256 bytes hold them costs the host 0.4 us).
+template <int N>
+struct RopeTurns {
+  int dim, layout;
+  float mul;
+  uint64_t turns[N];
+};
 struct RopeArgs {
-  RopeTable table;
   const int* pos;             // [T]
   const void* x;
   void* y;
@@ -379,10 +386,10 @@ struct RopeArgs {
   bool vec_behind;            // so are those behind the rotated part
   int tpw;                    // tokens of a workgroup (set by the launcher)
 };
-hipError_t launch_rope(RopeArgs a, hipStream_t s);
+hipError_t launch_rope(RopeArgs a, const RopeTable& table, hipStream_t s);
 
 struct KvWriteArgs {
-  RopeTable table;
+  RopeTurns<32> table;
   bool rotate;
   const int* pos;             // [T], if rotate
   const void* x;              // [T][576]

@@ -12,24 +12,24 @@ namespace fdm {
 // consecutive values (two runs of eight, R / 2 apart, for rotated ones in the
 // half layout), so a 16-bit head moves by 16-byte accesses.  Values that pass
 // through are items too, unless the call is in place.
-template <typename TX, typename TY, bool HALF>
-__global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
+template <typename TX, typename TY, bool HALF, int N>
+__global__ __launch_bounds__(256) void k_rope(RopeArgs a, RopeTurns<N> table) {
   extern __shared__ float2 sc[];  // [tpw][R / 2] (sine, cosine)
   const int t0 = blockIdx.x * a.tpw, nt = min(a.tpw, a.T - t0);
-  const int half = a.table.dim / 2;
+  const int half = table.dim / 2;
   for (int i = threadIdx.x; i < nt * half; i += 256) {
     const int t = i / half, p = i - t * half;
-    const uint64_t turns = (uint64_t)(int64_t)a.pos[t0 + t] * a.table.turns[p];
+    const uint64_t turns = (uint64_t)(int64_t)a.pos[t0 + t] * table.turns[p];
     float s, c;
     turn_sincos(turns, &s, &c);
-    sc[i] = make_float2(s * a.table.mul, c * a.table.mul);
+    sc[i] = make_float2(s * table.mul, c * table.mul);
   }
   __syncthreads();
   const bool vx = a.vec_x, vy = a.vec_y;
   const int rot_items = HALF ? half / 8 : half / 4;  // whole items; a tail of pairs follows
   const int rot_done = rot_items * (HALF ? 8 : 4);   // pairs they cover
   const int tail = half - rot_done;                  // pairs one by one
-  const int before = a.offset, behind = a.D - a.offset - a.table.dim;
+  const int before = a.offset, behind = a.D - a.offset - table.dim;
   const int pass0 = a.pass ? (before + 7) / 8 : 0, pass1 = a.pass ? (behind + 7) / 8 : 0;
   const int items = rot_items + tail + pass0 + pass1;
   const int total = nt * a.H * items;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
     }
     it -= tail;
     const bool first = it < pass0;
-    const int at = first ? 8 * it : a.offset + a.table.dim + 8 * (it - pass0);
+    const int at = first ? 8 * it : a.offset + table.dim + 8 * (it - pass0);
     const int n = min(8, (first ? a.offset : a.D) - at);
     // behind the rotated part the run starts where that ends: aligned if R is
     if (n == 8 && (first || a.vec_behind)) {
@@ -95,25 +95,38 @@ __global__ __launch_bounds__(256) void k_rope(RopeArgs a) {
 }
 
 namespace {
-template <typename TX, typename TY>
-void launch_layout(const RopeArgs& a, dim3 grid, size_t lds, hipStream_t s) {
-  if (a.table.layout)
-    k_rope<TX, TY, true><<<grid, 256, lds, s>>>(a);
+template <typename TX, typename TY, int N>
+void launch_layout(const RopeArgs& a, const RopeTable& table, dim3 grid, size_t lds, hipStream_t s) {
+  RopeTurns<N> t;
+  t.dim = table.dim;
+  t.layout = table.layout;
+  t.mul = table.mul;
+  for (int i = 0; i < N; ++i) t.turns[i] = table.turns[i];
+  if (table.layout)
+    k_rope<TX, TY, true, N><<<grid, 256, lds, s>>>(a, t);
   else
-    k_rope<TX, TY, false><<<grid, 256, lds, s>>>(a);
+    k_rope<TX, TY, false, N><<<grid, 256, lds, s>>>(a, t);
 }
-template <typename TX>
-void launch_to(const RopeArgs& a, dim3 grid, size_t lds, hipStream_t s) {
+template <typename TX, int N>
+void launch_to(const RopeArgs& a, const RopeTable& table, dim3 grid, size_t lds, hipStream_t s) {
   switch (a.y_type) {
-    case ElemType::f32: return launch_layout<TX, float>(a, grid, lds, s);
-    case ElemType::f16: return launch_layout<TX, _Float16>(a, grid, lds, s);
-    case ElemType::bf16: return launch_layout<TX, __bf16>(a, grid, lds, s);
+    case ElemType::f32: return launch_layout<TX, float, N>(a, table, grid, lds, s);
+    case ElemType::f16: return launch_layout<TX, _Float16, N>(a, table, grid, lds, s);
+    case ElemType::bf16: return launch_layout<TX, __bf16, N>(a, table, grid, lds, s);
+  }
+}
+template <int N>
+void launch_from(const RopeArgs& a, const RopeTable& table, dim3 grid, size_t lds, hipStream_t s) {
+  switch (a.x_type) {
+    case ElemType::f32: return launch_to<float, N>(a, table, grid, lds, s);
+    case ElemType::f16: return launch_to<_Float16, N>(a, table, grid, lds, s);
+    case ElemType::bf16: return launch_to<__bf16, N>(a, table, grid, lds, s);
   }
 }
 }  // namespace
 
-hipError_t launch_rope(RopeArgs a, hipStream_t s) {
-  const int half = a.table.dim / 2;
+hipError_t launch_rope(RopeArgs a, const RopeTable& table, hipStream_t s) {
+  const int half = table.dim / 2;
   const int per_token = a.H * ((a.D + 7) / 8);  // items of a token, about
   a.tpw = max(1, min(1024 / per_token, 2048 / half));
   const int wgs = (a.T + a.tpw - 1) / a.tpw;
@@ -121,11 +134,10 @@ hipError_t launch_rope(RopeArgs a, hipStream_t s) {
   const int split = max(1, min((a.tpw * per_token + 255) / 256, 2 * g_num_cus / wgs));
   const dim3 grid(wgs, split);
   const size_t lds = (size_t)a.tpw * half * sizeof(float2);
-  switch (a.x_type) {
-    case ElemType::f32: launch_to<float>(a, grid, lds, s); break;
-    case ElemType::f16: launch_to<_Float16>(a, grid, lds, s); break;
-    case ElemType::bf16: launch_to<__bf16>(a, grid, lds, s); break;
-  }
+  if (half <= 32)
+    launch_from<32>(a, table, grid, lds, s);
+  else
+    launch_from<kRopeMaxDim / 2>(a, table, grid, lds, s);
   return hipGetLastError();
 }
 
