@@ -2527,7 +2527,8 @@ int fdm_kv_read(const fdm_kv_cache* c, const int32_t* d_slots, int T, void* d_y,
 }
 
 static int check_mla_shape(int N, int H) {
-  if (N < 0 || H < 1 || H > FDM_MLA_MAX_HEADS) return fail(FDM_E_INVAL, "N=%d H=%d (1 .. %d heads)", N, H, FDM_MLA_MAX_HEADS);
+  if (N < 0 || N > FDM_MLA_MAX_TOKENS || H < 1 || H > FDM_MLA_MAX_HEADS)
+    return fail(FDM_E_INVAL, "N=%d (0 .. %d) H=%d (1 .. %d)", N, FDM_MLA_MAX_TOKENS, H, FDM_MLA_MAX_HEADS);
   return FDM_OK;
 }
 

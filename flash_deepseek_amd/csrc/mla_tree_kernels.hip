@@ -34,7 +34,8 @@ constexpr int kPBytes = kTileRows * kTilePos * 2;
 // three steps' rotary parts, the weights of two steps
 constexpr int kRotAt = 4 * kLatBytes, kPAt = kRotAt + 3 * kRotBytes, kStepLds = kPAt + 2 * kPBytes;
 constexpr size_t kPartFloats = (size_t)kTileRows * kLatDim;
-constexpr uint32_t kMaxSteps = 0x7FFFFFFFu;
+constexpr uint32_t kMaxUnits = 0x7FFFFFFFu;
+constexpr int kTileCost = 6;
 constexpr int kMaxGroups = 256;  // workgroups that share the work
 constexpr float kGrow = 8.0f;  // a row's maximum (log2) is moved when it grew by more
 
@@ -106,7 +107,13 @@ __device__ __forceinline__ float acc_put(float v) {
   asm("v_accvgpr_write_b32 %0, %1" : "=a"(a) : "v"(v));
   return a;
 }
-// before an ALU instruction reads what products have written
+__device__ __forceinline__ float acc_zero() {
+  float a;
+  asm volatile("v_accvgpr_write_b32 %0, 0" : "=a"(a));  // one each, not copies of one
+  return a;
+}
+// Before an ALU instruction reads what products have written, the compiler's
+// own copies where control flow meets among them.
 __device__ __forceinline__ void products_done() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("s_nop 11" ::: "memory");
@@ -166,10 +173,12 @@ __device__ __attribute__((aligned(16))) uint32_t zero_row[kLatDim * 2 / 4];  // 
 }  // namespace
 
 // ---- the work: tiles of rows, steps of positions --------------------------------------
-// A tile is g = 128 / H tokens of one sequence; it has a step for every 32
-// positions that its last token may see (one at least, so that rows that see
-// nothing are written).  All steps of all tiles in order (sequence, tile,
-// step) are cut into equal ranges, one a workgroup.
+// The (token, head) rows of a sequence, heads fastest, are cut into tiles of R.
+// A tile has a step for every S positions that its last token may see (one at
+// least, so that rows that see nothing are written) and counts kTileCost units
+// more, what beginning and ending it costs a workgroup (queries, first steps,
+// results: 12 to 14 us against 2.2 us a step).  The units of all tiles in order
+// (sequence, tile, unit) are cut into equal ranges, one a workgroup.
 struct SeqWork {
   int n, len, t0;  // tokens, positions, first token
 };
@@ -180,22 +189,164 @@ __device__ __forceinline__ SeqWork seq_work(const MlaTreeArgs& a, int b) {
   s.len = min(max(a.kv_len[b], 0), a.max_len);
   return s;
 }
-__device__ __forceinline__ int tile_steps(const SeqWork& s, int tile, int g, bool in_order) {
-  const int64_t seen = in_order ? (int64_t)s.len - s.n + min((tile + 1) * g, s.n) : s.len;
-  return max(1, (int)((seen + kTilePos - 1) / kTilePos));
+template <int R>
+__device__ __forceinline__ int tiles_of(const SeqWork& s, int H) { return (s.n * H + R - 1) / R; }
+template <int R, int S>
+__device__ __forceinline__ int tile_steps(const SeqWork& s, int tile, int H, bool in_order) {
+  const int last = min((R * (tile + 1) - 1) / H + 1, s.n);  // tokens up to the tile's last
+  const int64_t seen = in_order ? (int64_t)s.len - s.n + last : s.len;
+  return max(1, (int)((seen + S - 1) / S));
 }
-// ceil(1 / 32) + .. + ceil(x / 32)
+template <int R, int S>
+__device__ __forceinline__ int tile_units(const SeqWork& s, int tile, int H, bool in_order) {
+  return tile_steps<R, S>(s, tile, H, in_order) + kTileCost;
+}
+// ceil(1 / S) + .. + ceil(x / S)
+template <int S>
 __device__ __forceinline__ int64_t step_sum(int64_t x) {
-  const int64_t q = x / kTilePos, r = x % kTilePos;
-  return kTilePos * q * (q + 1) / 2 + r * (q + 1);
+  const int64_t q = x / S, r = x % S;
+  return S * q * (q + 1) / 2 + r * (q + 1);
 }
-// steps of the sequence's tiles 0 .. tiles - 1
-__device__ int64_t steps_before(const SeqWork& s, int tiles, int g, bool in_order) {
-  if (!in_order || s.n == 1) return (int64_t)tiles * tile_steps(s, 0, s.n, in_order);
-  if (g == 1 && s.len >= s.n) return step_sum(s.len - s.n + tiles) - step_sum(s.len - s.n);
+// units of the sequence's tiles 0 .. tiles - 1
+template <int R, int S>
+__device__ int64_t units_before(const SeqWork& s, int tiles, int H, bool in_order) {
+  if (!in_order || s.n <= 1) return (int64_t)tiles * tile_units<R, S>(s, 0, H, in_order);
+  if (H % R == 0 && s.len >= s.n) {  // whole tiles of one token
+    const int q = H / R, tokens = tiles / q;
+    const int64_t before = s.len - s.n;
+    return q * (step_sum<S>(before + tokens) - step_sum<S>(before)) +
+           (int64_t)(tiles % q) * ((before + tokens + 1 + S - 1) / S) + (int64_t)tiles * kTileCost;
+  }
   int64_t sum = 0;
-  for (int i = 0; i < tiles; ++i) sum += tile_steps(s, i, g, in_order);
+  for (int i = 0; i < tiles; ++i) sum += tile_units<R, S>(s, i, H, in_order);
   return sum;
+}
+
+// Units before each sequence into before[0 .. B], two sequences a thread of
+// 256.  A call's units are below 2^31; starts that make them more (sequences
+// that share tokens) are cut.
+template <int R, int S>
+__device__ __forceinline__ void count_units(const MlaTreeArgs& a, uint32_t* before, uint32_t* wave_total) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool in_order = a.mask == nullptr;
+  uint32_t mine[2], sum = 0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    mine[k] = sum;
+    const int b = 2 * tid + k;
+    if (b < a.B) {
+      const SeqWork s = seq_work(a, b);
+      sum = (uint32_t)min((int64_t)sum + units_before<R, S>(s, tiles_of<R>(s, a.H), a.H, in_order), (int64_t)kMaxUnits);
+    }
+  }
+  uint32_t upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t v = __shfl_up(upto, d);
+    if (lane >= d) upto = min(upto + v, kMaxUnits);
+  }
+  if (lane == 63) wave_total[wave] = upto;
+  const uint32_t inside = __shfl_up(upto, 1);
+  __syncthreads();
+  uint32_t base = 0;
+  for (int w = 0; w < wave; ++w) base = min(base + wave_total[w], kMaxUnits);
+  base = min(base + (lane ? inside : 0), kMaxUnits);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (2 * tid + k <= a.B) before[2 * tid + k] = min(base + mine[k], kMaxUnits);
+  if (tid == 255 && a.B == kMlaMaxSeqs) before[kMlaMaxSeqs] = min(base + sum, kMaxUnits);
+  __syncthreads();
+}
+
+// A workgroup's range of units, and the part of a tile that it is at.  Range g
+// of G over T units is [g T / G, (g + 1) T / G); unit u is in ((u + 1) G - 1) / T.
+struct Range {
+  uint32_t u, end;      // next unit, end
+  int group;            // number of the range
+  int b, tile, steps;   // sequence and tile of the part; all steps of the tile
+  int from, to;         // steps of the part
+  int parts;            // workgroups that have steps of the tile
+  SeqWork s;
+};
+// Ranges of two units at least: a part of one step is 256 KB of sums for 36 KB
+// of rows (one token over 1024 positions: 27.7 us, with ranges of one 30.0, of four 30.5).
+__device__ __forceinline__ uint32_t range_count(uint32_t total) { return min((uint32_t)gridDim.x, total / 2); }
+__device__ __forceinline__ Range range_of(const MlaTreeArgs& a, const uint32_t* before) {
+  Range r;
+  const uint32_t total = (uint32_t)uniform((int)before[a.B]), groups = range_count(total);
+  // Neighbours in the list on one XCD (workgroups go round the eight in turn),
+  // where they share rows; fewer ranges than workgroups are spread over all.
+  const bool full = groups == gridDim.x && gridDim.x % 8 == 0;
+  r.group = full ? (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
+  r.u = r.end = r.b = 0;
+  if ((uint32_t)r.group >= groups) return r;
+  r.u = (uint32_t)uniform((int)((uint64_t)r.group * total / groups));
+  r.end = (uint32_t)uniform((int)((uint64_t)(r.group + 1) * total / groups));
+  int hi = a.B - 1;  // the last sequence that starts at or before u
+  while (r.b < hi) {
+    const int mid = (r.b + hi + 1) / 2;
+    if ((uint32_t)uniform((int)before[mid]) <= r.u) r.b = mid;
+    else hi = mid - 1;
+  }
+  return r;
+}
+// The next part that has steps; false at the end of the range.
+template <int R, int S>
+__device__ __forceinline__ bool next_part(const MlaTreeArgs& a, const uint32_t* before, Range& r) {
+  const bool in_order = a.mask == nullptr;
+  while (r.u < r.end) {
+    while ((uint32_t)uniform((int)before[r.b + 1]) <= r.u) ++r.b;
+    r.s = seq_work(a, r.b);
+    r.s = {uniform(r.s.n), uniform(r.s.len), uniform(r.s.t0)};
+    const int64_t seq_u = (uint32_t)uniform((int)before[r.b]);
+    r.tile = 0;
+    {  // the last tile that starts at or before u
+      int hi = tiles_of<R>(r.s, a.H) - 1;
+      while (r.tile < hi) {
+        const int mid = (r.tile + hi + 1) / 2;
+        if (seq_u + units_before<R, S>(r.s, mid, a.H, in_order) <= r.u) r.tile = mid;
+        else hi = mid - 1;
+      }
+    }
+    const int64_t tile_u = seq_u + units_before<R, S>(r.s, r.tile, a.H, in_order) + kTileCost;  // its first step
+    r.steps = tile_steps<R, S>(r.s, r.tile, a.H, in_order);
+    r.from = (int)max((int64_t)r.u - tile_u, (int64_t)0);
+    r.to = (int)min((int64_t)r.steps, (int64_t)r.end - tile_u);
+    if (r.to > r.from) {
+      r.u = (uint32_t)(tile_u + r.to);
+      const uint32_t total = (uint32_t)uniform((int)before[a.B]), groups = range_count(total);
+      auto range_at = [&](uint64_t u) { return (int)(((u + 1) * groups - 1) / total); };
+      r.parts = uniform(range_at(tile_u + r.steps - 1) - range_at(tile_u) + 1);
+      return true;
+    }
+    if (r.to <= 0) break;  // the range ends before the tile's first step
+    r.u = (uint32_t)(tile_u + r.to);
+  }
+  return false;
+}
+
+// Which of the positions j0 .. j0 + 31 the sequence's token `place` sees (bits).
+__device__ __forceinline__ uint32_t sees(const MlaTreeArgs& a, const SeqWork& s, int place, int64_t j0) {
+  const int64_t d0 = j0 - (s.len - s.n);  // the token place of the first position
+  uint32_t see = d0 >= 0 ? 0u : d0 <= -32 ? ~0u : (1u << -d0) - 1;
+  if (d0 > -32) {
+    if (!a.mask) {
+      const int64_t last = place - d0;  // of the 32
+      see = last >= 31 ? ~0u : last < 0 ? see : (see | ((2u << last) - 1));
+    } else {
+      // bits d0 .. d0 + 31 of the mask
+      const uint64_t* mask = a.mask + (size_t)(s.t0 + place) * a.mask_words;
+      const int64_t at = d0 >= 0 ? d0 : 0;
+      const int64_t w = at >> 6;
+      uint64_t bits = w < a.mask_words ? mask[w] >> (at & 63) : 0;
+      if ((at & 63) && w + 1 < a.mask_words) bits |= mask[w + 1] << (64 - (at & 63));
+      see |= d0 >= 0 ? (uint32_t)bits : (uint32_t)bits << -d0;
+    }
+    // positions behind the sequence's end
+    const int64_t in = s.len - j0;
+    see &= in >= 32 ? ~0u : in <= 0 ? 0u : (1u << in) - 1;
+  }
+  return see;
 }
 
 template <int FMT>
@@ -207,101 +358,26 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   __shared__ float scale_by[2][kTileRows];   // what the rows' sums so far are scaled by
   __shared__ int moved[2][4];                // the step at which a wave's rows last were
   __shared__ int live[4];                    // bytes: which rows of a step exist
-  __shared__ uint32_t before[kMlaMaxSeqs + 1];  // steps before each sequence
+  __shared__ uint32_t before[kMlaMaxSeqs + 1];  // units before each sequence
   __shared__ uint32_t wave_total[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, h = lane >> 5;
-  const int g = kTileRows / a.H;
-  const bool in_order = a.mask == nullptr;
 
-  // steps before each sequence, two sequences a thread.  A call's steps are
-  // below 2^31; starts that make them more (sequences that share tokens) are cut.
-  {
-    uint32_t mine[2], sum = 0;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      mine[k] = sum;
-      const int b = 2 * tid + k;
-      if (b < a.B) {
-        const SeqWork s = seq_work(a, b);
-        sum = (uint32_t)min((int64_t)sum + steps_before(s, (s.n + g - 1) / g, g, in_order), (int64_t)kMaxSteps);
-      }
-    }
-    uint32_t upto = sum;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t v = __shfl_up(upto, d);
-      if (lane >= d) upto = min(upto + v, kMaxSteps);
-    }
-    if (lane == 63) wave_total[wave] = upto;
-    const uint32_t inside = __shfl_up(upto, 1);
-    __syncthreads();
-    uint32_t base = 0;
-    for (int w = 0; w < wave; ++w) base = min(base + wave_total[w], kMaxSteps);
-    base = min(base + (lane ? inside : 0), kMaxSteps);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (2 * tid + k <= a.B) before[2 * tid + k] = min(base + mine[k], kMaxSteps);
-    if (tid == 255 && a.B == kMlaMaxSeqs) before[kMlaMaxSeqs] = min(base + sum, kMaxSteps);
-    __syncthreads();
-  }
-  const int64_t total = (uint32_t)uniform((int)before[a.B]);
-  const int groups = gridDim.x;
-  // neighbours in the list on one XCD (workgroups go round the eight in turn)
-  const int group = groups % 8 ? blockIdx.x : (blockIdx.x % 8) * (groups / 8) + blockIdx.x / 8;
-  const int64_t per = uniform((total + groups - 1) / groups);
-  int64_t u = group * per;
-  const int64_t u_end = min(u + per, total);
-  const Space space = space_of(a.workspace, groups);
+  count_units<kTileRows, kTilePos>(a, before, wave_total);
+  Range range = range_of(a, before);
+  const int group = range.group;
+  const Space space = space_of(a.workspace, gridDim.x);
   JoinDesc desc = {0, 0, 0, 0};
 
-  int b = 0;
-  if (u < u_end) {  // the last sequence that starts at or before u
-    int hi = a.B - 1;
-    while (b < hi) {
-      const int mid = (b + hi + 1) / 2;
-      if ((uint32_t)uniform((int)before[mid]) <= u) b = mid;
-      else hi = mid - 1;
-    }
-  }
-  while (u < u_end) {
-    while ((uint32_t)uniform((int)before[b + 1]) <= u) ++b;
-    SeqWork s = seq_work(a, b);
-    s = {uniform(s.n), uniform(s.len), uniform(s.t0)};
-    const int64_t seq_u = (uint32_t)uniform((int)before[b]);
-    int tile = 0;
-    {  // the last tile that starts at or before u
-      int hi = (s.n + g - 1) / g - 1;
-      while (tile < hi) {
-        const int mid = (tile + hi + 1) / 2;
-        if (seq_u + steps_before(s, mid, g, in_order) <= u) tile = mid;
-        else hi = mid - 1;
-      }
-    }
-    const int64_t tile_u = seq_u + steps_before(s, tile, g, in_order);
-    const int steps = tile_steps(s, tile, g, in_order);
-    const int from = (int)(u - tile_u);
-    const int to = (int)min((int64_t)steps, u_end - tile_u);
-    const int n = s.n, len = s.len;
-    u = tile_u + to;
-    const int prefix = len - n;                // may be negative
-    const int first = s.t0 + tile * g;         // the tile's first token
-    const int rows = min(g, n - tile * g) * a.H;
+  while (next_part<kTileRows, kTilePos>(a, before, range)) {
+    const SeqWork s = range.s;
+    const int from = range.from, to = range.to, len = s.len;
+    const int prefix = len - s.n;  // may be negative
+    const int row0 = kTileRows * range.tile, rows = min(kTileRows, s.n * a.H - row0);
 
-    // the row of this lane's scores, and its query as the products' B operand
-    const int row = 32 * wave + l32;
-    const bool row_is = row < rows;
-    const int tok = row_is ? row / a.H : 0, head = row_is ? row - tok * a.H : 0;
-    x8 q[36];
-    {
-      const T* ql = static_cast<const T*>(a.q_lat) + (int64_t)(first + tok) * a.ql_token + head * a.ql_head + 8 * h;
-      const T* qr = static_cast<const T*>(a.q_rope) + (int64_t)(first + tok) * a.qr_token + head * a.qr_head + 8 * h;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) q[k] = *reinterpret_cast<const x8*>(ql + 16 * k);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) q[32 + k] = *reinterpret_cast<const x8*>(qr + 16 * k);
-    }
-
+    // The lane's scores are those of row 32 wave + l32.  What is needed of it is
+    // computed where it is needed: registers are short in the loop.
+    auto token_of = [&](int r) { return (row0 + min(r, rows - 1)) / a.H; };
     // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7, eight lanes
     // each, in kBring pieces of work.  16-bit rows go straight into LDS, one a
     // piece.  FP8 codes go into registers, and from there in the same turn as 16-bit
@@ -309,7 +385,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     constexpr bool kCodes = FMT == kKvFp8;
     constexpr int kBring = 9;
     const int my_row = 8 * wave + (lane >> 3);
-    const int* pages = a.pages + (size_t)b * a.pages_stride;
+    const int* pages = a.pages + (size_t)range.b * a.pages_stride;
     const char* none = reinterpret_cast<const char*>(zero_row);
     int page;                // of this lane's row in the step that is placed next
     int slot = 0;            // this lane's row in the step placed last; -1: none
@@ -381,20 +457,16 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 
     // ---- the products
     f32x16 o[8][2];  // [32 dims][32 rows]: dims 256 (wave & 1) + 32 i, rows 64 (wave >> 1) + 32 k
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][k][e] = acc_put(0.0f);
+    x8 q[36];        // the queries of the lane's row: the products' B operand
     float m = -__builtin_inff(), l = 0.0f;
     const int rh = wave >> 1, dh = wave & 1;
+    const bool works = 64 * rh < rows;  // otherwise the wave only brings
 
     // Operands come out of LDS kAhead reads before the product that wants them:
     // 36 of keys (position = l32, 8 dims at 16 k + 8 h), then 16 of values (dim =
     // l32 of a block of 32; positions 16 s + 4 h + {0 .. 3, 8 .. 11}, the ones
     // whose weights the lane has).
-    constexpr int kKeys = 36, kVals = 16, kAhead = kCodes ? 6 : 6;
+    constexpr int kKeys = 36, kVals = 16, kAhead = 4;
     static_assert(kKeys % kAhead == 0, "keys and values take the registers in turn");
     i32x4 f[kAhead];
     int key_at, rot_at, v0_at, v1_at;  // this lane's addresses
@@ -458,7 +530,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           const float keep = need ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
           m = need ? top : m;
           l *= keep;
-          scale_by[step & 1][row] = keep;  // both halves of the wave have it
+          scale_by[step & 1][here(32 * wave + l32)] = keep;  // both halves of the wave have it
           moved[step & 1][wave] = step;
         }
         off = m == -__builtin_inff() ? 0.0f : m;
@@ -503,27 +575,6 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    // which positions of the step the lane's row sees
-    auto seen = [&](int step, uint32_t exists) -> uint32_t {
-      const int64_t d0 = (int64_t)step * kTilePos - prefix;  // the token place of the step's first position
-      uint32_t see = d0 >= 0 ? 0u : d0 <= -32 ? ~0u : (1u << -d0) - 1;
-      if (d0 > -32) {
-        if (in_order) {
-          const int64_t last = tile * g + tok - d0;  // of the step's positions
-          see = last >= 31 ? ~0u : last < 0 ? see : (see | ((2u << last) - 1));
-        } else {
-          // bits d0 .. d0 + 31 of the mask
-          const uint64_t* mask = a.mask + (size_t)(first + tok) * a.mask_words;
-          const int64_t at = d0 >= 0 ? d0 : 0;
-          const int64_t w = at >> 6;
-          uint64_t bits = w < a.mask_words ? mask[w] >> (at & 63) : 0;
-          if ((at & 63) && w + 1 < a.mask_words) bits |= mask[w + 1] << (64 - (at & 63));
-          see |= d0 >= 0 ? (uint32_t)bits : (uint32_t)bits << -d0;
-        }
-      }
-      return see & exists;
-    };
-
     // In one turn step j's keys and then step j - 1's values are multiplied.
     // Step j + 1 is in LDS already, so its first keys are requested before the
     // turn ends, and the barrier stands among the keys' products: behind it the
@@ -539,14 +590,14 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
     };
-    bool dirty = false;   // step j - 1 has rows that not all tokens see
+    auto edge = [&](int j) { return (int64_t)(j + 1) * kTilePos > prefix; };  // not all tokens see all of step j
     int mv0 = -1, mv1 = -1;
     auto moves = [&](int j) {
       mv0 = moved[j & 1][2 * rh];
       mv1 = moved[j & 1][2 * rh + 1];
     };
     auto clear_of = [&](int j) {  // step j's values and the sums made ready for its weights
-      if (dirty) {
+      if (edge(j)) {
         clean(j);
         __syncthreads();
       }
@@ -558,6 +609,12 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       __builtin_amdgcn_sched_barrier(0);
       asm volatile("s_nop 4" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
+    };
+    auto next_rot = [&] {
+      const int r = rot_now;
+      rot_now = rot_next;
+      rot_next = rot_then;
+      rot_then = r;
     };
     auto turn = [&](int j, auto with_values) {
       constexpr bool VALUES = decltype(with_values)::value;
@@ -578,10 +635,8 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           bring(j + 2, (k - kBarrier - 2) / kApart, rot_then);
         __builtin_amdgcn_sched_barrier(0);
       }
-      const bool edge = (int64_t)(j + 1) * kTilePos > prefix;
       uint32_t see = (uint32_t)uniform(exists);
-      if (edge) see = seen(j, see);
-      dirty = edge;
+      if (edge(j)) see &= sees(a, s, token_of(here(32 * wave + l32)), (int64_t)j * kTilePos);
       if constexpr (VALUES) val_product(0, kKeys);
       products_done();
       if (__any(see != ~0u)) hide(see);
@@ -610,10 +665,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) fetch_key(k);
       }
-      const int r = rot_now;
-      rot_now = rot_next;
-      rot_next = rot_then;
-      rot_then = r;
+      next_rot();
     };
     page = page_of(from);
     __syncthreads();  // the tile before has left LDS
@@ -628,79 +680,124 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) widen(from + t, k);
     }
-    landed();
-    key_place(from, rot_now);
+    // the queries are requested behind the first rows, which take longer
+    {
+      const int tok = token_of(32 * wave + l32), head = row0 + min(32 * wave + l32, rows - 1) - tok * a.H;
+      const T* ql = static_cast<const T*>(a.q_lat) + (int64_t)(s.t0 + tok) * a.ql_token + head * a.ql_head + 8 * h;
+      const T* qr = static_cast<const T*>(a.q_rope) + (int64_t)(s.t0 + tok) * a.qr_token + head * a.qr_head + 8 * h;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) fetch_key(k);
-    turn(from, std::false_type{});
-#pragma nounroll
-    for (int j = from + 1; j < to; ++j) turn(j, std::true_type{});
-    landed();
-    moves(to - 1);
-    clear_of(to - 1);
-    val_place(to - 1);
-    fetch_weights(to - 1, 0);
-    fetch_weights(to - 1, 1);
+      for (int k = 0; k < 32; ++k) q[k] = *reinterpret_cast<const x8*>(ql + 16 * k);
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch_val(i, i);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < kVals; ++i) {
-      val_product(i, i);
-      if (i + kAhead < kVals) fetch_val(i + kAhead, i + kAhead);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int k = 0; k < 4; ++k) q[32 + k] = *reinterpret_cast<const x8*>(qr + 16 * k);
     }
-
-    // ---- the tile's results, or a part of them
-    products_done();
-    l = across_halves(l, [](float x, float y) { return x + y; });
-    __syncthreads();
-    float* stat = reinterpret_cast<float*>(lds + kPAt);  // [128] max, [128] sum
-    if (lane < 32) {
-      stat[row] = m;
-      stat[kTileRows + row] = l;
-    }
-    __syncthreads();
-    if (from == 0 && to == steps) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int r = 64 * rh + 32 * k + l32;
-        if (r < rows) {
-          const int t = r / a.H, hd = r - t * a.H;
-          const float sum = stat[kTileRows + r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          T* out = static_cast<T*>(a.out) + (int64_t)(first + t) * a.out_token + hd * a.out_head + 256 * dh + 4 * h;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x4 v;
-#pragma unroll
-              for (int c = 0; c < 4; ++c) v[c] = (T)(acc_get(o[i][k][4 * e + c]) * inv);
-              *reinterpret_cast<x4*>(out + 32 * i + 8 * e) = v;
-              __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-      }
-      if (a.lse && lane < 32 && row_is)
-        a.lse[(size_t)(first + tok) * a.H + head] =
-            l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
-    } else {
-      // the range's first tile may have begun in the workgroup before; its last goes on in the next
-      const int part = 2 * group + (from == 0 ? 1 : 0);
-      if (from == 0) desc = {b, tile, (int)((tile_u + steps - 1) / per) - group + 1, 0};
-      if (tid < kTileRows) space.stat[(size_t)part * kTileRows + tid] = make_float2(stat[tid], stat[kTileRows + tid]);
-      f32x4* to_part = reinterpret_cast<f32x4*>(space.part + (size_t)part * kPartFloats) + wave * 4096 + lane;
+    if (works) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            to_part[((i * 2 + k) * 4 + e) * 64] =
-                f32x4{acc_get(o[i][k][4 * e]), acc_get(o[i][k][4 * e + 1]), acc_get(o[i][k][4 * e + 2]),
-                      acc_get(o[i][k][4 * e + 3])};
-            __builtin_amdgcn_sched_barrier(0);
+          for (int e = 0; e < 16; ++e) o[i][k][e] = acc_zero();
+    }
+    landed();
+    if (works) {
+      key_place(from, rot_now);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) fetch_key(k);
+      turn(from, std::false_type{});
+#pragma nounroll
+      for (int j = from + 1; j < to; ++j) turn(j, std::true_type{});
+      landed();
+      moves(to - 1);
+      clear_of(to - 1);
+      val_place(to - 1);
+      fetch_weights(to - 1, 0);
+      fetch_weights(to - 1, 1);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fetch_val(i, i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kVals; ++i) {
+        val_product(i, i);
+        if (i + kAhead < kVals) fetch_val(i + kAhead, i + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      products_done();
+
+      // ---- the tile's results, or a part of them
+      l = across_halves(l, [](float x, float y) { return x + y; });
+      __syncthreads();
+      float* stat = reinterpret_cast<float*>(lds + kPAt);  // [128] max, [128] sum
+      if (lane < 32) {
+        stat[32 * wave + l32] = m;
+        stat[kTileRows + 32 * wave + l32] = l;
+      }
+      __syncthreads();
+      if (from == 0 && to == range.steps) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int r = 64 * rh + 32 * k + l32;
+          if (r < rows) {
+            const int t = (row0 + r) / a.H, hd = row0 + r - t * a.H;
+            const float sum = stat[kTileRows + r], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            T* out = static_cast<T*>(a.out) + (int64_t)(s.t0 + t) * a.out_token + hd * a.out_head + 256 * dh + 4 * h;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                x4 v;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[c] = (T)(acc_get(o[i][k][4 * e + c]) * inv);
+                *reinterpret_cast<x4*>(out + 32 * i + 8 * e) = v;
+                __builtin_amdgcn_sched_barrier(0);
+              }
           }
+        }
+        const int r = here(32 * wave + l32);
+        if (a.lse && lane < 32 && r < rows) {
+          const int tok = token_of(r);
+          a.lse[(size_t)(s.t0 + tok) * a.H + row0 + r - tok * a.H] =
+              l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+        }
+      } else {
+        // the range's first tile may have begun in the workgroup before; its last goes on in the next
+        const int part = 2 * group + (from == 0 ? 1 : 0);
+        if (from == 0) desc = {range.b, range.tile, range.parts, 0};
+        if (tid < kTileRows) space.stat[(size_t)part * kTileRows + tid] = make_float2(stat[tid], stat[kTileRows + tid]);
+        f32x4* to_part = reinterpret_cast<f32x4*>(space.part + (size_t)part * kPartFloats) + (2 * rh * 16 + 8 * dh) * 256 + lane;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (64 * rh + 32 * k >= rows) break;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              to_part[(k * 16 + i) * 256 + e * 64] =
+                  f32x4{acc_get(o[i][k][4 * e]), acc_get(o[i][k][4 * e + 1]), acc_get(o[i][k][4 * e + 2]),
+                        acc_get(o[i][k][4 * e + 3])};
+              __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+      }
+    } else {  // the same barriers
+#pragma nounroll
+      for (int j = from; j <= to; ++j) {
+        landed();
+        if (j > from && edge(j - 1)) {
+          clean(j - 1);
+          __syncthreads();
+        }
+        if (j == to) break;
+#pragma unroll
+        for (int k = 0; k < kBring; ++k) {
+          bring(j + 2, k, rot_then);
+          apart();
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) widen(j + 2, k);
+        next_rot();
+      }
+      __syncthreads();  // and those of the results
+      __syncthreads();
     }
   }
   if (tid == 0) space.desc[group] = desc;
@@ -712,7 +809,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 // tiles of many parts are bound by latency (I = 1, S = 4: one token over 1024
 // positions, 32 parts, 9.6 us), many of few by memory and by the dependent
 // reads before the first part (I = 8, S = 1).
-template <int FMT, int S, int I>
+template <int FMT, int R, int S, int I>
 __global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int groups) {
   typedef typename Half<FMT>::T T;
   typedef typename Half<FMT>::x4 x4;
@@ -739,19 +836,19 @@ __global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int gr
   __syncthreads();
   const int group = owner;
   if (group < 0) return;
-  const JoinDesc d = space.desc[group];
-  const int dim0 = (int)blockIdx.y / 4 * I;  // blocks of 32 dims, of 16
-  const int rh = ((int)blockIdx.y >> 1) & 1, k = blockIdx.y & 1, w = 2 * rh + dim0 / 8;
-  const int row0 = 64 * rh + 32 * k;
-  const int g = kTileRows / a.H;
+  JoinDesc d = space.desc[group];
+  d.parts = min(d.parts, groups - group);
+  constexpr int kBlocks = R / 32;  // of rows
+  const int dim0 = (int)blockIdx.y / kBlocks * I, rb = (int)blockIdx.y % kBlocks;  // first block of 32 dims, of 16
+  const int row0 = 32 * rb;
   const SeqWork s = seq_work(a, d.b);
-  const int first = s.t0 + d.tile * g, rows = min(g, s.n - d.tile * g) * a.H;
+  const int tile0 = R * d.tile, rows = min(R, s.n * a.H - tile0);
   if (row0 >= rows) return;
   auto part_of = [&](int p) { return (size_t)(p ? 2 * (group + p) : 2 * group + 1); };
   // the rows' weights of each part
   const int srow = tid & 31, slot = tid >> 5;
   float top = -__builtin_inff();
-  for (int p = slot; p < d.parts; p += kSlots) top = fmaxf(top, space.stat[part_of(p) * kTileRows + row0 + srow].x);
+  for (int p = slot; p < d.parts; p += kSlots) top = fmaxf(top, space.stat[part_of(p) * R + row0 + srow].x);
   red[slot][srow] = top;
   __syncthreads();
 #pragma unroll
@@ -760,7 +857,7 @@ __global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int gr
   const float off = top == -__builtin_inff() ? 0.0f : top;
   float l = 0.0f;
   for (int p = slot; p < d.parts; p += kSlots) {
-    const float2 st = space.stat[part_of(p) * kTileRows + row0 + srow];
+    const float2 st = space.stat[part_of(p) * R + row0 + srow];
     const float f = __builtin_amdgcn_exp2f(st.x - off);
     weight[p][srow] = f;
     l = fmaf(f, st.y, l);
@@ -773,18 +870,18 @@ __global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int gr
 #pragma unroll
   for (int t = 0; t < kSlots; ++t) l += red[t][l32];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int t = r / a.H, hd = r - t * a.H;
-  T* out = static_cast<T*>(a.out) + (int64_t)(first + t) * a.out_token + hd * a.out_head + 32 * dim0 + 8 * e + 4 * h;
+  const int t = (tile0 + r) / a.H, hd = tile0 + r - t * a.H;
+  T* out = static_cast<T*>(a.out) + (int64_t)(s.t0 + t) * a.out_token + hd * a.out_head + 32 * dim0 + 8 * e + 4 * h;
   constexpr int kFlight = I > 1 ? 4 : 8;
 #pragma unroll 2
   for (int i = 0; i < I; ++i) {
-    const f32x4* from = reinterpret_cast<const f32x4*>(space.part) + w * 4096 + (((dim0 % 8 + i) * 2 + k) * 4 + e) * 64 + lane;
+    const f32x4* from = reinterpret_cast<const f32x4*>(space.part) + (rb * 16 + dim0 + i) * 256 + e * 64 + lane;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int p0 = ps; p0 < d.parts; p0 += kFlight * S) {
       f32x4 v[kFlight];
 #pragma unroll
       for (int t = 0; t < kFlight; ++t)
-        if (p0 + t * S < d.parts) v[t] = from[part_of(p0 + t * S) * (kPartFloats / 4)];
+        if (p0 + t * S < d.parts) v[t] = from[part_of(p0 + t * S) * (R * kLatDim / 4)];
 #pragma unroll
       for (int t = 0; t < kFlight; ++t)
         if (p0 + t * S < d.parts) {
@@ -810,8 +907,8 @@ __global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int gr
   }
   if (a.lse && r < rows && dim0 == 0 && e == 0 && h == 0) {
     top = -__builtin_inff();
-    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, space.stat[part_of(p) * kTileRows + r].x);
-    a.lse[(size_t)(first + t) * a.H + hd] =
+    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, space.stat[part_of(p) * R + r].x);
+    a.lse[(size_t)(s.t0 + t) * a.H + hd] =
         l == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
   }
 }
@@ -824,17 +921,21 @@ size_t mla_tree_workspace(int, int) {
 }
 
 namespace {
+template <int FMT, int R>
+void join_parts(const MlaTreeArgs& a, int groups, hipStream_t s) {
+  // no more tiles than these, whatever the sequences' sizes
+  const int64_t most = ((int64_t)a.N * a.H + R - 1) / R + a.B;
+  const int tiles = (int)min((int64_t)groups, most);
+  if (tiles * 16 <= groups)  // 16 parts a tile, if all workgroups have work
+    k_mla_tree_join<FMT, R, 4, 1><<<dim3(tiles, R / 32 * 16), 1024, 0, s>>>(a, groups);
+  else
+    k_mla_tree_join<FMT, R, 1, 8><<<dim3(tiles, R / 32 * 2), 256, 0, s>>>(a, groups);
+}
 template <int FMT>
 void launch_fmt(const MlaTreeArgs& a, hipStream_t s) {
   const int groups = mla_tree_groups();
   k_mla_tree<FMT><<<groups, 256, 0, s>>>(a);
-  // no more tiles than these, whatever the sequences' sizes
-  const int g = kTileRows / a.H;
-  const int tiles = min(groups, min(a.N, a.N / g + a.B));
-  if (tiles * 16 <= groups)  // 16 parts a tile, if all workgroups have work
-    k_mla_tree_join<FMT, 4, 1><<<dim3(tiles, 64), 1024, 0, s>>>(a, groups);
-  else
-    k_mla_tree_join<FMT, 1, 8><<<dim3(tiles, 8), 256, 0, s>>>(a, groups);
+  join_parts<FMT, kTileRows>(a, groups, s);
 }
 }  // namespace
 

@@ -529,7 +529,7 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
  * else BF16; strides in elements, multiples of 8, 16-byte aligned.  lse
  * (optional) fp32 [N][H].  Products of the 16-bit values accumulate in fp32 and
  * softmax weights round to 16 bits before the second product.  1 <= H <=
- * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS.  max_kv: the longest kv_len the
+ * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS, N <= FDM_MLA_MAX_TOKENS.  max_kv: the longest kv_len the
  * caller expects (0: unknown); it only chooses among kernels.
  * d_workspace: at least fdm_mla_workspace(N, H) bytes, 256-byte aligned, used
  * by the call alone until it has run on its stream: calls that may overlap, and
@@ -537,6 +537,7 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
  * may be captured.  The same arguments give the same bits. */
 #define FDM_MLA_MAX_HEADS 128
 #define FDM_MLA_MAX_SEQS 512
+#define FDM_MLA_MAX_TOKENS 1048576
 typedef struct fdm_mla_batch {
   int B, N, H;
   const int32_t *d_q_start;  /* [B + 1]          */

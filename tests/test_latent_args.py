@@ -99,7 +99,7 @@ def attend(c=None, **kw):
     return _lib.lib.fdm_mla_attend(cache() if c is None else c, ctypes.byref(batch), *{**CALL, **kw}.values())
 
 
-@pytest.mark.parametrize("bad", [dict(B=0), dict(B=513), dict(N=-1), dict(H=0), dict(H=129), dict(pages_stride=0), dict(max_kv=-1),
+@pytest.mark.parametrize("bad", [dict(B=0), dict(B=513), dict(N=-1), dict(N=(1 << 20) + 1), dict(H=0), dict(H=129), dict(pages_stride=0), dict(max_kv=-1),
                                  dict(mask=P), dict(mask_words=1), dict(mask=P, mask_words=-1), dict(mask=P + 4, mask_words=1),
                                  dict(q_start=None), dict(kv_len=None), dict(pages=None), dict(ql=None), dict(qr=None), dict(out=None),
                                  dict(ws=None), dict(ws=P + 128), dict(ql=P + 8), dict(qr=P + 8), dict(out=P + 8), dict(ql0=2052),
