@@ -133,6 +133,15 @@ __device__ __forceinline__ void lds_load16(uint64_t base, int off, char* to) {
   const int at = (int)(uintptr_t)(FDM_LDS char*)to;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
 }
+// Two rows of a base's next four: the loads' offset moves both of their ends.
+template <int ROW>
+__device__ __forceinline__ void lds_load_rows(uint64_t base, int off0, int off1, char* to) {
+  const int at = (int)(uintptr_t)(FDM_LDS char*)to;
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3 offset:%4\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:%5" ::"s"(at), "v"(off0), "v"(off1), "s"(base), "n"(ROW * 1024), "n"(ROW * 1024 + 1024)
+      : "memory");
+}
 // four rows x 16 columns of 16-bit values, lane i of 16 pointing at four
 // columns of row i / 4: lane i gets column i of the four rows
 __device__ __forceinline__ f16x4 read_turned(const char* p, f16x4) {
@@ -160,6 +169,20 @@ __device__ __forceinline__ int here(int v) {
   return v;
 }
 
+// A condition whose code stands out of the way: a taken branch costs a wave
+// that has its SIMD alone some 60 cycles.
+__device__ __forceinline__ bool rare(bool v) { return __builtin_expect(v, 0); }
+
+// f with the constants 0 .. N - 1
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  unrolled(f, std::make_integer_sequence<int, N>{});
+}
+
 // the value of lane ^ 32, combined
 template <typename F>
 __device__ __forceinline__ float across_halves(float v, F f) {
@@ -168,7 +191,7 @@ __device__ __forceinline__ float across_halves(float v, F f) {
   return f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
-__device__ __attribute__((aligned(16))) uint32_t zero_row[kLatDim * 2 / 4];  // stands for a row that is none
+__device__ __attribute__((aligned(16))) uint32_t zero_row[8 * kLatDim * 2 / 4];  // stands for eight rows that are none
 
 }  // namespace
 
@@ -349,7 +372,7 @@ __device__ __forceinline__ uint32_t sees(const MlaTreeArgs& a, const SeqWork& s,
   return see;
 }
 
-template <int FMT>
+template <int FMT, bool WHOLE>
 __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   typedef typename Half<FMT>::T T;
   typedef typename Half<FMT>::x4 x4;
@@ -378,80 +401,110 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     // The lane's scores are those of row 32 wave + l32.  What is needed of it is
     // computed where it is needed: registers are short in the loop.
     auto token_of = [&](int r) { return (row0 + min(r, rows - 1)) / a.H; };
-    // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7, eight lanes
-    // each, in kBring pieces of work.  16-bit rows go straight into LDS, one a
-    // piece.  FP8 codes go into registers, and from there in the same turn as 16-bit
+    // ---- a step's rows into LDS: wave w brings rows 8 w .. 8 w + 7, in kBring
+    // pieces of work.  16-bit rows go straight into LDS.  FP8 codes go into
+    // registers, eight lanes a row, and from there in the same turn as 16-bit
     // values (exact) into LDS.  A row that is none reads zeros.
+    // WHOLE: all rows of a step lie in one page (pages of 32 and more).  Where
+    // they are is known to all lanes, and a piece is two rows; positions behind
+    // the sequence's end are read as they are, and hidden.  Otherwise a lane
+    // looks after the row that it is one of eight of, and a piece is one row,
+    // which costs 85 of 640 instructions more a step: 512 tokens of 128 heads over
+    // 4608 positions 636 us against 615, 32 sequences of 16 over 16384 1333 against 1283.
     constexpr bool kCodes = FMT == kKvFp8;
-    constexpr int kBring = 9;
+    constexpr int kBring = kCodes || WHOLE ? 8 : 12;
     const int my_row = 8 * wave + (lane >> 3);
     const int* pages = a.pages + (size_t)range.b * a.pages_stride;
     const char* none = reinterpret_cast<const char*>(zero_row);
-    int page;                // of this lane's row in the step that is placed next
-    int slot = 0;            // this lane's row in the step placed last; -1: none
+    int page;                // of the next step to be placed (this lane's row)
+    int slot = 0;            // the step placed last: this lane's row, WHOLE: the wave's first; -1: none
+    uint32_t exist = 0;      // WHOLE: bit step & 3
     const char* mine;        // 16 bits: that row
     uint64_t base;           //   the row that the next piece brings
     u32x4 code[4];           // FP8: that row's codes (16 of each group) and scales
     uint32_t code_scale = 0;
-    auto page_of = [&](int step) { return pages[min(step * kTilePos + my_row, max(len - 1, 0)) >> a.page_shift]; };
+    auto page_of = [&](int step) {
+      return pages[min(step * kTilePos + (WHOLE ? 0 : my_row), max(len - 1, 0)) >> a.page_shift];
+    };
     auto place = [&](int step) {
-      const int j = step * kTilePos + my_row;
-      const bool is = (unsigned)page < (unsigned)a.n_pages && j < len && step < to;
-      slot = is ? (page << a.page_shift) + (j & ((1 << a.page_shift) - 1)) : -1;
-      page = page_of(step + 1);
+      const int j = step * kTilePos + (WHOLE ? 0 : my_row);
+      const int at = WHOLE ? uniform(page) : page;
+      const bool is = (unsigned)at < (unsigned)a.n_pages & j < len & step < to;
+      slot = is ? (at << a.page_shift) + (j & ((1 << a.page_shift) - 1)) + (WHOLE ? 8 * wave : 0) : -1;
+      if constexpr (WHOLE) exist = (exist & ~(1u << (step & 3))) | (uint32_t)is << (step & 3);
     };
     auto announce = [&](int step, int rot_at) {  // which rows exist, and their rotary parts
-      const uint64_t all = __ballot(slot >= 0);
-      uint32_t byte = 0xFF;
-      if (all != ~0ull) {
-        byte = 0;
+      const int swap = 16 * ((lane & 7) ^ ((my_row >> 1) & 7));
+      if constexpr (WHOLE) {
+        const char* rp = slot >= 0 ? static_cast<const char*>(a.rope) + (size_t)slot * (kRotDim * 2) : none;
+        lds_load16((uint64_t)rp, here((lane >> 3) * (kRotDim * 2) + swap), lds + rot_at + wave * 1024);
+      } else {
+        const uint64_t all = __ballot(slot >= 0);
+        uint32_t byte = 0xFF;
+        if (all != ~0ull) {
+          byte = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) byte |= (uint32_t)((all >> (8 * k)) & 1) << k;
+          for (int k = 0; k < 8; ++k) byte |= (uint32_t)((all >> (8 * k)) & 1) << k;
+        }
+        reinterpret_cast<uint8_t*>(&live[step & 3])[wave] = (uint8_t)byte;
+        const char* rp = static_cast<const char*>(a.rope) + (size_t)max(slot, 0) * (kRotDim * 2) + here(swap);
+        lds_load16(slot >= 0 ? rp : none, lds + rot_at + wave * 1024);
       }
-      reinterpret_cast<uint8_t*>(&live[step & 3])[wave] = (uint8_t)byte;
-      const char* rp = static_cast<const char*>(a.rope) + (size_t)max(slot, 0) * (kRotDim * 2) + here(16 * ((lane & 7) ^ ((my_row >> 1) & 7)));
-      lds_load16(slot >= 0 ? rp : none, lds + rot_at + wave * 1024);
     };
     auto base_of = [&](int k) {
       return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uintptr_t)mine, 8 * k) |
              (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)((uintptr_t)mine >> 32), 8 * k) << 32;
     };
-    auto load_codes = [&](int k) {
-      const char* p = static_cast<const char*>(a.latent) + (size_t)max(slot, 0) * kLatDim + here(16 * (lane & 7));
-      p = slot >= 0 ? p : none;
-      if (k == 0)
-        code_scale = *reinterpret_cast<const uint32_t*>(slot >= 0 ? reinterpret_cast<const char*>(a.scale) + (size_t)slot * 4 : none);
-      code[k] = *reinterpret_cast<const u32x4*>(p + 128 * k);
+    auto load_scales = [&] {
+      const char* sc = slot >= 0 ? reinterpret_cast<const char*>(a.scale) + (size_t)slot * 4 : none;
+      code_scale = *reinterpret_cast<const uint32_t*>(WHOLE ? sc + (uint32_t)here((lane >> 3) * 4) : sc);
     };
-    auto widen = [&](int step, int k) {
-      char* at = lds + (step & 3) * kLatBytes;
-      const int widen_at = here(my_row * 1024 + (((2 * (lane & 7)) ^ row_swap(my_row)) << 4));
-      const float sc = scale_value((int)((code_scale >> (8 * k)) & 0xFF));
+    auto load_codes = [&](int k) {
+      const char* p = slot >= 0 ? static_cast<const char*>(a.latent) + (size_t)slot * kLatDim : none;
+      const int at = here(WHOLE ? (lane >> 3) * kLatDim + 16 * (lane & 7) : 16 * (lane & 7));
+      code[k] = *reinterpret_cast<const u32x4*>(p + (uint32_t)at + 128 * k);
+    };
+    auto widen = [&](int step, int piece) {  // in eight pieces
       if constexpr (kCodes) {
-        u32x4 v[2];
+        const int k = piece >> 1, half = piece & 1;
+        const int at = here((step & 3) * kLatBytes + my_row * 1024 + (((2 * (lane & 7)) ^ row_swap(my_row)) << 4));
+        const float sc = scale_value((int)((code_scale >> (8 * k)) & 0xFF));
+        u32x4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i >> 1][2 * (i & 1)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, false));
-          v[i >> 1][2 * (i & 1) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][i], sc, true));
+        for (int i = 0; i < 2; ++i) {
+          v[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][2 * half + i], sc, false));
+          v[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code[k][2 * half + i], sc, true));
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4*>(at + (widen_at ^ (16 * i)) + 256 * k) = v[i];
+        *reinterpret_cast<u32x4*>(lds + (at ^ (16 * half)) + 256 * k) = v;
       }
     };
-    auto bring = [&](int step, int piece, int rot_at) {
-      if constexpr (kCodes) {
-        if (piece == 0) place(step), announce(step, rot_at);
-        else if (piece < 5) load_codes(piece - 1);
-      } else if (piece == 0) {
+    auto bring = [&](int step, auto piece, int rot_at) {
+      constexpr int P = decltype(piece)::value;
+      if constexpr (P == 0) {
         place(step);
+      } else if constexpr (P == 1) {
+        page = page_of(step + 1);
+      } else if constexpr (P == 2) {
         announce(step, rot_at);
-        mine = slot >= 0 ? static_cast<const char*>(a.latent) + (size_t)slot * (kLatDim * 2) : none;
-        base = base_of(0);
+      } else if constexpr (P == 3 && kCodes) {
+        load_scales();
+      } else if constexpr (P == 3) {
+        const char* at = slot >= 0 ? static_cast<const char*>(a.latent) + (size_t)slot * (kLatDim * 2) : none;
+        if constexpr (WHOLE) base = (uint64_t)at;
+        else mine = at, base = base_of(0);
+      } else if constexpr (kCodes) {
+        load_codes(P - 4);
       } else {
-        const int k = piece - 1, r = 8 * wave + k;
-        lds_load16(base, here((lane ^ ((2 * wave) & 3)) << 4) ^ (((k >> 2) << 4) | ((k & 3) << 6)),
-                   lds + (step & 3) * kLatBytes + r * 1024);
-        if (k < 7) base = base_of(k + 1);
+        constexpr int K = WHOLE ? 2 * P - 8 : P - 4;  // first row
+        const int swap = here((lane ^ ((2 * wave) & 3)) << 4) ^ ((K >> 2) << 4);
+        char* to = lds + (step & 3) * kLatBytes + (8 * wave + (WHOLE ? K & 4 : K)) * 1024;
+        if constexpr (WHOLE) {
+          lds_load_rows<(K & 3)>(base, swap ^ ((K & 3) << 6), swap ^ (((K + 1) & 3) << 6), to);
+          if (K == 2) base += 4 * kLatDim * 2;
+        } else {
+          lds_load16(base, swap ^ ((K & 3) << 6), to);
+          if (K < 7) base = base_of(K + 1);
+        }
       }
     };
 
@@ -503,13 +556,14 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       if (k == 0) mfma_score<FMT, true>(c, f[0], b);
       else mfma_score<FMT, false>(c, f[k % kAhead], b);
     };
-    auto val_product = [&](int i, int place) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) mfma_out<FMT>(o[i & 7][k], f[place % kAhead], w[i >> 3][k]);
-    };
+    auto val_product = [&](int i, int place, int k) { mfma_out<FMT>(o[i & 7][k], f[place % kAhead], w[i >> 3][k]); };
 
-    // The step's weights from its scores, in kWeigh pieces; the last two put them into LDS.
-    constexpr int kWeigh = 12;
+    // The step's weights from its scores, in kWeigh pieces.  A wave issues in
+    // order and has its SIMD alone, so a piece is what is issued while one product
+    // is worked on, and nothing stands next to what it needs: one piece has a
+    // pair's exponents, one the sum and rounding of the pair before and the
+    // products of the pair after the next.
+    constexpr int kWeigh = 23;
     float top = 0.0f, off = 0.0f;
     auto hide = [&](uint32_t see) {
       const uint32_t mine = see >> (4 * h);
@@ -520,13 +574,16 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     i32x4 p8[2];
     auto weigh = [&](int step, int piece) {
       if (piece == 0) {
-        top = c[0];
+        float t[4];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, c[e]);
+        for (int i = 0; i < 4; ++i) t[i] = fmaxf(c[i], c[4 + i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = fmaxf(fmaxf(t[i], c[8 + i]), c[12 + i]);
+        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       } else if (piece == 1) {
         top = across_halves(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
         const bool need = top > m + kGrow;
-        if (__any(need)) {
+        if (rare(__any(need))) {
           const float keep = need ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
           m = need ? top : m;
           l *= keep;
@@ -534,18 +591,29 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           moved[step & 1][wave] = step;
         }
         off = m == -__builtin_inff() ? 0.0f : m;
-      } else if (piece < 10) {
-        const int i = piece - 2;
-        typedef T x2 __attribute__((ext_vector_type(2)));
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(c[2 * i], a.scale_log2, -off));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(c[2 * i + 1], a.scale_log2, -off));
-        l += p0;
-        l += p1;
-        p8[i >> 2][i & 3] = __builtin_bit_cast(int, x2{(T)p0, (T)p1});
-      } else {
-        const int ks = piece - 10;
-        *reinterpret_cast<i32x4*>(lds + kPAt + (step & 1) * kPBytes + here((wave * 64 + lane) * 16) + ks * 4096) = p8[ks];
       }
+      auto scaled = [&](int i) {
+        c[2 * i] = fmaf(c[2 * i], a.scale_log2, -off);
+        c[2 * i + 1] = fmaf(c[2 * i + 1], a.scale_log2, -off);
+      };
+      if (piece == 3) scaled(0), scaled(1);
+      const int p = (piece - 4) >> 1;  // a pair
+      if (piece >= 4 && piece % 2 == 0 && p < 8) {
+        c[2 * p] = __builtin_amdgcn_exp2f(c[2 * p]);
+        c[2 * p + 1] = __builtin_amdgcn_exp2f(c[2 * p + 1]);
+      }
+      if (piece >= 5 && piece % 2 == 1) {
+        if (p + 2 < 8) scaled(p + 2);
+        if (p >= 1 && p < 9) {
+          const int i = p - 1;
+          typedef T x2 __attribute__((ext_vector_type(2)));
+          p8[i >> 2][i & 3] = __builtin_bit_cast(int, x2{(T)c[2 * i], (T)c[2 * i + 1]});
+          l += c[2 * i] + c[2 * i + 1];
+        }
+      }
+      if (piece == 14 || piece == 22)
+        *reinterpret_cast<i32x4*>(lds + kPAt + (step & 1) * kPBytes + here((wave * 64 + lane) * 16) + (piece == 22) * 4096) =
+            p8[piece == 22];
     };
     // the rows' sums so far follow a moved maximum
     auto follow = [&](int step, int mv0, int mv1) {
@@ -580,11 +648,15 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     // turn ends, and the barrier stands among the keys' products: behind it the
     // weights of step j - 1 are whole, step j + 2 may be brought where step j - 2
     // was, and what was brought in the turn before has landed.  Beside the values
-    // step j's weights are computed.  The order of issue is the source's: a piece
-    // of that work behind each product, its operand requested six products ahead.
-    constexpr int kBarrier = 6;  // after so many of the keys' products
-    constexpr int kApart = kCodes ? 5 : 6;  // products between two pieces of what is brought
-    static_assert(kBarrier + 2 + 4 * kApart < kKeys, "five pieces have a place beside the keys");
+    // step j's weights are computed.  The order of issue is the source's: behind
+    // each product about as much of that work as is issued in its 32 cycles.
+    // A step takes some 4150 cycles for 2176 of products, at 1.9 to 2.1 GHz: with
+    // fewer cycles (4270 before the work was cut so finely) the clock falls.
+    constexpr int kBarrier = 6;             // after so many of the keys' products
+    constexpr int kClear = kBarrier + 14;   // marks of moved maxima read by then, values not yet
+    constexpr int kApart = 3;               // products between two pieces of what is brought
+    constexpr int kBesideKeys = 8;          // so many pieces, the others beside the values
+    static_assert(kBarrier + 2 + (kBesideKeys - 1) * kApart < kKeys, "the pieces have a place beside the keys");
     int rot_now = kRotAt, rot_next = kRotAt + kRotBytes, rot_then = kRotAt + 2 * kRotBytes;
     auto landed = [&] {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -597,13 +669,15 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       mv1 = moved[j & 1][2 * rh + 1];
     };
     auto clear_of = [&](int j) {  // step j's values and the sums made ready for its weights
-      if (edge(j)) {
-        clean(j);
-        __syncthreads();
-      }
       mv0 = uniform(mv0);
       mv1 = uniform(mv1);
-      if ((mv0 == j || mv1 == j) && j > from) follow(j, mv0, mv1);  // the first step's sums are zeros
+      if (rare(edge(j) | (mv0 == j) | (mv1 == j))) {
+        if (edge(j)) {
+          clean(j);
+          __syncthreads();
+        }
+        if ((mv0 == j || mv1 == j) && j > from) follow(j, mv0, mv1);  // the first step's sums are zeros
+      }
     };
     auto apart = [&] {  // v_readlane's scalar and the load that it is the address of
       __builtin_amdgcn_sched_barrier(0);
@@ -618,9 +692,9 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     };
     auto turn = [&](int j, auto with_values) {
       constexpr bool VALUES = decltype(with_values)::value;
-      const int exists = live[j & 3];
-#pragma unroll
-      for (int k = 0; k < kKeys; ++k) {
+      const int exists = WHOLE ? -(int)((exist >> (j & 3)) & 1) : live[j & 3];
+      unrolled<kKeys>([&](auto at) {
+        constexpr int k = decltype(at)::value;
         key_product(k);
         if (k + kAhead < kKeys) fetch_key(k + kAhead);
         else if (VALUES) fetch_val(k + kAhead - kKeys, k + kAhead);
@@ -628,40 +702,47 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           landed();
           if (VALUES) moves(j - 1);
         }
-        if (VALUES && k == kBarrier + 1) clear_of(j - 1);
-        if (VALUES && k == kBarrier + 2) val_place(j - 1);
+        if (VALUES && k == kClear) clear_of(j - 1);
+        if (VALUES && k == kClear + 1) val_place(j - 1);
         if (VALUES && k == kKeys - 4) fetch_weights(j - 1, 0);
-        if (k >= kBarrier + 2 && (k - kBarrier - 2) % kApart == 0 && (k - kBarrier - 2) / kApart < 5)
-          bring(j + 2, (k - kBarrier - 2) / kApart, rot_then);
+        constexpr int from_barrier = k - kBarrier - 2;
+        if constexpr (from_barrier >= 0 && from_barrier % kApart == 0 && from_barrier / kApart < kBesideKeys)
+          bring(j + 2, std::integral_constant<int, from_barrier / kApart>{}, rot_then);
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
       uint32_t see = (uint32_t)uniform(exists);
-      if (edge(j)) see &= sees(a, s, token_of(here(32 * wave + l32)), (int64_t)j * kTilePos);
-      if constexpr (VALUES) val_product(0, kKeys);
+      if (rare(edge(j))) see &= sees(a, s, token_of(here(32 * wave + l32)), (int64_t)j * kTilePos);
+      if constexpr (VALUES) val_product(0, kKeys, 0), val_product(0, kKeys, 1);
       products_done();
-      if (__any(see != ~0u)) hide(see);
+      if (rare(__any(see != ~0u))) hide(see);
       key_place(j + 1, rot_next);
       if constexpr (VALUES) {
-#pragma unroll
-        for (int i = 0; i < kVals; ++i) {
-          if (i) val_product(i, kKeys + i);
+        unrolled<kVals>([&](auto at) {
+          constexpr int i = decltype(at)::value;
+          if (i) val_product(i, kKeys + i, 0);
+          weigh(j, 2 * i);
+          if (i >= kVals - 4) widen(j + 2, 2 * (i - (kVals - 4)));
+          __builtin_amdgcn_sched_barrier(0);
+          if (i) val_product(i, kKeys + i, 1);
           if (i + kAhead < kVals) fetch_val(i + kAhead, kKeys + i + kAhead);
           else fetch_key((kKeys + i) % kAhead);  // the register that this product has left
           if (i == 4) fetch_weights(j - 1, 1);
-          if (i < kWeigh) weigh(j, i);
-          else widen(j + 2, i - kWeigh);
-          if (!kCodes && i % 4 == 1) bring(j + 2, 5 + i / 4, rot_then);
+          weigh(j, 2 * i + 1);
+          if (i >= kVals - 4) widen(j + 2, 2 * (i - (kVals - 4)) + 1);
+          if constexpr (i % 4 == 1 && kBesideKeys + i / 4 < kBring)
+            bring(j + 2, std::integral_constant<int, kBesideKeys + i / 4>{}, rot_then);
           __builtin_amdgcn_sched_barrier(0);
-        }
-        static_assert(kWeigh + 4 == kVals, "all pieces have a place");
+        });
+        static_assert(kWeigh <= 2 * kVals, "all pieces have a place");
       } else {
 #pragma unroll
         for (int i = 0; i < kWeigh; ++i) weigh(j, i);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          widen(j + 2, i);
-          if (!kCodes) bring(j + 2, 5 + i, rot_then), apart();
-        }
+        for (int i = 0; i < 8; ++i) widen(j + 2, i);
+        unrolled<kBring - kBesideKeys>([&](auto i) {
+          bring(j + 2, std::integral_constant<int, kBesideKeys + decltype(i)::value>{}, rot_then);
+          apart();
+        });
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) fetch_key(k);
       }
@@ -672,13 +753,12 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     if (tid < 8) moved[tid >> 2][tid & 3] = -1;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int k = 0; k < kBring; ++k) {
+      unrolled<kBring>([&](auto k) {
         bring(from + t, k, t ? rot_next : rot_now);
         if constexpr (!kCodes) apart();
-      }
+      });
 #pragma unroll
-      for (int k = 0; k < 4; ++k) widen(from + t, k);
+      for (int k = 0; k < 8; ++k) widen(from + t, k);
     }
     // the queries are requested behind the first rows, which take longer
     {
@@ -717,7 +797,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kVals; ++i) {
-        val_product(i, i);
+        val_product(i, i, 0), val_product(i, i, 1);
         if (i + kAhead < kVals) fetch_val(i + kAhead, i + kAhead);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -787,13 +867,12 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
           __syncthreads();
         }
         if (j == to) break;
-#pragma unroll
-        for (int k = 0; k < kBring; ++k) {
+        unrolled<kBring>([&](auto k) {
           bring(j + 2, k, rot_then);
           apart();
-        }
+        });
 #pragma unroll
-        for (int k = 0; k < 4; ++k) widen(j + 2, k);
+        for (int k = 0; k < 8; ++k) widen(j + 2, k);
         next_rot();
       }
       __syncthreads();  // and those of the results
@@ -934,7 +1013,8 @@ void join_parts(const MlaTreeArgs& a, int groups, hipStream_t s) {
 template <int FMT>
 void launch_fmt(const MlaTreeArgs& a, hipStream_t s) {
   const int groups = mla_tree_groups();
-  k_mla_tree<FMT><<<groups, 256, 0, s>>>(a);
+  if ((1 << a.page_shift) >= kTilePos) k_mla_tree<FMT, true><<<groups, 256, 0, s>>>(a);
+  else k_mla_tree<FMT, false><<<groups, 256, 0, s>>>(a);
   join_parts<FMT, kTileRows>(a, groups, s);
 }
 }  // namespace
