@@ -451,6 +451,11 @@ def kv_cache(format, n_pages, page_size=64):
     return KvCache(codes, rope_plane, torch.zeros(*lead, 4, dtype=torch.uint8, device=dev).view(torch.float8_e8m0fnu))
 
 
+def _on_cache_device(fn, cache):
+    if _device is not None and cache.device != _device:
+        _refuse(fn, f"the cache is on device {cache.device}, the library on device {_device}")
+
+
 def _rows(fn, name, t, T):
     if t.shape != (T, _lib.KV_LATENT + _lib.KV_ROPE) or t.stride(1) != 1:
         _refuse(fn, f"{name}: [{T}, {_lib.KV_LATENT + _lib.KV_ROPE}] with contiguous rows is wanted, got {tuple(t.shape)}")
@@ -469,6 +474,7 @@ def kv_write(cache, kv, slots, norm_w=None, table=None, pos=None, stream=None):
         pos = None
     elif pos is None:
         _refuse("kv_write", "a rotation needs positions")
+    _on_cache_device("kv_write", cache)
     _on_device("kv_write", kv, slots, norm_w, pos)
     call("fdm_kv_write", ctypes.byref(cache.desc), kv.data_ptr(), _elem("kv_write", "kv", kv.dtype), kv.stride(0),
          None if norm_w is None else _vector("kv_write", "norm_w", norm_w, _lib.KV_LATENT, _f32),
@@ -482,6 +488,7 @@ def kv_read(cache, slots, out, stream=None):
     _rows("kv_read", "out", out, T)
     if not _types:
         _load_types()
+    _on_cache_device("kv_read", cache)
     _on_device("kv_read", slots, out)
     call("fdm_kv_read", ctypes.byref(cache.desc), _vector("kv_read", "slots", slots, T, _i32), T, out.data_ptr(),
          _elem("kv_read", "out", out.dtype), out.stride(0), _call_stream(stream))
@@ -495,8 +502,7 @@ def mla_workspace(N, H):
     return torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", _device or 0))
 
 
-def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=None, lse=None, workspace=None, max_kv=0,
-               stream=None):
+def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=None, lse=None, workspace=None, stream=None):
     """Latent attention of B sequences' query tokens over the paged cache.
 
     q_lat [N, H, 512] (the absorbed queries) and q_rope [N, H, 64]; sequence b has
@@ -506,7 +512,7 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
     of its mask (int64 [N, words], bit d: the sequence's token d) or, without
     one, those up to itself.  out [N, H, 512] = sum of softmax(scale q k) latent;
     lse (float32 [N, H]) the log of the sums.  workspace: mla_workspace's (None:
-    allocated for the call).  max_kv: the longest kv_len to expect, if known."""
+    allocated for the call)."""
     fn = "mla_attend"
     if q_lat.dim() != 3 or q_lat.shape[2] != _lib.KV_LATENT:
         _refuse(fn, f"q_lat: [N, H, {_lib.KV_LATENT}] is wanted, got {tuple(q_lat.shape)}")
@@ -525,6 +531,7 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
         _refuse(fn, f"pages: [{B}, P] is wanted, got {tuple(pages.shape)}")
     if not _types:
         _load_types()
+    _on_cache_device(fn, cache)
     _on_device(fn, q_lat, q_rope, q_start, kv_len, pages, out, mask, lse, workspace)
     words = 0
     if mask is not None:
@@ -537,7 +544,7 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
             _refuse(fn, f"lse: {(N, H)} is wanted, got {tuple(lse.shape)}")
         lse = _vector(fn, "lse", lse, N * H, _f32)
     batch = _lib.MlaBatch(B, N, H, _vector(fn, "q_start", q_start, B + 1, _i32), _vector(fn, "kv_len", kv_len, B, _i32),
-                          _vector(fn, "pages", pages, pages.numel(), _i32), pages.shape[1], max_kv, mask, words)
+                          _vector(fn, "pages", pages, pages.numel(), _i32), pages.shape[1], mask, words)
     handle = _call_stream(stream)
     if workspace is None:  # torch's allocator keeps it for the stream that it is made on
         import torch

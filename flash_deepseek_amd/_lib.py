@@ -69,7 +69,7 @@ class MlaBatch(ctypes.Structure):
     """struct fdm_mla_batch."""
     _fields_ = [("B", ctypes.c_int), ("N", ctypes.c_int), ("H", ctypes.c_int), ("q_start", ctypes.c_void_p),
                 ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("pages_stride", ctypes.c_int),
-                ("max_kv", ctypes.c_int), ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_int)]
+                ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_int)]
 
 
 EXPERT_Q4K_BYTES = 24772608

@@ -2461,7 +2461,7 @@ int fdm_kv_write(const fdm_kv_cache* c, const void* d_x, int x_type, int64_t x_s
   KvWriteArgs a{};
   ElemType t;
   if (int rc = elem_type(x_type, &t, "x")) return rc;
-  if (T < 0) return fail(FDM_E_INVAL, "T=%d", T);
+  if (T < 0 || T > FDM_KV_MAX_ROWS) return fail(FDM_E_INVAL, "T=%d: 0 .. %d", T, FDM_KV_MAX_ROWS);
   if (table) {
     if (int rc = check_table(table)) return rc;
     if (table->dim != FDM_KV_ROPE) return fail(FDM_E_INVAL, "rope table of dim %d: the cache's rows have %d", table->dim, FDM_KV_ROPE);
@@ -2503,7 +2503,7 @@ int fdm_kv_read(const fdm_kv_cache* c, const int32_t* d_slots, int T, void* d_y,
   if (int rc = check_cache(c)) return rc;
   ElemType t;
   if (int rc = elem_type(y_type, &t, "y")) return rc;
-  if (T < 0) return fail(FDM_E_INVAL, "T=%d", T);
+  if (T < 0 || T > FDM_KV_MAX_ROWS) return fail(FDM_E_INVAL, "T=%d: 0 .. %d", T, FDM_KV_MAX_ROWS);
   if (T == 0) return check_ready();
   if (!d_y || !d_slots) return fail(FDM_E_INVAL, "null pointer");
   if (!aligned(d_y, elem_size(t)) || !aligned(d_slots, 4)) return fail(FDM_E_INVAL, "misaligned pointer");
@@ -2549,7 +2549,6 @@ int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_
   if (int rc = check_mla_shape(b->N, b->H)) return rc;
   if (b->B < 1 || b->B > FDM_MLA_MAX_SEQS) return fail(FDM_E_INVAL, "%d sequences: 1 .. %d", b->B, FDM_MLA_MAX_SEQS);
   if (b->pages_stride < 1) return fail(FDM_E_INVAL, "pages_stride %d", b->pages_stride);
-  if (b->max_kv < 0) return fail(FDM_E_INVAL, "max_kv %d", b->max_kv);
   if (b->d_mask ? b->mask_words < 1 : b->mask_words != 0) return fail(FDM_E_INVAL, "mask_words %d", b->mask_words);
   if (!(scale > 0.0f) || !isfinite(scale)) return fail(FDM_E_INVAL, "scale %g: above 0", (double)scale);
   if (b->N == 0) return check_ready();

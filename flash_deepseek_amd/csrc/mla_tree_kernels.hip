@@ -225,24 +225,55 @@ __device__ __forceinline__ int tile_units(const SeqWork& s, int tile, int H, boo
   return tile_steps<R, S>(s, tile, H, in_order) + kTileCost;
 }
 // ceil(1 / S) + .. + ceil(x / S)
-template <int S>
-__device__ __forceinline__ int64_t step_sum(int64_t x) {
+__device__ __forceinline__ int64_t step_sum(int64_t x, int S) {
   const int64_t q = x / S, r = x % S;
-  return S * q * (q + 1) / 2 + r * (q + 1);
+  return S * (q * (q + 1) / 2) + r * (q + 1);
+}
+// Whether the sequence's tiles are of one size or grow by k = R / H whole
+// tokens that divide a step: their units have a sum in closed form.
+template <int R, int S>
+__device__ __forceinline__ bool even_tiles(const SeqWork& s, int H, bool in_order) {
+  return !in_order || s.n <= 1 || (s.len >= s.n && R % H == 0 && S % (R / H) == 0);
 }
 // units of the sequence's tiles 0 .. tiles - 1
 template <int R, int S>
 __device__ int64_t units_before(const SeqWork& s, int tiles, int H, bool in_order) {
   if (!in_order || s.n <= 1) return (int64_t)tiles * tile_units<R, S>(s, 0, H, in_order);
-  if (H % R == 0 && s.len >= s.n) {  // whole tiles of one token
-    const int q = H / R, tokens = tiles / q;
-    const int64_t before = s.len - s.n;
-    return q * (step_sum<S>(before + tokens) - step_sum<S>(before)) +
-           (int64_t)(tiles % q) * ((before + tokens + 1 + S - 1) / S) + (int64_t)tiles * kTileCost;
-  }
   int64_t sum = 0;
+  if (even_tiles<R, S>(s, H, in_order)) {
+    // sum of ceil((p + k i) / S), p positions before the tokens: with p in whole
+    // k, rounded up, the same as ceil((p / k + i) / (S / k))
+    const int k = R / H, per = S / k, whole = min(tiles, s.n / k);
+    const int64_t p = ((int64_t)(s.len - s.n) + k - 1) / k;
+    sum = step_sum(p + whole, per) - step_sum(p, per);
+    if (tiles > whole) sum += (s.len + S - 1) / S;  // the last, of fewer tokens
+    return sum + (int64_t)tiles * kTileCost;
+  }
   for (int i = 0; i < tiles; ++i) sum += tile_units<R, S>(s, i, H, in_order);
   return sum;
+}
+// The last tile that starts at or before unit u of the sequence, and its start.
+template <int R, int S>
+__device__ int tile_at(const SeqWork& s, int64_t u, int H, bool in_order, int64_t& start) {
+  const int tiles = tiles_of<R>(s, H);
+  int tile = 0;
+  start = 0;
+  if (even_tiles<R, S>(s, H, in_order)) {
+    int hi = tiles - 1;
+    while (tile < hi) {
+      const int mid = (tile + hi + 1) / 2;
+      if (units_before<R, S>(s, mid, H, in_order) <= u) tile = mid;
+      else hi = mid - 1;
+    }
+    start = units_before<R, S>(s, tile, H, in_order);
+  } else {
+    for (; tile < tiles - 1; ++tile) {
+      const int64_t next = start + tile_units<R, S>(s, tile, H, in_order);
+      if (next > u) break;
+      start = next;
+    }
+  }
+  return tile;
 }
 
 // Units before each sequence into before[0 .. B], two sequences a thread of
@@ -286,9 +317,8 @@ __device__ __forceinline__ void count_units(const MlaTreeArgs& a, uint32_t* befo
 struct Range {
   uint32_t u, end;      // next unit, end
   int group;            // number of the range
-  int b, tile, steps;   // sequence and tile of the part; all steps of the tile
-  int from, to;         // steps of the part
-  int parts;            // workgroups that have steps of the tile
+  int b, tile;          // sequence and tile of the part
+  int from, to;         // steps of the part; it ends before unit u
   SeqWork s;
 };
 // Ranges of two units at least: a part of one step is 256 KB of sums for 36 KB
@@ -322,30 +352,22 @@ __device__ __forceinline__ bool next_part(const MlaTreeArgs& a, const uint32_t* 
     r.s = seq_work(a, r.b);
     r.s = {uniform(r.s.n), uniform(r.s.len), uniform(r.s.t0)};
     const int64_t seq_u = (uint32_t)uniform((int)before[r.b]);
-    r.tile = 0;
-    {  // the last tile that starts at or before u
-      int hi = tiles_of<R>(r.s, a.H) - 1;
-      while (r.tile < hi) {
-        const int mid = (r.tile + hi + 1) / 2;
-        if (seq_u + units_before<R, S>(r.s, mid, a.H, in_order) <= r.u) r.tile = mid;
-        else hi = mid - 1;
-      }
-    }
-    const int64_t tile_u = seq_u + units_before<R, S>(r.s, r.tile, a.H, in_order) + kTileCost;  // its first step
-    r.steps = tile_steps<R, S>(r.s, r.tile, a.H, in_order);
+    int64_t start;
+    r.tile = uniform(tile_at<R, S>(r.s, r.u - seq_u, a.H, in_order, start));
+    const int64_t tile_u = uniform(seq_u + start) + kTileCost;  // its first step
     r.from = (int)max((int64_t)r.u - tile_u, (int64_t)0);
-    r.to = (int)min((int64_t)r.steps, (int64_t)r.end - tile_u);
-    if (r.to > r.from) {
-      r.u = (uint32_t)(tile_u + r.to);
-      const uint32_t total = (uint32_t)uniform((int)before[a.B]), groups = range_count(total);
-      auto range_at = [&](uint64_t u) { return (int)(((u + 1) * groups - 1) / total); };
-      r.parts = uniform(range_at(tile_u + r.steps - 1) - range_at(tile_u) + 1);
-      return true;
-    }
+    r.to = (int)min((int64_t)tile_steps<R, S>(r.s, r.tile, a.H, in_order), (int64_t)r.end - tile_u);
     if (r.to <= 0) break;  // the range ends before the tile's first step
     r.u = (uint32_t)(tile_u + r.to);
+    if (r.to > r.from) return true;
   }
   return false;
+}
+// Workgroups that have steps of the part's tile of so many steps.
+__device__ __forceinline__ int parts_of(const MlaTreeArgs& a, const uint32_t* before, const Range& r, int steps) {
+  const uint32_t total = before[a.B], groups = range_count(total), first = r.u - r.to;
+  auto range_at = [&](uint64_t u) { return (int)(((u + 1) * groups - 1) / total); };
+  return range_at((uint64_t)first + steps - 1) - range_at(first) + 1;
 }
 
 // Which of the positions j0 .. j0 + 31 the sequence's token `place` sees (bits).
@@ -390,12 +412,12 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   Range range = range_of(a, before);
   const int group = range.group;
   const Space space = space_of(a.workspace, gridDim.x);
-  JoinDesc desc = {0, 0, 0, 0};
+  if (tid == 0) space.desc[group] = {0, 0, 0, 0};  // unless it begins a tile that others go on with
 
   while (next_part<kTileRows, kTilePos>(a, before, range)) {
     const SeqWork s = range.s;
     const int from = range.from, to = range.to, len = s.len;
-    const int prefix = len - s.n;  // may be negative
+    const int first_edge = max(len - s.n, 0) / kTilePos;  // from this step on not all tokens see all positions
     const int row0 = kTileRows * range.tile, rows = min(kTileRows, s.n * a.H - row0);
 
     // The lane's scores are those of row 32 wave + l32.  What is needed of it is
@@ -662,7 +684,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __syncthreads();
     };
-    auto edge = [&](int j) { return (int64_t)(j + 1) * kTilePos > prefix; };  // not all tokens see all of step j
+    auto edge = [&](int j) { return j >= first_edge; };
     int mv0 = -1, mv1 = -1;
     auto moves = [&](int j) {
       mv0 = moved[j & 1][2 * rh];
@@ -812,7 +834,8 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
         stat[kTileRows + 32 * wave + l32] = l;
       }
       __syncthreads();
-      if (from == 0 && to == range.steps) {
+      const int steps = tile_steps<kTileRows, kTilePos>(s, range.tile, a.H, a.mask == nullptr);
+      if (from == 0 && to == steps) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int r = 64 * rh + 32 * k + l32;
@@ -841,7 +864,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       } else {
         // the range's first tile may have begun in the workgroup before; its last goes on in the next
         const int part = 2 * group + (from == 0 ? 1 : 0);
-        if (from == 0) desc = {range.b, range.tile, range.parts, 0};
+        if (from == 0 && tid == 0) space.desc[group] = {range.b, range.tile, parts_of(a, before, range, steps), 0};
         if (tid < kTileRows) space.stat[(size_t)part * kTileRows + tid] = make_float2(stat[tid], stat[kTileRows + tid]);
         f32x4* to_part = reinterpret_cast<f32x4*>(space.part + (size_t)part * kPartFloats) + (2 * rh * 16 + 8 * dh) * 256 + lane;
 #pragma unroll
@@ -879,7 +902,6 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       __syncthreads();
     }
   }
-  if (tid == 0) space.desc[group] = desc;
 }
 
 // A tile's parts put together: M = max m, out = sum 2^(m - M) part / sum 2^(m - M) l.

@@ -495,6 +495,7 @@ int fdm_rope(const fdm_rope_table *table, const int32_t *d_pos, int T, int H, in
  * row of y as it was. */
 #define FDM_KV_LATENT 512
 #define FDM_KV_ROPE 64
+#define FDM_KV_MAX_ROWS 33554432 /* of one call */
 #define FDM_KV_F16 0
 #define FDM_KV_BF16 1
 #define FDM_KV_FP8 2
@@ -529,8 +530,7 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
  * else BF16; strides in elements, multiples of 8, 16-byte aligned.  lse
  * (optional) fp32 [N][H].  Products of the 16-bit values accumulate in fp32 and
  * softmax weights round to 16 bits before the second product.  1 <= H <=
- * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS, N <= FDM_MLA_MAX_TOKENS.  max_kv: the longest kv_len the
- * caller expects (0: unknown); it only chooses among kernels.
+ * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS, N <= FDM_MLA_MAX_TOKENS.
  * d_workspace: at least fdm_mla_workspace(N, H) bytes, 256-byte aligned, used
  * by the call alone until it has run on its stream: calls that may overlap, and
  * graphs that may run at once, need one each.  The call allocates nothing and
@@ -544,7 +544,6 @@ typedef struct fdm_mla_batch {
   const int32_t *d_kv_len;   /* [B]              */
   const int32_t *d_pages;    /* [B][pages_stride] */
   int pages_stride;
-  int max_kv;
   const uint64_t *d_mask;    /* [N][mask_words], or NULL */
   int mask_words;
 } fdm_mla_batch;

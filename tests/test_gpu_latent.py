@@ -476,17 +476,28 @@ def test_attend_streams_and_graph(fdm):
         turned.zero_()
 
 
-def test_attend_is_repeatable_and_takes_no_heed_of_max_kv(fdm):
+def test_attend_is_repeatable(fdm):
     g = rng(43)
     cache, rows = filled(fdm, "bf16", 40, 64, g)
     pages = torch.arange(40).reshape(1, 40).tolist()
     q = queries(g, "bf16", 1, 128)
     say("mla_attend repeated")
     first = run_attend(fdm, cache, rows, 64, *q, [0, 1], [2500], pages)
-    for max_kv in (0, 1, 2500, 1 << 30):
-        out, lse = run_attend(fdm, cache, rows, 64, *q, [0, 1], [2500], pages, max_kv=max_kv)
-        if max_kv == 0:
-            assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+    again = run_attend(fdm, cache, rows, 64, *q, [0, 1], [2500], pages)
+    assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+
+
+@pytest.mark.parametrize("H,counts,extra", [(128, [37, 2], 70), (64, [81, 3], 31), (32, [150, 1], 5), (16, [300, 9], 33), (8, [200, 17], 64),
+                                            (4, [333, 33], 1), (2, [400, 65], 40), (1, [300, 129], 0), (40, [90, 7], 50), (127, [25, 3], 64)])
+def test_attend_prompts(fdm, H, counts, extra):
+    """Many tokens in order, so that the tiles of one sequence differ in length and are found by their units, for heads that divide a tile and not."""
+    g = rng(91 + H)
+    page, lens = 32, [counts[0] + extra, counts[1] + 3 * extra]
+    per = -(-max(lens) // page)
+    cache, rows = filled(fdm, "bf16", 2 * per, page, g)
+    pages = torch.randperm(2 * per, generator=g).reshape(2, per).tolist()
+    say(f"mla_attend prompts H={H} {counts} {lens}")
+    run_attend(fdm, cache, rows, page, *queries(g, "bf16", sum(counts), H), [0, counts[0], sum(counts)], lens, pages)
 
 
 def test_refusals(fdm):
@@ -530,7 +541,6 @@ def test_refusals(fdm):
         lambda: fdm.mla_attend(cache, q, r, *a, 1.0, o, lse=cuda(2, 3)),
         lambda: fdm.mla_attend(cache, q, r, *a, 1.0, o, workspace=cuda(8, dtype=torch.uint8)),
         lambda: fdm.mla_attend(cache, q, r, *a, 1.0, o[:, :1].expand(2, 4, 512)),
-        lambda: fdm.mla_attend(cache, q, r, *a, 1.0, o, max_kv=-1),
         lambda: fdm.mla_attend(cache, cuda(2, 129, 512, dtype=torch.bfloat16), cuda(2, 129, 64, dtype=torch.bfloat16), *a, 1.0,
                                cuda(2, 129, 512, dtype=torch.bfloat16)),
     ):

@@ -82,15 +82,15 @@ def test_cache_refusals(bad):
 
 def test_write_and_read_refusals():
     t = ctypes.byref(table()[1])
-    for bad in (dict(x=None), dict(slots=None), dict(xt=12), dict(T=-1), dict(x=P + 1), dict(slots=P + 2), dict(t=t), dict(w=P + 2),
+    for bad in (dict(x=None), dict(slots=None), dict(xt=12), dict(T=-1), dict(T=(1 << 25) + 1), dict(x=P + 1), dict(slots=P + 2), dict(t=t), dict(w=P + 2),
                 dict(t=t, pos=P + 2), dict(t=ctypes.byref(table(32)[1]), pos=P)):
         assert write(**bad) == INVAL, bad
-    for bad in (dict(y=None), dict(slots=None), dict(yt=12), dict(T=-1), dict(y=P + 2), dict(stride=575), dict(stride=0)):
+    for bad in (dict(y=None), dict(slots=None), dict(yt=12), dict(T=-1), dict(T=(1 << 25) + 1), dict(y=P + 2), dict(stride=575), dict(stride=0)):
         assert read(**bad) == INVAL, bad
     assert _lib.lib.fdm_kv_write(None, P, 0, 576, None, None, None, P, 2, None) == INVAL
 
 
-BATCH = dict(B=2, N=3, H=4, q_start=P, kv_len=P, pages=P, pages_stride=4, max_kv=0, mask=None, mask_words=0)
+BATCH = dict(B=2, N=3, H=4, q_start=P, kv_len=P, pages=P, pages_stride=4, mask=None, mask_words=0)
 CALL = dict(ql=P, ql0=2048, ql1=512, qr=P, qr0=256, qr1=64, scale=0.1, out=2 * P, o0=2048, o1=512, lse=None, ws=P, size=1 << 40, stream=None)
 
 
@@ -99,7 +99,7 @@ def attend(c=None, **kw):
     return _lib.lib.fdm_mla_attend(cache() if c is None else c, ctypes.byref(batch), *{**CALL, **kw}.values())
 
 
-@pytest.mark.parametrize("bad", [dict(B=0), dict(B=513), dict(N=-1), dict(N=(1 << 20) + 1), dict(H=0), dict(H=129), dict(pages_stride=0), dict(max_kv=-1),
+@pytest.mark.parametrize("bad", [dict(B=0), dict(B=513), dict(N=-1), dict(N=(1 << 20) + 1), dict(H=0), dict(H=129), dict(pages_stride=0),
                                  dict(mask=P), dict(mask_words=1), dict(mask=P, mask_words=-1), dict(mask=P + 4, mask_words=1),
                                  dict(q_start=None), dict(kv_len=None), dict(pages=None), dict(ql=None), dict(qr=None), dict(out=None),
                                  dict(ws=None), dict(ws=P + 128), dict(ql=P + 8), dict(qr=P + 8), dict(out=P + 8), dict(ql0=2052),
@@ -118,3 +118,20 @@ def test_good_arguments_get_as_far_as_the_device():
     assert _lib.lib.fdm_mla_workspace(4, 128, ctypes.byref(ctypes.c_size_t())) == STATE
     assert _lib.lib.fdm_mla_workspace(4, 129, ctypes.byref(ctypes.c_size_t())) == INVAL
     assert copy.copy(table()[1]).dim == 64
+
+
+def test_a_cache_of_another_device(monkeypatch):
+    """The planes' device is the one that they were given with, whatever the library's is now."""
+    import types
+
+    import torch
+
+    import flash_deepseek_amd as fdm
+    elsewhere = types.SimpleNamespace(device=1, half=torch.bfloat16)
+    monkeypatch.setattr(fdm, "_device", 0)
+    x, q, r = torch.zeros(2, 576), torch.zeros(2, 4, 512, dtype=torch.bfloat16), torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: fdm.kv_write(elsewhere, x, i), lambda: fdm.kv_read(elsewhere, i, x),
+                 lambda: fdm.mla_attend(elsewhere, q, r, i, i[:1], i[None], 1.0, q)):
+        with pytest.raises(fdm.FdmError, match="the cache is on device 1"):
+            call()
