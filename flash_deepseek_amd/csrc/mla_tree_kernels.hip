@@ -11,7 +11,15 @@
 // the rows of two matrix products with the cached rows, 1088 products a pair
 // and position: 242 flops a byte of a BF16 cache with 128 heads, about what
 // separates the matrix cores from HBM.  A workgroup takes 128 such rows (one
-// token of 128 heads, eight of 16) and walks a range of positions, 32 at a time.
+// token of 128 heads, eight of 16), four waves that each have a SIMD and its 512
+// registers to themselves: 256 of them hold 64 rows x 256 of the result's dims,
+// 144 the queries of 32 rows, so that of each step of 32 positions only the cached
+// rows move, once into LDS and from there as either product's operand.
+// The bound is what a single wave issues around its products (a step takes 4150
+// cycles, 2176 of them products) and, as soon as that is better, the power: the
+// clock falls from 2.4 to 1.9 GHz.  512 tokens of 128 heads over 4608 positions
+// 585 to 620 us with the card, 1.0 to 1.06 PFLOP/s, where a library product of
+// 8192^3 reaches 1.21.
 #include "latent_device.h"
 
 namespace fdm {
@@ -427,37 +435,36 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     // pieces of work.  16-bit rows go straight into LDS.  FP8 codes go into
     // registers, eight lanes a row, and from there in the same turn as 16-bit
     // values (exact) into LDS.  A row that is none reads zeros.
-    // WHOLE: all rows of a step lie in one page (pages of 32 and more).  Where
-    // they are is known to all lanes, and a piece is two rows; positions behind
+    // WHOLE: a wave's eight rows lie in one page (pages of 8 and more).  Where
+    // they are is known to all its lanes, and a piece is two rows; positions behind
     // the sequence's end are read as they are, and hidden.  Otherwise a lane
-    // looks after the row that it is one of eight of, and a piece is one row,
-    // which costs 85 of 640 instructions more a step: 512 tokens of 128 heads over
-    // 4608 positions 636 us against 615, 32 sequences of 16 over 16384 1333 against 1283.
+    // looks after the row that it is one of eight of, and a piece is one row: 85
+    // instructions more a step, 74 us against 69 for 128 sequences of three tokens
+    // of 16 heads over 2048 positions, 635 against 621 for 512 tokens of 128 over 4608.
     constexpr bool kCodes = FMT == kKvFp8;
     constexpr int kBring = kCodes || WHOLE ? 8 : 12;
     const int my_row = 8 * wave + (lane >> 3);
     const int* pages = a.pages + (size_t)range.b * a.pages_stride;
     const char* none = reinterpret_cast<const char*>(zero_row);
     int page;                // of the next step to be placed (this lane's row)
-    int slot = 0;            // the step placed last: this lane's row, WHOLE: the wave's first; -1: none
-    uint32_t exist = 0;      // WHOLE: bit step & 3
+    int slot = 0;            // the step placed last: this lane's row (WHOLE: the wave's first); -1: none
     const char* mine;        // 16 bits: that row
     uint64_t base;           //   the row that the next piece brings
     u32x4 code[4];           // FP8: that row's codes (16 of each group) and scales
     uint32_t code_scale = 0;
     auto page_of = [&](int step) {
-      return pages[min(step * kTilePos + (WHOLE ? 0 : my_row), max(len - 1, 0)) >> a.page_shift];
+      return pages[min(step * kTilePos + (WHOLE ? 8 * wave : my_row), max(len - 1, 0)) >> a.page_shift];
     };
     auto place = [&](int step) {
-      const int j = step * kTilePos + (WHOLE ? 0 : my_row);
+      const int j = step * kTilePos + (WHOLE ? 8 * wave : my_row);
       const int at = WHOLE ? uniform(page) : page;
       const bool is = (unsigned)at < (unsigned)a.n_pages & j < len & step < to;
-      slot = is ? (at << a.page_shift) + (j & ((1 << a.page_shift) - 1)) + (WHOLE ? 8 * wave : 0) : -1;
-      if constexpr (WHOLE) exist = (exist & ~(1u << (step & 3))) | (uint32_t)is << (step & 3);
+      slot = is ? (at << a.page_shift) + (j & ((1 << a.page_shift) - 1)) : -1;
     };
     auto announce = [&](int step, int rot_at) {  // which rows exist, and their rotary parts
       const int swap = 16 * ((lane & 7) ^ ((my_row >> 1) & 7));
       if constexpr (WHOLE) {
+        reinterpret_cast<uint8_t*>(&live[step & 3])[wave] = (uint8_t)(slot >= 0 ? 0xFF : 0);
         const char* rp = slot >= 0 ? static_cast<const char*>(a.rope) + (size_t)slot * (kRotDim * 2) : none;
         lds_load16((uint64_t)rp, here((lane >> 3) * (kRotDim * 2) + swap), lds + rot_at + wave * 1024);
       } else {
@@ -714,7 +721,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     };
     auto turn = [&](int j, auto with_values) {
       constexpr bool VALUES = decltype(with_values)::value;
-      const int exists = WHOLE ? -(int)((exist >> (j & 3)) & 1) : live[j & 3];
+      const int exists = live[j & 3];
       unrolled<kKeys>([&](auto at) {
         constexpr int k = decltype(at)::value;
         key_product(k);
@@ -1035,7 +1042,7 @@ void join_parts(const MlaTreeArgs& a, int groups, hipStream_t s) {
 template <int FMT>
 void launch_fmt(const MlaTreeArgs& a, hipStream_t s) {
   const int groups = mla_tree_groups();
-  if ((1 << a.page_shift) >= kTilePos) k_mla_tree<FMT, true><<<groups, 256, 0, s>>>(a);
+  if (a.page_shift >= 3) k_mla_tree<FMT, true><<<groups, 256, 0, s>>>(a);
   else k_mla_tree<FMT, false><<<groups, 256, 0, s>>>(a);
   join_parts<FMT, kTileRows>(a, groups, s);
 }
