@@ -24,6 +24,10 @@ __device__ __forceinline__ float wave_sum(float v) {
 // power-of-two scale of fp8_scale_byte, n 2^-e rounded to e4m3; r in bf16.
 // Power-of-two scales make n 2^-e and what is read back exact: the code is
 // the only rounding.
+// One wave a row, so that the norm's sum and a group's maximum stay in registers
+// and need no barrier, four rows a workgroup.  Bound by memory: 32768 fp32 rows
+// into BF16 23.9 us a call, 113 MB at 4.75 TB/s; 64 rows are 4 us of kernel (load,
+// sum, rotation, store one after the other) and the host's 6 us a call.
 template <typename TX, int FMT>
 __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
   const int lane = threadIdx.x & 63;
@@ -98,7 +102,8 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
 
 // The row's values, widened: code 2^e and the rotary part, rounded once to
 // the output's type.  Rows whose slot is none of the cache's are left as they
-// were.
+// were.  Bound by memory: 16384 FP8 rows into BF16 6.6 us, 29.5 MB at 4.4 TB/s;
+// 1000 rows are 2.9 us of kernel and the host's 5.5 us a call.
 template <typename TY, int FMT>
 __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
   const int lane = threadIdx.x & 63;

@@ -12,6 +12,9 @@ namespace fdm {
 // consecutive values (two runs of eight, R / 2 apart, for rotated ones in the
 // half layout), so a 16-bit head moves by 16-byte accesses.  Values that pass
 // through are items too, unless the call is in place.
+// Bound by memory: 4097 tokens of 64 x 128 BF16 values 27.5 us a call, 134 MB
+// at 4.9 TB/s, where a large copy reaches 5.1.  A step of 16 tokens is 3 us of
+// kernel and the host's 6 us a call.
 template <typename TX, typename TY, bool HALF, int N>
 __global__ __launch_bounds__(256) void k_rope(RopeArgs a, RopeTurns<N> table) {
   extern __shared__ float2 sc[];  // [tpw][R / 2] (sine, cosine)
