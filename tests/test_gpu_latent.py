@@ -376,6 +376,32 @@ def test_attend_empty_rows_and_unseen_values(fdm):
     assert torch.equal(got[2].cpu(), cache.latent.view(-1, 512)[0].cpu().expand(H, 512))  # sees position 0 alone
 
 
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "fp8"])
+@pytest.mark.parametrize("page", [1, 4, 8, 16, 32, 128])
+def test_attend_among_rows_that_are_no_numbers(fdm, fmt, page):
+    """Every row that belongs to no position of a sequence is NaN, the workspace full of ones."""
+    g = rng(1000 + page)
+    lens, counts = [1, 7, 33, 64, 95, 161], [1, 2, 1, 5, 3, 1]
+    per = -(-max(lens) // page) + 1
+    n_pages = len(lens) * per
+    cache, _ = filled(fdm, fmt, n_pages, page, g)
+    pages = torch.randperm(n_pages, generator=g).reshape(len(lens), per)
+    used = torch.zeros(n_pages * page, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        j = torch.arange(n)
+        used[pages[b, j // page] * page + j % page] = True
+    for plane, none in ((cache.latent, 0x7F if fmt == "fp8" else 0xFF), (cache.rope, 0xFF), (cache.scale, 0xFF)):
+        if plane is not None:
+            raw = plane.view(torch.uint8)
+            raw.view(n_pages * page, -1)[~used.cuda()] = none
+    rows = C.widened(*planes(cache))
+    assert rows[~used].isnan().all() and rows[used].isfinite().all()
+    workspace = fdm.mla_workspace(sum(counts), 16).fill_(0xFF)
+    start = [0] + np.cumsum(counts).tolist()
+    say(f"mla_attend {fmt} page={page} among NaN")
+    run_attend(fdm, cache, rows, page, *queries(g, fmt, sum(counts), 16), start, lens, pages.tolist(), tree(g, counts), workspace=workspace)
+
+
 def test_attend_pages_outside_the_cache(fdm):
     """A page number that is none of the cache's: its positions are unseen, nothing is read."""
     g = rng(29)
