@@ -50,7 +50,7 @@ constexpr float kGrow = 8.0f;  // a row's maximum (log2) is moved when it grew b
 // A tile that several workgroups share is put together from their parts; the
 // workgroup that has its first part says so.
 struct JoinDesc {
-  int b, tile, parts, spare;
+  int t0, tile, parts, rows;  // its sequence's first token; rows of the tile
 };
 
 // workspace: JoinDesc [groups], row statistics [2 groups][128] (max, sum),
@@ -872,7 +872,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       } else {
         // the range's first tile may have begun in the workgroup before; its last goes on in the next
         const int part = 2 * group + (from == 0 ? 1 : 0);
-        if (from == 0 && tid == 0) space.desc[group] = {range.b, range.tile, parts_of(a, before, range, steps), 0};
+        if (from == 0 && tid == 0) space.desc[group] = {s.t0, range.tile, parts_of(a, before, range, steps), rows};
         if (tid < kTileRows) space.stat[(size_t)part * kTileRows + tid] = make_float2(stat[tid], stat[kTileRows + tid]);
         f32x4* to_part = reinterpret_cast<f32x4*>(space.part + (size_t)part * kPartFloats) + (2 * rh * 16 + 8 * dh) * 256 + lane;
 #pragma unroll
@@ -914,113 +914,124 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 
 // A tile's parts put together: M = max m, out = sum 2^(m - M) part / sum 2^(m - M) l.
 // Workgroup (x, y): of the x-th tile that has parts, 32 rows and I blocks of 32
-// dims; 256 threads of four dims each, S times over for every S-th part.  Few
-// tiles of many parts are bound by latency (I = 1, S = 4: one token over 1024
-// positions, 16 parts, 6.6 us), many of few by memory and by the dependent
-// reads before the first part (I = 8, S = 1: 64 sequences of one token over 4095
-// positions, 82 MB of parts, 20 us).
+// dims; 256 threads of four dims each, S times over for every S-th part.  A thread
+// reads its row's statistics itself, twice, from the caches, and requests the first
+// parts before them.  Few tiles of many parts are bound by latency (I = 1, S = 4:
+// one token over 1024 positions, 16 parts, 4.8 us; I = 8, S = 1 would have 8
+// workgroups there), many of few by memory (I = 8, S = 1: 64 sequences of one token
+// over 4095 positions, 82 MB of parts, 17.5 us; blocks of four at a time 1 % more of
+// the whole).
 template <int FMT, int R, int S, int I>
 __global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int groups) {
   typedef typename Half<FMT>::T T;
   typedef typename Half<FMT>::x4 x4;
-  constexpr int kSlots = 8 * S;  // parts side by side in the statistics
-  __shared__ float weight[kMaxGroups][32];
-  __shared__ float red[kSlots][32];
+  constexpr int kFlight = S > 1 ? 8 : 4;  // parts requested at a time
+  __shared__ int first[4];                // tiles that begin in the groups before a wave's 64
   __shared__ int owner;
-  __shared__ f32x4 sums[S > 1 ? S - 1 : 1][256];
+  __shared__ JoinDesc found;
+  __shared__ float4 red[S > 1 ? S - 1 : 1][256];
+  __shared__ float red_l[S > 1 ? S - 1 : 1][32];
+  __shared__ float red_top[S][32];
   const Space space = space_of(a.workspace, groups);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // the x-th group that has the first part of a tile
-  if (wave == 0) {
-    int before = 0, found = -1;
-    for (int at = 0; at < groups && found < 0; at += 64) {
-      const uint64_t has = __ballot(at + lane < groups && space.desc[at + lane].parts != 0);
-      const int n = __popcll(has);
-      const int mine = before + __popcll(has & ((1ull << lane) - 1));
-      const uint64_t hit = __ballot(((has >> lane) & 1) && mine == (int)blockIdx.x);
-      if (hit) found = at + __builtin_ctzll(hit);
-      before += n;
+  if (tid == 0) owner = -1;
+  const JoinDesc mine = space.desc[min(tid, groups - 1)];
+  const uint64_t has = __ballot(tid < groups && mine.parts != 0);
+  if (wave < 4 && lane == 0) first[wave] = __popcll(has);
+  __syncthreads();
+  if (wave < 4) {
+    int before = 0;
+    for (int w = 0; w < wave; ++w) before += first[w];
+    if (((has >> lane) & 1) && before + __popcll(has & ((1ull << lane) - 1)) == (int)blockIdx.x) {
+      owner = tid;
+      found = mine;
     }
-    if (lane == 0) owner = found;
   }
   __syncthreads();
   const int group = owner;
   if (group < 0) return;
-  JoinDesc d = space.desc[group];
-  d.parts = min(d.parts, groups - group);
+  const int parts = min(found.parts, groups - group), rows = found.rows, tile0 = R * found.tile, t0 = found.t0;
   constexpr int kBlocks = R / 32;  // of rows
   const int dim0 = (int)blockIdx.y / kBlocks * I, rb = (int)blockIdx.y % kBlocks;  // first block of 32 dims, of 16
-  const int row0 = 32 * rb;
-  const SeqWork s = seq_work(a, d.b);
-  const int tile0 = R * d.tile, rows = min(R, s.n * a.H - tile0);
-  if (row0 >= rows) return;
+  if (32 * rb >= rows) return;
+  const int id = tid & 255, ps = tid >> 8, e = id >> 6, l32 = lane & 31, h = lane >> 5;
+  const int r = 32 * rb + l32;
   auto part_of = [&](int p) { return (size_t)(p ? 2 * (group + p) : 2 * group + 1); };
-  // the rows' weights of each part
-  const int srow = tid & 31, slot = tid >> 5;
-  float top = -__builtin_inff();
-  for (int p = slot; p < d.parts; p += kSlots) top = fmaxf(top, space.stat[part_of(p) * R + row0 + srow].x);
-  red[slot][srow] = top;
-  __syncthreads();
+  const float2* stat = space.stat + r;
+  const f32x4* part = reinterpret_cast<const f32x4*>(space.part) + (rb * 16 + dim0) * 256 + e * 64 + lane;
+  f32x4 v[I][kFlight];
+  auto request = [&](int p0) {
 #pragma unroll
-  for (int t = 0; t < kSlots; ++t) top = fmaxf(top, red[t][srow]);
-  __syncthreads();
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+      for (int t = 0; t < kFlight; ++t)
+        if (p0 + t * S < parts) v[i][t] = __builtin_nontemporal_load(part + part_of(p0 + t * S) * (R * kLatDim / 4) + i * 256);
+  };
+  request(ps);  // ahead of the statistics that they wait for
+  // the row's maximum
+  float top = -__builtin_inff();
+  for (int p0 = ps; p0 < parts; p0 += kFlight * S) {
+    float m[kFlight];
+#pragma unroll
+    for (int t = 0; t < kFlight; ++t) m[t] = p0 + t * S < parts ? stat[part_of(p0 + t * S) * R].x : -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < kFlight; ++t) top = fmaxf(top, m[t]);
+  }
+  if constexpr (S > 1) {
+    if (e == 0 && h == 0) red_top[ps][l32] = top;
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < S; ++t) top = fmaxf(top, red_top[t][l32]);
+  }
   const float off = top == -__builtin_inff() ? 0.0f : top;
   float l = 0.0f;
-  for (int p = slot; p < d.parts; p += kSlots) {
-    const float2 st = space.stat[part_of(p) * R + row0 + srow];
-    const float f = __builtin_amdgcn_exp2f(st.x - off);
-    weight[p][srow] = f;
-    l = fmaf(f, st.y, l);
-  }
-  red[slot][srow] = l;
-  __syncthreads();
-  const int id = tid & 255, ps = tid >> 8, e = id >> 6, l32 = lane & 31, h = lane >> 5;
-  const int r = row0 + l32;
-  l = 0.0f;
+  f32x4 sum[I];
 #pragma unroll
-  for (int t = 0; t < kSlots; ++t) l += red[t][l32];
+  for (int i = 0; i < I; ++i) sum[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p0 = ps; p0 < parts; p0 += kFlight * S) {
+    if (p0 != ps) request(p0);
+#pragma unroll
+    for (int t = 0; t < kFlight; ++t)
+      if (p0 + t * S < parts) {
+        const float2 st = stat[part_of(p0 + t * S) * R];
+        const float f = __builtin_amdgcn_exp2f(st.x - off);
+        l = fmaf(f, st.y, l);
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[i][c] = fmaf(f, v[i][t][c], sum[i][c]);
+      }
+  }
+  if constexpr (S > 1) {
+    static_assert(I == 1, "one block of dims where parts are shared out");
+    if (ps) {
+      red[ps - 1][id] = make_float4(sum[0][0], sum[0][1], sum[0][2], sum[0][3]);
+      if (e == 0 && h == 0) red_l[ps - 1][l32] = l;
+    }
+    __syncthreads();
+    if (ps) return;
+#pragma unroll
+    for (int t = 0; t < S - 1; ++t) {
+      const float4 other = red[t][id];
+      sum[0] += f32x4{other.x, other.y, other.z, other.w};
+      l += red_l[t][l32];
+    }
+  }
+  if (r >= rows) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int t = (tile0 + r) / a.H, hd = tile0 + r - t * a.H;
-  T* out = static_cast<T*>(a.out) + (int64_t)(s.t0 + t) * a.out_token + hd * a.out_head + 32 * dim0 + 8 * e + 4 * h;
-  constexpr int kFlight = I > 1 ? 4 : 8;
-#pragma unroll 2
+  T* out = static_cast<T*>(a.out) + (int64_t)(t0 + t) * a.out_token + hd * a.out_head + 32 * dim0 + 8 * e + 4 * h;
+#pragma unroll
   for (int i = 0; i < I; ++i) {
-    const f32x4* from = reinterpret_cast<const f32x4*>(space.part) + (rb * 16 + dim0 + i) * 256 + e * 64 + lane;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p0 = ps; p0 < d.parts; p0 += kFlight * S) {
-      f32x4 v[kFlight];
+    x4 y;
 #pragma unroll
-      for (int t = 0; t < kFlight; ++t)
-        if (p0 + t * S < d.parts) v[t] = from[part_of(p0 + t * S) * (R * kLatDim / 4)];
-#pragma unroll
-      for (int t = 0; t < kFlight; ++t)
-        if (p0 + t * S < d.parts) {
-          const float f = weight[p0 + t * S][l32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sum[c] = fmaf(f, v[t][c], sum[c]);
-        }
-    }
-    if constexpr (S > 1) {
-      static_assert(I == 1, "one block of dims where parts are shared out");
-      if (ps) sums[ps - 1][id] = sum;
-      __syncthreads();
-      if (ps) return;
-#pragma unroll
-      for (int t = 0; t < S - 1; ++t) sum += sums[t][id];
-    }
-    if (r < rows) {
-      x4 v;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) v[c] = (T)(sum[c] * inv);
-      *reinterpret_cast<x4*>(out + 32 * i) = v;
-    }
+    for (int c = 0; c < 4; ++c) y[c] = (T)(sum[i][c] * inv);
+    *reinterpret_cast<x4*>(out + 32 * i) = y;
   }
-  if (a.lse && r < rows && dim0 == 0 && e == 0 && h == 0) {
-    top = -__builtin_inff();
-    for (int p = 0; p < d.parts; ++p) top = fmaxf(top, space.stat[part_of(p) * R + r].x);
-    a.lse[(size_t)(s.t0 + t) * a.H + hd] =
+  if (a.lse && dim0 == 0 && e == 0 && h == 0)
+    a.lse[(size_t)(t0 + t) * a.H + hd] =
         l == 0.0f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
-  }
 }
 
 static int mla_tree_groups() { return min(max(1, g_num_cus), kMaxGroups); }
