@@ -233,56 +233,67 @@ template <int R, int S>
 __device__ __forceinline__ int tile_units(const SeqWork& s, int tile, int H, bool in_order) {
   return tile_steps<R, S>(s, tile, H, in_order) + kTileCost;
 }
-// ceil(1 / S) + .. + ceil(x / S)
-__device__ __forceinline__ int64_t step_sum(int64_t x, int S) {
-  const int64_t q = x / S, r = x % S;
-  return S * (q * (q + 1) / 2) + r * (q + 1);
+// ceil(1 / 2^k) + .. + ceil(x / 2^k)
+__device__ __forceinline__ int64_t step_sum(int64_t x, int k) {
+  const int64_t q = x >> k, r = x & ((1 << k) - 1);
+  return ((q * (q + 1) / 2) << k) + r * (q + 1);
 }
-// Whether the sequence's tiles are of one size or grow by k = R / H whole
-// tokens that divide a step: their units have a sum in closed form.
-template <int R, int S>
-__device__ __forceinline__ bool even_tiles(const SeqWork& s, int H, bool in_order) {
-  return !in_order || s.n <= 1 || (s.len >= s.n && R % H == 0 && S % (R / H) == 0);
+// sum over i < n of floor((a i + b) / m): whole parts of a and b are taken out,
+// and the points under what is left of the line are counted along the other axis.
+__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
+  uint64_t sum = 0;
+  for (;;) {
+    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const uint64_t end = a * n + b;
+    if (end < m) return sum;
+    n = end / m;
+    b = end % m;
+    const uint64_t t = m;
+    m = a;
+    a = t;
+  }
 }
 // units of the sequence's tiles 0 .. tiles - 1
 template <int R, int S>
-__device__ int64_t units_before(const SeqWork& s, int tiles, int H, bool in_order) {
+__device__ __forceinline__ int64_t units_before(const SeqWork& s, int tiles, int H, bool in_order) {
   if (!in_order || s.n <= 1) return (int64_t)tiles * tile_units<R, S>(s, 0, H, in_order);
   int64_t sum = 0;
-  if (even_tiles<R, S>(s, H, in_order)) {
-    // sum of ceil((p + k i) / S), p positions before the tokens: with p in whole
-    // k, rounded up, the same as ceil((p / k + i) / (S / k))
-    const int k = R / H, per = S / k, whole = min(tiles, s.n / k);
-    const int64_t p = ((int64_t)(s.len - s.n) + k - 1) / k;
-    sum = step_sum(p + whole, per) - step_sum(p, per);
-    if (tiles > whole) sum += (s.len + S - 1) / S;  // the last, of fewer tokens
+  if (s.len < s.n) {  // tokens before the first position: tiles of one step
+    for (int i = 0; i < tiles; ++i) sum += tile_steps<R, S>(s, i, H, in_order);
     return sum + (int64_t)tiles * kTileCost;
   }
-  for (int i = 0; i < tiles; ++i) sum += tile_units<R, S>(s, i, H, in_order);
-  return sum;
-}
-// The last tile that starts at or before unit u of the sequence, and its start.
-template <int R, int S>
-__device__ int tile_at(const SeqWork& s, int64_t u, int H, bool in_order, int64_t& start) {
-  const int tiles = tiles_of<R>(s, H);
-  int tile = 0;
-  start = 0;
-  if (even_tiles<R, S>(s, H, in_order)) {
-    int hi = tiles - 1;
-    while (tile < hi) {
-      const int mid = (tile + hi + 1) / 2;
-      if (units_before<R, S>(s, mid, H, in_order) <= u) tile = mid;
-      else hi = mid - 1;
-    }
-    start = units_before<R, S>(s, tile, H, in_order);
-  } else {
-    for (; tile < tiles - 1; ++tile) {
-      const int64_t next = start + tile_units<R, S>(s, tile, H, in_order);
-      if (next > u) break;
-      start = next;
+  // ceil((before + last) / S) each, before the positions in front of the tokens
+  // and last the tile's last token (from 1): k (i + 1) with k = R / H whole tokens a
+  // tile, else floor((R (i + 1) - 1) / H) + 1; the sequence's last tile may have fewer
+  const int64_t before = s.len - s.n;
+  const int whole = tiles == tiles_of<R>(s, H) ? tiles - 1 : tiles, k = R / H;
+  if (whole < tiles) sum = (s.len + S - 1) / S;
+  if (whole > 0) {
+    if (R % H == 0 && S % k == 0) {  // with before in whole k, rounded up, ceil((before / k + i) / (S / k))
+      const int kb = __builtin_ctz(k), per = __builtin_ctz(S) - kb;
+      const int64_t p = (before + k - 1) >> kb;
+      sum += step_sum(p + whole, per) - step_sum(p, per);
+    } else {
+      sum += (int64_t)floor_sum(whole, (uint64_t)H * S, R, R - 1 + (uint64_t)H * (before + S));
     }
   }
-  return tile;
+  return sum + (int64_t)tiles * kTileCost;
+}
+// The last tile that starts at or before unit u of the sequence; every lane of a
+// wave looks at one of 64 at a time.
+template <int R, int S>
+__device__ __forceinline__ int tile_at(const SeqWork& s, int64_t u, int H, bool in_order) {
+  int lo = 0, n = tiles_of<R>(s, H);  // it is among lo .. lo + n - 1
+  while (n > 1) {
+    const int every = (n + 63) / 64, at = (int)(threadIdx.x & 63) * every;
+    const bool starts = at < n && units_before<R, S>(s, lo + at, H, in_order) <= u;
+    const int last = 63 - __builtin_clzll(__ballot(starts) | 1);
+    lo += last * every;
+    n = min(every, n - last * every);
+  }
+  return uniform(lo);
 }
 
 // Units before each sequence into before[0 .. B], two sequences a thread of
@@ -326,21 +337,30 @@ __device__ __forceinline__ void count_units(const MlaTreeArgs& a, uint32_t* befo
 struct Range {
   uint32_t u, end;      // next unit, end
   int group;            // number of the range
-  int b, tile;          // sequence and tile of the part
+  int b, tile;          // sequence and tile of the part (tile -1: to be looked for)
   int from, to;         // steps of the part; it ends before unit u
   SeqWork s;
 };
-// Ranges of two units at least: a part of one step is 256 KB of sums for 36 KB
-// of rows (one token over 1024 positions: 27.7 us, with ranges of one 30.0, of four 30.5).
-__device__ __forceinline__ uint32_t range_count(uint32_t total) { return min((uint32_t)gridDim.x, total / 2); }
+// A range that is cut out of a tile costs a part, 256 KB written and read again,
+// so few units are not spread over all workgroups: U units over G take 2 U / G us
+// of steps and about 0.13 G us of parts, least at G = sqrt(15 U); but no fewer than
+// there are tiles, and two units at least.  One token of 128 heads over 1024
+// positions in ranges of two 27.7 us, of one 30.0; over 32768 in ranges of eight 48,
+// of four 62; eight sequences of one token over 4096 47 and 52.
+__device__ __forceinline__ uint32_t range_count(const MlaTreeArgs& a, uint32_t total) {
+  const uint32_t tiles = (uint32_t)(((int64_t)a.N * a.H + kTileRows - 1) / kTileRows) + a.B;  // at most
+  const uint32_t few = max((uint32_t)__builtin_amdgcn_sqrtf(15.0f * (float)total), tiles);
+  return (uint32_t)uniform((int)min((uint32_t)gridDim.x, min(few, total / 2)));
+}
 __device__ __forceinline__ Range range_of(const MlaTreeArgs& a, const uint32_t* before) {
   Range r;
-  const uint32_t total = (uint32_t)uniform((int)before[a.B]), groups = range_count(total);
+  const uint32_t total = (uint32_t)uniform((int)before[a.B]), groups = range_count(a, total);
   // Neighbours in the list on one XCD (workgroups go round the eight in turn),
   // where they share rows; fewer ranges than workgroups are spread over all.
   const bool full = groups == gridDim.x && gridDim.x % 8 == 0;
   r.group = full ? (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
   r.u = r.end = r.b = 0;
+  r.tile = -1;
   if ((uint32_t)r.group >= groups) return r;
   r.u = (uint32_t)uniform((int)((uint64_t)r.group * total / groups));
   r.end = (uint32_t)uniform((int)((uint64_t)(r.group + 1) * total / groups));
@@ -357,13 +377,18 @@ template <int R, int S>
 __device__ __forceinline__ bool next_part(const MlaTreeArgs& a, const uint32_t* before, Range& r) {
   const bool in_order = a.mask == nullptr;
   while (r.u < r.end) {
-    while ((uint32_t)uniform((int)before[r.b + 1]) <= r.u) ++r.b;
+    while ((uint32_t)uniform((int)before[r.b + 1]) <= r.u) ++r.b, r.tile = -1;
     r.s = seq_work(a, r.b);
     r.s = {uniform(r.s.n), uniform(r.s.len), uniform(r.s.t0)};
     const int64_t seq_u = (uint32_t)uniform((int)before[r.b]);
-    int64_t start;
-    r.tile = uniform(tile_at<R, S>(r.s, r.u - seq_u, a.H, in_order, start));
-    const int64_t tile_u = uniform(seq_u + start) + kTileCost;  // its first step
+    int64_t start = r.u;  // the tile behind the one before starts here
+    if (r.tile >= 0) {
+      ++r.tile;
+    } else {
+      r.tile = r.u == seq_u ? 0 : tile_at<R, S>(r.s, r.u - seq_u, a.H, in_order);
+      start = uniform(seq_u + units_before<R, S>(r.s, r.tile, a.H, in_order));
+    }
+    const int64_t tile_u = start + kTileCost;  // its first step
     r.from = (int)max((int64_t)r.u - tile_u, (int64_t)0);
     r.to = (int)min((int64_t)tile_steps<R, S>(r.s, r.tile, a.H, in_order), (int64_t)r.end - tile_u);
     if (r.to <= 0) break;  // the range ends before the tile's first step
@@ -374,7 +399,7 @@ __device__ __forceinline__ bool next_part(const MlaTreeArgs& a, const uint32_t* 
 }
 // Workgroups that have steps of the part's tile of so many steps.
 __device__ __forceinline__ int parts_of(const MlaTreeArgs& a, const uint32_t* before, const Range& r, int steps) {
-  const uint32_t total = before[a.B], groups = range_count(total), first = r.u - r.to;
+  const uint32_t total = before[a.B], groups = range_count(a, total), first = r.u - r.to;
   auto range_at = [&](uint64_t u) { return (int)(((u + 1) * groups - 1) / total); };
   return range_at((uint64_t)first + steps - 1) - range_at(first) + 1;
 }
@@ -426,8 +451,9 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   while (next_part<kTileRows, kTilePos>(a, before, range)) {
     const SeqWork s = range.s;
     const int from = range.from, to = range.to, len = s.len;
-    const int first_edge = max(len - s.n, 0) / kTilePos;  // from this step on not all tokens see all positions
     const int row0 = kTileRows * range.tile, rows = min(kTileRows, s.n * a.H - row0);
+    // from this step on not all of the tile's tokens see all positions
+    const int first_edge = max(len - s.n + (a.mask ? 0 : row0 / a.H + 1), 0) / kTilePos;
 
     // The lane's scores are those of row 32 wave + l32.  What is needed of it is
     // computed where it is needed: registers are short in the loop.
