@@ -18,7 +18,7 @@
 // The bound is what a single wave issues around its products (a step takes 4150
 // cycles, 2176 of them products) and, as soon as that is better, the power: the
 // clock falls from 2.4 to 1.9 GHz.  512 tokens of 128 heads over 4608 positions
-// 585 to 620 us with the card, 1.0 to 1.06 PFLOP/s, where a library product of
+// 560 to 580 us with the card, 1.07 to 1.1 PFLOP/s, where a library product of
 // 8192^3 reaches 1.21.
 #include "latent_device.h"
 
