@@ -402,6 +402,25 @@ def test_attend_among_rows_that_are_no_numbers(fdm, fmt, page):
     run_attend(fdm, cache, rows, page, *queries(g, fmt, sum(counts), 16), start, lens, pages.tolist(), tree(g, counts), workspace=workspace)
 
 
+def test_attend_as_many_sequences_as_a_call_takes(fdm):
+    """512 of them: without tokens, without positions, and one that is longer than all others together."""
+    g = rng(512)
+    B, page = 512, 8
+    counts = [i % 3 for i in range(B)]
+    lens = [0 if i % 7 == 3 else max(counts[i], i % 11) for i in range(B)]
+    counts[300], lens[300] = 2, 4000
+    per = [max(1, -(-n // page)) for n in lens]
+    cache, rows = filled(fdm, "bf16", sum(per), page, g)
+    pages = torch.full((B, max(per)), -1, dtype=torch.int64)
+    at = 0
+    for b in range(B):
+        pages[b, :per[b]] = torch.arange(at, at + per[b])
+        at += per[b]
+    start = [0] + np.cumsum(counts).tolist()
+    say("mla_attend 512 sequences")
+    run_attend(fdm, cache, rows, page, *queries(g, "bf16", start[-1], 5), start, lens, pages.tolist())
+
+
 def test_attend_pages_outside_the_cache(fdm):
     """A page number that is none of the cache's: its positions are unseen, nothing is read."""
     g = rng(29)
