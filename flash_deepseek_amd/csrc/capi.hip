@@ -288,6 +288,23 @@ void free_workspace(Workspace& w) {
   w = Workspace();
 }
 
+// Zeroes words that kernels rely on, and returns when they are zero.  Nothing
+// orders a caller's stream behind the null stream (torch's streams do not wait
+// for it), so a clear that is only queued there could land while the stream's
+// first kernels run and take arrivals and tags away that their waits are for.
+// On a stream of its own: neither behind what the caller has queued, nor
+// recorded where the caller captures.
+int clear_words(std::initializer_list<std::pair<void*, size_t>> parts) {
+  hipStream_t s = nullptr;
+  FDM_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
+  hipError_t e = hipSuccess;
+  for (const auto& p : parts)
+    if (e == hipSuccess) e = hipMemsetAsync(p.first, 0, p.second, s);
+  if (e == hipSuccess) e = hipStreamSynchronize(s);
+  (void)hipStreamDestroy(s);
+  return e == hipSuccess ? FDM_OK : hip_fail(e, "clearing a workspace");
+}
+
 int alloc_workspace(Workspace& w) {
   FDM_HIP(hipMalloc(&w.xd, kXdGroups * sizeof(XGroup)));
   FDM_HIP(hipMalloc(&w.logits, (size_t)FDM_MAX_TOKENS * FDM_N_EXPERTS * sizeof(float)));
@@ -296,21 +313,16 @@ int alloc_workspace(Workspace& w) {
   FDM_HIP(hipMalloc(&w.act, (size_t)(FDM_MAX_K + 1) * FDM_MOE_FFN * sizeof(float)));
   FDM_HIP(hipMalloc(&w.act_xd, (size_t)(FDM_MAX_K + 1) * (FDM_MOE_FFN / 64) * sizeof(XGroup)));
   FDM_HIP(hipMalloc(&w.gu_count, (FDM_MAX_K + 1) * 64 * sizeof(int)));
-  FDM_HIP(hipMemset(w.gu_count, 0, (FDM_MAX_K + 1) * 64 * sizeof(int)));
   FDM_HIP(hipMalloc(&w.dn_count, 448 * sizeof(int)));
-  FDM_HIP(hipMemset(w.dn_count, 0, 448 * sizeof(int)));
   FDM_HIP(hipMalloc(&w.eo, (size_t)(FDM_MAX_K + 1) * FDM_HIDDEN * sizeof(float)));
   FDM_HIP(hipMalloc(&w.layer_cnt, (size_t)kLayerCounters * kLayerStride * sizeof(int)));
-  FDM_HIP(hipMemset(w.layer_cnt, 0, (size_t)kLayerCounters * kLayerStride * sizeof(int)));
   FDM_HIP(hipMalloc(&w.layer_flags, (size_t)kLayerFlags * kLayerStride * sizeof(unsigned)));
-  FDM_HIP(hipMemset(w.layer_flags, 0, (size_t)kLayerFlags * kLayerStride * sizeof(unsigned)));
   FDM_HIP(hipMalloc(&w.b_seg, (FDM_N_EXPERTS + 1) * sizeof(int)));
   FDM_HIP(hipMalloc(&w.b_pair_tok, (size_t)FDM_MAX_TOKENS * FDM_MAX_K * sizeof(int)));
   FDM_HIP(hipMalloc(&w.b_pair_of, (size_t)FDM_MAX_TOKENS * FDM_MAX_K * sizeof(int)));
   FDM_HIP(hipMalloc(&w.b_distinct, FDM_N_EXPERTS * sizeof(int)));
   FDM_HIP(hipMalloc(&w.b_ndistinct, sizeof(int)));
   FDM_HIP(hipMalloc(&w.layer_tagged, kLayerTagged * sizeof(uint64_t)));
-  FDM_HIP(hipMemset(w.layer_tagged, 0, kLayerTagged * sizeof(uint64_t)));
   FDM_HIP(hipMalloc(&w.stage_x, FDM_HIDDEN * sizeof(float)));
   FDM_HIP(hipMalloc(&w.stage_y, FDM_HIDDEN * sizeof(float)));
   FDM_HIP(hipMalloc(&w.stage_idx, FDM_MAX_K * sizeof(int)));
@@ -318,7 +330,11 @@ int alloc_workspace(Workspace& w) {
   FDM_HIP(hipMalloc(&w.dense_act, kDenseMaxFfn * sizeof(float)));
   FDM_HIP(hipMalloc(&w.q_chunks, 2 * kQMaxChunks * sizeof(int4)));
   FDM_HIP(hipMalloc(&w.q_nchunks, 2 * sizeof(int)));
-  return FDM_OK;
+  return clear_words({{w.gu_count, (FDM_MAX_K + 1) * 64 * sizeof(int)},
+                      {w.dn_count, 448 * sizeof(int)},
+                      {w.layer_cnt, (size_t)kLayerCounters * kLayerStride * sizeof(int)},
+                      {w.layer_flags, (size_t)kLayerFlags * kLayerStride * sizeof(unsigned)},
+                      {w.layer_tagged, kLayerTagged * sizeof(uint64_t)}});
 }
 
 // The workspace of the calls on stream s.  Calls on one stream run in stream
