@@ -21,6 +21,7 @@
 #include "../../include/fdm.h"
 #include "epoch_book.h"
 #include "fdm_internal.h"
+#include "launch_turns.h"
 
 namespace fdm {
 // ---- the scratch of fdm_moe_forward_batched_noalloc ------------------------------------
@@ -242,6 +243,9 @@ struct State {
   Workspace ws;  // the null stream's
   std::mutex ws_mu;  // guards stream_ws
   std::vector<std::pair<hipStream_t, std::unique_ptr<Workspace>>> stream_ws;  // any other stream's
+  std::mutex turn_mu;  // held from a one-launch kernel's wait to its event
+  LaunchTurns turns;
+  hipEvent_t turn_done = nullptr;
   Layer layers[FDM_MAX_LAYERS];
   DenseLayer dense[FDM_MAX_LAYERS];
   std::unique_ptr<StreamedLayer> streamed[FDM_MAX_LAYERS];
@@ -519,6 +523,47 @@ struct ProfScope {
   }
 };
 
+// A one-launch kernel's turn (launch_turns.h): begin() before the launch, end()
+// behind it; the streams' launches are kept apart until the scope ends.
+class OneLaunch {
+ public:
+  explicit OneLaunch(hipStream_t s) : s_(s), lock_(g.turn_mu) {}
+  int begin() {
+    const LaunchTurns::Step step = g.turns.before(s_);
+    if (step == LaunchTurns::kGo) return FDM_OK;
+    // a stream that was destroyed without a release: wait for the device instead
+    if (step == LaunchTurns::kMarkAndWait && hipEventRecord(g.turn_done, static_cast<hipStream_t>(g.turns.last)) != hipSuccess) {
+      (void)hipGetLastError();
+      FDM_HIP(hipDeviceSynchronize());
+      return FDM_OK;
+    }
+    FDM_HIP(hipStreamWaitEvent(s_, g.turn_done, 0));
+    return FDM_OK;
+  }
+  int end() {
+    if (!g.turns.after(s_)) return FDM_OK;
+    const hipError_t e = hipEventRecord(g.turn_done, s_);
+    g.turns.marked = e == hipSuccess;
+    return e == hipSuccess ? FDM_OK : hip_fail(e, "hipEventRecord");
+  }
+
+ private:
+  hipStream_t s_;
+  std::lock_guard<std::mutex> lock_;
+};
+
+// The waits of a one-launch kernel are tied to its call's epoch: a replayed launch
+// would find the tags of the replay before and go on with its values, and no
+// event orders replays.
+int check_not_captured(hipStream_t s, const char* what) {
+  if (!s) return FDM_OK;
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  FDM_HIP(hipStreamIsCapturing(s, &st));
+  if (st != hipStreamCaptureStatusNone)
+    return fail(FDM_E_STATE, "%s cannot be captured into a graph: its kernel's waits are tied to the call", what);
+  return FDM_OK;
+}
+
 SlotTable slots_for(const Layer& L, const int* idx, const float* w, int K, bool with_shared) {
   SlotTable t;
   t.experts = L.experts;
@@ -771,6 +816,10 @@ int fdm_init(int device) {
     free_workspace(g.ws);
     return rc;
   }
+  if (hipError_t ev = hipEventCreateWithFlags(&g.turn_done, hipEventDisableTiming)) {
+    free_workspace(g.ws);
+    return hip_fail(ev, "hipEventCreateWithFlags");
+  }
   g.device = device;
   g.ready = true;
   return FDM_OK;
@@ -787,6 +836,9 @@ int fdm_shutdown(void) {
   for (auto& e : g.stream_ws) free_workspace(*e.second);
   g.stream_ws.clear();
   free_workspace(g.ws);
+  if (g.turn_done) (void)hipEventDestroy(g.turn_done);
+  g.turn_done = nullptr;
+  g.turns = LaunchTurns();
   for (int i = 0; i < g.prof.created; ++i) {
     (void)hipEventDestroy(g.prof.start[i]);
     (void)hipEventDestroy(g.prof.stop[i]);
@@ -881,6 +933,10 @@ int fdm_stream_release(void* stream) {
   }
   if (!w) return FDM_OK;
   FDM_HIP(hipDeviceSynchronize());  // the stream itself may already be destroyed
+  {
+    std::lock_guard<std::mutex> lock(g.turn_mu);
+    g.turns.forget(s);
+  }
   free_workspace(*w);
   return FDM_OK;
 }
@@ -970,6 +1026,7 @@ int run_matvec(bool q6, const void* d_W, const float* d_x, float* d_y, uint32_t 
     return FDM_OK;
   }
   if (!q6 && matvec2_supported((int)in_dim, (int)out_dim, part_words)) {
+    if (int rc = check_not_captured(s, "this matvec")) return rc;
     Matvec2Args a;
     a.W = W;
     a.x = d_x;
@@ -979,11 +1036,16 @@ int run_matvec(bool q6, const void* d_W, const float* d_x, float* d_y, uint32_t 
     a.err = w->layer_flags + kLayerFlagErr * kLayerStride;
     a.epoch = w->epochs.next();
     a.spin_limit = g_layer_spin_limit;
-    ProfScope p(FDM_PROF_MATVEC, s);
-    FDM_HIP(launch_matvec2_q4k(a, (int)in_dim, s));
-    return FDM_OK;
+    OneLaunch turn(s);
+    if (int rc = turn.begin()) return rc;
+    {
+      ProfScope p(FDM_PROF_MATVEC, s);
+      FDM_HIP(launch_matvec2_q4k(a, (int)in_dim, s));
+    }
+    return turn.end();
   }
   if (matvec1_supported(q6, (int)in_dim)) {
+    if (int rc = check_not_captured(s, "this matvec")) return rc;
     MatvecArgs a;
     a.W = W;
     a.x = d_x;
@@ -996,9 +1058,13 @@ int run_matvec(bool q6, const void* d_W, const float* d_x, float* d_y, uint32_t 
     a.err = w->layer_flags + kLayerFlagErr * kLayerStride;
     a.epoch = w->epochs.next();
     a.spin_limit = g_layer_spin_limit;
-    ProfScope p(FDM_PROF_MATVEC, s);
-    FDM_HIP(launch_matvec1(a, q6, s));
-    return FDM_OK;
+    OneLaunch turn(s);
+    if (int rc = turn.begin()) return rc;
+    {
+      ProfScope p(FDM_PROF_MATVEC, s);
+      FDM_HIP(launch_matvec1(a, q6, s));
+    }
+    return turn.end();
   }
   {
     ProfScope p(FDM_PROF_XDIGITS, s);
@@ -1043,6 +1109,7 @@ int fdm_expert_ffn(const void* d_blob, size_t expert_size, const float* d_x, flo
   hipStream_t s = as_stream(stream);
   // one launch of the fp32 expert kernel (expert_kernels.hip) on the
   // caller's packed blob, Q4_K or Q6_K down
+  if (int rc = check_not_captured(s, "fdm_expert_ffn")) return rc;
   Workspace* ws = nullptr;
   if (int rc = stream_workspace(s, &ws)) return rc;
   LayerArgs a;
@@ -1063,12 +1130,14 @@ int fdm_expert_ffn(const void* d_blob, size_t expert_size, const float* d_x, flo
   a.w = ws->w;
   layer_workspace_args(a, ws);
   a.act_out = d_act;
+  OneLaunch turn(s);
+  if (int rc = turn.begin()) return rc;
   {
     ProfScope p(FDM_PROF_GATEUP, s);
     // the fp32 expert kernel (gate/up items, one activation hand-off, down items)
     FDM_HIP(launch_expert_f32(a, s));
   }
-  return FDM_OK;
+  return turn.end();
 }
 
 // ---- router -----------------------------------------------------------------
@@ -1365,16 +1434,19 @@ int run_layer(int L, const float* h, const float* norm_w, float* h_post_out, con
   a.down_q6 = y->down_q6 ? 1 : 0;
   a.K = K;
   a.n_slots = K + (y->shared ? 1 : 0);
+  if (int rc = check_not_captured(s, "the batch-1 layer")) return rc;
   Workspace* ws = nullptr;
   if (int rc = stream_workspace(s, &ws)) return rc;
   a.idx = idx ? idx : ws->idx;
   a.w = w ? w : ws->w;
   layer_workspace_args(a, ws);
+  OneLaunch turn(s);
+  if (int rc = turn.begin()) return rc;
   {
     ProfScope p(FDM_PROF_LAYER, s);
     FDM_HIP(launch_layer(a, s));
   }
-  return FDM_OK;
+  return turn.end();
 }
 }  // namespace
 }  // namespace fdm

@@ -21,7 +21,8 @@
 // products (4 (q - 32)) x summed, then scaled by d sc / 4.
 //
 // Final items only wait for gate/up items, which come first in the list and
-// never wait: the grid drains whatever the dispatch order.  The wait is
+// never wait: the grid drains in whatever order it is dispatched, beside other
+// work that ends by itself (two grids with waits: launch_turns.h).  The wait is
 // bounded: one that gives up records the call's epoch in the error flag
 // (fdm_stream_sync reports it) and releases every other wait.
 #include "fdm_internal.h"

@@ -42,7 +42,10 @@
 // before they wait for the activations).  Workgroups are dispatched in
 // list order within each XCD, so the earliest unfinished item is always
 // resident or dispatchable and never waits on anything unfinished: the
-// grid drains.  Every wait is bounded as well: one that times out records
+// grid drains.  That holds for one such grid at a time: with two, an XCD full
+// of waiting workgroups of one may have no place for the item that an XCD full
+// of the other's waits for.  The host orders them over all streams
+// (launch_turns.h).  Every wait is bounded as well: one that times out records
 // the call's epoch in the error flag, which releases every other wait, so
 // the launch always completes (the host reports the error on its next
 // sync).

@@ -186,9 +186,10 @@ hipError_t launch_matvec_q6k(const uint8_t* W, const XGroup* xd, float* y, int r
 // item requests its weights first, then waits for the digit flag (set by
 // the last digit item to arrive), stages the records with coherent 16-byte
 // loads and finishes; the digits' latency hides behind the weight loads and
-// no second launch is paid.  Digit items never wait, so the grid drains
-// whatever the dispatch order; the flag wait is bounded as well (a wait that
-// gives up records the epoch in the error flag, which fdm_stream_sync reports).
+// no second launch is paid.  Digit items never wait, and are dispatched first, so
+// the grid drains, one such grid at a time (launch_turns.h); the flag wait is
+// bounded as well (a wait that gives up records the epoch in the error flag,
+// which fdm_stream_sync reports).
 
 __device__ __forceinline__ int mv_digit_items(int gr) { return (gr + 1) / 2; }
 

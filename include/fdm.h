@@ -87,7 +87,14 @@ int fdm_stream_sync(void *stream);
  * made by fdm_init; another stream's at its first call, kept until
  * fdm_stream_release(stream) or fdm_shutdown (at most 64 streams at a time:
  * FDM_E_STATE beyond).  Release a stream's workspace before destroying the
- * stream if its handle may be reused.  Shared across streams, by design:
+ * stream if its handle may be reused.  The kernels whose workgroups wait for
+ * one another (fdm_moe_layer, fdm_moe_layer_norm, fdm_expert_ffn, and
+ * fdm_matvec_* where it is one launch with digits or column parts) take turns
+ * over all streams: such a call on another stream than the latest one's waits
+ * on the device, not on the host, until that one's kernel has run.  They cannot
+ * be captured into a graph (FDM_E_STATE), because their waits are tied to the
+ * call.  Nothing orders them with those of another process on the same device.
+ * Shared across streams, by design:
  * a streamed layer's expert cache (calls take turns), an attention layer's
  * KV cache (one sequence: one stream at a time), the scratch of
  * fdm_moe_forward_batched_noalloc, and the timing pool of fdm_prof_*.
@@ -253,9 +260,10 @@ int fdm_moe_forward_host(int L, const float *h_post, const int *exp_idx, const f
  * shared expert, combine, and the residual:
  *   hidden = h_in + sum_k w[k] E_k(h_post) + S(h_post).
  * d_h_in may be NULL (no residual).  d_idx / d_w (optional) receive the
- * routing.  One launch; its scratch is the stream's workspace, so calls on
- * different streams may overlap.  A launch whose internal waits
- * time out (never expected; it would mean a broken device) completes with
+ * routing.  One launch; its scratch is the stream's workspace, so several
+ * threads may call on streams of their own (their kernels take turns).  A launch
+ * whose internal waits time out (never expected; it would mean a broken device
+ * or another process's waiting kernels beside it) completes with
  * an unspecified result and makes the next fdm_stream_sync return
  * FDM_E_STATE. */
 int fdm_moe_layer(int L, const float *d_h_post, const float *d_h_in, int K, float *d_hidden,
