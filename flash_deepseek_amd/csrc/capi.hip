@@ -22,6 +22,7 @@
 #include "epoch_book.h"
 #include "fdm_internal.h"
 #include "launch_turns.h"
+#include "mla_work.h"
 
 namespace fdm {
 // ---- the scratch of fdm_moe_forward_batched_noalloc ------------------------------------
@@ -2650,6 +2651,10 @@ int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_
     if (s % 8) return fail(FDM_E_INVAL, "stride %lld: a multiple of 8 elements", (long long)s);
   if (!rows_apart(out_head, b->H, out_token, b->N, FDM_KV_LATENT))
     return fail(FDM_E_INVAL, "out: rows of %d overlap", FDM_KV_LATENT);
+  const int max_len = (int)std::min<int64_t>((int64_t)b->pages_stride * c->page_size, INT32_MAX - 4096);
+  const uint64_t units = most_units(b->N, b->H, b->B, max_len);
+  if (units > kMaxUnits)
+    return fail(FDM_E_INVAL, "%d tokens of %d heads with tables of %d positions: more work than a call takes", b->N, b->H, max_len);
   if (int rc = check_ready()) return rc;
   if (workspace_bytes < mla_tree_workspace(b->N, b->H))
     return fail(FDM_E_INVAL, "workspace of %zu bytes: %zu are needed", workspace_bytes, mla_tree_workspace(b->N, b->H));
@@ -2661,7 +2666,8 @@ int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_
   a.page_shift = __builtin_ctz(c->page_size);
   a.pages = b->d_pages;
   a.pages_stride = b->pages_stride;
-  a.max_len = (int)std::min<int64_t>((int64_t)b->pages_stride * c->page_size, INT32_MAX - 4096);
+  a.max_len = max_len;
+  a.wide_units = units > INT32_MAX;
   a.q_start = b->d_q_start;
   a.kv_len = b->d_kv_len;
   a.B = b->B;

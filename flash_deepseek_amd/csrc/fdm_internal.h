@@ -413,7 +413,6 @@ struct KvReadArgs {
 };
 hipError_t launch_kv_read(const KvReadArgs& a, int fmt, ElemType y, hipStream_t s);
 
-constexpr int kMlaMaxSeqs = 512;  // FDM_MLA_MAX_SEQS
 struct MlaTreeArgs {
   const void *latent, *rope;  // the cache's planes
   const uint8_t* scale;
@@ -424,6 +423,7 @@ struct MlaTreeArgs {
   int B, N, H;
   const uint64_t* mask;       // [N][mask_words] or null: in order
   int mask_words;
+  bool wide_units;            // the work may count 2^31 units and more
   const void *q_lat, *q_rope;
   int64_t ql_token, ql_head, qr_token, qr_head;
   float scale_log2;           // score scale x log2(e)

@@ -21,6 +21,7 @@
 // 560 to 580 us with the card, 1.07 to 1.1 PFLOP/s, where a library product of
 // 8192^3 reaches 1.21.
 #include "latent_device.h"
+#include "mla_work.h"
 
 namespace fdm {
 
@@ -34,16 +35,12 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kTileRows = 128;  // (token, head) rows of a workgroup
-constexpr int kTilePos = 32;    // positions of a step
 constexpr int kLatBytes = kTilePos * kLatDim * 2, kRotBytes = kTilePos * kRotDim * 2;
 constexpr int kPBytes = kTileRows * kTilePos * 2;
 // LDS: four steps' latent rows (one's values, one's keys, one landed, one landing),
 // three steps' rotary parts, the weights of two steps
 constexpr int kRotAt = 4 * kLatBytes, kPAt = kRotAt + 3 * kRotBytes, kStepLds = kPAt + 2 * kPBytes;
 constexpr size_t kPartFloats = (size_t)kTileRows * kLatDim;
-constexpr uint32_t kMaxUnits = 0x7FFFFFFFu;
-constexpr int kTileCost = 6;
 constexpr int kMaxGroups = 256;  // workgroups that share the work
 constexpr float kGrow = 8.0f;  // a row's maximum (log2) is moved when it grew by more
 
@@ -203,83 +200,13 @@ __device__ __attribute__((aligned(16))) uint32_t zero_row[8 * kLatDim * 2 / 4]; 
 
 }  // namespace
 
-// ---- the work: tiles of rows, steps of positions --------------------------------------
-// The (token, head) rows of a sequence, heads fastest, are cut into tiles of R.
-// A tile has a step for every S positions that its last token may see (one at
-// least, so that rows that see nothing are written) and counts kTileCost units
-// more, what beginning and ending it costs a workgroup (queries, first steps,
-// results: about 12 us against 2 us a step; 64 sequences of one token over 4095
-// positions 119 us without, 114 with four, 112 with six).  The units of all tiles
-// in order (sequence, tile, unit) are cut into equal ranges, one a workgroup.
-struct SeqWork {
-  int n, len, t0;  // tokens, positions, first token
-};
+// ---- the work: tiles of rows, steps of positions (mla_work.h) ---------------------------
 __device__ __forceinline__ SeqWork seq_work(const MlaTreeArgs& a, int b) {
   SeqWork s;
   s.t0 = min(max(a.q_start[b], 0), a.N);
   s.n = max(min(a.q_start[b + 1], a.N) - s.t0, 0);
   s.len = min(max(a.kv_len[b], 0), a.max_len);
   return s;
-}
-template <int R>
-__device__ __forceinline__ int tiles_of(const SeqWork& s, int H) { return (s.n * H + R - 1) / R; }
-template <int R, int S>
-__device__ __forceinline__ int tile_steps(const SeqWork& s, int tile, int H, bool in_order) {
-  const int last = min((R * (tile + 1) - 1) / H + 1, s.n);  // tokens up to the tile's last
-  const int64_t seen = in_order ? (int64_t)s.len - s.n + last : s.len;
-  return max(1, (int)((seen + S - 1) / S));
-}
-template <int R, int S>
-__device__ __forceinline__ int tile_units(const SeqWork& s, int tile, int H, bool in_order) {
-  return tile_steps<R, S>(s, tile, H, in_order) + kTileCost;
-}
-// ceil(1 / 2^k) + .. + ceil(x / 2^k)
-__device__ __forceinline__ int64_t step_sum(int64_t x, int k) {
-  const int64_t q = x >> k, r = x & ((1 << k) - 1);
-  return ((q * (q + 1) / 2) << k) + r * (q + 1);
-}
-// sum over i < n of floor((a i + b) / m): whole parts of a and b are taken out,
-// and the points under what is left of the line are counted along the other axis.
-__device__ __forceinline__ uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
-  uint64_t sum = 0;
-  for (;;) {
-    sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
-    const uint64_t end = a * n + b;
-    if (end < m) return sum;
-    n = end / m;
-    b = end % m;
-    const uint64_t t = m;
-    m = a;
-    a = t;
-  }
-}
-// units of the sequence's tiles 0 .. tiles - 1
-template <int R, int S>
-__device__ __forceinline__ int64_t units_before(const SeqWork& s, int tiles, int H, bool in_order) {
-  if (!in_order || s.n <= 1) return (int64_t)tiles * tile_units<R, S>(s, 0, H, in_order);
-  int64_t sum = 0;
-  if (s.len < s.n) {  // tokens before the first position: tiles of one step
-    for (int i = 0; i < tiles; ++i) sum += tile_steps<R, S>(s, i, H, in_order);
-    return sum + (int64_t)tiles * kTileCost;
-  }
-  // ceil((before + last) / S) each, before the positions in front of the tokens
-  // and last the tile's last token (from 1): k (i + 1) with k = R / H whole tokens a
-  // tile, else floor((R (i + 1) - 1) / H) + 1; the sequence's last tile may have fewer
-  const int64_t before = s.len - s.n;
-  const int whole = tiles == tiles_of<R>(s, H) ? tiles - 1 : tiles, k = R / H;
-  if (whole < tiles) sum = (s.len + S - 1) / S;
-  if (whole > 0) {
-    if (R % H == 0 && S % k == 0) {  // with before in whole k, rounded up, ceil((before / k + i) / (S / k))
-      const int kb = __builtin_ctz(k), per = __builtin_ctz(S) - kb;
-      const int64_t p = (before + k - 1) >> kb;
-      sum += step_sum(p + whole, per) - step_sum(p, per);
-    } else {
-      sum += (int64_t)floor_sum(whole, (uint64_t)H * S, R, R - 1 + (uint64_t)H * (before + S));
-    }
-  }
-  return sum + (int64_t)tiles * kTileCost;
 }
 // The last tile that starts at or before unit u of the sequence; every lane of a
 // wave looks at one of 64 at a time.
@@ -296,46 +223,46 @@ __device__ __forceinline__ int tile_at(const SeqWork& s, int64_t u, int H, bool 
   return uniform(lo);
 }
 
-// Units before each sequence into before[0 .. B], two sequences a thread of
-// 256.  A call's units are below 2^31; starts that make them more (sequences
-// that share tokens) are cut.
-template <int R, int S>
-__device__ __forceinline__ void count_units(const MlaTreeArgs& a, uint32_t* before, uint32_t* wave_total) {
+// Units before each sequence into before[0 .. B], two sequences a thread of 256.
+// U: of 32 bits unless the call can have more.
+template <int R, int S, typename U>
+__device__ __forceinline__ void count_units(const MlaTreeArgs& a, UnitMarks& before, uint64_t* wave_total) {
+  constexpr U kMost = sizeof(U) == 8 ? (U)kMaxUnits : (U)0x7FFFFFFF;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const bool in_order = a.mask == nullptr;
-  uint32_t mine[2], sum = 0;
+  U mine[2], sum = 0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     mine[k] = sum;
     const int b = 2 * tid + k;
     if (b < a.B) {
       const SeqWork s = seq_work(a, b);
-      sum = (uint32_t)min((int64_t)sum + units_before<R, S>(s, tiles_of<R>(s, a.H), a.H, in_order), (int64_t)kMaxUnits);
+      sum = (U)min((uint64_t)sum + (uint64_t)units_before<R, S>(s, tiles_of<R>(s, a.H), a.H, in_order), (uint64_t)kMost);
     }
   }
-  uint32_t upto = sum;
+  U upto = sum;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t v = __shfl_up(upto, d);
-    if (lane >= d) upto = min(upto + v, kMaxUnits);
+    const U v = __shfl_up(upto, d);
+    if (lane >= d) upto = min(upto + v, kMost);
   }
   if (lane == 63) wave_total[wave] = upto;
-  const uint32_t inside = __shfl_up(upto, 1);
+  const U inside = __shfl_up(upto, 1);
   __syncthreads();
-  uint32_t base = 0;
-  for (int w = 0; w < wave; ++w) base = min(base + wave_total[w], kMaxUnits);
-  base = min(base + (lane ? inside : 0), kMaxUnits);
+  U base = 0;
+  for (int w = 0; w < wave; ++w) base = min(base + (U)wave_total[w], kMost);
+  base = min(base + (lane ? inside : 0), kMost);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (2 * tid + k <= a.B) before[2 * tid + k] = min(base + mine[k], kMaxUnits);
-  if (tid == 255 && a.B == kMlaMaxSeqs) before[kMlaMaxSeqs] = min(base + sum, kMaxUnits);
+    if (2 * tid + k <= a.B) before.put(2 * tid + k, min(base + mine[k], kMost));
+  if (tid == 255 && a.B == kMlaMaxSeqs) before.put(kMlaMaxSeqs, min(base + sum, kMost));
   __syncthreads();
 }
+__device__ __forceinline__ uint64_t units_at(const UnitMarks& before, int b) { return uniform((int64_t)before.at(b)); }
 
-// A workgroup's range of units, and the part of a tile that it is at.  Range g
-// of G over T units is [g T / G, (g + 1) T / G); unit u is in ((u + 1) G - 1) / T.
+// A workgroup's range of units, and the part of a tile that it is at.
 struct Range {
-  uint32_t u, end;      // next unit, end
+  uint64_t u, end;      // next unit, end
   int group;            // number of the range
   int b, tile;          // sequence and tile of the part (tile -1: to be looked for)
   int from, to;         // steps of the part; it ends before unit u
@@ -347,61 +274,64 @@ struct Range {
 // there are tiles, and two units at least.  One token of 128 heads over 1024
 // positions in ranges of two 27.7 us, of one 30.0; over 32768 in ranges of eight 48,
 // of four 62; eight sequences of one token over 4096 47 and 52.
-__device__ __forceinline__ uint32_t range_count(const MlaTreeArgs& a, uint32_t total) {
+__device__ __forceinline__ uint32_t range_count(const MlaTreeArgs& a, uint64_t total) {
   const uint32_t tiles = (uint32_t)(((int64_t)a.N * a.H + kTileRows - 1) / kTileRows) + a.B;  // at most
   const uint32_t few = max((uint32_t)__builtin_amdgcn_sqrtf(15.0f * (float)total), tiles);
-  return (uint32_t)uniform((int)min((uint32_t)gridDim.x, min(few, total / 2)));
+  return (uint32_t)uniform((int)min((uint64_t)min((uint32_t)gridDim.x, few), total / 2));
 }
-__device__ __forceinline__ Range range_of(const MlaTreeArgs& a, const uint32_t* before) {
+__device__ __forceinline__ Range range_of(const MlaTreeArgs& a, const UnitMarks& before) {
   Range r;
-  const uint32_t total = (uint32_t)uniform((int)before[a.B]), groups = range_count(a, total);
+  const uint64_t total = units_at(before, a.B);
+  const uint32_t groups = range_count(a, total);
   // Neighbours in the list on one XCD (workgroups go round the eight in turn),
   // where they share rows; fewer ranges than workgroups are spread over all.
   const bool full = groups == gridDim.x && gridDim.x % 8 == 0;
   r.group = full ? (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8 : blockIdx.x;
-  r.u = r.end = r.b = 0;
+  r.u = r.end = 0;
+  r.b = 0;
   r.tile = -1;
   if ((uint32_t)r.group >= groups) return r;
-  r.u = (uint32_t)uniform((int)((uint64_t)r.group * total / groups));
-  r.end = (uint32_t)uniform((int)((uint64_t)(r.group + 1) * total / groups));
+  const Ranges ranges(total, groups);
+  r.u = uniform((int64_t)ranges.start(r.group));
+  r.end = uniform((int64_t)ranges.start(r.group + 1));
   int hi = a.B - 1;  // the last sequence that starts at or before u
   while (r.b < hi) {
     const int mid = (r.b + hi + 1) / 2;
-    if ((uint32_t)uniform((int)before[mid]) <= r.u) r.b = mid;
+    if (units_at(before, mid) <= r.u) r.b = mid;
     else hi = mid - 1;
   }
   return r;
 }
 // The next part that has steps; false at the end of the range.
 template <int R, int S>
-__device__ __forceinline__ bool next_part(const MlaTreeArgs& a, const uint32_t* before, Range& r) {
+__device__ __forceinline__ bool next_part(const MlaTreeArgs& a, const UnitMarks& before, Range& r) {
   const bool in_order = a.mask == nullptr;
   while (r.u < r.end) {
-    while ((uint32_t)uniform((int)before[r.b + 1]) <= r.u) ++r.b, r.tile = -1;
-    const int64_t seq_u = (uint32_t)uniform((int)before[r.b]);
+    while (units_at(before, r.b + 1) <= r.u) ++r.b, r.tile = -1;
+    const int64_t seq_u = units_at(before, r.b);
     int64_t start = r.u;  // the tile behind the one before starts here
     if (r.tile >= 0) {
       ++r.tile;
     } else {
       r.s = seq_work(a, r.b);
       r.s = {uniform(r.s.n), uniform(r.s.len), uniform(r.s.t0)};
-      r.tile = r.u == seq_u ? 0 : tile_at<R, S>(r.s, r.u - seq_u, a.H, in_order);
+      r.tile = (int64_t)r.u == seq_u ? 0 : tile_at<R, S>(r.s, r.u - seq_u, a.H, in_order);
       start = uniform(seq_u + units_before<R, S>(r.s, r.tile, a.H, in_order));
     }
     const int64_t tile_u = start + kTileCost;  // its first step
     r.from = (int)max((int64_t)r.u - tile_u, (int64_t)0);
     r.to = (int)min((int64_t)tile_steps<R, S>(r.s, r.tile, a.H, in_order), (int64_t)r.end - tile_u);
     if (r.to <= 0) break;  // the range ends before the tile's first step
-    r.u = (uint32_t)(tile_u + r.to);
+    r.u = tile_u + r.to;
     if (r.to > r.from) return true;
   }
   return false;
 }
 // Workgroups that have steps of the part's tile of so many steps.
-__device__ __forceinline__ int parts_of(const MlaTreeArgs& a, const uint32_t* before, const Range& r, int steps) {
-  const uint32_t total = before[a.B], groups = range_count(a, total), first = r.u - r.to;
-  auto range_at = [&](uint64_t u) { return (int)(((u + 1) * groups - 1) / total); };
-  return range_at((uint64_t)first + steps - 1) - range_at(first) + 1;
+__device__ __forceinline__ int parts_of(const MlaTreeArgs& a, const UnitMarks& before, const Range& r, int steps) {
+  const uint64_t total = units_at(before, a.B), first = r.u - r.to;
+  const Ranges ranges(total, range_count(a, total));
+  return ranges.at(first + steps - 1) - ranges.at(first) + 1;
 }
 
 // Which of the positions j0 .. j0 + 31 the sequence's token `place` sees (bits).
@@ -437,12 +367,13 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   __shared__ float scale_by[2][kTileRows];   // what the rows' sums so far are scaled by
   __shared__ int moved[2][4];                // the step at which a wave's rows last were
   __shared__ int live[4];                    // bytes: which rows of a step exist
-  __shared__ uint32_t before[kMlaMaxSeqs + 1];  // units before each sequence
-  __shared__ uint32_t wave_total[4];
+  __shared__ UnitMarks before;               // units before each sequence
+  __shared__ uint64_t wave_total[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, h = lane >> 5;
 
-  count_units<kTileRows, kTilePos>(a, before, wave_total);
+  if (a.wide_units) count_units<kTileRows, kTilePos, uint64_t>(a, before, wave_total);
+  else count_units<kTileRows, kTilePos, uint32_t>(a, before, wave_total);
   Range range = range_of(a, before);
   const int group = range.group;
   const Space space = space_of(a.workspace, gridDim.x);

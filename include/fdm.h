@@ -532,13 +532,14 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
  * itself.  A token that sees nothing gets out = 0, lse = -infinity.  Values of
  * positions that no token sees are not used, whatever they are; a page number
  * outside the cache makes its positions unseen.  kv_len is cut to 0 .. pages_stride *
- * page_size, q_start to 0 .. N.  Rows of out and lse outside every sequence
+ * page_size (and 2^31 - 4097), q_start to 0 .. N.  Rows of out and lse outside every sequence
  * are left as they were; sequences must not share tokens.
  * q_lat [N][H][512], q_rope [N][H][64], out [N][H][512]: F16 for an F16 cache,
  * else BF16; strides in elements, multiples of 8, 16-byte aligned.  lse
  * (optional) fp32 [N][H].  Products of the 16-bit values accumulate in fp32 and
  * softmax weights round to 16 bits before the second product.  1 <= H <=
- * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS, N <= FDM_MLA_MAX_TOKENS.
+ * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS, N <= FDM_MLA_MAX_TOKENS, and
+ * (N H / 128 + 1 + B) (pages_stride page_size / 32 + 8) <= 2^40, whatever the lengths.
  * d_workspace: at least fdm_mla_workspace(N, H) bytes, 256-byte aligned, used
  * by the call alone until it has run on its stream: calls that may overlap, and
  * graphs that may run at once, need one each.  The call allocates nothing and
