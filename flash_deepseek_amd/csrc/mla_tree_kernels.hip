@@ -42,7 +42,15 @@ constexpr int kPBytes = kTileRows * kTilePos * 2;
 constexpr int kRotAt = 4 * kLatBytes, kPAt = kRotAt + 3 * kRotBytes, kStepLds = kPAt + 2 * kPBytes;
 constexpr size_t kPartFloats = (size_t)kTileRows * kLatDim;
 constexpr int kMaxGroups = 256;  // workgroups that share the work
-constexpr float kGrow = 8.0f;  // a row's maximum (log2) is moved when it grew by more
+// Weights are 2^(s - m), s in log2.  A row's m is kAbove under its maximum when it is
+// moved, which is when the maximum grew by more than kGrow since: a weight is at
+// most 2^(kAbove + kGrow).  That uses F16's numbers above 1: rounded to it, a weight
+// is off by 2^-32 of the row's largest at most, where with m the maximum itself
+// weights of 2^-25 were none, and 32768 of them 9e-4 of the values.  BF16 reaches as
+// far down as the fp32 sums.
+constexpr float kGrow = 8.0f;
+template <int FMT>
+constexpr float kAbove = FMT == kKvF16 ? 7.0f : 0.0f;
 
 // A tile that several workgroups share is put together from their parts; the
 // workgroup that has its first part says so.
@@ -569,10 +577,11 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
         top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       } else if (piece == 1) {
         top = across_halves(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
-        const bool need = top > m + kGrow;
+        const bool need = top > m + (kGrow + kAbove<FMT>);
         if (rare(__any(need))) {
-          const float keep = need ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
-          m = need ? top : m;
+          const float to_m = top - kAbove<FMT>;
+          const float keep = need ? __builtin_amdgcn_exp2f(m - to_m) : 1.0f;
+          m = need ? to_m : m;
           l *= keep;
           scale_by[step & 1][here(32 * wave + l32)] = keep;  // both halves of the wave have it
           moved[step & 1][wave] = step;
@@ -793,7 +802,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
       // ---- the tile's results, or a part of them
       l = across_halves(l, [](float x, float y) { return x + y; });
       __syncthreads();
-      float* stat = reinterpret_cast<float*>(lds + kPAt);  // [128] max, [128] sum
+      float* stat = reinterpret_cast<float*>(lds + kPAt);  // [128] m, [128] sum
       if (lane < 32) {
         stat[32 * wave + l32] = m;
         stat[kTileRows + 32 * wave + l32] = l;
@@ -879,7 +888,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
   }
 }
 
-// A tile's parts put together: M = max m, out = sum 2^(m - M) part / sum 2^(m - M) l.
+// A tile's parts put together: M = max m (not the maximum, but near it), out = sum 2^(m - M) part / sum 2^(m - M) l.
 // Workgroup (x, y): of the x-th tile that has parts, 32 rows and I blocks of 32
 // dims; 256 threads of four dims each, S times over for every S-th part.  A thread
 // reads its row's statistics itself, twice, from the caches, and requests the first
@@ -936,7 +945,7 @@ __global__ __launch_bounds__(256 * S) void k_mla_tree_join(MlaTreeArgs a, int gr
         if (p0 + t * S < parts) v[i][t] = __builtin_nontemporal_load(part + part_of(p0 + t * S) * (R * kLatDim / 4) + i * 256);
   };
   request(ps);  // ahead of the statistics that they wait for
-  // the row's maximum
+  // the largest m of the row
   float top = -__builtin_inff();
   for (int p0 = ps; p0 < parts; p0 += kFlight * S) {
     float m[kFlight];

@@ -537,7 +537,9 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
  * q_lat [N][H][512], q_rope [N][H][64], out [N][H][512]: F16 for an F16 cache,
  * else BF16; strides in elements, multiples of 8, 16-byte aligned.  lse
  * (optional) fp32 [N][H].  Products of the 16-bit values accumulate in fp32 and
- * softmax weights round to 16 bits before the second product.  1 <= H <=
+ * softmax weights round to 16 bits before the second product (relative; in F16 by
+ * no less than 2^-32 of the row's largest, so that weights below that add to lse
+ * alone).  1 <= H <=
  * FDM_MLA_MAX_HEADS, 1 <= B <= FDM_MLA_MAX_SEQS, N <= FDM_MLA_MAX_TOKENS, and
  * (N H / 128 + 1 + B) (pages_stride page_size / 32 + 8) <= 2^40, whatever the lengths.
  * d_workspace: at least fdm_mla_workspace(N, H) bytes, 256-byte aligned, used

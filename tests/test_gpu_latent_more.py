@@ -55,3 +55,40 @@ def test_tables_of_2_to_31_positions(fdm):
                         SCALE, None if mask is None else mask.cpu()[at])
         C.check(got[0][0][at], want[0], want[2], "out")
         C.check(got[0][1][at], want[1], want[3], "lse")
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16"])
+@pytest.mark.parametrize("strong", [0, 5000, 32768])
+def test_one_strong_position_among_many_weak_ones(fdm, fmt, strong):
+    """Weights of 2^-25 of the row's largest, 32768 of them: 1e-3 of the values, all of
+    those that the strong position has none of.  The tolerance is C.attend's, and
+    for F16 weights half a step of its smallest numbers, 2^-25, where the row's
+    largest weight is at least 2^7: 2^-32 a position.  512 sequences of one token
+    share the pages, so that a workgroup walks each from end to end."""
+    g = rng(6)
+    page, L, H, B = 64, 32769, 4, 512
+    t = C.DTYPES[fmt]
+    rows = torch.rand(L, C.LAT, generator=g) + 0.5
+    rows[:, 0] = 0.0
+    rows[strong] = normal(g, C.LAT)
+    rows[strong, 1:256] = 0.0
+    rows[strong, 0] = 4.34375  # with q 4 and scale 1: 17.375, or 2^25.07
+    cache = fdm.kv_cache(fmt, -(-L // page), page)
+    cache.latent.flatten(0, 1)[:L].copy_(rows)
+    q_lat, q_rope = torch.zeros(1, H, C.LAT, dtype=t), torch.zeros(1, H, C.ROT, dtype=t)
+    q_lat[:, :, 0] = 4.0
+    pages = torch.arange(cache.n_pages, dtype=torch.int32)[None]
+    out, lse = torch.empty(B, H, C.LAT, dtype=t, device="cuda"), torch.empty(B, H, device="cuda")
+    say(f"mla_attend {fmt}, the strong position at {strong} of {L}")
+    fdm.mla_attend(cache, q_lat.expand(B, -1, -1).cuda(), q_rope.expand(B, -1, -1).cuda(), i32(*range(B + 1)), i32(*[L] * B),
+                   pages.expand(B, -1).contiguous().cuda(), 1.0, out, lse=lse)
+    torch.cuda.synchronize()
+    assert torch.equal(out, out[:1].expand_as(out)) and torch.equal(lse, lse[:1].expand_as(lse))
+    k = C.widened(cache.latent.cpu(), cache.rope.cpu())
+    want, wlse, tol, ltol = C.attend(k, page, q_lat, q_rope, [0, 1], [L], pages, 1.0)
+    tail = want[0, 0, 1:256].mean()
+    assert 8e-4 < tail < 1.1e-3
+    if fmt == "f16":
+        tol = tol + 2.0 ** -32 * k[:L, :C.LAT].abs().sum(0)
+    C.check(out[:1].cpu(), want, tol, "out")
+    C.check(lse[:1].cpu(), wlse, ltol, "lse")
