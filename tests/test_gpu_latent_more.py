@@ -92,3 +92,30 @@ def test_one_strong_position_among_many_weak_ones(fdm, fmt, strong):
         tol = tol + 2.0 ** -32 * k[:L, :C.LAT].abs().sum(0)
     C.check(out[:1].cpu(), want, tol, "out")
     C.check(lse[:1].cpu(), wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "fp8"])
+@pytest.mark.parametrize("step", [0.3, 3.0])
+def test_scores_that_grow_along_the_sequence(fdm, fmt, step):
+    """Every 32 positions have a larger maximum than all before them, by `step` in
+    log2 a position: the running maximum moves again and again in every row."""
+    g = rng(7)
+    page, L, H, n = 16, 700, 24, 5
+    t = torch.float16 if fmt == "f16" else torch.bfloat16
+    cache = fdm.kv_cache(fmt, -(-L // page), page)
+    kv = normal(g, L, C.LAT + C.ROT)
+    kv[:, C.LAT] = torch.arange(L) * step * math.log(2.0) / 2.0  # rotary parts keep 16 bits in every format
+    fdm.kv_write(cache, kv.cuda(), torch.arange(L, dtype=torch.int32, device="cuda"))
+    q_lat, q_rope = normal(g, n, H, C.LAT, std=0.02).to(t), torch.zeros(n, H, C.ROT, dtype=t)
+    q_rope[:, :, 0] = 2.0
+    pages = torch.arange(cache.n_pages, dtype=torch.int32)[None]
+    out, lse = torch.empty(n, H, C.LAT, dtype=t, device="cuda"), torch.empty(n, H, device="cuda")
+    say(f"mla_attend {fmt}, scores growing by 2^{step} a position")
+    fdm.mla_attend(cache, q_lat.cuda(), q_rope.cuda(), i32(0, n), i32(L), pages.cuda(), 1.0, out, lse=lse)
+    torch.cuda.synchronize()
+    k = C.widened(cache.latent.cpu(), cache.rope.cpu(), None if cache.scale is None else cache.scale.cpu())
+    score = k[:, C.LAT] * 2.0 / math.log(2.0)
+    assert (score[32::32] - score[:-32:32][:score[32::32].numel()] > 8.0).all() or step < 1.0  # past what a weight may grow by
+    want, wlse, tol, ltol = C.attend(k, page, q_lat, q_rope, [0, n], [L], pages, 1.0)
+    C.check(out.cpu(), want, tol + (2.0 ** -32 * k[:L, :C.LAT].abs().sum(0) if fmt == "f16" else 0.0), "out")
+    C.check(lse.cpu(), wlse, ltol, "lse")
