@@ -2465,7 +2465,8 @@ int fdm_rope_table_init(const fdm_rope_params* p, fdm_rope_table* out) {
     // in double, as the definition: floor and ceil may turn on the last bit
     auto c = [&](double turns) { return p->dim * log(p->orig_ctx / (2.0 * M_PI * turns)) / (2.0 * log(p->base)); };
     lo = fmax(floor(c(p->beta_fast)), 0.0);
-    hi = fmin(ceil(c(p->beta_slow)), (double)(half - 1));
+    // cut at dim - 1, as the method has it: past the last pair, the ramp ends short of 1
+    hi = fmin(ceil(c(p->beta_slow)), (double)(p->dim - 1));
     if (hi < lo + 1) hi = lo + 1;
   }
   memset(out, 0, sizeof *out);

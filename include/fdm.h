@@ -441,8 +441,9 @@ int fdm_attn_release(int L);
  * f_i = base^(-2i / dim), for longer contexts scaled:
  *   FDM_ROPE_LINEAR  f_i / factor
  *   FDM_ROPE_YARN    f_i ((1 - m) / factor + m), m = 1 - clamp((i - lo) / (hi - lo), 0, 1),
- *     lo = max(floor(c(beta_fast)), 0), hi = min(ceil(c(beta_slow)), dim / 2 - 1), at least lo + 1,
- *     c(b) = dim ln(orig_ctx / (2 pi b)) / (2 ln base)   (infer.m:586-624)
+ *     lo = max(floor(c(beta_fast)), 0), hi = min(ceil(c(beta_slow)), dim - 1), at least lo + 1,
+ *     c(b) = dim ln(orig_ctx / (2 pi b)) / (2 ln base)   (infer.m:586-624 for dim 64, base
+ *     10000, orig_ctx 4096, where its cut at dim / 2 - 1 is the same: hi is 23)
  * fdm_rope_table_init fills a table on the host (no fdm_init needed): dim even,
  * 2 .. FDM_ROPE_MAX_DIM, base > 1, factor >= 1, mul finite (0: 1).  A table is
  * plain data and may be copied.  Its frequencies are fractions of a turn in
