@@ -535,8 +535,9 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
     _on_device(fn, q_lat, q_rope, q_start, kv_len, pages, out, mask, lse, workspace)
     words = 0
     if mask is not None:
-        if mask.dim() != 2 or mask.shape[0] != N:
-            _refuse(fn, f"mask: [{N}, words] is wanted, got {tuple(mask.shape)}")
+        # (without words it would have no address, which means no mask: tokens in order)
+        if mask.dim() != 2 or mask.shape[0] != N or mask.shape[1] < 1:
+            _refuse(fn, f"mask: [{N}, words] is wanted, a word at least, got {tuple(mask.shape)}")
         words = mask.shape[1]
         mask = _vector(fn, "mask", mask, N * words, _i64)
     if lse is not None:

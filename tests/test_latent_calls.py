@@ -1,0 +1,39 @@
+"""What the Python entry points of the latent operators hand on and what they refuse, on
+the CPU: the library's call is replaced by one that keeps its arguments."""
+import types
+
+import pytest
+import torch
+
+import flash_deepseek_amd as fdm
+
+BF = torch.bfloat16
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+    monkeypatch.setattr(fdm, "_on_device", lambda *a: None)
+    monkeypatch.setattr(fdm, "_call_stream", lambda s: 0)
+    monkeypatch.setattr(fdm, "call", lambda name, *a: made.append((name, a)))
+    return made
+
+
+def attend(N=3, H=4, B=2, **kw):
+    from flash_deepseek_amd import _lib
+    cache = types.SimpleNamespace(device=0, half=BF, desc=_lib.KvCacheDesc())
+    i = torch.zeros(B + 1, dtype=torch.int32)
+    a = dict(workspace=torch.zeros(1024, dtype=torch.uint8))
+    a.update(kw)
+    fdm.mla_attend(cache, torch.zeros(N, H, 512, dtype=BF), torch.zeros(N, H, 64, dtype=BF), i, i[:B], torch.zeros(B, 4, dtype=torch.int32), 1.0,
+                   torch.zeros(N, H, 512, dtype=BF), **a)
+
+
+def test_a_mask_without_words_is_refused(calls):
+    with pytest.raises(fdm.FdmError, match="a word at least"):
+        attend(mask=torch.zeros(3, 0, dtype=torch.int64))
+    assert calls == []
+    attend(mask=torch.zeros(3, 1, dtype=torch.int64))
+    attend()
+    batch = [a[1]._obj for _, a in calls]
+    assert batch[0].mask_words == 1 and batch[0].mask and batch[1].mask_words == 0 and not batch[1].mask
