@@ -552,6 +552,8 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
         with torch.cuda.stream(torch.cuda.current_stream(q_lat.device) if stream is None
                                else torch.cuda.ExternalStream(handle, device=q_lat.device)):
             workspace = mla_workspace(N, H)
+    elif not workspace.is_contiguous():  # its numel would not be the bytes behind its address
+        _refuse(fn, "workspace: contiguous memory is wanted")
     call("fdm_mla_attend", ctypes.byref(cache.desc), ctypes.byref(batch), q_lat.data_ptr(), lt, lh, q_rope.data_ptr(), rt,
          rh, scale, out.data_ptr(), ot, oh, lse, workspace.data_ptr(), workspace.numel() * workspace.element_size(), handle)
 

@@ -37,3 +37,14 @@ def test_a_mask_without_words_is_refused(calls):
     attend()
     batch = [a[1]._obj for _, a in calls]
     assert batch[0].mask_words == 1 and batch[0].mask and batch[1].mask_words == 0 and not batch[1].mask
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(1, dtype=torch.uint8).expand(1 << 40), torch.zeros(2048, dtype=torch.uint8)[::2],
+                                       torch.zeros(32, 64, dtype=torch.uint8).t()])
+def test_a_workspace_that_is_not_contiguous_is_refused(calls, workspace):
+    """A size in elements says how many bytes lie behind the address only then."""
+    with pytest.raises(fdm.FdmError, match="contiguous"):
+        attend(workspace=workspace)
+    assert calls == []
+    attend(workspace=torch.zeros(64, 32, dtype=torch.float32))
+    assert calls[0][1][-2] == 64 * 32 * 4
