@@ -538,8 +538,8 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
         # (without words it would have no address, which means no mask: tokens in order)
         if mask.dim() != 2 or mask.shape[0] != N or mask.shape[1] < 1:
             _refuse(fn, f"mask: [{N}, words] is wanted, a word at least, got {tuple(mask.shape)}")
-        words = mask.shape[1]
-        mask = _vector(fn, "mask", mask, N * words, _i64)
+        words = mask.shape[1] if N else 0  # no tokens: no words either
+        mask = _vector(fn, "mask", mask, N * words, _i64) if N else None
     if lse is not None:
         if lse.shape != (N, H):
             _refuse(fn, f"lse: {(N, H)} is wanted, got {tuple(lse.shape)}")

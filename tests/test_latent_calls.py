@@ -48,3 +48,13 @@ def test_a_workspace_that_is_not_contiguous_is_refused(calls, workspace):
     assert calls == []
     attend(workspace=torch.zeros(64, 32, dtype=torch.float32))
     assert calls[0][1][-2] == 64 * 32 * 4
+
+
+def test_a_step_without_tokens_may_have_a_mask(calls):
+    attend(N=0, mask=torch.zeros(0, 2, dtype=torch.int64))
+    batch = calls[0][1][1]._obj
+    assert batch.N == 0 and batch.mask_words == 0 and not batch.mask
+    # what the library takes that for
+    from flash_deepseek_amd import _lib
+    from tests.test_latent_args import INVAL, attend as c_attend
+    assert c_attend(N=0, ql=None) in (_lib.FDM_E_STATE, _lib.FDM_OK) and c_attend(N=0, ql=None, mask_words=2) == INVAL
