@@ -70,23 +70,24 @@ template <int R, int S>
 FDM_HD int64_t units_before(const SeqWork& s, int tiles, int H, bool in_order) {
   if (!in_order || s.n <= 1) return (int64_t)tiles * tile_units<R, S>(s, 0, H, in_order);
   int64_t sum = 0;
-  if (s.len < s.n) {  // tokens before the first position: tiles of one step
-    for (int i = 0; i < tiles; ++i) sum += tile_steps<R, S>(s, i, H, in_order);
-    return sum + (int64_t)tiles * kTileCost;
-  }
   // ceil((before + last) / S) each, before the positions in front of the tokens
   // and last the tile's last token (from 1): k (i + 1) with k = R / H whole tokens a
   // tile, else floor((R (i + 1) - 1) / H) + 1; the sequence's last tile may have fewer
-  const int64_t before = s.len - s.n;
+  // than R rows.  Tokens before the first position (before < 0): the tiles that see
+  // nothing, those of the first -before H rows, have one step.
+  const int64_t before = (int64_t)s.len - s.n;
   const int whole = tiles == tiles_of<R>(s, H) ? tiles - 1 : tiles, k = R / H;
-  if (whole < tiles) sum = (s.len + S - 1) / S;
+  if (whole < tiles) sum = s.len > S ? ((int64_t)s.len + S - 1) / S : 1;
   if (whole > 0) {
-    if (R % H == 0 && S % k == 0) {  // with before in whole k, rounded up, ceil((before / k + i) / (S / k))
+    if (before >= 0 && R % H == 0 && S % k == 0) {  // with before in whole k, rounded up, ceil((before / k + i) / (S / k))
       const int kb = __builtin_ctz(k), per = __builtin_ctz(S) - kb;
       const int64_t p = (before + k - 1) >> kb;
       sum += step_sum(p + whole, per) - step_sum(p, per);
     } else {
-      sum += (int64_t)floor_sum(whole, (uint64_t)H * S, R, R - 1 + (uint64_t)H * (before + S));
+      const int dark = before < 0 ? (int)(-before * H) / R : 0, none = dark < whole ? dark : whole;
+      sum += none;
+      if (none < whole)
+        sum += (int64_t)floor_sum(whole - none, (uint64_t)H * S, R, (uint64_t)(R - 1 + (int64_t)R * none + H * (before + S)));
     }
   }
   return sum + (int64_t)tiles * kTileCost;

@@ -119,3 +119,23 @@ def test_scores_that_grow_along_the_sequence(fdm, fmt, step):
     want, wlse, tol, ltol = C.attend(k, page, q_lat, q_rope, [0, n], [L], pages, 1.0)
     C.check(out.cpu(), want, tol + (2.0 ** -32 * k[:L, :C.LAT].abs().sum(0) if fmt == "f16" else 0.0), "out")
     C.check(lse.cpu(), wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("n,L,H", [(300, 70, 40), (260, 0, 16), (150, 149, 128), (40, 33, 7)])
+def test_more_tokens_than_positions(fdm, n, L, H):
+    """Tokens in order that stand before the first position see nothing, over several tiles."""
+    g = rng(n)
+    page = 8
+    cache = fdm.kv_cache("bf16", 16 * 2, page)
+    cache.latent.copy_(normal(g, *cache.latent.shape))
+    cache.rope.copy_(normal(g, *cache.rope.shape))
+    q_lat, q_rope = normal(g, n + 3, H, C.LAT, std=0.6).bfloat16(), normal(g, n + 3, H, C.ROT, std=0.6).bfloat16()
+    pages = torch.randperm(32, generator=g)[:19 + 3].to(torch.int32)[None].expand(2, -1).contiguous()
+    out, lse = torch.full((n + 3, H, C.LAT), 7.0, dtype=torch.bfloat16, device="cuda"), torch.full((n + 3, H), 7.0, device="cuda")
+    say(f"mla_attend of {n} tokens in order over {L} positions, {H} heads, beside three over 170")
+    fdm.mla_attend(cache, q_lat.cuda(), q_rope.cuda(), i32(0, n, n + 3), i32(L, 170), pages.cuda(), SCALE, out, lse=lse)
+    torch.cuda.synchronize()
+    want, wlse, tol, ltol = C.attend(C.widened(cache.latent.cpu(), cache.rope.cpu()), page, q_lat, q_rope, [0, n, n + 3], [L, 170], pages, SCALE)
+    assert (wlse[:n - L] == -math.inf).all() and (want[:n - L] == 0).all()
+    C.check(out.cpu(), want, tol, "out")
+    C.check(lse.cpu(), wlse, ltol, "lse")

@@ -96,18 +96,38 @@ int main() {
 }
 """,
 }
+DRIVERS["quick"] = r"""
+#include <ctime>
+// sequences of more tokens than positions: counted without a walk over their tiles
+int main() {
+  const clock_t start = std::clock();
+  int64_t all = 0;
+  for (int len : {0, 1, 100, 5000, 1048575}) {
+    const SeqWork s{1 << 20, len, 0};
+    for (int H : {128, 127, 16, 1})
+      for (int t = 0; t < 2000; ++t) all += units_before<R, S>(s, tiles_of<R>(s, H) - t, H, true);
+  }
+  const double seconds = (double)(std::clock() - start) / CLOCKS_PER_SEC;
+  std::printf("%.3f s for 40000 sums (%lld)", seconds, (long long)all);
+  return seconds > 2.0;  // 40000 sums of a few divisions; a walk over up to 2^20 tiles each takes minutes
+}
+"""
 
 
 def run(tmp_path, name):
     src, exe = tmp_path / f"{name}.cpp", tmp_path / name
     src.write_text(HEAD + DRIVERS[name])
     subprocess.run(["g++", "-std=c++17", "-O2", "-w", "-D__HIP_PLATFORM_AMD__", "-I", CSRC, "-I", "/opt/rocm/include", str(src), "-o", str(exe)], check=True)
-    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600)
     assert out.returncode == 0, out.stdout
 
 
 def test_sums_over_tiles(tmp_path):
     run(tmp_path, "sums")
+
+
+def test_more_tokens_than_positions(tmp_path):
+    run(tmp_path, "quick")
 
 
 def test_more_than_32_bits_of_units(tmp_path):
