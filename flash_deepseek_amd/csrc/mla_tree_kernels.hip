@@ -86,8 +86,9 @@ struct Half {
 // for one, so the source sees to them:
 //  - an operand that an ALU instruction wrote needs two states before the
 //    product: every operand here was loaded, from LDS or memory;
-//  - a result needs 11 states (8 passes and 3) before an ALU instruction reads
-//    it: products_done() stands before such reads;
+//  - a result needs 12 states before an ALU instruction reads it (what this
+//    compiler keeps behind its own such products on gfx950): products_done()
+//    stands before such reads;
 //  - products that add to one sum need none between them.
 #define FDM_MFMA_OF(FMT, form, ...)                               \
   if constexpr (FMT == kKvF16) {                                  \
