@@ -2648,7 +2648,9 @@ int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_
       !aligned(d_lse, 4) || !aligned(d_workspace, 256) || !aligned(d_q_lat, 16) || !aligned(d_q_rope, 16) ||
       !aligned(d_out, 16))
     return fail(FDM_E_INVAL, "misaligned pointer (q_lat, q_rope, out: 16 bytes, workspace: 256)");
-  for (int64_t s : {q_lat_token, q_lat_head, q_rope_token, q_rope_head, out_token, out_head})
+  // (strides of a single token or head say nothing)
+  for (int64_t s : {b->N > 1 ? q_lat_token : 0, b->H > 1 ? q_lat_head : 0, b->N > 1 ? q_rope_token : 0,
+                    b->H > 1 ? q_rope_head : 0, b->N > 1 ? out_token : 0, b->H > 1 ? out_head : 0})
     if (s % 8) return fail(FDM_E_INVAL, "stride %lld: a multiple of 8 elements", (long long)s);
   if (!rows_apart(out_head, b->H, out_token, b->N, FDM_KV_LATENT))
     return fail(FDM_E_INVAL, "out: rows of %d overlap", FDM_KV_LATENT);

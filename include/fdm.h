@@ -536,7 +536,8 @@ int fdm_kv_read(const fdm_kv_cache *cache, const int32_t *d_slots, int T, void *
  * page_size (and 2^31 - 4097), q_start to 0 .. N.  Rows of out and lse outside every sequence
  * are left as they were; sequences must not share tokens.
  * q_lat [N][H][512], q_rope [N][H][64], out [N][H][512]: F16 for an F16 cache,
- * else BF16; strides in elements, multiples of 8, 16-byte aligned.  lse
+ * else BF16; strides in elements, multiples of 8 where there is more than one
+ * token or head, 16-byte aligned.  lse
  * (optional) fp32 [N][H].  Products of the 16-bit values accumulate in fp32 and
  * softmax weights round to 16 bits before the second product (relative; in F16 by
  * no less than 2^-32 of the row's largest, so that weights below that add to lse

@@ -58,3 +58,17 @@ def test_a_step_without_tokens_may_have_a_mask(calls):
     from flash_deepseek_amd import _lib
     from tests.test_latent_args import INVAL, attend as c_attend
     assert c_attend(N=0, ql=None) in (_lib.FDM_E_STATE, _lib.FDM_OK) and c_attend(N=0, ql=None, mask_words=2) == INVAL
+
+
+def test_strides_of_a_single_token_or_head_are_free():
+    """A tensor's stride along an axis of one element may be anything (a column turned into a row has 1)."""
+    from flash_deepseek_amd import _lib
+    from tests.test_latent_args import INVAL, STATE, attend as c_attend
+    if _lib.lib.fdm_available():
+        pytest.skip("library already initialised in this process")
+    row = torch.zeros(512, 1).t()[:, None]
+    assert row.shape == (1, 1, 512) and row.stride()[0] == 1
+    assert c_attend(N=1, ql0=1, qr0=3, o0=1) == STATE
+    assert c_attend(H=1, ql1=1, qr1=3, o1=1) == STATE
+    for bad in (dict(ql0=1), dict(qr0=3), dict(o0=2049), dict(ql1=1), dict(qr1=3), dict(o1=513)):
+        assert c_attend(**bad) == INVAL, bad
