@@ -281,8 +281,8 @@ struct Range {
 // so few units are not spread over all workgroups: U units over G take 2 U / G us
 // of steps and about 0.13 G us of parts, least at G = sqrt(15 U); but no fewer than
 // there are tiles, and two units at least.  One token of 128 heads over 1024
-// positions in ranges of two 27.7 us, of one 30.0; over 32768 in ranges of eight 48,
-// of four 62; eight sequences of one token over 4096 47 and 52.
+// positions in ranges of two 20.3 us, of one 21.4; over 32768 in ranges of eight 47,
+// of four 60; eight sequences of one token over 4096 44 and 52.
 __device__ __forceinline__ uint32_t range_count(const MlaTreeArgs& a, uint64_t total) {
   const uint32_t tiles = (uint32_t)(((int64_t)a.N * a.H + kTileRows - 1) / kTileRows) + a.B;  // at most
   const uint32_t few = max((uint32_t)__builtin_amdgcn_sqrtf(15.0f * (float)total), tiles);
@@ -406,8 +406,8 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     // they are is known to all its lanes, and a piece is two rows; positions behind
     // the sequence's end are read as they are, and hidden.  Otherwise a lane
     // looks after the row that it is one of eight of, and a piece is one row: 85
-    // instructions more a step, 74 us against 69 for 128 sequences of three tokens
-    // of 16 heads over 2048 positions, 635 against 621 for 512 tokens of 128 over 4608.
+    // instructions more a step, 81 us against 77 for 128 sequences of three tokens
+    // of 16 heads over 2048 positions, 577 against 562 for 512 tokens of 128 over 4608.
     constexpr bool kCodes = FMT == kKvFp8;
     constexpr int kBring = kCodes || WHOLE ? 8 : 12;
     const int my_row = 8 * wave + (lane >> 3);
@@ -558,7 +558,10 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
     // order and has its SIMD alone, so a piece is what is issued while one product
     // is worked on, and nothing stands next to what it needs: one piece has a
     // pair's exponents, one the sum and rounding of the pair before and the
-    // products of the pair after the next.
+    // products of the pair after the next.  Weights round to the cache's 16-bit type,
+    // the only one that the second product takes beside its values (in two 16-bit
+    // halves they would double its 32 of a step's 68 matrix instructions); their sum is
+    // that of the unrounded ones, in fp32.
     constexpr int kWeigh = 23;
     float top = 0.0f, off = 0.0f;
     auto hide = [&](uint32_t see) {
@@ -894,7 +897,7 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
 // dims; 256 threads of four dims each, S times over for every S-th part.  A thread
 // reads its row's statistics itself, twice, from the caches, and requests the first
 // parts before them.  Few tiles of many parts are bound by latency (I = 1, S = 4:
-// one token over 1024 positions, 16 parts, 4.8 us; I = 8, S = 1 would have 8
+// one token over 1024 positions, 16 parts, 4.6 us; I = 8, S = 1 would have 8
 // workgroups there), many of few by memory (I = 8, S = 1: 64 sequences of one token
 // over 4095 positions, 82 MB of parts, 17.5 us; blocks of four at a time 1 % more of
 // the whole).

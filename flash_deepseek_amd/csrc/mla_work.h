@@ -6,7 +6,7 @@
 // least, so that rows that see nothing are written) and counts kTileCost units
 // more, what beginning and ending it costs a workgroup (queries, first steps,
 // results: about 12 us against 2 us a step; 64 sequences of one token over 4095
-// positions 119 us without, 114 with four, 112 with six).  The units of all tiles
+// FP8 positions 94.5 us without, 90.9 with four, 86.3 with six).  The units of all tiles
 // in order (sequence, tile, unit) are cut into equal ranges, one a workgroup.
 #pragma once
 
@@ -48,8 +48,9 @@ FDM_HD int64_t step_sum(int64_t x, int k) {
   const int64_t q = x >> k, r = x & ((1 << k) - 1);
   return ((q * (q + 1) / 2) << k) + r * (q + 1);
 }
-// sum over i < n of floor((a i + b) / m): whole parts of a and b are taken out,
-// and the points under what is left of the line are counted along the other axis.
+// sum over i < n of floor((a i + b) / m), the lattice points under a line, by the
+// known reduction along Euclid's algorithm: whole parts of a and b are taken out, and
+// the points under what is left of the line are counted along the other axis.
 FDM_HD uint64_t floor_sum(uint64_t n, uint64_t m, uint64_t a, uint64_t b) {
   uint64_t sum = 0;
   for (;;) {
