@@ -580,10 +580,11 @@ __global__ __launch_bounds__(256, 1) void k_mla_tree(MlaTreeArgs a) {
         for (int i = 0; i < 4; ++i) t[i] = fmaxf(fmaxf(t[i], c[8 + i]), c[12 + i]);
         top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       } else if (piece == 1) {
-        top = across_halves(top, [](float x, float y) { return fmaxf(x, y); }) * a.scale_log2;
-        const bool need = top > m + (kGrow + kAbove<FMT>);
+        // s - m rounded as a weight's is, so that none passes its limit however coarse s is
+        top = across_halves(top, [](float x, float y) { return fmaxf(x, y); });
+        const bool need = fmaf(top, a.scale_log2, -m) > kGrow + kAbove<FMT>;
         if (rare(__any(need))) {
-          const float to_m = top - kAbove<FMT>;
+          const float to_m = fmaf(top, a.scale_log2, -kAbove<FMT>);
           const float keep = need ? __builtin_amdgcn_exp2f(m - to_m) : 1.0f;
           m = need ? to_m : m;
           l *= keep;

@@ -139,3 +139,32 @@ def test_more_tokens_than_positions(fdm, n, L, H):
     assert (wlse[:n - L] == -math.inf).all() and (want[:n - L] == 0).all()
     C.check(out.cpu(), want, tol, "out")
     C.check(lse.cpu(), wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16"])
+@pytest.mark.parametrize("grow,scale", [(1, 2.0794), (2, 2.0794), (1, 0.75), (5, 0.5123)])
+def test_scores_of_2_to_25(fdm, fmt, grow, scale):
+    """Scores whose fp32 neighbours are 4 apart (exact sums: 2^25 and multiples of 4): the
+    reference of a row is rounded by up to 4 in log2, and no weight may pass the type's
+    range for it.  With (1, 2.0794) a comparison of rounded maxima let one reach 2^20.
+    Weights round by half a step of the type, exponents by 2^-18 with the exponential's own."""
+    g = rng(8)
+    page, L, H, B = 32, 128, 2, 512
+    t, step = C.DTYPES[fmt], C.HALF_STEP[C.DTYPES[fmt]]
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    rows = normal(g, L, C.LAT)
+    rows[:, 0], rows[:, 1] = 8192.0, 4.0 * grow * (torch.arange(L) // 32)
+    cache = fdm.kv_cache(fmt, L // page, page)
+    cache.latent.flatten(0, 1).copy_(rows)
+    q_lat, q_rope = torch.zeros(B, H, C.LAT, dtype=t), torch.zeros(B, H, C.ROT, dtype=t)
+    q_lat[:, :, 0], q_lat[:, :, 1] = 4096.0, 1.0
+    pages = torch.arange(L // page, dtype=torch.int32)[None].expand(B, -1).contiguous()
+    out = torch.empty(B, H, C.LAT, dtype=t, device="cuda")
+    say(f"mla_attend {fmt}, scores of 2^25 growing by {4 * grow} times {scale}")
+    fdm.mla_attend(cache, q_lat.cuda(), q_rope.cuda(), i32(*range(B + 1)), i32(*[L] * B), pages.cuda(), scale, out)
+    torch.cuda.synchronize()
+    k = cache.latent.cpu().flatten(0, 1).double()
+    p = torch.softmax(k[:, 1] * scale, 0)  # the 2^25 is the same in all
+    want = p @ k
+    tol = p @ k.abs() * (step + 2.0 ** -18) + (2.0 ** -32 * k.abs().sum(0) if fmt == "f16" else 0.0) + want.abs() * step
+    C.check(out.cpu(), want.expand(B, H, -1), tol, "out")
