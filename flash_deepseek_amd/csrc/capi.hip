@@ -247,6 +247,7 @@ struct State {
   std::mutex turn_mu;  // held from a one-launch kernel's wait to its event
   LaunchTurns turns;
   hipEvent_t turn_done = nullptr;
+  std::mutex mla_mu;  // held from the launch of an attention to that of its join
   Layer layers[FDM_MAX_LAYERS];
   DenseLayer dense[FDM_MAX_LAYERS];
   std::unique_ptr<StreamedLayer> streamed[FDM_MAX_LAYERS];
@@ -2691,6 +2692,9 @@ int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_
   a.lse = d_lse;
   a.workspace = d_workspace;
   OnDevice dev;
+  // two threads' calls on one stream may share a workspace: one's join must not stand
+  // behind the other's parts
+  std::lock_guard<std::mutex> lock(g.mla_mu);
   ProfScope prof(FDM_PROF_MLA, as_stream(stream));
   FDM_HIP(launch_mla_tree(a, c->format, as_stream(stream)));
   return FDM_OK;

@@ -168,3 +168,45 @@ def test_scores_of_2_to_25(fdm, fmt, grow, scale):
     want = p @ k
     tol = p @ k.abs() * (step + 2.0 ** -18) + (2.0 ** -32 * k.abs().sum(0) if fmt == "f16" else 0.0) + want.abs() * step
     C.check(out.cpu(), want.expand(B, H, -1), tol, "out")
+
+
+def test_two_threads_on_one_stream_share_a_workspace(fdm):
+    """Calls on one stream run in its order, from whichever thread they come: a call's
+    two launches follow each other."""
+    import threading
+    g = rng(9)
+    page, H = 64, 128
+    cache = fdm.kv_cache("bf16", 64, page)
+    cache.latent.copy_(normal(g, *cache.latent.shape))
+    cache.rope.copy_(normal(g, *cache.rope.shape))
+    pages = torch.randperm(64, generator=g).to(torch.int32)[None].cuda()
+    space = fdm.mla_workspace(4, H)
+    sizes = [(1, 4000), (3, 2100)]  # one tile of many parts; three tiles
+    args = []
+    for n, L in sizes:
+        q_lat, q_rope = normal(g, n, H, C.LAT, std=0.6).bfloat16().cuda(), normal(g, n, H, C.ROT, std=0.6).bfloat16().cuda()
+        args.append((cache, q_lat, q_rope, i32(0, n), i32(L), pages, SCALE))
+    want = [torch.empty_like(a[1]) for a in args]
+    for a, o in zip(args, want):
+        fdm.mla_attend(*a, o, workspace=space)
+    torch.cuda.synchronize()
+    say("two threads x 300 calls on the null stream, one workspace")
+    got = [[torch.empty_like(w) for _ in range(300)] for w in want]
+    errors = []
+
+    def worker(i):
+        try:
+            for o in got[i]:
+                fdm.mla_attend(*args[i], o, workspace=space, stream=0)
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=worker, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=60)
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for w, outs in zip(want, got):
+        assert all(torch.equal(o, w) for o in outs)
