@@ -17,7 +17,8 @@ for this path, over the C ABI of libfdm.so (include/fdm.h):
   expert streaming (flash)      :1478-1602 stream_layer / moe_layer_streamed
   mla_forward                   :766-903   attn_upload / attn_forward
     (its parts for several          -      rope / kv_write / kv_read / mla_attend
-     sequences and drafted tokens)
+     sequences and drafted tokens,         kv_grow / kv_trim / add_rms_norm / project
+     what stands between them)
   layer_forward dense branch    :1852-1868 dense_ffn (weights: upload_dense /
                                            attach_dense / load_dense_gguf)
 
@@ -38,6 +39,7 @@ __all__ = [
     "moe_forward_host", "moe_layer", "f32_to_f16", "upload_dense", "attach_dense", "load_dense_gguf",
     "release_dense", "dense_info", "dense_ffn", "DENSE_FFN", "stream_layer", "moe_layer_streamed",
     "stream_stats", "rope_table", "rope", "KvCache", "kv_cache", "kv_write", "kv_read", "mla_workspace", "mla_attend",
+    "KvPages", "kv_pages", "kv_grow", "kv_trim", "add_rms_norm", "Adapters", "project_workspace", "project",
     "attn_upload", "attn_load_gguf", "attn_forward", "attn_reset", "attn_len", "attn_release", "set_batch_kernel", "BATCH_AUTO", "BATCH_DOT4", "BATCH_MFMA", "prof_enable", "prof_reset", "prof_read", "synth_q4k", "synth_q6k", "synth_normal", "FdmError",
     "QK_K", "Q4K_BLOCK_SIZE", "Q6K_BLOCK_SIZE", "HIDDEN", "MOE_FFN", "N_EXPERTS", "MAX_K",
     "MAX_LAYERS", "MAX_TOKENS", "EXPERT_Q4K_BYTES", "EXPERT_Q6K_BYTES",
@@ -324,7 +326,7 @@ ROPE_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 KV_FORMATS = {"f16": _lib.KV_F16, "bf16": _lib.KV_BF16, "fp8": _lib.KV_FP8}
 _device = None  # of init()
 _types = {}     # torch dtype -> element type
-_i32 = _i64 = _f32 = None  # torch's (imported lazily)
+_i32 = _i64 = _f32 = _f16 = _bf16 = _e4m3 = None  # torch's (imported lazily)
 
 
 def _refuse(fn, why):
@@ -332,9 +334,10 @@ def _refuse(fn, why):
 
 
 def _load_types():
-    global _i32, _i64, _f32
+    global _i32, _i64, _f32, _f16, _bf16, _e4m3
     import torch
     _i32, _i64, _f32 = torch.int32, torch.int64, torch.float32
+    _f16, _bf16, _e4m3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
     _types.update({torch.float32: _lib.GGML_F32, torch.float16: _lib.GGML_F16, torch.bfloat16: _lib.GGML_BF16})
 
 
@@ -558,6 +561,200 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
          rh, scale, out.data_ptr(), ot, oh, lse, workspace.data_ptr(), workspace.numel() * workspace.element_size(), handle)
 
 
+# ---- what stands between the attention of one layer and of the next ---------------------
+class KvPages:
+    """The books of a paged cache (int32 tensors of the caller, kept alive here and
+    changed in place): pages [B, P] the page numbers of each sequence, kv_len [B]
+    its cached positions, free [n_pages] a stack of free pages, n_free [1] how
+    many.  No two sequences have a page in common."""
+
+    def __init__(self, pages, kv_len, free, n_free, page_size):
+        import torch
+        fn = "KvPages"
+        if pages.dim() != 2:
+            _refuse(fn, f"pages: [sequences, pages of each] is wanted, got {tuple(pages.shape)}")
+        if not _types:
+            _load_types()
+        (B, P), n = pages.shape, free.numel()
+        _on_device(fn, pages, kv_len, free, n_free)
+        at = [_vector(fn, name, t, k, _i32) for name, t, k in (("pages", pages, B * P), ("kv_len", kv_len, B), ("free", free, n),
+                                                               ("n_free", n_free, 1))]
+        if page_size < 1 or page_size & (page_size - 1):
+            _refuse(fn, f"page_size {page_size}: a power of two")
+        self.pages, self.kv_len, self.free, self.n_free, self.page_size = pages, kv_len, free, n_free, page_size
+        self._turn = torch.zeros(1, dtype=torch.int32, device=pages.device)
+        self.desc = _lib.KvPagesDesc(*at, self._turn.data_ptr(), B, P, n, page_size)
+        self.device = pages.get_device()
+
+
+def kv_pages(B, pages_per_seq, n_pages, page_size=64):
+    """KvPages of B empty sequences with room for pages_per_seq pages each, over a
+    cache of n_pages, all of them free."""
+    import torch
+    dev = torch.device("cuda", torch.cuda.current_device() if _device is None else _device)
+    return KvPages(torch.full((B, pages_per_seq), -1, dtype=torch.int32, device=dev), torch.zeros(B, dtype=torch.int32, device=dev),
+                   torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev),
+                   torch.full((1,), n_pages, dtype=torch.int32, device=dev), page_size)
+
+
+def _on_books_device(fn, pages):
+    if _device is not None and pages.device != _device:
+        _refuse(fn, f"the pages are on device {pages.device}, the library on device {_device}")
+
+
+def kv_grow(pages, new, q_start, pos, slots, refused=None, stream=None):
+    """Places for new [B] tokens of every sequence: pages are taken where they need
+    them, and q_start [B + 1] (their ranges), pos and slots [N] (position and slot
+    of each, what kv_write and mla_attend take) written; places behind the last
+    token get position 0 and slot -1.  A sequence whose row, whose pages or whose
+    places do not suffice gets none and stays as it was; refused [1] is their
+    number.  All int32."""
+    fn, B, N = "kv_grow", pages.desc.B, slots.numel()
+    if not _types:
+        _load_types()
+    _on_books_device(fn, pages)
+    _on_device(fn, new, q_start, pos, slots, refused)
+    call("fdm_kv_grow", ctypes.byref(pages.desc), _vector(fn, "new", new, B, _i32), N, _vector(fn, "q_start", q_start, B + 1, _i32),
+         _vector(fn, "pos", pos, N, _i32), _vector(fn, "slots", slots, N, _i32),
+         None if refused is None else _vector(fn, "refused", refused, 1, _i32), _call_stream(stream))
+
+
+def kv_trim(pages, keep, stream=None):
+    """Every sequence keeps its first keep [B] int32 positions (below 0, or more than
+    it has: all; 0 ends it); the pages behind them are free again."""
+    if not _types:
+        _load_types()
+    _on_books_device("kv_trim", pages)
+    _on_device("kv_trim", keep)
+    call("fdm_kv_trim", ctypes.byref(pages.desc), _vector("kv_trim", "keep", keep, pages.desc.B, _i32), _call_stream(stream))
+
+
+def _matrix(fn, name, t, shape):
+    """The row stride of a tensor of `shape` whose rows are contiguous."""
+    if t.shape != shape or (t.stride(1) != 1 and shape[1] > 1):
+        _refuse(fn, f"{name}: {tuple(shape)} with contiguous rows is wanted, got {tuple(t.shape)} of strides {t.stride()}")
+    return t.stride(0)
+
+
+def add_rms_norm(x, add, norm_w, out, scale=None, sum=None, eps=1e-6, stream=None):
+    """out = s / sqrt(mean(s^2) + eps) * norm_w with s = x + add, rows [T, d] in
+    float32, float16 or bfloat16; sum (x's type, may be x) receives s.  add and
+    norm_w (float32 [d]) may be None.  With scale (uint8 or float8_e8m0fnu
+    [T, ceil(d / 128)]) out is float8_e4m3fn: codes, and a power of two for every
+    128 values."""
+    fn = "add_rms_norm"
+    if x.dim() != 2:
+        _refuse(fn, f"x: [T, d] is wanted, got {tuple(x.shape)}")
+    T, d = shape = x.shape
+    if not _types:
+        _load_types()
+    _on_device(fn, x, add, norm_w, out, scale, sum)
+    xt = _elem(fn, "x", x.dtype)
+    if scale is None:
+        yt, ss = _elem(fn, "out", out.dtype), 0
+    else:
+        if out.dtype is not _e4m3 or scale.element_size() != 1:
+            _refuse(fn, f"with scales out is float8_e4m3fn and scale bytes, got {out.dtype} and {scale.dtype}")
+        yt, ss = _lib.E4M3, _matrix(fn, "scale", scale, (T, (d + 127) // 128))
+    if sum is not None and sum.dtype is not x.dtype:
+        _refuse(fn, f"sum: x's type {x.dtype} is wanted, got {sum.dtype}")
+    call("fdm_add_rms_norm", x.data_ptr(), xt, _matrix(fn, "x", x, shape),
+         None if add is None else add.data_ptr(), 0 if add is None else _elem(fn, "add", add.dtype),
+         0 if add is None else _matrix(fn, "add", add, shape),
+         None if sum is None else sum.data_ptr(), 0 if sum is None else _matrix(fn, "sum", sum, shape),
+         None if norm_w is None else _vector(fn, "norm_w", norm_w, d, _f32), eps, out.data_ptr(), yt,
+         _matrix(fn, "out", out, shape), None if scale is None else scale.data_ptr(), ss, T, d, _call_stream(stream))
+
+
+class Adapters:
+    """Low-rank adapters of one projection (tensors of the caller, kept alive here):
+    a [n, rank, in] and b [n, out, rank] in float16 (for float16 rows) or bfloat16,
+    times [n] float32 (None: 1) what their product is multiplied by."""
+
+    def __init__(self, a, b, times=None):
+        fn = "Adapters"
+        if not _types:
+            _load_types()
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            _refuse(fn, f"a, b: [n, rank, in] and [n, out, rank] are wanted, got {tuple(a.shape)} and {tuple(b.shape)}")
+        if a.dtype is not b.dtype or a.dtype not in (_f16, _bf16):
+            _refuse(fn, f"a, b: both float16 or both bfloat16 are wanted, got {a.dtype} and {b.dtype}")
+        if not a.is_contiguous() or not b.is_contiguous():
+            _refuse(fn, "a, b: not contiguous")
+        _on_device(fn, a, b, times)
+        self.n, self.rank, self.in_dim = a.shape
+        self.out_dim, self.dtype = b.shape[1], a.dtype
+        if not self.n or not self.rank:
+            _refuse(fn, "no adapters")
+        self.a, self.b, self.times = a, b, times
+        self.at = a.data_ptr(), b.data_ptr(), None if times is None else _vector(fn, "times", times, self.n, _f32)
+        self.device = a.get_device()
+
+
+def project_workspace(T, in_dim, out_dim, rank=0):
+    """A workspace for project calls of up to T rows of such a projection (with adapters
+    of that rank) that run one after the other."""
+    import torch
+    n = ctypes.c_size_t()
+    call("fdm_project_workspace", T, in_dim, out_dim, rank, ctypes.byref(n))
+    return torch.empty(n.value, dtype=torch.uint8, device=torch.device("cuda", _device or 0))
+
+
+def project(x, w, out, x_scale=None, w_scale=None, adapters=None, q_start=None, adapter=None, workspace=None, stream=None):
+    """out [T, out] = x [T, in] w^T, and beside it times_k b_k (a_k x_t) for row t of
+    request r with k = adapter[r] (int32 [B]; outside 0 .. n - 1: none), whose rows
+    are q_start[r] .. q_start[r + 1] - 1.  x and w [out, in] in float16 or
+    bfloat16, or float8_e4m3fn with x_scale [T, ceil(in / 128)] and w_scale
+    [ceil(out / 128), ceil(in / 128)] (uint8 or float8_e8m0fnu); out in float32,
+    float16 or bfloat16.  workspace: project_workspace's (None: allocated for
+    the call)."""
+    fn = "project"
+    if x.dim() != 2 or w.dim() != 2:
+        _refuse(fn, f"x, w: [T, in] and [out, in] are wanted, got {tuple(x.shape)} and {tuple(w.shape)}")
+    if not _types:
+        _load_types()
+    (T, inner), n_out = x.shape, w.shape[0]
+    fp8 = x.dtype is _e4m3
+    if w.dtype is not x.dtype or not (fp8 or x.dtype is _f16 or x.dtype is _bf16):
+        _refuse(fn, f"x, w: both float16, bfloat16 or float8_e4m3fn are wanted, got {x.dtype} and {w.dtype}")
+    if (x_scale is None) == fp8 or (w_scale is None) == fp8:
+        _refuse(fn, "scales: float8_e4m3fn rows and matrices have them, the others none")
+    _on_device(fn, x, w, out, x_scale, w_scale, q_start, adapter, workspace)
+    xs = 0
+    if fp8:
+        groups = (inner + 127) // 128
+        xs = _matrix(fn, "x_scale", x_scale, (T, groups))
+        if x_scale.element_size() != 1 or w_scale.element_size() != 1 or w_scale.shape != ((n_out + 127) // 128, groups) or not w_scale.is_contiguous():
+            _refuse(fn, f"scales: bytes, w_scale {((n_out + 127) // 128, groups)} contiguous, got {x_scale.dtype}, {w_scale.dtype} {tuple(w_scale.shape)}")
+    p = _lib.Projection(_lib.E4M3 if fp8 else _types[x.dtype], T, inner, n_out, x.data_ptr(), _matrix(fn, "x", x, (T, inner)),
+                        None if x_scale is None else x_scale.data_ptr(), xs, w.data_ptr(), _matrix(fn, "w", w, (n_out, inner)),
+                        None if w_scale is None else w_scale.data_ptr(), out.data_ptr(), _matrix(fn, "out", out, (T, n_out)),
+                        _elem(fn, "out", out.dtype))
+    rank = 0
+    if adapters is not None:
+        if adapters.in_dim != inner or adapters.out_dim != n_out:
+            _refuse(fn, f"the adapters are {adapters.out_dim} x {adapters.in_dim}, the matrix {n_out} x {inner}")
+        if adapters.dtype is not (_f16 if x.dtype is _f16 else _bf16):
+            _refuse(fn, f"adapters of {adapters.dtype} beside {x.dtype}")
+        if _device is not None and adapters.device != _device:
+            _refuse(fn, f"the adapters are on device {adapters.device}, the library on device {_device}")
+        if q_start is None or adapter is None:
+            _refuse(fn, "adapters need q_start and adapter")
+        p.n_adapters, p.rank, p.B = adapters.n, adapters.rank, adapter.numel()
+        p.a, p.b, p.times = adapters.at
+        p.q_start, p.adapter = _vector(fn, "q_start", q_start, p.B + 1, _i32), _vector(fn, "adapter", adapter, p.B, _i32)
+        rank = adapters.rank
+    handle = _call_stream(stream)
+    if workspace is None:  # torch's allocator keeps it for the stream that it is made on
+        import torch
+        with torch.cuda.stream(torch.cuda.current_stream(x.device) if stream is None
+                               else torch.cuda.ExternalStream(handle, device=x.device)):
+            workspace = project_workspace(T, inner, n_out, rank)
+    elif not workspace.is_contiguous():  # its numel would not be the bytes behind its address
+        _refuse(fn, "workspace: contiguous memory is wanted")
+    call("fdm_project", ctypes.byref(p), workspace.data_ptr(), workspace.numel() * workspace.element_size(), handle)
+
+
 # ---- dense FFN layers (layer_forward's branch for L < 3) ------------------------------
 def f32_to_f16(src, dst, n=None, stream=None):
     """(__fp16) cast of f32_to_f16_alloc on the device: fp32 -> F16 bits."""
@@ -605,7 +802,7 @@ PHASES = {"router": _lib.PROF_ROUTER, "gateup": _lib.PROF_GATEUP, "down": _lib.P
           "xdigits": _lib.PROF_XDIGITS, "matvec": _lib.PROF_MATVEC, "layer": _lib.PROF_LAYER,
           "batch": _lib.PROF_BATCH, "prefill": _lib.PROF_PREFILL, "dense": _lib.PROF_DENSE,
           "attn": _lib.PROF_ATTN, "ceiling": _lib.PROF_CEILING, "rope": _lib.PROF_ROPE, "kv": _lib.PROF_KV,
-          "mla": _lib.PROF_MLA}
+          "mla": _lib.PROF_MLA, "norm": _lib.PROF_NORM, "project": _lib.PROF_PROJECT}
 
 
 def prof_enable(on=True):

@@ -20,7 +20,8 @@ FDM_E_IO = -7
 FDM_E_FORMAT = -8
 
 (PROF_ROUTER, PROF_GATEUP, PROF_DOWN, PROF_XDIGITS, PROF_MATVEC, PROF_LAYER, PROF_BATCH,
- PROF_PREFILL, PROF_DENSE, PROF_ATTN, PROF_CEILING, PROF_ROPE, PROF_KV, PROF_MLA) = range(14)
+ PROF_PREFILL, PROF_DENSE, PROF_ATTN, PROF_CEILING, PROF_ROPE, PROF_KV, PROF_MLA,
+ PROF_NORM, PROF_PROJECT) = range(16)
 
 QK_K = 256
 Q4K_BLOCK_SIZE = 144
@@ -43,6 +44,7 @@ class AttnWeights(ctypes.Structure):
 
 ROPE_MAX_DIM = 256
 GGML_F32, GGML_F16, GGML_BF16 = 0, 1, 30  # element types
+E4M3 = 100
 KV_LATENT, KV_ROPE = 512, 64
 KV_F16, KV_BF16, KV_FP8 = range(3)
 
@@ -70,6 +72,22 @@ class MlaBatch(ctypes.Structure):
     _fields_ = [("B", ctypes.c_int), ("N", ctypes.c_int), ("H", ctypes.c_int), ("q_start", ctypes.c_void_p),
                 ("kv_len", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("pages_stride", ctypes.c_int),
                 ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_int)]
+
+
+class KvPagesDesc(ctypes.Structure):
+    """struct fdm_kv_pages."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("pages", "kv_len", "free", "n_free", "turn")] + [
+        (n, ctypes.c_int) for n in ("B", "pages_stride", "n_pages", "page_size")]
+
+
+class Projection(ctypes.Structure):
+    """struct fdm_projection."""
+    _fields_ = [("type", ctypes.c_int), ("T", ctypes.c_int), ("in_dim", ctypes.c_int), ("out_dim", ctypes.c_int),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("x_scale", ctypes.c_void_p),
+                ("x_scale_stride", ctypes.c_int64), ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64),
+                ("w_scale", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("y_type", ctypes.c_int),
+                ("n_adapters", ctypes.c_int), ("rank", ctypes.c_int), ("B", ctypes.c_int), ("a", ctypes.c_void_p),
+                ("b", ctypes.c_void_p), ("times", ctypes.c_void_p), ("q_start", ctypes.c_void_p), ("adapter", ctypes.c_void_p)]
 
 
 EXPERT_Q4K_BYTES = 24772608
@@ -143,6 +161,11 @@ SIGNATURES = {
     "fdm_mla_workspace": [_i, _i, ctypes.POINTER(_sz)],
     "fdm_mla_attend": [ctypes.POINTER(KvCacheDesc), ctypes.POINTER(MlaBatch), _vp, _i64, _i64, _vp, _i64, _i64, _f,
                        _vp, _i64, _i64, _vp, _vp, _sz, _vp],
+    "fdm_kv_grow": [ctypes.POINTER(KvPagesDesc), _vp, _i, _vp, _vp, _vp, _vp, _vp],
+    "fdm_kv_trim": [ctypes.POINTER(KvPagesDesc), _vp, _vp],
+    "fdm_add_rms_norm": [_vp, _i, _i64, _vp, _i, _i64, _vp, _i64, _vp, _f, _vp, _i, _i64, _vp, _i64, _i, _i, _vp],
+    "fdm_project_workspace": [_i, _i, _i, _i, ctypes.POINTER(_sz)],
+    "fdm_project": [ctypes.POINTER(Projection), _vp, _sz, _vp],
     "fdm_prof_enable": [_i],
     "fdm_prof_reset": [],
     "fdm_prof_read": [_i, ctypes.POINTER(_i), ctypes.POINTER(ctypes.c_double),

@@ -36,6 +36,9 @@ SOURCES = [
     "rope_kernels.hip",
     "kvcache_kernels.hip",
     "mla_tree_kernels.hip",
+    "kvpages_kernels.hip",
+    "norm_kernels.hip",
+    "project_kernels.hip",
     "gguf_host.hip",
     "capi.hip",
 ]

@@ -21,6 +21,7 @@
 #include "../../include/fdm.h"
 #include "epoch_book.h"
 #include "fdm_internal.h"
+#include "project_work.h"
 #include "launch_turns.h"
 #include "mla_work.h"
 
@@ -248,6 +249,7 @@ struct State {
   LaunchTurns turns;
   hipEvent_t turn_done = nullptr;
   std::mutex mla_mu;  // held from the launch of an attention to that of its join
+  std::mutex project_mu;  // held over the launches of a projection
   Layer layers[FDM_MAX_LAYERS];
   DenseLayer dense[FDM_MAX_LAYERS];
   std::unique_ptr<StreamedLayer> streamed[FDM_MAX_LAYERS];
@@ -2407,7 +2409,8 @@ int fdm_dense_ffn(int L, const float* d_h_post, const float* d_h_in, float* d_hi
 // Arguments are checked before anything of the device is needed.
 static_assert(sizeof(RopeTable) == sizeof(fdm_rope_table) && kRopeMaxDim == FDM_ROPE_MAX_DIM, "one table");
 static_assert(kKvF16 == FDM_KV_F16 && kKvBf16 == FDM_KV_BF16 && kKvFp8 == FDM_KV_FP8, "formats");
-static_assert(kMlaMaxSeqs == FDM_MLA_MAX_SEQS, "sequences");
+static_assert(kMlaMaxSeqs == FDM_MLA_MAX_SEQS && kKvMaxSeqs == FDM_KV_MAX_SEQS && kProjectMaxSeqs == FDM_PROJECT_MAX_SEQS, "sequences");
+static_assert(kNormMaxDim == FDM_NORM_MAX_DIM && kMaxAdapters == FDM_MAX_ADAPTERS && kMaxRank == FDM_MAX_RANK, "sizes");
 
 // The calling thread's device is the library's while this lives.
 struct OnDevice {
@@ -2697,6 +2700,215 @@ int fdm_mla_attend(const fdm_kv_cache* c, const fdm_mla_batch* b, const void* d_
   std::lock_guard<std::mutex> lock(g.mla_mu);
   ProfScope prof(FDM_PROF_MLA, as_stream(stream));
   FDM_HIP(launch_mla_tree(a, c->format, as_stream(stream)));
+  return FDM_OK;
+}
+
+// ---- the paged cache's books ----------------------------------------------------------
+static int check_pages(const fdm_kv_pages* p) {
+  if (!p) return fail(FDM_E_INVAL, "null pages");
+  if (p->B < 1 || p->B > FDM_KV_MAX_SEQS) return fail(FDM_E_INVAL, "%d sequences: 1 .. %d", p->B, FDM_KV_MAX_SEQS);
+  if (p->pages_stride < 1 || (int64_t)p->B * p->pages_stride > INT32_MAX)
+    return fail(FDM_E_INVAL, "a table of %d x %d pages: below 2^31 in all", p->B, p->pages_stride);
+  if (p->page_size < 1 || (p->page_size & (p->page_size - 1)) || p->n_pages < 1 ||
+      (int64_t)p->n_pages * p->page_size > INT32_MAX)
+    return fail(FDM_E_INVAL, "%d pages of %d rows: a power of two each, below 2^31 in all", p->n_pages, p->page_size);
+  const void* all[] = {p->d_pages, p->d_kv_len, p->d_free, p->d_n_free, p->d_turn};
+  for (const void* q : all)
+    if (!q || !aligned(q, 4)) return fail(FDM_E_INVAL, "pages: null or misaligned pointer");
+  return FDM_OK;
+}
+
+static KvPagesArgs pages_args(const fdm_kv_pages* p) {
+  KvPagesArgs a{};
+  a.pages = p->d_pages;
+  a.kv_len = p->d_kv_len;
+  a.free = p->d_free;
+  a.n_free = p->d_n_free;
+  a.turn = p->d_turn;
+  a.B = p->B;
+  a.P = p->pages_stride;
+  a.n_pages = p->n_pages;
+  a.shift = __builtin_ctz(p->page_size);
+  a.max_len = (int)std::min<int64_t>((int64_t)p->pages_stride * p->page_size, INT32_MAX - 4096);
+  return a;
+}
+
+int fdm_kv_grow(const fdm_kv_pages* p, const int32_t* d_new, int N, int32_t* d_q_start, int32_t* d_pos, int32_t* d_slots,
+                int32_t* d_refused, void* stream) {
+  if (int rc = check_pages(p)) return rc;
+  if (N < 0 || N > FDM_KV_MAX_ROWS) return fail(FDM_E_INVAL, "N=%d: 0 .. %d", N, FDM_KV_MAX_ROWS);
+  if (!d_new || !d_q_start || (N && (!d_pos || !d_slots))) return fail(FDM_E_INVAL, "null pointer");
+  if (!aligned(d_new, 4) || !aligned(d_q_start, 4) || !aligned(d_pos, 4) || !aligned(d_slots, 4) || !aligned(d_refused, 4))
+    return fail(FDM_E_INVAL, "misaligned pointer");
+  if (int rc = check_ready()) return rc;
+  const KvGrowArgs g{d_new, N, d_q_start, d_pos, d_slots, d_refused, aligned(d_pos, 16) && aligned(d_slots, 16)};
+  OnDevice dev;
+  ProfScope prof(FDM_PROF_KV, as_stream(stream));
+  FDM_HIP(launch_kv_grow(pages_args(p), g, as_stream(stream)));
+  return FDM_OK;
+}
+
+int fdm_kv_trim(const fdm_kv_pages* p, const int32_t* d_keep, void* stream) {
+  if (int rc = check_pages(p)) return rc;
+  if (!d_keep || !aligned(d_keep, 4)) return fail(FDM_E_INVAL, "keep: null or misaligned pointer");
+  if (int rc = check_ready()) return rc;
+  OnDevice dev;
+  ProfScope prof(FDM_PROF_KV, as_stream(stream));
+  FDM_HIP(launch_kv_trim(pages_args(p), d_keep, as_stream(stream)));
+  return FDM_OK;
+}
+
+// ---- the residual's addition and its norm ----------------------------------------------
+int fdm_add_rms_norm(const void* d_x, int x_type, int64_t x_stride, const void* d_add, int add_type, int64_t add_stride,
+                     void* d_sum, int64_t sum_stride, const float* d_w, float eps, void* d_y, int y_type,
+                     int64_t y_stride, uint8_t* d_scale, int64_t scale_stride, int T, int d, void* stream) {
+  NormArgs a{};
+  if (int rc = elem_type(x_type, &a.x_type, "x")) return rc;
+  a.add_type = a.x_type;
+  if (d_add)
+    if (int rc = elem_type(add_type, &a.add_type, "add")) return rc;
+  const bool fp8 = y_type == FDM_E4M3;
+  if (!fp8)
+    if (int rc = elem_type(y_type, &a.y_type, "y")) return rc;
+  if (T < 0 || d < 1 || d > FDM_NORM_MAX_DIM) return fail(FDM_E_INVAL, "T=%d d=%d (1 .. %d)", T, d, FDM_NORM_MAX_DIM);
+  if (!(eps >= 0.0f) || !isfinite(eps)) return fail(FDM_E_INVAL, "eps %g", (double)eps);
+  if (fp8 ? !d_scale && T > 0 : d_scale != nullptr) return fail(FDM_E_INVAL, "scale: E4M3 rows have one, the others none");
+  if (T == 0) return check_ready();
+  if (!d_x || !d_y) return fail(FDM_E_INVAL, "null pointer");
+  const int64_t xs = elem_size(a.x_type), as = elem_size(a.add_type), ys = fp8 ? 1 : elem_size(a.y_type);
+  if (!aligned(d_x, xs) || !aligned(d_add, as) || !aligned(d_sum, xs) || !aligned(d_y, ys) || !aligned(d_w, 4))
+    return fail(FDM_E_INVAL, "misaligned pointer");
+  for (int64_t s : {x_stride, add_stride, sum_stride, y_stride, scale_stride})
+    if (llabs(s) > INT64_MAX / 16) return fail(FDM_E_INVAL, "stride %lld", (long long)s);
+  const int groups = (d + 127) / 128;
+  if (T > 1 && (llabs(y_stride) < d || (d_sum && llabs(sum_stride) < d) || (fp8 && llabs(scale_stride) < groups)))
+    return fail(FDM_E_INVAL, "rows of y, sum or scale overlap");
+  // a place of its own is written behind its reads by the same thread; rows at another
+  // stride would be written before they are read
+  auto same = [&](const void* out, const void* in, int64_t s_out, int64_t s_in) { return out != in || T == 1 || s_out == s_in; };
+  const int64_t xb = x_stride * xs, ab = add_stride * as, sb = sum_stride * xs, yb = y_stride * ys;
+  if (d_sum && (!same(d_sum, d_x, sb, xb) || (d_add && !same(d_sum, d_add, sb, ab)) || d_sum == d_y || (d_sum == d_add && as != xs)))
+    return fail(FDM_E_INVAL, "sum: in x's place (or add's, of one size) with its stride, or elsewhere; not in y's");
+  if ((d_y == d_x && ys != xs) || (d_add && d_y == d_add && ys != as) || !same(d_y, d_x, yb, xb) || (d_add && !same(d_y, d_add, yb, ab)))
+    return fail(FDM_E_INVAL, "y: in x's or add's place with its size and stride, or elsewhere");
+  if (int rc = check_ready()) return rc;
+  a.x = d_x;
+  a.add = d_add;
+  a.sum = d_sum;
+  a.y = d_y;
+  a.scale = fp8 ? d_scale : nullptr;
+  a.w = d_w;
+  a.x_bytes = xb;
+  a.add_bytes = ab;
+  a.sum_bytes = sb;
+  a.y_bytes = yb;
+  a.scale_bytes = scale_stride;
+  a.T = T;
+  a.d = d;
+  a.eps = eps;
+  // accesses of eight values: 16 bytes, of codes 8
+  auto rows = [&](const void* q, int64_t bytes, int64_t at) { return !q || (aligned(q, at) && (T == 1 || bytes % at == 0)); };
+  a.vec = d % 8 == 0 && rows(d_x, xb, 16) && rows(d_add, ab, 16) && rows(d_sum, sb, 16) && rows(d_y, yb, fp8 ? 8 : 16) &&
+          aligned(d_w, 16);
+  OnDevice dev;
+  ProfScope prof(FDM_PROF_NORM, as_stream(stream));
+  FDM_HIP(launch_add_rms_norm(a, as_stream(stream)));
+  return FDM_OK;
+}
+
+// ---- projections with the requests' adapters -------------------------------------------
+static int check_projection_shape(int T, int in, int out, int rank) {
+  if (T < 0 || T > FDM_PROJECT_MAX_ROWS || in < 8 || in > FDM_PROJECT_MAX_DIM || in % 8 || out < 1 || out > FDM_PROJECT_MAX_DIM)
+    return fail(FDM_E_INVAL, "T=%d (0 .. %d) in=%d (eights) out=%d (up to %d)", T, FDM_PROJECT_MAX_ROWS, in, out, FDM_PROJECT_MAX_DIM);
+  if (rank < 0 || rank > FDM_MAX_RANK || rank % 8) return fail(FDM_E_INVAL, "rank %d: eights, up to %d", rank, FDM_MAX_RANK);
+  return FDM_OK;
+}
+
+int fdm_project_workspace(int T, int in_dim, int out_dim, int rank, size_t* bytes) {
+  if (int rc = check_projection_shape(T, in_dim, out_dim, rank)) return rc;
+  if (!bytes) return fail(FDM_E_INVAL, "null pointer");
+  if (int rc = check_ready()) return rc;
+  *bytes = project_most_bytes(T, in_dim, out_dim, rank, g_num_cus);
+  return FDM_OK;
+}
+
+int fdm_project(const fdm_projection* p, void* d_workspace, size_t workspace_bytes, void* stream) {
+  if (!p) return fail(FDM_E_INVAL, "null projection");
+  int fmt;
+  switch (p->type) {
+    case FDM_GGML_F16: fmt = 0; break;
+    case FDM_GGML_BF16: fmt = 1; break;
+    case FDM_E4M3: fmt = 2; break;
+    default: return fail(FDM_E_INVAL, "type %d is none of F16, BF16, E4M3", p->type);
+  }
+  ProjectArgs a{};
+  if (int rc = elem_type(p->y_type, &a.y_type, "y")) return rc;
+  const bool fp8 = fmt == 2, adapters = p->n_adapters != 0;
+  const int size = fp8 ? 1 : 2;
+  if (int rc = check_projection_shape(p->T, p->in_dim, p->out_dim, adapters ? p->rank : 0)) return rc;
+  if (fp8 && p->in_dim % 16) return fail(FDM_E_INVAL, "in=%d: sixteens in E4M3", p->in_dim);
+  if (p->n_adapters < 0 || p->n_adapters > FDM_MAX_ADAPTERS || (adapters && p->rank < 8))
+    return fail(FDM_E_INVAL, "%d adapters (0 .. %d) of rank %d", p->n_adapters, FDM_MAX_ADAPTERS, p->rank);
+  if (adapters && (p->B < 1 || p->B > FDM_PROJECT_MAX_SEQS)) return fail(FDM_E_INVAL, "%d requests: 1 .. %d", p->B, FDM_PROJECT_MAX_SEQS);
+  if (p->T == 0) return check_ready();
+  if (!p->d_x || !p->d_w || !p->d_y || !d_workspace) return fail(FDM_E_INVAL, "null pointer");
+  if (adapters && (!p->d_a || !p->d_b || !p->d_q_start || !p->d_adapter)) return fail(FDM_E_INVAL, "adapters: null pointer");
+  if (fp8 ? !p->d_x_scale || !p->d_w_scale : p->d_x_scale || p->d_w_scale)
+    return fail(FDM_E_INVAL, "scales: E4M3 rows and matrices have them, the others none");
+  const int ys = (int)elem_size(a.y_type), groups = (p->in_dim + 127) / 128;
+  if (!aligned(p->d_x, 16) || !aligned(p->d_w, 16) || !aligned(d_workspace, 256) || !aligned(p->d_y, ys))
+    return fail(FDM_E_INVAL, "misaligned pointer (x, w: 16 bytes, workspace: 256)");
+  if (adapters && (!aligned(p->d_a, 16) || !aligned(p->d_b, 16) || !aligned(p->d_times, 4) || !aligned(p->d_q_start, 4) || !aligned(p->d_adapter, 4)))
+    return fail(FDM_E_INVAL, "adapters: misaligned pointer (a, b: 16 bytes)");
+  // (strides of a single row say nothing)
+  const int64_t x_stride = p->T > 1 ? p->x_stride : p->in_dim, w_stride = p->out_dim > 1 ? p->w_stride : p->in_dim;
+  for (int64_t s : {x_stride, w_stride})
+    if (s % (16 / size) || llabs(s) > FDM_PROJECT_MAX_STRIDE)
+      return fail(FDM_E_INVAL, "stride %lld: whole 16 bytes, up to %d elements", (long long)s, FDM_PROJECT_MAX_STRIDE);
+  const int64_t y_stride = p->T > 1 ? p->y_stride : p->out_dim;
+  if (llabs(y_stride) < p->out_dim || llabs(y_stride) > FDM_PROJECT_MAX_STRIDE)
+    return fail(FDM_E_INVAL, "y: rows of %d at stride %lld", p->out_dim, (long long)y_stride);
+  if (fp8 && llabs(p->x_scale_stride) > FDM_PROJECT_MAX_STRIDE) return fail(FDM_E_INVAL, "scale stride %lld", (long long)p->x_scale_stride);
+  if (int rc = check_ready()) return rc;
+  const ProjectPlan plan = project_plan(p->T, (int64_t)p->in_dim * size, p->out_dim, adapters, g_num_cus);
+  const int rank = adapters ? p->rank : 0;
+  if (workspace_bytes < project_bytes(plan, p->T, p->out_dim, rank))
+    return fail(FDM_E_INVAL, "workspace of %zu bytes: %zu are needed", workspace_bytes, project_bytes(plan, p->T, p->out_dim, rank));
+  a.x = p->d_x;
+  a.w = p->d_w;
+  a.x_scale = p->d_x_scale;
+  a.w_scale = p->d_w_scale;
+  a.x_bytes = x_stride * size;
+  a.w_bytes = w_stride * size;
+  a.x_scale_bytes = p->T > 1 ? p->x_scale_stride : groups;
+  a.w_scale_bytes = groups;
+  a.y = p->d_y;
+  a.y_bytes = y_stride * ys;
+  a.vec_y = aligned(p->d_y, 16) && (p->T == 1 || a.y_bytes % 16 == 0);
+  a.vec_part = p->out_dim % 4 == 0;
+  a.T = p->T;
+  a.in = p->in_dim;
+  a.out = p->out_dim;
+  a.row_bytes = p->in_dim * size;
+  a.steps = steps_of(a.row_bytes);
+  a.a = p->d_a;
+  a.b = p->d_b;
+  a.times = p->d_times;
+  a.n_adapters = p->n_adapters;
+  a.rank = rank;
+  a.q_start = p->d_q_start;
+  a.adapter = p->d_adapter;
+  a.B = p->B;
+  a.planes = a.y_type == ElemType::f32 && fmt != 0 ? 3 : 2;
+  a.u = static_cast<float*>(d_workspace);
+  a.part = plan.join ? a.u + (project_u_floats(plan, p->T, rank) + 63) / 64 * 64 : nullptr;
+  a.splits = plan.splits;
+  a.u_splits = plan.u_splits;
+  OnDevice dev;
+  // two threads' calls on one stream may share a workspace: their launches must not mix
+  std::lock_guard<std::mutex> lock(g.project_mu);
+  ProfScope prof(FDM_PROF_PROJECT, as_stream(stream));
+  FDM_HIP(launch_project(a, plan, fp8 && a.y_type == ElemType::f32 ? 3 : fmt, as_stream(stream)));
   return FDM_OK;
 }
 

@@ -7,6 +7,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <functional>
 #include <string>
 #include <unordered_map>
@@ -434,6 +435,62 @@ struct MlaTreeArgs {
 };
 size_t mla_tree_workspace(int N, int H);
 hipError_t launch_mla_tree(const MlaTreeArgs& a, int fmt, hipStream_t s);
+
+// kvpages_kernels.hip
+constexpr int kKvMaxSeqs = 4096;  // FDM_KV_MAX_SEQS
+struct KvPagesArgs {
+  int* pages;                 // [B][P]
+  int *kv_len, *free, *n_free;
+  unsigned* turn;             // counts the workgroups of a launch; zero between launches
+  int B, P, n_pages, shift;   // shift: log2 of a page's rows
+  int max_len;                // positions that a row of the table has room for
+};
+struct KvGrowArgs {
+  const int* more;            // [B] tokens asked for
+  int N;                      // places of pos and slots
+  int *q_start, *pos, *slots, *refused;  // refused may be null
+  bool vec;                   // pos and slots are 16-byte aligned
+};
+hipError_t launch_kv_grow(const KvPagesArgs& a, const KvGrowArgs& g, hipStream_t s);
+hipError_t launch_kv_trim(const KvPagesArgs& a, const int* keep, hipStream_t s);
+
+// norm_kernels.hip
+constexpr int kNormMaxDim = 32768;  // FDM_NORM_MAX_DIM
+struct NormArgs {
+  const void *x, *add;        // [T][d]; add may be null
+  void* sum;                  // x + add in x's type, or null
+  void* y;
+  uint8_t* scale;             // e4m3 rows: [T][ceil(d / 128)]; null: y_type
+  const float* w;             // [d] or null
+  int64_t x_bytes, add_bytes, sum_bytes, y_bytes, scale_bytes;  // from row to row
+  ElemType x_type, add_type, y_type;
+  int T, d;
+  float eps;
+  bool vec;                   // rows of whole eights, aligned for accesses of eight values
+};
+hipError_t launch_add_rms_norm(const NormArgs& a, hipStream_t s);
+
+// project_kernels.hip
+struct ProjectArgs {
+  const void *x, *w;          // [T][in], [out][in]
+  const uint8_t *x_scale, *w_scale;  // e4m3: [T][ceil(in / 128)], [ceil(out / 128)][ceil(in / 128)]
+  int64_t x_bytes, w_bytes, x_scale_bytes, w_scale_bytes, y_bytes;  // from row to row
+  void* y;                    // [T][out]
+  ElemType y_type;
+  bool vec_y, vec_part;       // rows aligned for accesses of eight values
+  int T, in, out, row_bytes, steps;
+  const void *a, *b;          // [n][rank][in], [n][out][rank]
+  const float* times;         // [n] or null
+  int n_adapters, rank;       // 0: none
+  const int *q_start, *adapter;  // [B + 1], [B]
+  int B;
+  int planes;                 // 16-bit numbers that stand for one of u on the matrix cores
+  float* u;                   // workspace [u_splits][T][rank]
+  float* part;                // workspace [splits][T][out]; null: straight into y
+  int splits, u_splits;
+};
+struct ProjectPlan;           // project_work.h
+hipError_t launch_project(const ProjectArgs& a, const ProjectPlan& p, int fmt, hipStream_t s);
 
 // synth_kernels.hip
 hipError_t launch_synth_q4k(uint8_t* dst, size_t n_blocks, uint64_t seed, hipStream_t s);

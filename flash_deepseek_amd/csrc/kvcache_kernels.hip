@@ -71,17 +71,8 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
 #pragma unroll
     for (int d = 8; d >= 1; d >>= 1) m = amax_bits(m, __shfl_xor(m, d));
     const int byte = fp8_scale_byte(m);
-    const float inv = scale_value(byte == kScaleNan ? 127 : 254 - byte);  // 2^-e
     uint32_t code[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float q[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q[j] = fminf(fmaxf(v[4 * k + j] * inv, -448.0f), 448.0f);
-      int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-      code[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
-    }
-    if (byte == kScaleNan) code[0] = code[1] = 0x7F7F7F7Fu;  // e4m3's NaN
+    fp8_codes8(v, byte, code);
     *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.latent) + at * kLatDim + 8 * lane) = make_uint2(code[0], code[1]);
     if ((lane & 15) == 0) a.scale[at * 4 + (lane >> 4)] = (uint8_t)byte;
     if (lane < 32) {

@@ -1,0 +1,210 @@
+// kvpages_kernels.hip -- the books of the paged latent cache: which pages a
+// sequence has, which are free, and where a step's tokens go.
+//   free[0 .. n_free - 1] is a stack.  Sequence b holds the pages
+//   pages[b][0 .. ceil(kv_len[b] / page) - 1].
+// Pages are taken from the stack's top in the order of (sequence, page) and given
+// back in the opposite one, so that what a call took and another gives back leaves
+// the stack as it was, and the same calls give the same pages.
+#include "fdm_internal.h"
+
+namespace fdm {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Exclusive sums over the workgroup's threads; *total gets the sum of all.
+template <typename T>
+__device__ __forceinline__ T scan(T mine, T* of_wave, T* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T v = __shfl_up(upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 63) of_wave[wave] = upto;
+  __syncthreads();
+  T before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < wave) before += of_wave[w];
+    all += of_wave[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + upto - mine;
+}
+
+// The last b of start[0 .. B] (not falling) with start[b] <= i.
+__device__ __forceinline__ int owner(const int* start, int B, int i) {
+  int lo = 0, hi = B;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (start[mid] <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int pages_for(int len, int shift) { return (int)(((int64_t)len + (1 << shift) - 1) >> shift); }
+
+// Whether this workgroup is the last of the launch to come here: the others have
+// read the state that it may now change.  The word counts up to the workgroups
+// and starts again.
+__device__ __forceinline__ bool is_last(unsigned* turn, int* said) {
+  if (gridDim.x == 1) {
+    __syncthreads();
+    return true;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) *said = atomicInc(turn, gridDim.x - 1) == gridDim.x - 1;
+  __syncthreads();
+  return *said;
+}
+
+}  // namespace
+
+// Every workgroup counts all sequences itself (B <= 4096, 16 a thread), so that one
+// launch needs no second one behind it; the last one to come to its end changes the
+// state that the others read.  A workgroup gives 1024 places at a time, four a
+// thread: a token's sequence is searched for in LDS, and the first token of a new
+// page names the page in the table.
+__global__ __launch_bounds__(kThreads) void k_kv_grow(KvPagesArgs a, KvGrowArgs g) {
+  __shared__ int start[kKvMaxSeqs + 1], first[kKvMaxSeqs], len[kKvMaxSeqs];
+  __shared__ int64_t wide[kThreads / 64];
+  __shared__ int narrow[kThreads / 64], said;
+  const int tid = threadIdx.x, per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(b0 + per, a.B);
+  const int n_free = min(max(*a.n_free, 0), a.n_pages);
+  // what the sequences that have room ask for, up to each
+  int64_t pages = 0, tokens = 0, all64;
+  for (int b = b0; b < b1; ++b) {
+    const int l = min(max(a.kv_len[b], 0), a.max_len), n = max(g.more[b], 0);
+    const bool room = n <= a.max_len - l;
+    len[b] = l;
+    start[b] = room ? n : -1;
+    first[b] = room ? pages_for(l + n, a.shift) - pages_for(l, a.shift) : 0;
+    pages += first[b];
+    tokens += room ? n : 0;
+  }
+  pages = scan(pages, wide, &all64);
+  tokens = scan(tokens, wide, &all64);
+  // who is served
+  int n_sum = 0, need_sum = 0, refused = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = start[b], need = first[b];
+    pages += need;
+    tokens += max(n, 0);
+    const bool served = n >= 0 && (need == 0 || pages <= n_free) && tokens <= g.N;
+    refused += !served && n != 0;
+    start[b] = served ? n : 0;
+    first[b] = served ? need : 0;
+    n_sum += start[b];
+    need_sum += first[b];
+  }
+  int total, taken, n_refused;
+  int at = scan(n_sum, narrow, &total), page_at = scan(need_sum, narrow, &taken);
+  scan(refused, narrow, &n_refused);
+  for (int b = b0; b < b1; ++b) {
+    const int n = start[b], need = first[b];
+    start[b] = at;
+    first[b] = page_at;
+    at += n;
+    page_at += need;
+  }
+  if (tid == 0) start[a.B] = total;
+  __syncthreads();
+  const int inside = (1 << a.shift) - 1;
+  for (int64_t t0 = 4 * ((int64_t)blockIdx.x * kThreads + tid); t0 < g.N; t0 += (int64_t)4 * kThreads * gridDim.x) {
+    int pos[4], slot[4];
+    int b = t0 < total ? owner(start, a.B, (int)t0) : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t t = t0 + k;
+      pos[k] = 0;
+      slot[k] = -1;
+      if (t < total) {
+        while (start[b + 1] <= t) ++b;
+        pos[k] = len[b] + (int)(t - start[b]);
+        const int p = pos[k] >> a.shift, have = pages_for(len[b], a.shift);
+        int* entry = a.pages + (int64_t)b * a.P + p;
+        int page;
+        if (p < have) {
+          page = *entry;
+        } else {
+          page = a.free[n_free - 1 - (first[b] + p - have)];
+          if ((pos[k] & inside) == 0) *entry = page;
+        }
+        if (page >= 0 && page < a.n_pages) slot[k] = (page << a.shift) | (pos[k] & inside);
+      }
+    }
+    if (g.vec && t0 + 4 <= g.N) {
+      *reinterpret_cast<int4*>(g.pos + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<int4*>(g.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (t0 + k < g.N) {
+          g.pos[t0 + k] = pos[k];
+          g.slots[t0 + k] = slot[k];
+        }
+    }
+  }
+  if (!is_last(a.turn, &said)) return;
+  for (int b = b0; b < b1; ++b) {
+    g.q_start[b] = start[b];
+    a.kv_len[b] = len[b] + start[b + 1] - start[b];
+  }
+  if (tid == 0) {
+    g.q_start[a.B] = total;
+    *a.n_free = n_free - taken;
+    if (g.refused) *g.refused = n_refused;
+  }
+}
+
+// The pages behind what each sequence keeps, onto the stack; one launch as above.
+__global__ __launch_bounds__(kThreads) void k_kv_trim(KvPagesArgs a, const int* keep) {
+  __shared__ int before[kKvMaxSeqs + 1], stay[kKvMaxSeqs], len[kKvMaxSeqs];
+  __shared__ int narrow[kThreads / 64], said;
+  const int tid = threadIdx.x, per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(b0 + per, a.B);
+  const int n_free = min(max(*a.n_free, 0), a.n_pages);
+  int sum = 0, total;
+  for (int b = b0; b < b1; ++b) {
+    const int l = min(max(a.kv_len[b], 0), a.max_len), k = keep[b] < 0 ? l : min(keep[b], l);
+    len[b] = k;
+    stay[b] = pages_for(k, a.shift);
+    before[b] = pages_for(l, a.shift) - stay[b];
+    sum += before[b];
+  }
+  int at = scan(sum, narrow, &total);
+  for (int b = b0; b < b1; ++b) {
+    const int n = before[b];
+    before[b] = at;
+    at += n;
+  }
+  if (tid == 0) before[a.B] = total;
+  __syncthreads();
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < total; i += (int64_t)kThreads * gridDim.x) {
+    const int b = owner(before, a.B, (int)i);
+    const int64_t to = (int64_t)n_free + total - 1 - i;
+    if (to < a.n_pages) a.free[to] = a.pages[(int64_t)b * a.P + stay[b] + (i - before[b])];
+  }
+  if (!is_last(a.turn, &said)) return;
+  for (int b = b0; b < b1; ++b) a.kv_len[b] = len[b];
+  if (tid == 0) *a.n_free = (int)min((int64_t)n_free + total, (int64_t)a.n_pages);
+}
+
+// Workgroups: one for every 1024 places (tokens, or entries of the table, of which
+// a call seldom gives back many), a CU's worth at most.
+hipError_t launch_kv_grow(const KvPagesArgs& a, const KvGrowArgs& g, hipStream_t s) {
+  const int wgs = (int)std::min<int64_t>(std::max<int64_t>(((int64_t)g.N + 1023) / 1024, 1), g_num_cus);
+  k_kv_grow<<<wgs, kThreads, 0, s>>>(a, g);
+  return hipGetLastError();
+}
+hipError_t launch_kv_trim(const KvPagesArgs& a, const int* keep, hipStream_t s) {
+  const int wgs = (int)std::min<int64_t>(((int64_t)a.B * a.P + 8191) / 8192, g_num_cus);
+  k_kv_trim<<<wgs, kThreads, 0, s>>>(a, keep);
+  return hipGetLastError();
+}
+
+}  // namespace fdm

@@ -90,6 +90,20 @@ __device__ __forceinline__ float scale_value(int byte) {
   return __builtin_bit_cast(float, byte == kScaleNan ? 0x7FC00000u : (uint32_t)max(byte, 1) << 23);
 }
 
+// e4m3 codes of eight values of a group with that scale byte, four a word.
+__device__ __forceinline__ void fp8_codes8(const float* v, int byte, uint32_t* code) {
+  const float up = scale_value(byte == kScaleNan ? 127 : 254 - byte);  // 2^-e
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q[j] = fminf(fmaxf(v[4 * k + j] * up, -448.0f), 448.0f);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    code[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+  }
+  if (byte == kScaleNan) code[0] = code[1] = 0x7F7F7F7Fu;  // e4m3's NaN
+}
+
 // max over |v| that keeps infinities and NaN (a NaN's bits, sign cleared, are
 // above every number's)
 __device__ __forceinline__ float amax_bits(float m, float v) {

@@ -566,6 +566,115 @@ int fdm_mla_attend(const fdm_kv_cache *cache, const fdm_mla_batch *batch, const 
                    void *d_out, int64_t out_token, int64_t out_head, float *d_lse, void *d_workspace,
                    size_t workspace_bytes, void *stream);
 
+/* ---- the books of the paged cache: which pages each sequence has, which are
+ * free, and where a step's tokens go (no counterpart in the reference, whose
+ * cache holds one sequence).  d_free [n_pages] is a stack of free pages, its
+ * first *d_n_free entries; sequence b has the pages d_pages[b][0 ..
+ * ceil(kv_len[b] / page_size) - 1], which no other sequence has.  All of it is
+ * the caller's device memory and changes in place; d_turn is a word of the
+ * library's, zero at first.  kv_len is cut to 0 .. pages_stride * page_size (and
+ * 2^31 - 4097), *d_n_free to 0 .. n_pages, as they are read.  Calls on the same
+ * pages follow each other on one stream; they may be captured.
+ *
+ * fdm_kv_grow: d_new [B] tokens for each sequence (below 0: none).  A sequence is
+ * served if its row of the table has room for them, and if the pages that it
+ * needs (if any) and the tokens are there when all sequences with room up to it
+ * ask for theirs: the free pages, and N places.  One that is not served stays as
+ * it was and has no tokens; *d_refused (may be NULL) is how many with tokens
+ * asked for were not.  Pages are taken from the stack's top, for the first
+ * sequence first.  Then kv_len[b] counts the new tokens, q_start [B + 1] their
+ * ranges (as fdm_mla_attend takes them), and pos [N] and slots [N] their
+ * positions and slots (as fdm_kv_write takes them; a page number outside the
+ * cache: slot -1).  Places behind the last token get position 0 and slot -1.
+ * fdm_kv_trim: every sequence keeps its first d_keep [B] positions (below 0 or
+ * past kv_len: all); 0 ends it.  The pages behind them go back, the last
+ * sequence's last one first, so that what a grow took and a trim gives back
+ * leaves the stack as it was.  Entries of the table behind a sequence's pages
+ * stay as they were. */
+#define FDM_KV_MAX_SEQS 4096
+typedef struct fdm_kv_pages {
+  int32_t *d_pages;   /* [B][pages_stride] */
+  int32_t *d_kv_len;  /* [B]               */
+  int32_t *d_free;    /* [n_pages]         */
+  int32_t *d_n_free;  /* [1]               */
+  uint32_t *d_turn;   /* [1]               */
+  int B, pages_stride, n_pages, page_size;
+} fdm_kv_pages;
+int fdm_kv_grow(const fdm_kv_pages *pages, const int32_t *d_new, int N, int32_t *d_q_start, int32_t *d_pos,
+                int32_t *d_slots, int32_t *d_refused, void *stream);
+int fdm_kv_trim(const fdm_kv_pages *pages, const int32_t *d_keep, void *stream);
+
+/* ---- the residual's addition and its norm for several tokens (infer.m:369-374
+ * and the additions of 1846-1850, 1922, without fdm_rms_norm's order of sums):
+ *   s = x + add (d_add NULL: x),  y = s / sqrt(mean(s^2) + eps) * w (d_w fp32 [d], NULL: 1),
+ * T rows of d values (1 .. FDM_NORM_MAX_DIM), strides in elements, in fp32, each
+ * output rounded once: d_sum (may be NULL) receives s in x's type, d_y the norm of s
+ * as it was before that rounding.  Types are FDM_GGML_F32, _F16, _BF16; y_type may
+ * be FDM_E4M3: codes with a scale byte for every 128 values of a row, d_scale
+ * [T][ceil(d / 128)], by the rule of FDM_KV_FP8 (zeros: 27, an infinity or NaN: 255).
+ * d_sum may be d_x, d_y may be d_x or d_add (same size of elements and stride);
+ * otherwise they must not overlap.  Rows of whole eights, 16-byte aligned, with add
+ * in x's type or BF16, move by 16-byte accesses, any other value by value. */
+#define FDM_NORM_MAX_DIM 32768
+#define FDM_E4M3 100 /* 8-bit floats, no GGML type: an element type where it is named */
+int fdm_add_rms_norm(const void *d_x, int x_type, int64_t x_stride, const void *d_add, int add_type,
+                     int64_t add_stride, void *d_sum, int64_t sum_stride, const float *d_w, float eps, void *d_y,
+                     int y_type, int64_t y_stride, uint8_t *d_scale, int64_t scale_stride, int T, int d, void *stream);
+
+/* ---- a shared projection and the low-rank adapters of many requests beside it
+ * (mv_f16, infer.m:459-513, for several tokens; adapters have no counterpart there):
+ *   y_t = W x_t + times_a B_a (A_a x_t),
+ * T rows x [T][in] through W [out][in], a = d_adapter[b] the adapter of the request b
+ * that row t is a token of (q_start[b] .. q_start[b + 1] - 1, as fdm_kv_grow writes
+ * them); a row of no request, or of one whose adapter is outside 0 .. n_adapters - 1,
+ * is W x_t alone.  type is that of x and W:
+ *   FDM_GGML_F16, _BF16  no scales;
+ *   FDM_E4M3             codes; d_x_scale [T][ceil(in / 128)] a byte e + 127 for every 128
+ *     values of a row (code 2^e, as fdm_add_rms_norm writes them), d_w_scale
+ *     [ceil(out / 128)][ceil(in / 128)] one for every 128 x 128 of W, contiguous;
+ *     255 makes its values NaN.
+ * A [n][rank][in] and B [n][out][rank] are contiguous, F16 beside F16, else BF16;
+ * d_times [n] fp32 (NULL: 1).  n_adapters 0: none, and the fields behind are not read.
+ * y_type F32, F16 or BF16.  Strides in elements; x, W, A, B 16-byte aligned, rows of x
+ * and W whole 16 bytes apart (strides of a single row are free).  in is a multiple of 8
+ * (16 in E4M3), rank of 8; in, out <= FDM_PROJECT_MAX_DIM.  y must not overlap the inputs,
+ * requests must not share rows.
+ * Sums and A x are fp32, products exact but for E4M3 with a 16-bit y: there every eight
+ * neighbouring products are added with what lies under 2^-13 of their largest cut off
+ * (1e-4 of a result of 7168 normal values).  Where B (A x) runs on the matrix cores A x is
+ * held as two numbers of the adapters' type (three for an fp32 y beside BF16), 2^-16 of itself
+ * and less.  A row's result depends on its own values and adapter alone, whatever else is
+ * in the call; its sums' order on T and the sizes.  The same arguments give the same bits.
+ * d_workspace: at least fdm_project_workspace(T, in, out, rank) bytes (rank 0: no
+ * adapters), 256-byte aligned, used by the call alone until it has run on its
+ * stream.  The call allocates nothing and may be captured. */
+#define FDM_PROJECT_MAX_ROWS 1048576
+#define FDM_PROJECT_MAX_DIM 262144
+#define FDM_PROJECT_MAX_STRIDE 4194304
+#define FDM_PROJECT_MAX_SEQS 4096
+#define FDM_MAX_ADAPTERS 1024
+#define FDM_MAX_RANK 128
+typedef struct fdm_projection {
+  int type, T, in_dim, out_dim;
+  const void *d_x;
+  int64_t x_stride;
+  const uint8_t *d_x_scale;
+  int64_t x_scale_stride;
+  const void *d_w;
+  int64_t w_stride;
+  const uint8_t *d_w_scale;
+  void *d_y;
+  int64_t y_stride;
+  int y_type;
+  int n_adapters, rank, B;
+  const void *d_a, *d_b;
+  const float *d_times;
+  const int32_t *d_q_start; /* [B + 1] */
+  const int32_t *d_adapter; /* [B]     */
+} fdm_projection;
+int fdm_project_workspace(int T, int in_dim, int out_dim, int rank, size_t *bytes);
+int fdm_project(const fdm_projection *p, void *d_workspace, size_t workspace_bytes, void *stream);
+
 /* ---- dense FFN layers (the layers before the first MoE layer, L < 3 in
  * R1): replaces the dense branch of layer_forward (infer.m:1852-1868),
  *   hidden = h_in + W_down . (silu(W_gate . h_post) * (W_up . h_post)),
@@ -610,9 +719,11 @@ int fdm_dense_ffn(int L, const float *d_h_post, const float *d_h_in, float *d_hi
 #define FDM_PROF_ATTN 9     /* fdm_attn_forward: the whole token        */
 #define FDM_PROF_CEILING 10 /* fdm_layer_read_ceiling                   */
 #define FDM_PROF_ROPE 11    /* fdm_rope                                 */
-#define FDM_PROF_KV 12      /* fdm_kv_write / fdm_kv_read               */
+#define FDM_PROF_KV 12      /* fdm_kv_write / _read / _grow / _trim     */
 #define FDM_PROF_MLA 13     /* fdm_mla_attend: both launches            */
-#define FDM_PROF_PHASES 14
+#define FDM_PROF_NORM 14    /* fdm_add_rms_norm                         */
+#define FDM_PROF_PROJECT 15 /* fdm_project: all launches                */
+#define FDM_PROF_PHASES 16
 int fdm_prof_enable(int on);
 int fdm_prof_reset(void);
 int fdm_prof_read(int phase, int *count, double *total_ms, double *min_ms, double *max_ms);
