@@ -2863,15 +2863,15 @@ int fdm_project(const fdm_projection* p, void* d_workspace, size_t workspace_byt
   // (strides of a single row say nothing)
   const int64_t x_stride = p->T > 1 ? p->x_stride : p->in_dim, w_stride = p->out_dim > 1 ? p->w_stride : p->in_dim;
   for (int64_t s : {x_stride, w_stride})
-    if (s % (16 / size) || llabs(s) > FDM_PROJECT_MAX_STRIDE)
+    if (s % (16 / size) || s < 0 || s > FDM_PROJECT_MAX_STRIDE)
       return fail(FDM_E_INVAL, "stride %lld: whole 16 bytes, up to %d elements", (long long)s, FDM_PROJECT_MAX_STRIDE);
   const int64_t y_stride = p->T > 1 ? p->y_stride : p->out_dim;
   if (llabs(y_stride) < p->out_dim || llabs(y_stride) > FDM_PROJECT_MAX_STRIDE)
     return fail(FDM_E_INVAL, "y: rows of %d at stride %lld", p->out_dim, (long long)y_stride);
   if (fp8 && llabs(p->x_scale_stride) > FDM_PROJECT_MAX_STRIDE) return fail(FDM_E_INVAL, "scale stride %lld", (long long)p->x_scale_stride);
   if (int rc = check_ready()) return rc;
-  const ProjectPlan plan = project_plan(p->T, (int64_t)p->in_dim * size, p->out_dim, adapters, g_num_cus);
-  const int rank = adapters ? p->rank : 0;
+  const int rank = adapters ? p->rank : 0, u_tiles = adapters ? adapter_tiles(p->T, p->B, p->n_adapters) * rank_parts(rank) : 0;
+  const ProjectPlan plan = project_plan(p->T, (int64_t)p->in_dim * size, p->out_dim, u_tiles, g_num_cus);
   if (workspace_bytes < project_bytes(plan, p->T, p->out_dim, rank))
     return fail(FDM_E_INVAL, "workspace of %zu bytes: %zu are needed", workspace_bytes, project_bytes(plan, p->T, p->out_dim, rank));
   a.x = p->d_x;
@@ -2885,7 +2885,6 @@ int fdm_project(const fdm_projection* p, void* d_workspace, size_t workspace_byt
   a.y = p->d_y;
   a.y_bytes = y_stride * ys;
   a.vec_y = aligned(p->d_y, 16) && (p->T == 1 || a.y_bytes % 16 == 0);
-  a.vec_part = p->out_dim % 4 == 0;
   a.T = p->T;
   a.in = p->in_dim;
   a.out = p->out_dim;
@@ -2901,7 +2900,8 @@ int fdm_project(const fdm_projection* p, void* d_workspace, size_t workspace_byt
   a.B = p->B;
   a.planes = a.y_type == ElemType::f32 && fmt != 0 ? 3 : 2;
   a.u = static_cast<float*>(d_workspace);
-  a.part = plan.join ? a.u + (project_u_floats(plan, p->T, rank) + 63) / 64 * 64 : nullptr;
+  a.part = a.u + (project_u_floats(plan, p->T, rank) + 63) / 64 * 64;
+  a.full = plan.full;
   a.splits = plan.splits;
   a.u_splits = plan.u_splits;
   OnDevice dev;

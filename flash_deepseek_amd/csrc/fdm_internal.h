@@ -477,7 +477,7 @@ struct ProjectArgs {
   int64_t x_bytes, w_bytes, x_scale_bytes, w_scale_bytes, y_bytes;  // from row to row
   void* y;                    // [T][out]
   ElemType y_type;
-  bool vec_y, vec_part;       // rows aligned for accesses of eight values
+  bool vec_y;                 // rows aligned for accesses of eight values
   int T, in, out, row_bytes, steps;
   const void *a, *b;          // [n][rank][in], [n][out][rank]
   const float* times;         // [n] or null
@@ -486,8 +486,9 @@ struct ProjectArgs {
   int B;
   int planes;                 // 16-bit numbers that stand for one of u on the matrix cores
   float* u;                   // workspace [u_splits][T][rank]
-  float* part;                // workspace [splits][T][out]; null: straight into y
-  int splits, u_splits;
+  float* part;                // workspace [splits][tiles - full][rows][cols]
+  int full, splits, u_splits;
+  int u_groups;               // workgroups of the adapters' first product before the others (set by the launcher)
 };
 struct ProjectPlan;           // project_work.h
 hipError_t launch_project(const ProjectArgs& a, const ProjectPlan& p, int fmt, hipStream_t s);

@@ -28,8 +28,10 @@ struct Half {
   typedef std::conditional_t<FMT == kRowF16, _Float16, __bf16> T;
   typedef std::conditional_t<FMT == kRowF16, f16x8, bf16x8> x8;
 };
-__device__ __forceinline__ f32x16 mfma16(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mfma16(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
 __device__ __attribute__((aligned(16))) uint32_t zeros16[4];  // stands for 16 bytes behind a row's end
 
@@ -40,6 +42,17 @@ __device__ __attribute__((aligned(16))) uint32_t zeros16[4];  // stands for 16 b
 __device__ __forceinline__ void lds_load16(const char* from, char* to) {
   const int at = (int)(uintptr_t)(FDM_LDS char*)to;
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+}
+// The same from a scalar base (not one that v_readlane wrote within the last five states)
+// and a byte offset a lane.
+__device__ __forceinline__ void lds_load16(const char* base, uint32_t off, char* to) {
+  const int at = (int)(uintptr_t)(FDM_LDS char*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off), "s"(base) : "memory");
+}
+// A byte a lane, widened to four: lane i's land at `to` + 4 i.
+__device__ __forceinline__ void lds_load_byte(const uint8_t* from, char* to) {
+  const int at = (int)(uintptr_t)(FDM_LDS char*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(at), "v"(from) : "memory");
 }
 // Sixteen e4m3 codes times a power of two, in BF16: exact, four bits of significand.
 __device__ __forceinline__ void widen16(i32x4 c, float scale, bf16x8* v) {
@@ -53,6 +66,12 @@ __device__ __forceinline__ void widen16(i32x4 c, float scale, bf16x8* v) {
     v[k / 2][4 * (k % 2) + 3] = hi[1];
   }
 }
+// Eight codes.
+__device__ __forceinline__ bf16x8 widen8(uint2 c, float scale) {
+  const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, scale, true);
+  const auto d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, scale, false), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, scale, true);
+  return bf16x8{a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
 // at most N of the wave's loads are still in flight, and none of its LDS reads
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
@@ -62,87 +81,230 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
-// A row's 16-byte piece c lies at c ^ piece_swap(row): sixteen rows' same piece
-// lie in sixteen bank groups.
-__device__ __forceinline__ int piece_swap(int row) { return (row >> 1) & 7; }
-
-// The request whose tokens row t is among; -1: none.
-__device__ __forceinline__ int request_of(const int* q_start, int B, int t) {
-  int lo = 0, hi = B + 1;  // the first b with q_start[b] > t, B + 1 if none
+// The request whose tokens row t is among, its adapter; -1: none.
+__device__ __forceinline__ int adapter_of(const ProjectArgs& a, int t) {
+  if (t >= a.T) return -1;
+  int lo = 0, hi = a.B + 1;  // the first b with q_start[b] > t, B + 1 if none
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
-    if (q_start[mid] <= t) lo = mid + 1;
+    if (a.q_start[mid] <= t) lo = mid + 1;
     else hi = mid;
   }
-  return lo <= B ? lo - 1 : -1;
-}
-__device__ __forceinline__ int adapter_of(const ProjectArgs& a, int t) {
-  if (!a.n_adapters || t >= a.T) return -1;
-  const int b = request_of(a.q_start, a.B, t);
-  const int k = b < 0 ? -1 : a.adapter[b];
+  if (lo < 1 || lo > a.B) return -1;
+  const int k = a.adapter[lo - 1];
   return k < a.n_adapters ? k : -1;
 }
 
-}  // namespace
+// ---- a wave's sums -----------------------------------------------------------------------
+// The matrix's rows are the products' first operand and x's the second, so that a lane
+// holds one row of the result a block.  Products of 16-bit values are 16 x 16 x 32: 32 x 32 x 16
+// ones have the same rate but draw more, 1.80 against 2.11 PFLOP/s where the power
+// limits them (random values, nothing beside the products).  fp8 ones are 32 x 32 x 64.
+// Which row of the matrix stands in which place of the first operand is chosen such that
+// a lane's columns, over its NB blocks, are neighbours.
+template <int FMT>
+struct Block {
+  static constexpr bool k32 = FMT == kRowFp8;
+  static constexpr int kRows = k32 ? 32 : 16;  // of x, and columns
+  static constexpr int kOf = k32 ? 16 : 4;     // a lane's columns
+  typedef std::conditional_t<k32, f32x16, f32x4> sum_t;
+};
+// The matrix's row (of a wave's) in place i of block j's operand.
+template <int FMT, int NB>
+__device__ __forceinline__ int matrix_row(int i, int j) {
+  return Block<FMT>::k32 ? (i >> 2 & 1) * 16 * NB + 16 * j + (i >> 3) * 4 + (i & 3) : (i >> 2) * 4 * NB + 4 * j + (i & 3);
+}
+// Where a row's 16-byte piece c of a step lies: at c ^ swap8(row).  A read of 16 bytes a lane
+// is served sixteen lanes at a time, 0-3, 12-15, 20-23 and 24-27 of each 32 and then the
+// others; the swap is such that these, four rows each from four places of an operand above
+// (and with 16 x 16 blocks two pieces), find sixteen bank groups.
+template <int FMT>
+__device__ __forceinline__ int swap8(int row) {
+  const int q = row >> 2 & 3, upper = Block<FMT>::k32 ? q : q ^ (row >> 4 & 3);
+  return upper << 1 | (row >> 1 & 1);
+}
+
+// The adapters' second product on a wave's sums: for every adapter among the rows of a
+// block, B_a u on the matrix cores, u as sums of 16-bit numbers (a.planes of them: 8 bits
+// each in BF16, 11 in F16), kept by the rows that are the adapter's own.  A row that
+// has another keeps its sum untouched, whatever B_a holds.
+template <int FMT, int NB>
+__device__ __forceinline__ void add_adapters(const ProjectArgs& a, int m, int id, int n0, typename Block<FMT>::sum_t* acc) {
+  typedef typename Half<FMT>::T T16;
+  typedef typename Half<FMT>::x8 x8;
+  constexpr int kRows = Block<FMT>::kRows, kK = 8 * 64 / kRows;  // values of the rank that a product takes
+  const int lane = threadIdx.x & 63, i0 = lane % kRows, g = lane / kRows;
+  uint64_t left = __ballot(id >= 0);
+  const float* u = a.u + (int64_t)m * a.rank;
+  const int64_t next = (int64_t)a.T * a.rank;  // part of the inner dimension
+  // F16 planes: the row's largest brought to [1, 2), so that none overflows and few are lost
+  float up = 1.0f, down = 1.0f;
+  if constexpr (FMT == kRowF16) {
+    float top = 0.0f;
+    if (id >= 0)
+      for (int j = 0; j < a.rank; ++j) {
+        float v = 0.0f;
+        for (int p = 0; p < a.u_splits; ++p) v += u[p * next + j];
+        top = fmaxf(top, fabsf(v));
+      }
+    const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 100);
+    up = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+    down = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+  }
+  while (left) {
+    const int k = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+    const bool mine = id == k;
+    left &= ~__ballot(mine);
+    const T16* B = static_cast<const T16*>(a.b) + (int64_t)k * a.out * a.rank;
+    typename Block<FMT>::sum_t sum[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < Block<FMT>::kOf; ++i) sum[nb][i] = 0.0f;
+    for (int j0 = 0; j0 < a.rank; j0 += kK) {
+      const int j = j0 + 8 * g;
+      float v[8];
+      x8 bv[NB];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bv[nb][i] = (T16)0.0f;
+      if (j < a.rank) {
+        if (mine)
+          for (int p = 0; p < a.u_splits; ++p) {
+            float part[8];
+            load8(u + p * next + j, true, part);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += part[i];
+          }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int n = min(n0 + matrix_row<FMT, NB>(i0, nb), a.out - 1);
+          bv[nb] = *reinterpret_cast<const x8*>(B + (int64_t)n * a.rank + j);
+        }
+      }
+      for (int p = 0; p < a.planes; ++p) {
+        x8 w;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (p == 0) v[i] *= up;
+          w[i] = (T16)v[i];
+          const float rest = v[i] - (float)w[i];
+          v[i] = fabsf(rest) < __builtin_inff() ? rest : 0.0f;  // an infinity has no rest
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) sum[nb] = mfma(bv[nb], w, sum[nb]);
+      }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < Block<FMT>::kOf; ++i) acc[nb][i] = mine ? fmaf(sum[nb][i], down, acc[nb][i]) : acc[nb][i];
+  }
+}
+
+// A lane's columns n .. n + COUNT - 1 of a row.
+template <int COUNT, typename TY, typename S>
+__device__ __forceinline__ void store_columns(TY* y, int n, int out, bool vec, const S* c) {
+  constexpr int kOf = sizeof(S) / 4;
+#pragma unroll
+  for (int p = 0; p < COUNT; p += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c[(p + i) / kOf][(p + i) % kOf];
+    if (vec && n + p + 8 <= out) {
+      store8(y + n + p, true, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + p + i < out) y[n + p + i] = (TY)v[i];
+    }
+  }
+}
+
+// A wave's sums, MB blocks of rows by NB of columns, that begin at row m0 and column n0 of the
+// result: into y with the adapters' part, or (part not null) into the part's tile of `width`
+// columns, where they begin at `part`.  ids: the rows' adapters.
+template <int FMT, int MB, int NB>
+__device__ __forceinline__ void store_tile(const ProjectArgs& a, typename Block<FMT>::sum_t (*acc)[NB], float* part, int width, int m0, int n0,
+                                           const int* ids) {
+  constexpr int kRows = Block<FMT>::kRows, kCount = NB * Block<FMT>::kOf;
+  const int lane = threadIdx.x & 63, i0 = lane % kRows, col = lane / kRows * kCount;
+#pragma unroll
+  for (int i = 0; i < MB; ++i) {
+    const int m = m0 + kRows * i + i0;
+    if (part) {
+      if (m < a.T) store_columns<kCount>(part + (kRows * i + i0) * width, col, width, true, acc[i]);
+      continue;
+    }
+    if (a.n_adapters) add_adapters<FMT, NB>(a, m, ids[kRows * i + i0], n0, acc[i]);
+    if (m >= a.T) continue;
+    char* y = static_cast<char*>(a.y) + (int64_t)m * a.y_bytes;
+    if (a.y_type == ElemType::f32) store_columns<kCount>(reinterpret_cast<float*>(y), n0 + col, a.out, a.vec_y, acc[i]);
+    else if (a.y_type == ElemType::f16) store_columns<kCount>(reinterpret_cast<_Float16*>(y), n0 + col, a.out, a.vec_y, acc[i]);
+    else store_columns<kCount>(reinterpret_cast<__bf16*>(y), n0 + col, a.out, a.vec_y, acc[i]);
+  }
+}
 
 // ---- the adapters' first product: u_t = c_a A_a x_t ----------------------------------
 // A workgroup takes up to 32 rows of one adapter, wherever they stand: all count the
-// requests' rows by adapter in LDS, and the grid's y-th tile of the list (adapters in
-// order, their rows in order) is found from that; tiles <= rows / 32 + adapters in use.
-// Four waves share the part of the inner dimension; their sums meet in LDS.
-template <int FMT, int RB>
-__global__ __launch_bounds__(256) void k_adapter_in(ProjectArgs a) {
-  __shared__ int count[kMaxAdapters];
-  __shared__ int list[32];
-  __shared__ int chosen[3];  // adapter, its first row of the tile, rows of the adapter
-  __shared__ int of_wave[4];
-  __shared__ float sums[4][32][36];
+// requests' rows by adapter in LDS, and tile `mine` of the list (adapters in order,
+// their rows in order) is found from that; tiles <= rows / 32 + adapters in use.  The waves
+// share the values of part `split` of `splits` of the inner dimension, 128 bytes of a
+// row of x at a time, the next ones on their way; their sums meet in LDS.  Ranks above 64
+// are two halves, tiles of their own (more sums and operands do not fit the registers).
+struct AdapterLds {
+  int count[kMaxAdapters];
+  int list[32], chosen[2], of_wave[8];
+  float sums[8][32][20];
+};
+template <int FMT, int RB, int WAVES>
+__device__ __forceinline__ void adapter_in(const ProjectArgs& a, int split, int splits, int mine, int rank0, AdapterLds& l) {
+  constexpr int kThreads = 64 * WAVES, kEach = kMaxAdapters / kThreads;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int i = tid; i < a.n_adapters; i += 256) count[i] = 0;
-  if (tid == 0) chosen[0] = -1;
-  if (tid < 32) list[tid] = -1;
+  for (int i = tid; i < a.n_adapters; i += kThreads) l.count[i] = 0;
+  if (tid == 0) l.chosen[0] = -1;
+  if (tid < 32) l.list[tid] = -1;
   __syncthreads();
-  for (int b = tid; b < a.B; b += 256) {
+  for (int b = tid; b < a.B; b += kThreads) {
     const int k = a.adapter[b], t0 = min(max(a.q_start[b], 0), a.T), n = min(a.q_start[b + 1], a.T) - t0;
-    if (k >= 0 && k < a.n_adapters && n > 0) atomicAdd(&count[k], n);
+    if (k >= 0 && k < a.n_adapters && n > 0) atomicAdd(&l.count[k], n);
   }
   __syncthreads();
-  // tiles before each adapter, four consecutive ones a thread
+  // tiles before each adapter, kEach consecutive ones a thread
   int tiles = 0;
 #pragma unroll
-  for (int i = 0; i < kMaxAdapters / 256; ++i) {
-    const int k = tid * (kMaxAdapters / 256) + i;
-    if (k < a.n_adapters) tiles += (count[k] + 31) / 32;
-  }
+  for (int i = 0; i < kEach; ++i)
+    if (tid * kEach + i < a.n_adapters) tiles += (l.count[tid * kEach + i] + 31) / 32;
   int upto = tiles;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const int v = __shfl_up(upto, d);
     if (lane >= d) upto += v;
   }
-  if (lane == 63) of_wave[wave] = upto;
+  if (lane == 63) l.of_wave[wave] = upto;
   __syncthreads();
   int before = upto - tiles;
-  for (int w = 0; w < wave; ++w) before += of_wave[w];
-  const int mine = blockIdx.y;
+  for (int w = 0; w < wave; ++w) before += l.of_wave[w];
 #pragma unroll
-  for (int i = 0; i < kMaxAdapters / 256; ++i) {
-    const int k = tid * (kMaxAdapters / 256) + i;
+  for (int i = 0; i < kEach; ++i) {
+    const int k = tid * kEach + i;
     if (k >= a.n_adapters) break;
-    const int n = (count[k] + 31) / 32;
+    const int n = (l.count[k] + 31) / 32;
     if (mine >= before && mine < before + n) {
-      chosen[0] = k;
-      chosen[1] = 32 * (mine - before);
-      chosen[2] = count[k];
+      l.chosen[0] = k;
+      l.chosen[1] = 32 * (mine - before);
     }
     before += n;
   }
   __syncthreads();
-  const int k = chosen[0], row0 = chosen[1];
+  const int k = __builtin_amdgcn_readfirstlane(l.chosen[0]), row0 = l.chosen[1];
   if (k < 0) return;  // no such tile
   // the adapter's rows row0 .. row0 + 31
   int seen = 0;
-  for (int b0 = 0; b0 < a.B && seen < row0 + 32; b0 += 256) {
+  for (int b0 = 0; b0 < a.B && seen < row0 + 32; b0 += kThreads) {
     const int b = b0 + tid;
     int t0 = 0, n = 0;
     if (b < a.B && a.adapter[b] == k) {
@@ -156,394 +318,478 @@ __global__ __launch_bounds__(256) void k_adapter_in(ProjectArgs a) {
       if (lane >= d) sum += v;
     }
     __syncthreads();
-    if (lane == 63) of_wave[wave] = sum;
+    if (lane == 63) l.of_wave[wave] = sum;
     __syncthreads();
     int at = seen + sum - n;
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) at += of_wave[w];
-      seen += of_wave[w];
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) at += l.of_wave[w];
+      seen += l.of_wave[w];
     }
-    for (int i = max(at, row0); i < min(at + n, row0 + 32); ++i) list[i - row0] = t0 + (i - at);
+    for (int i = max(at, row0); i < min(at + n, row0 + 32); ++i) l.list[i - row0] = t0 + (i - at);
   }
   __syncthreads();
 
   typedef typename Half<FMT>::T T16;
   typedef typename Half<FMT>::x8 x8;
-  const int r = lane & 31, h = lane >> 5;
-  const int t = max(list[r], 0);
-  const int units = (a.in + 15) / 16;  // of sixteen values; each lane has eight
-  const int parts = gridDim.x * 4, part = blockIdx.x * 4 + wave;
-  const int u0 = (int)((int64_t)units * part / parts), u1 = (int)((int64_t)units * (part + 1) / parts);
-  const char* x = static_cast<const char*>(a.x) + (int64_t)t * a.x_bytes;
-  const T16* A = static_cast<const T16*>(a.a) + (int64_t)k * a.rank * a.in;
-  f32x16 acc[RB];
+  constexpr bool kCodes = FMT == kRowFp8 || FMT == kRowFp8Wide;
+  typedef std::conditional_t<kCodes, uint2, x8> piece_t;  // eight values of x
+  constexpr int kUnits = kCodes ? 4 : 2;                  // products of 32 values in 128 bytes of x
+  const int r = lane & 15, g = lane >> 4;
+  const int steps = a.steps, parts = splits * WAVES, part = split * WAVES + wave;
+  const int s0 = (int)((int64_t)steps * part / parts), s1 = (int)((int64_t)steps * (part + 1) / parts);
+  const char* x[2];
+  const uint8_t* scale[2] = {};
 #pragma unroll
-  for (int j = 0; j < RB; ++j)
+  for (int m = 0; m < 2; ++m) {
+    const int t = max(l.list[16 * m + r], 0);
+    x[m] = static_cast<const char*>(a.x) + (int64_t)t * a.x_bytes;
+    if (kCodes) scale[m] = a.x_scale + (int64_t)t * a.x_scale_bytes;
+  }
+  const int rank = min(a.rank - rank0, kRankPart);
+  const T16* A = static_cast<const T16*>(a.a) + ((int64_t)k * a.rank + rank0) * a.in;
+  f32x4 acc[2][RB];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[j][i] = 0.0f;
-  for (int u = u0; u < u1; ++u) {
-    const int at = 16 * u + 8 * h;
-    x8 xv, av[RB];
+  for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) xv[i] = (T16)0.0f;
+    for (int j = 0; j < RB; ++j) acc[m][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  struct Step {
+    piece_t x[2][kUnits];
+    x8 a[RB][kUnits];
+    int scale[2];
+  };
+  auto load = [&](int s, Step& v) {
 #pragma unroll
-    for (int j = 0; j < RB; ++j) av[j] = xv;
-    if (at < a.in) {
-      if constexpr (FMT == kRowFp8 || FMT == kRowFp8Wide) {
-        const uint2 c = *reinterpret_cast<const uint2*>(x + at);
-        const float s = scale_value(a.x_scale[(int64_t)t * a.x_scale_bytes + at / 128]);
+    for (int q = 0; q < kUnits; ++q) {
+      const int at = (s * kUnits + q) * 32 + 8 * g;
+      const bool in = at < a.in;
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t word = w ? c.y : c.x;
-          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
-          xv[4 * w] = (T16)(lo[0] * s);  // exact: four bits of significand
-          xv[4 * w + 1] = (T16)(lo[1] * s);
-          xv[4 * w + 2] = (T16)(hi[0] * s);
-          xv[4 * w + 3] = (T16)(hi[1] * s);
-        }
-      } else {
-        xv = *reinterpret_cast<const x8*>(x + 2 * at);
-      }
+      for (int m = 0; m < 2; ++m) v.x[m][q] = in ? *reinterpret_cast<const piece_t*>(x[m] + at * (kCodes ? 1 : 2)) : piece_t{};
 #pragma unroll
-      for (int j = 0; j < RB; ++j) {
-        const int row = 32 * j + r;
-        if (row < a.rank) av[j] = *reinterpret_cast<const x8*>(A + (int64_t)row * a.in + at);
-      }
+      for (int j = 0; j < RB; ++j) v.a[j][q] = in && 16 * j + r < rank ? *reinterpret_cast<const x8*>(A + (int64_t)(16 * j + r) * a.in + at) : x8{};
     }
+    if constexpr (kCodes)
 #pragma unroll
-    for (int j = 0; j < RB; ++j) acc[j] = mfma16(av[j], xv, acc[j]);
+      for (int m = 0; m < 2; ++m) v.scale[m] = scale[m][s];
+  };
+  auto use = [&](const Step& v) {
+#pragma unroll
+    for (int q = 0; q < kUnits; ++q)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        x8 xv;
+        if constexpr (kCodes) xv = widen8(v.x[m][q], scale_value(v.scale[m]));
+        else xv = v.x[m][q];
+#pragma unroll
+        for (int j = 0; j < RB; ++j) acc[m][j] = mfma(v.a[j][q], xv, acc[m][j]);
+      }
+  };
+  Step v[2];
+  if (s0 < s1) load(s0, v[0]);
+  for (int s = s0; s < s1; s += 2) {
+    if (s + 1 < s1) load(s + 1, v[1]);
+    use(v[0]);
+    if (s + 2 < s1) load(s + 2, v[0]);
+    if (s + 1 < s1) use(v[1]);
   }
   const float c = a.times ? a.times[k] : 1.0f;
 #pragma unroll
   for (int j = 0; j < RB; ++j) {
-    // lane: row r, columns 8 q + 4 h + 0 .. 3 of the block
+    // lane: rows r and 16 + r, columns 4 g + 0 .. 3 of the block
     if (j) __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<f32x4*>(&sums[wave][r][8 * q + 4 * h]) =
-          f32x4{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+    for (int m = 0; m < 2; ++m) *reinterpret_cast<f32x4*>(&l.sums[wave][16 * m + r][4 * g]) = acc[m][j];
     __syncthreads();
-    for (int i = tid; i < 32 * 32; i += 256) {
-      const int m = i / 32, col = i % 32;
-      if (list[m] < 0 || 32 * j + col >= a.rank) continue;
-      const float s = (sums[0][m][col] + sums[1][m][col]) + (sums[2][m][col] + sums[3][m][col]);
-      a.u[((int64_t)blockIdx.x * a.T + list[m]) * a.rank + 32 * j + col] = s * c;
+    for (int i = tid; i < 32 * 16; i += kThreads) {
+      const int m = i / 16, col = i % 16;
+      if (l.list[m] < 0 || 16 * j + col >= rank) continue;
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) s += l.sums[w][m][col];
+      a.u[((int64_t)split * a.T + l.list[m]) * a.rank + rank0 + 16 * j + col] = s * c;
     }
   }
 }
-
-// ---- the projection --------------------------------------------------------------------
-// The adapters' second product on a wave's sums: for every adapter among the 32 rows of
-// a block, B_a u on the matrix cores, u as sums of 16-bit numbers (PLANES of them: 8 bits
-// each in BF16, 11 in F16), kept by the rows that are the adapter's own.  A row that
-// has another keeps its sum untouched, whatever B_a holds.
-template <int FMT, int NB>
-__device__ __forceinline__ void add_adapters(const ProjectArgs& a, int m, int id, int n0, f32x16* acc, int planes) {
-  typedef typename Half<FMT>::T T16;
-  typedef typename Half<FMT>::x8 x8;
-  const int lane = threadIdx.x & 63, h = lane >> 5;
-  uint64_t left = __ballot(id >= 0);
-  const float* u = a.u + (int64_t)m * a.rank;
-  // F16 planes: the row's largest brought to [1, 2), so that none overflows and few are lost
-  float up = 1.0f, down = 1.0f;
-  if constexpr (FMT == kRowF16) {
-    float top = 0.0f;
-    if (id >= 0)
-      for (int j = 0; j < a.rank; ++j) top = fmaxf(top, fabsf(u[j]));
-    const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 100);
-    up = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-    down = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
-  }
-  while (left) {
-    const int k = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-    const bool mine = id == k;
-    left &= ~__ballot(mine);
-    const T16* B = static_cast<const T16*>(a.b) + (int64_t)k * a.out * a.rank;
-    f32x16 sum[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum[nb][i] = 0.0f;
-    for (int j0 = 0; j0 < a.rank; j0 += 16) {
-      const int j = j0 + 8 * h;
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-      x8 bv[NB];
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) bv[nb][i] = (T16)0.0f;
-      if (j < a.rank) {
-        if (mine) load8(u + j, true, v);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          const int n = min(n0 + 32 * nb + (lane & 31), a.out - 1);
-          bv[nb] = *reinterpret_cast<const x8*>(B + (int64_t)n * a.rank + j);
-        }
-      }
-      for (int p = 0; p < planes; ++p) {
-        x8 w;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (p == 0) v[i] *= up;
-          w[i] = (T16)v[i];
-          const float rest = v[i] - (float)w[i];
-          v[i] = fabsf(rest) < __builtin_inff() ? rest : 0.0f;  // an infinity has no rest
-        }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) sum[nb] = mfma16(bv[nb], w, sum[nb]);
-      }
-    }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[nb][i] = mine ? fmaf(sum[nb][i], down, acc[nb][i]) : acc[nb][i];
-  }
+template <int FMT, int WAVES>
+__device__ __forceinline__ void adapter_in(const ProjectArgs& a, int split, int splits, int mine, int rank0, AdapterLds& l) {
+  if (a.rank <= 16) adapter_in<FMT, 1, WAVES>(a, split, splits, mine, rank0, l);
+  else if (a.rank <= 32) adapter_in<FMT, 2, WAVES>(a, split, splits, mine, rank0, l);
+  else adapter_in<FMT, 4, WAVES>(a, split, splits, mine, rank0, l);
 }
 
-__device__ __forceinline__ float swap_halves(float lo, float hi, float* other) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi), false, false);
-  *other = __builtin_bit_cast(float, (uint32_t)r[1]);
-  return __builtin_bit_cast(float, (uint32_t)r[0]);
+}  // namespace
+
+template <int FMT, int RB>
+__global__ __launch_bounds__(512) void k_adapter_in(ProjectArgs a) {
+  __shared__ AdapterLds l;
+  adapter_in<FMT, RB, 8>(a, blockIdx.x, gridDim.x, blockIdx.y, blockIdx.z * kRankPart, l);
 }
 
-// Row m's columns n0 .. n0 + 31 of a block's sums: lane (m, h) has the columns
-// 8 q + 4 h + 0 .. 3; the halves exchange so that each has eight neighbours twice.
-template <typename TY>
-__device__ __forceinline__ void store_block(TY* y, bool live, int n0, int out, bool vec, const f32x16& c) {
-  const int h = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = swap_halves(c[8 * p + i], c[8 * p + 4 + i], &v[4 + i]);
-    const int n = n0 + 16 * p + 8 * h;
-    if (!live) continue;
-    if (vec && n + 8 <= out) {
-      store8(y + n, true, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (n + i < out) y[n + i] = (TY)v[i];
-    }
-  }
+// ---- the tiles -----------------------------------------------------------------------------
+// Tiles of a projection in the order in which workgroups take them.  Neighbours in the list
+// run on one XCD (workgroups go round the eight in turn) and share what they read: bands of
+// four tiles of rows, down and then along.
+struct Place {
+  int part, m, n;
+};
+__device__ __forceinline__ int on_xcd(int i, int count) {
+  const int xcd = i % 8;
+  return xcd * (count / 8) + min(xcd, count % 8) + i / 8;
+}
+__device__ __forceinline__ Place place_of(int tile, int m_tiles, int n_tiles) {
+  const int band = tile / (4 * n_tiles), high = min(4, m_tiles - 4 * band), in_band = tile - band * 4 * n_tiles;
+  return {0, 4 * band + in_band % high, in_band / high};
 }
 
-// A tile of 32 MB WM rows of x by 32 NB WN rows of the matrix, WM x WN waves, over the
-// steps of its part.  Each step's 128 bytes of every row go straight into LDS (STAGES
-// steps there at a time, so that STAGES - 1 are under way), and from there as operands:
-// the matrix's rows first, so that a lane holds one row of the result.
-template <int FMT, int MB, int NB, int WM, int WN, int STAGES>
+// A tile of BM rows of x by BN of the matrix, WM x WN waves, over the steps (128 bytes of
+// every row) of its part of the inner dimension.  Steps go straight into LDS, into a ring of
+// RING, RING - 1 of them under way, and from there as operands.  Whole lines of 128 bytes,
+// because half a line costs a CU's loads as much as a whole one (32 against 53 bytes a cycle).
+// TURN (eight waves, two a SIMD; 0: without): a wave's turn is TURN bytes of the rows and has
+// two parts, its operands' LDS reads, in a step's first turn with the requests for a step to
+// come, and the products; the two waves of a SIMD take opposite parts, with a barrier
+// between, so that the products of one run while the other reads:
+//   interval   2 j         2 j + 1       2 j + 2
+//   waves 0-3  read j      products j    read j + 1
+//   waves 4-7  products    read j        products j
+// The requests for step s + RING - 1 fill the place of s - 1, which both have read an interval
+// before.  Without turns all read, then multiply.
+// The first a.u_groups workgroups do the adapters' first product, the next a.full a tile
+// each, the others a part of one.
+template <int FMT, int BM, int BN, int WM, int WN, int RING, int TURN>
 __global__ __launch_bounds__(64 * WM * WN) void k_project(ProjectArgs a) {
-  constexpr int kWaves = WM * WN, BM = 32 * MB * WM, BN = 32 * NB * WN, kRows = BM + BN;
-  constexpr int kStage = kRows * kStepBytes;
-  constexpr int kLoads = kRows / 8 / kWaves;  // of a wave and step, eight rows each
-  static_assert(kRows % (8 * kWaves) == 0 && BM % 8 == 0, "whole loads");
-  __shared__ __attribute__((aligned(16))) char lds[STAGES * kStage];
+  constexpr bool kCodes = FMT == kRowFp8 || FMT == kRowFp8Wide;
+  constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, kStage = (BM + BN) * kStepBytes;
+  constexpr int kLoadsX = BM / 8 / kWaves, kLoads = (BM + BN) / 8 / kWaves;  // of a wave and step, eight rows each
+  constexpr int kBlock = Block<FMT>::kRows, MB = BM / WM / kBlock, NB = BN / WN / kBlock;
+  constexpr int kPieces = kBlock / 16;         // 16-byte pieces of a lane's operand
+  constexpr int kHalves = TURN == 64 ? 1 : 2;  // of a step (a product each) that are read at a time
+  constexpr int kGroups = BN / 128, kScales = (BM + kGroups + 63) / 64 * 64;
+  static_assert(BM % (8 * kWaves) == 0 && BN % (8 * kWaves) == 0 && BN % 128 == 0, "whole loads and groups");
+  static_assert(MB * WM * kBlock == BM && NB * WN * kBlock == BN && kScales <= kThreads && (!TURN || kWaves == 8), "whole blocks");
+  static_assert(sizeof(AdapterLds) <= RING * kStage, "LDS");
+  typedef std::conditional_t<kCodes, i32x4, typename Half<FMT>::x8> piece_t;
+  __shared__ __attribute__((aligned(16))) char lds[RING * kStage];
+  __shared__ __attribute__((aligned(16))) int scales[kCodes ? RING : 1][kScales];  // rows of x, then the matrix's groups
   __shared__ int ids[BM];
+  if ((int)blockIdx.x < a.u_groups) {
+    const int halves = (a.rank + kRankPart - 1) / kRankPart, tile = blockIdx.x / a.u_splits;
+    adapter_in<FMT, kWaves>(a, blockIdx.x % a.u_splits, a.u_splits, tile / halves, tile % halves * kRankPart, *reinterpret_cast<AdapterLds*>(lds));
+    return;
+  }
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int r = lane & 31, h = lane >> 5;
-  const int m_tiles = (a.T + BM - 1) / BM;
-  const int tile = blockIdx.x;
-  const int m0 = tile % m_tiles * BM, n0 = tile / m_tiles * BN;
-  const int part = blockIdx.y;
-  const int step0 = (int)((int64_t)a.steps * part / gridDim.y), step1 = (int)((int64_t)a.steps * (part + 1) / gridDim.y);
+  const int r = lane % kBlock, h = lane / kBlock;
+  const bool second = wave >= 4;
+  const int m_tiles = (a.T + BM - 1) / BM, n_tiles = (a.out + BN - 1) / BN, tiles = m_tiles * n_tiles;
+  const int group = (int)blockIdx.x - a.u_groups;
+  int tile, part = 0, parts = 1;
+  if (group < a.full) {
+    tile = on_xcd(group, a.full);
+  } else {
+    const int rest = tiles - a.full, at = on_xcd(group - a.full, rest * a.splits);
+    part = at / rest;
+    parts = a.splits;
+    tile = a.full + at - part * rest;
+  }
+  const Place place = place_of(tile, m_tiles, n_tiles);
+  const int m0 = BM * place.m, n0 = BN * place.n;
+  const int step0 = (int)((int64_t)a.steps * part / parts), step1 = (int)((int64_t)a.steps * (part + 1) / parts);
+  const int whole = a.row_bytes / kStepBytes;  // steps
 
-  // this wave's loads: their rows' addresses; rows past the end are the last one's again
-  const char* from[kLoads];
+  // this wave's loads: offsets of their rows, those past the end being the last one again
+  const char* base_x = static_cast<const char*>(a.x) + (int64_t)m0 * a.x_bytes;
+  const char* base_w = static_cast<const char*>(a.w) + (int64_t)n0 * a.w_bytes;
+  uint32_t off[kLoads];
   int piece[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int row = 8 * (wave * kLoads + i) + lane / 8;
-    piece[i] = ((lane & 7) ^ piece_swap(row)) * 16;
-    from[i] = row < BM ? static_cast<const char*>(a.x) + (int64_t)min(m0 + row, a.T - 1) * a.x_bytes
-                       : static_cast<const char*>(a.w) + (int64_t)min(n0 + row - BM, a.out - 1) * a.w_bytes;
+    const bool of_x = i < kLoadsX;
+    const int row = (kWaves * (of_x ? i : i - kLoadsX) + wave) * 8 + lane / 8;
+    piece[i] = ((lane & 7) ^ swap8<FMT>(row)) * 16;
+    off[i] = (of_x ? (uint32_t)(min(row, a.T - 1 - m0) * a.x_bytes) : (uint32_t)(min(row, a.out - 1 - n0) * a.w_bytes)) + piece[i];
   }
   auto bring = [&](int step) {
-    char* to = lds + (step % STAGES) * kStage + wave * kLoads * 1024;
+    if (step >= step1) return;
+    char* to = lds + (unsigned)step % RING * kStage + wave * 1024;
+    auto at = [&](int i) { return to + (i < kLoadsX ? i * kWaves * 1024 : BM * kStepBytes + (i - kLoadsX) * kWaves * 1024); };
+    if (step < whole) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = step * kStepBytes + piece[i];
-      lds_load16(at < a.row_bytes ? from[i] + at : reinterpret_cast<const char*>(zeros16), to + 1024 * i);
+      for (int i = 0; i < kLoads; ++i) lds_load16((i < kLoadsX ? base_x : base_w) + (int64_t)step * kStepBytes, off[i], at(i));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int b = step * kStepBytes + piece[i];
+        lds_load16(b < a.row_bytes ? (i < kLoadsX ? base_x : base_w) + off[i] + step * kStepBytes : reinterpret_cast<const char*>(zeros16), at(i));
+      }
     }
   };
+  // the scales of a step: a byte a thread, by the waves that have some
+  const bool scaler = kCodes && wave * 64 < kScales;
+  const uint8_t* scale_at = nullptr;
+  if constexpr (kCodes)
+    scale_at = tid < BM ? a.x_scale + (int64_t)min(m0 + tid, a.T - 1) * a.x_scale_bytes
+                        : a.w_scale + (int64_t)min(n0 / 128 + (tid - BM) % kGroups, (a.out - 1) / 128) * a.w_scale_bytes;
+  auto bring_scales = [&](int step) {
+    if (scaler && step < step1) lds_load_byte(scale_at + step, reinterpret_cast<char*>(&scales[(unsigned)step % RING][64 * wave]));
+  };
 
-  f32x16 acc[MB][NB];
+  typename Block<FMT>::sum_t acc[MB][NB];
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+      for (int e = 0; e < Block<FMT>::kOf; ++e) acc[i][j][e] = 0.0f;
 
+  // where a lane's pieces of a step's first half lie, for the first block of x's rows and for
+  // each of the matrix's: the pieces kPieces h + 0 .. kPieces - 1; of the second half 64 bytes apart
   const int wm = wave / WN, wn = wave % WN;
-  const int row_m = 32 * MB * wm + r, row_n = BM + 32 * NB * wn + r;  // in a stage
-  const int swap = piece_swap(r);
+  int at_x[kPieces], at_w[NB][kPieces];
+  auto place_in = [&](int row, int c) { return row * kStepBytes + (c ^ swap8<FMT>(row)) * 16; };
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (step0 + s < step1) bring(step0 + s);
-  for (int step = step0; step < step1; ++step) {
-    // (the last steps wait for everything: nothing is under way behind them)
-    if (step + STAGES - 1 <= step1) wait_loads<(STAGES - 2) * kLoads>();
-    else wait_loads<0>();
-    barrier();
-    if (step + STAGES - 1 < step1) bring(step + STAGES - 1);
-    const char* stage = lds + (step % STAGES) * kStage;
-    int xs[MB], ws[NB];
-    if constexpr (FMT == kRowFp8 || FMT == kRowFp8Wide) {
+  for (int p = 0; p < kPieces; ++p) {
+    at_x[p] = place_in(BM / WM * wm + r, kPieces * h + p);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) xs[i] = a.x_scale[(int64_t)min(m0 + row_m + 32 * i, a.T - 1) * a.x_scale_bytes + step];
+    for (int j = 0; j < NB; ++j) at_w[j][p] = BM * kStepBytes + place_in(BN / WN * wn + matrix_row<FMT, NB>(r, j), kPieces * h + p);
+  }
+
+  piece_t xv[MB][kHalves][kPieces], wv[NB][kHalves][kPieces];
+  int xs[MB] = {}, ws = 0;
+  auto read = [&](int step, int half0) {
+    const char* s = lds + (unsigned)step % RING * kStage;
 #pragma unroll
-      for (int j = 0; j < NB; ++j) ws[j] = a.w_scale[(int64_t)(min(n0 + row_n - BM + 32 * j, a.out - 1) / 128) * a.w_scale_bytes + step];
-    }
-    if constexpr (FMT == kRowFp8Wide) {
+    for (int k = 0; k < kHalves; ++k)
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int at = ((2 * s + h) ^ swap) << 4;
-        bf16x8 xv[MB][2], wv[NB][2];
+      for (int p = 0; p < kPieces; ++p) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) widen16(*reinterpret_cast<const i32x4*>(stage + (row_m + 32 * i) * kStepBytes + at), scale_value(xs[i]), xv[i]);
+        for (int i = 0; i < NB; ++i) wv[i][k][p] = *reinterpret_cast<const piece_t*>(s + (at_w[i][p] ^ (half0 + k) << 6));
 #pragma unroll
-        for (int j = 0; j < NB; ++j) widen16(*reinterpret_cast<const i32x4*>(stage + (row_n + 32 * j) * kStepBytes + at), scale_value(ws[j]), wv[j]);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j] = mfma16(wv[j][k], xv[i][k], acc[i][j]);
+        for (int i = 0; i < MB; ++i)  // (row kBlock i + r's swap is that of kBlock i and of r)
+          xv[i][k][p] = *reinterpret_cast<const piece_t*>(s + (at_x[p] ^ ((half0 + k) << 6 ^ swap8<FMT>(kBlock * i) << 4)) + kBlock * kStepBytes * i);
       }
-    } else if constexpr (FMT == kRowFp8) {
+    if constexpr (kCodes) {
+      if (half0 == 0) {
+        const int* c = scales[(unsigned)step % RING];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        auto operand = [&](int row) {
-          const char* p = stage + row * kStepBytes;
-          const i32x4 lo = *reinterpret_cast<const i32x4*>(p + (((4 * s + 2 * h) ^ swap) << 4));
-          const i32x4 hi = *reinterpret_cast<const i32x4*>(p + (((4 * s + 2 * h + 1) ^ swap) << 4));
-          return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        };
-        i32x8 xv[MB], wv[NB];
+        for (int i = 0; i < MB; ++i) xs[i] = c[BM / WM * wm + r + kBlock * i];
+        ws = c[BM + BN / WN * wn / 128];
+      }
+    }
+  };
+  auto products = [&]() {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) xv[i] = operand(row_m + 32 * i);
-#pragma unroll
-        for (int j = 0; j < NB; ++j) wv[j] = operand(row_n + 32 * j);
+    for (int k = 0; k < kHalves; ++k) {
+      if constexpr (FMT == kRowFp8) {
+        auto eight = [](const piece_t* v) { return i32x8{v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]}; };
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
           for (int j = 0; j < NB; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[j], xv[i], acc[i][j], 0, 0, 0, ws[j], 0, xs[i]);
-      }
-    } else {
-      typedef typename Half<FMT>::x8 x8;
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(eight(wv[j][k]), eight(xv[i][k]), acc[i][j], 0, 0, 0, ws, 0, xs[i]);
+      } else if constexpr (FMT == kRowFp8Wide) {
+        bf16x8 w[NB][2];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int at = ((2 * s + h) ^ swap) << 4;
-        x8 xv[MB], wv[NB];
+        for (int j = 0; j < NB; ++j) widen16(wv[j][k][0], scale_value(ws), w[j]);
 #pragma unroll
-        for (int i = 0; i < MB; ++i) xv[i] = *reinterpret_cast<const x8*>(stage + (row_m + 32 * i) * kStepBytes + at);
+        for (int i = 0; i < MB; ++i) {
+          bf16x8 x[2];
+          widen16(xv[i][k][0], scale_value(xs[i]), x);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) wv[j] = *reinterpret_cast<const x8*>(stage + (row_n + 32 * j) * kStepBytes + at);
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = mfma(w[j][e], x[e], acc[i][j]);
+        }
+      } else {
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
-          for (int j = 0; j < NB; ++j) acc[i][j] = mfma16(wv[j], xv[i], acc[i][j]);
+          for (int j = 0; j < NB; ++j) acc[i][j] = mfma(wv[j][k][0], xv[i][k][0], acc[i][j]);
       }
     }
-  }
+  };
+  // Step s + 1 has landed when no more are under way than the requests behind its own: those
+  // of RING - 2 steps, with a scales' one each; near the end, when none follow, all have.
+  auto landed = [&](int step) {
+    if (step + RING - 1 >= step1) wait_loads<0>();
+    else if (scaler) wait_loads<(RING - 2) * (kLoads + 1)>();
+    else wait_loads<(RING - 2) * kLoads>();
+  };
 
-  const bool direct = a.part == nullptr;
-  if (direct && a.n_adapters) {
-    for (int i = tid; i < BM; i += 64 * kWaves) ids[i] = adapter_of(a, m0 + i);
-    __syncthreads();
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s) {
+    bring(step0 + s);
+    if constexpr (kCodes) bring_scales(step0 + s);
   }
+  if (a.n_adapters && group < a.full)
+    for (int i = tid; i < BM; i += kThreads) ids[i] = adapter_of(a, m0 + i);
+  landed(step0 - 1);
+  if constexpr (TURN) {
+    barrier();
+    if (second) barrier();
+  }
+  for (int step = step0; step < step1; ++step) {
+    if constexpr (!TURN) {
+      if (step > step0) landed(step - 1);
+      barrier();
+      read(step, 0);
+      bring(step + RING - 1);
+      if constexpr (kCodes) bring_scales(step + RING - 1);
+      products();
+    } else {
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int m = m0 + row_m + 32 * i, nb0 = n0 + row_n - BM - r;
-    if (direct && a.n_adapters) add_adapters<FMT, NB>(a, m, ids[row_m + 32 * i], nb0, acc[i], a.planes);
-    const bool live = m < a.T;
+      for (int turn = 0; turn < 2 / kHalves; ++turn) {
+        const bool last = turn == 2 / kHalves - 1;
+        read(step, turn);
+        if (turn == 0) {
+          bring(step + RING - 1);
+          if constexpr (kCodes) bring_scales(step + RING - 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (last && second) landed(step);
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        barrier();
+        __builtin_amdgcn_s_setprio(1);
+        __builtin_amdgcn_sched_barrier(0);
+        products();
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int n = nb0 + 32 * j;
-      if (!direct) {
-        store_block(a.part + ((int64_t)part * a.T + m) * a.out, live, n, a.out, a.vec_part, acc[i][j]);
-      } else {
-        char* y = static_cast<char*>(a.y) + (int64_t)m * a.y_bytes;
-        if (a.y_type == ElemType::f32) store_block(reinterpret_cast<float*>(y), live, n, a.out, a.vec_y, acc[i][j]);
-        else if (a.y_type == ElemType::f16) store_block(reinterpret_cast<_Float16*>(y), live, n, a.out, a.vec_y, acc[i][j]);
-        else store_block(reinterpret_cast<__bf16*>(y), live, n, a.out, a.vec_y, acc[i][j]);
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int e = 0; e < NB; ++e) asm volatile("" : "+v"(acc[i][e]));  // here, not where the sums are next used
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(0);
+        if (last && !second) landed(step);
+        barrier();
       }
     }
   }
+  if constexpr (TURN)
+    if (!second) barrier();
+
+  float* to = nullptr;
+  if (group >= a.full)
+    to = a.part + ((int64_t)part * (tiles - a.full) + tile - a.full) * (BM * BN) + BM / WM * wm * BN + BN / WN * wn;
+  store_tile<FMT, MB, NB>(a, acc, to, BN, m0 + BM / WM * wm, n0 + BN / WN * wn, ids + BM / WM * wm);
 }
 
 // ---- parts and the adapters' second product, added -------------------------------------
-// One row a workgroup of 256 columns; u in LDS.
-template <int FMT>
+// CHUNKS times 256 neighbouring values of a tile's parts a workgroup, 256 / BN rows each: summed
+// by the four waves together, four values a lane, while the rows' adapters are looked up;
+// then a value a thread, B's row of an adapter read once for the neighbouring rows that have it.
+template <int FMT, int BM, int BN, int CHUNKS>
 __global__ __launch_bounds__(256) void k_project_join(ProjectArgs a) {
   typedef typename Half<FMT>::T T16;
   typedef typename Half<FMT>::x8 x8;
-  __shared__ float u[kMaxRank];
-  const int t = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
-  const int k = adapter_of(a, t);
-  if (k >= 0)
-    for (int j = threadIdx.x; j < a.rank; j += 256) {
+  constexpr int kSub = 256 / BN, kRows = CHUNKS * kSub;
+  __shared__ __attribute__((aligned(16))) float sums[4][256];
+  __shared__ float u[kRows][kMaxRank];
+  __shared__ int ids[kRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int m_tiles = (a.T + BM - 1) / BM, n_tiles = (a.out + BN - 1) / BN, rest = m_tiles * n_tiles - a.full;
+  const Place place = place_of(a.full + blockIdx.x, m_tiles, n_tiles);
+  const int t0 = BM * place.m + kRows * (int)blockIdx.y, rows = min(kRows, a.T - t0);
+  if (rows <= 0) return;
+  const int sub = tid / BN, n = BN * place.n + tid % BN;
+  if (a.n_adapters) {
+    if (tid < kRows) ids[tid] = -1;
+    __syncthreads();
+    for (int b = tid; b < a.B; b += 256) {
+      const int k = a.adapter[b], from = max(a.q_start[b], t0), to = min(a.q_start[b + 1], t0 + rows);
+      if (k >= 0 && k < a.n_adapters)
+        for (int t = from; t < to; ++t) ids[t - t0] = k;
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * a.rank; i += 256) {
+      const int m = i / a.rank, j = i % a.rank;
+      if (ids[m] < 0) continue;
       float s = 0.0f;
-      for (int p = 0; p < a.u_splits; ++p) s += a.u[((int64_t)p * a.T + t) * a.rank + j];
-      u[j] = s;
+      for (int p = 0; p < a.u_splits; ++p) s += a.u[((int64_t)p * a.T + t0 + m) * a.rank + j];
+      u[m][j] = s;
     }
-  __syncthreads();
-  if (n >= a.out) return;
-  float y = 0.0f;
-  for (int p = 0; p < a.splits; ++p) y += a.part[((int64_t)p * a.T + t) * a.out + n];
-  if (k >= 0) {
-    const T16* B = static_cast<const T16*>(a.b) + ((int64_t)k * a.out + n) * a.rank;
-    float d = 0.0f;
-    for (int j = 0; j < a.rank; j += 8) {
-      const x8 v = *reinterpret_cast<const x8*>(B + j);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) d = fmaf(u[j + i], (float)v[i], d);
-    }
-    y += d;
   }
-  char* to = static_cast<char*>(a.y) + (int64_t)t * a.y_bytes;
-  if (a.y_type == ElemType::f32) reinterpret_cast<float*>(to)[n] = y;
-  else if (a.y_type == ElemType::f16) reinterpret_cast<_Float16*>(to)[n] = (_Float16)y;
-  else reinterpret_cast<__bf16*>(to)[n] = (__bf16)y;
+  float y[CHUNKS];
+#pragma unroll
+  for (int m = 0; m < CHUNKS; ++m) {
+    if (m * kSub >= rows) break;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float* part = a.part + (int64_t)blockIdx.x * (BM * BN) + (kRows * (int)blockIdx.y + m * kSub) * BN + 4 * lane;
+    const int64_t next = (int64_t)rest * (BM * BN);
+#pragma unroll 4
+    for (int p = wave; p < a.splits; p += 4) s += *reinterpret_cast<const f32x4*>(part + p * next);
+    if (m) __syncthreads();
+    *reinterpret_cast<f32x4*>(&sums[wave][4 * lane]) = s;
+    __syncthreads();
+    y[m] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
+  }
+  if (n >= a.out) return;
+  if (a.n_adapters) {
+    const int own = (rows - sub + kSub - 1) / kSub;  // chunks that hold a row of this thread's
+    for (int m = 0; m < own;) {
+      const int k = ids[m * kSub + sub];
+      int end = m + 1;
+      while (end < own && ids[end * kSub + sub] == k) ++end;
+      if (k >= 0) {
+        const T16* B = static_cast<const T16*>(a.b) + ((int64_t)k * a.out + n) * a.rank;
+        for (int j = 0; j < a.rank; j += 8) {
+          const x8 v = *reinterpret_cast<const x8*>(B + j);
+#pragma unroll
+          for (int i = 0; i < CHUNKS; ++i)
+            if (i >= m && i < end) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[i] = fmaf(u[i * kSub + sub][j + e], (float)v[e], y[i]);
+            }
+        }
+      }
+      m = end;
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < CHUNKS; ++m) {
+    const int row = m * kSub + sub;
+    if (row >= rows) break;
+    char* to = static_cast<char*>(a.y) + (int64_t)(t0 + row) * a.y_bytes;
+    if (a.y_type == ElemType::f32) reinterpret_cast<float*>(to)[n] = y[m];
+    else if (a.y_type == ElemType::f16) reinterpret_cast<_Float16*>(to)[n] = (_Float16)y[m];
+    else reinterpret_cast<__bf16*>(to)[n] = (__bf16)y[m];
+  }
 }
 
 namespace {
 
 template <int FMT>
 hipError_t launch_adapter_in(const ProjectArgs& a, hipStream_t s) {
-  const dim3 grid(a.u_splits, (a.T + 31) / 32 + std::min(a.B, a.n_adapters));
-  if (a.rank <= 32) k_adapter_in<FMT, 1><<<grid, 256, 0, s>>>(a);
-  else if (a.rank <= 64) k_adapter_in<FMT, 2><<<grid, 256, 0, s>>>(a);
-  else k_adapter_in<FMT, 4><<<grid, 256, 0, s>>>(a);
+  const dim3 grid(a.u_splits, adapter_tiles(a.T, a.B, a.n_adapters), rank_parts(a.rank));
+  if (a.rank <= 16) k_adapter_in<FMT, 1><<<grid, 512, 0, s>>>(a);
+  else if (a.rank <= 32) k_adapter_in<FMT, 2><<<grid, 512, 0, s>>>(a);
+  else k_adapter_in<FMT, 4><<<grid, 512, 0, s>>>(a);
   return hipGetLastError();
 }
 
-template <int FMT, int MB, int NB, int WM, int WN, int STAGES>
-hipError_t launch_tiles(const ProjectArgs& a, hipStream_t s) {
-  constexpr int BM = 32 * MB * WM, BN = 32 * NB * WN;
-  const dim3 grid(((a.T + BM - 1) / BM) * ((a.out + BN - 1) / BN), a.splits);
-  k_project<FMT, MB, NB, WM, WN, STAGES><<<grid, 64 * WM * WN, 0, s>>>(a);
+template <int FMT, int BM, int BN, int WM, int WN, int RING, int TURN>
+hipError_t launch_tiles(ProjectArgs a, const ProjectPlan& p, hipStream_t s) {
+  const int m_tiles = (a.T + BM - 1) / BM, tiles = m_tiles * ((a.out + BN - 1) / BN), rest = tiles - a.full;
+  a.u_groups = 0;
+  if (a.n_adapters && a.full) {
+    const hipError_t e = launch_adapter_in<FMT>(a, s);
+    if (e != hipSuccess) return e;
+  } else if (a.n_adapters) {
+    a.u_groups = adapter_tiles(a.T, a.B, a.n_adapters) * rank_parts(a.rank) * a.u_splits;
+  }
+  k_project<FMT, BM, BN, WM, WN, RING, TURN><<<a.u_groups + a.full + rest * a.splits, 64 * WM * WN, 0, s>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !rest) return e;
+  const int rows = std::min(BM, a.T), of_one = 256 / BN;
+  if (a.T <= 64) k_project_join<FMT, BM, BN, 1><<<dim3(rest, (rows + of_one - 1) / of_one), 256, 0, s>>>(a);
+  else k_project_join<FMT, BM, BN, 8><<<dim3(rest, (rows + 8 * of_one - 1) / (8 * of_one)), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
 template <int FMT>
 hipError_t launch_fmt(const ProjectArgs& a, const ProjectPlan& p, hipStream_t s) {
-  hipError_t e = hipSuccess;
-  if (a.n_adapters) e = launch_adapter_in<FMT>(a, s);
-  if (e != hipSuccess) return e;
   switch (p.tile) {
-    case kTile32: e = launch_tiles<FMT, 1, 1, 1, 4, 6>(a, s); break;
-    case kTile64: e = launch_tiles<FMT, 2, 1, 1, 4, 5>(a, s); break;
-    case kTile128: e = launch_tiles<FMT, 2, 2, 2, 2, 4>(a, s); break;
-    default: e = launch_tiles<FMT, 4, 2, 2, 4, 2>(a, s);
+    case kTile32: return launch_tiles<FMT, 32, 128, 1, 4, 6, 0>(a, p, s);
+    case kTile64: return launch_tiles<FMT, 64, 128, 2, 4, 5, 128>(a, p, s);
+    case kTile128: return launch_tiles<FMT, 128, 128, 2, 4, 4, 128>(a, p, s);
+    default: return launch_tiles<FMT, 256, 256, 2, 4, 2, 64>(a, p, s);
   }
-  if (e != hipSuccess || !p.join) return e;
-  k_project_join<FMT><<<dim3((a.out + 255) / 256, a.T), 256, 0, s>>>(a);
-  return hipGetLastError();
 }
 
 }  // namespace
