@@ -671,16 +671,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_project(ProjectArgs a) {
 }
 
 // ---- parts and the adapters' second product, added -------------------------------------
-// CHUNKS times 256 neighbouring values of a tile's parts a workgroup, 256 / BN rows each: summed
-// by the four waves together, four values a lane, while the rows' adapters are looked up;
-// then a value a thread, B's row of an adapter read once for the neighbouring rows that have it.
+// CHUNKS times 256 neighbouring values of a tile's parts a workgroup, 256 / BN rows each, a
+// value a thread and chunk.  All of a thread's parts are requested before the rows' adapters
+// are looked up; where there is one chunk the four waves share them, four values a lane.  B's row
+// of an adapter is read once for the neighbouring rows that have it.
 template <int FMT, int BM, int BN, int CHUNKS>
 __global__ __launch_bounds__(256) void k_project_join(ProjectArgs a) {
   typedef typename Half<FMT>::T T16;
   typedef typename Half<FMT>::x8 x8;
   constexpr int kSub = 256 / BN, kRows = CHUNKS * kSub;
   __shared__ __attribute__((aligned(16))) float sums[4][256];
-  __shared__ float u[kRows][kMaxRank];
+  __shared__ __attribute__((aligned(16))) float u[kRows][kMaxRank];
   __shared__ int ids[kRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int m_tiles = (a.T + BM - 1) / BM, n_tiles = (a.out + BN - 1) / BN, rest = m_tiles * n_tiles - a.full;
@@ -688,6 +689,22 @@ __global__ __launch_bounds__(256) void k_project_join(ProjectArgs a) {
   const int t0 = BM * place.m + kRows * (int)blockIdx.y, rows = min(kRows, a.T - t0);
   if (rows <= 0) return;
   const int sub = tid / BN, n = BN * place.n + tid % BN;
+  const float* part = a.part + (int64_t)blockIdx.x * (BM * BN) + kRows * (int)blockIdx.y * BN;
+  const int64_t next = (int64_t)rest * (BM * BN);
+  float y[CHUNKS];
+  if constexpr (CHUNKS == 1) {
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int p = wave; p < a.splits; p += 4) s += *reinterpret_cast<const f32x4*>(part + p * next + 4 * lane);
+    *reinterpret_cast<f32x4*>(&sums[wave][4 * lane]) = s;
+  } else {
+#pragma unroll
+    for (int m = 0; m < CHUNKS; ++m) y[m] = part[256 * m + tid];
+    for (int p = 1; p < a.splits; ++p) {
+#pragma unroll
+      for (int m = 0; m < CHUNKS; ++m) y[m] += part[p * next + 256 * m + tid];
+    }
+  }
   if (a.n_adapters) {
     if (tid < kRows) ids[tid] = -1;
     __syncthreads();
@@ -697,28 +714,18 @@ __global__ __launch_bounds__(256) void k_project_join(ProjectArgs a) {
         for (int t = from; t < to; ++t) ids[t - t0] = k;
     }
     __syncthreads();
-    for (int i = tid; i < rows * a.rank; i += 256) {
-      const int m = i / a.rank, j = i % a.rank;
+    const int quads = a.rank / 4;
+    for (int i = tid; i < rows * quads; i += 256) {
+      const int m = i / quads, j = 4 * (i - m * quads);
       if (ids[m] < 0) continue;
-      float s = 0.0f;
-      for (int p = 0; p < a.u_splits; ++p) s += a.u[((int64_t)p * a.T + t0 + m) * a.rank + j];
-      u[m][j] = s;
+      f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int p = 0; p < a.u_splits; ++p) s += *reinterpret_cast<const f32x4*>(a.u + ((int64_t)p * a.T + t0 + m) * a.rank + j);
+      *reinterpret_cast<f32x4*>(&u[m][j]) = s;
     }
   }
-  float y[CHUNKS];
-#pragma unroll
-  for (int m = 0; m < CHUNKS; ++m) {
-    if (m * kSub >= rows) break;
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    const float* part = a.part + (int64_t)blockIdx.x * (BM * BN) + (kRows * (int)blockIdx.y + m * kSub) * BN + 4 * lane;
-    const int64_t next = (int64_t)rest * (BM * BN);
-#pragma unroll 4
-    for (int p = wave; p < a.splits; p += 4) s += *reinterpret_cast<const f32x4*>(part + p * next);
-    if (m) __syncthreads();
-    *reinterpret_cast<f32x4*>(&sums[wave][4 * lane]) = s;
-    __syncthreads();
-    y[m] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
-  }
+  __syncthreads();
+  if constexpr (CHUNKS == 1) y[0] = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
   if (n >= a.out) return;
   if (a.n_adapters) {
     const int own = (rows - sub + kSub - 1) / kSub;  // chunks that hold a row of this thread's
@@ -728,13 +735,17 @@ __global__ __launch_bounds__(256) void k_project_join(ProjectArgs a) {
       while (end < own && ids[end * kSub + sub] == k) ++end;
       if (k >= 0) {
         const T16* B = static_cast<const T16*>(a.b) + ((int64_t)k * a.out + n) * a.rank;
+#pragma unroll 4
         for (int j = 0; j < a.rank; j += 8) {
           const x8 v = *reinterpret_cast<const x8*>(B + j);
 #pragma unroll
           for (int i = 0; i < CHUNKS; ++i)
             if (i >= m && i < end) {
+              const f32x4 lo = *reinterpret_cast<const f32x4*>(&u[i * kSub + sub][j]), hi = *reinterpret_cast<const f32x4*>(&u[i * kSub + sub][j + 4]);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[i] = fmaf(u[i * kSub + sub][j + e], (float)v[e], y[i]);
+              for (int e = 0; e < 4; ++e) y[i] = fmaf(lo[e], (float)v[e], y[i]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[i] = fmaf(hi[e], (float)v[4 + e], y[i]);
             }
         }
       }
@@ -776,9 +787,10 @@ hipError_t launch_tiles(ProjectArgs a, const ProjectPlan& p, hipStream_t s) {
   k_project<FMT, BM, BN, WM, WN, RING, TURN><<<a.u_groups + a.full + rest * a.splits, 64 * WM * WN, 0, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !rest) return e;
-  const int rows = std::min(BM, a.T), of_one = 256 / BN;
-  if (a.T <= 64) k_project_join<FMT, BM, BN, 1><<<dim3(rest, (rows + of_one - 1) / of_one), 256, 0, s>>>(a);
-  else k_project_join<FMT, BM, BN, 8><<<dim3(rest, (rows + 8 * of_one - 1) / (8 * of_one)), 256, 0, s>>>(a);
+  // one chunk a workgroup where there are few in all
+  const int rows = std::min(BM, a.T), chunks = (rows * BN + 255) / 256;
+  if (rest * chunks <= 4 * g_num_cus) k_project_join<FMT, BM, BN, 1><<<dim3(rest, chunks), 256, 0, s>>>(a);
+  else k_project_join<FMT, BM, BN, 8><<<dim3(rest, (chunks + 7) / 8), 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -786,8 +798,8 @@ template <int FMT>
 hipError_t launch_fmt(const ProjectArgs& a, const ProjectPlan& p, hipStream_t s) {
   switch (p.tile) {
     case kTile32: return launch_tiles<FMT, 32, 128, 1, 4, 6, 0>(a, p, s);
-    case kTile64: return launch_tiles<FMT, 64, 128, 2, 4, 5, 128>(a, p, s);
-    case kTile128: return launch_tiles<FMT, 128, 128, 2, 4, 4, 128>(a, p, s);
+    case kTile64: return launch_tiles<FMT, 64, 128, 2, 4, 5, 0>(a, p, s);
+    case kTile128: return launch_tiles<FMT, 128, 128, 2, 4, 4, 0>(a, p, s);
     default: return launch_tiles<FMT, 256, 256, 2, 4, 2, 64>(a, p, s);
   }
 }

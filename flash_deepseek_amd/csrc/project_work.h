@@ -40,29 +40,53 @@ inline int rank_parts(int rank) { return (rank + kRankPart - 1) / kRankPart; }
 
 // Rounds of tiles over the CUs (a workgroup has one to itself) leave some of them idle in the
 // last; its tiles are cut into parts of the inner dimension where that is worth what parts
-// cost, their sums being written and read again.
-//   us a step of 128 bytes in a workgroup: 1.7 of the largest tiles, 0.8 of the others
-//   us a part: 0.1 (256 KB) and 0.03; 8 us for the joining launch
+// cost, their sums being written and read again.  What a cut takes, in us, from what was
+// measured over 1 to 8192 rows of 1536 to 16384 values:
+//   a step of 128 bytes in a workgroup  0.3, 0.42, 0.53, 1.6 by tile; 3 a round for its two ends
+//   a part                              0.015, 0.02, 0.03, 0.13; 5 for the joining launch
+// (500 rows of 16384 BF16 values by 7168: tiles of 128 rows 137 us, of 256 in four parts 138;
+// 1000 rows 276 and, in two parts, 238; 256 rows 79 and 93; 128 rows of 7168 by 576 in tiles
+// of 64 rows 11.9, of 128 15.1; of 1536 by 24576 23.7 and 17.2.)
+constexpr double kStepUs[] = {0.3, 0.42, 0.53, 1.6}, kPartUs[] = {0.015, 0.02, 0.03, 0.13};
+// Parts at most: two for every CU, one of the largest tiles (64 MB of sums).
+inline int most_parts(int tile, int cus) { return tile == kTile256 ? cus : 2 * cus; }
+// Tiles that are mostly rows past the end are not considered.
+inline bool tile_fits(int tile, int T) { return tile == kTile32 ? T <= 64 : T > kTiles[tile].rows / 2; }
+
+struct ProjectCut {
+  int64_t full;
+  int splits;
+  double us;
+};
+inline ProjectCut project_cut(int tile, int T, int out, int steps, bool join, int cus) {
+  const int64_t tiles = tiles_of(tile, T, out), rest = tiles % cus;
+  auto round = [&](int n) { return n * kStepUs[tile] + 3; };
+  const double rounds = (double)(tiles / cus) * round(steps);
+  ProjectCut c{tiles - rest, 1, rounds + (rest ? round(steps) : 0) + (join ? rest * kPartUs[tile] : 0)};
+  for (int s = 2; s <= steps && rest * s <= most_parts(tile, cus); ++s) {
+    const double us = rounds + (double)((rest * s + cus - 1) / cus) * round((steps + s - 1) / s) + rest * s * kPartUs[tile] + (join ? 0 : 5);
+    if (us < c.us) c.us = us, c.splits = s;
+  }
+  if (c.splits == 1 && !join) c.full = tiles;
+  return c;
+}
 // u_tiles: workgroups that the adapters' first product takes at least, 0: no adapters.
 inline ProjectPlan project_plan(int T, int64_t row_bytes, int out, int u_tiles, int cus) {
   ProjectPlan p{};
   const int steps = steps_of(row_bytes);
-  p.tile = T <= 32 ? kTile32 : T <= 64 ? kTile64 : kTile128;
-  if (T > 128 && tiles_of(kTile256, T, out) * 4 >= cus * 3) p.tile = kTile256;
-  const int64_t tiles = tiles_of(p.tile, T, out), rest = tiles % cus;
-  const double step = p.tile == kTile256 ? 1.7 : 0.8, part = p.tile == kTile256 ? 0.1 : 0.03;
-  p.full = (int)(tiles - rest);
-  p.splits = 1;
   // few rows: the adapters' first product runs beside the matrix's, the joining launch has the second
   const bool join = u_tiles && T <= 64;
-  double least = step * steps + (join ? rest * part : 0);
-  for (int s = 2; s <= steps && rest * s <= 2 * cus; ++s) {
-    const double t = (double)((rest * s + cus - 1) / cus) * ((steps + s - 1) / s) * step + rest * s * part + (join ? 0 : 8);
-    if (t < least) least = t, p.splits = s;
+  ProjectCut c{0, 1, 0.0};
+  bool any = false;
+  for (int tile = kTile32; tile <= kTile256; ++tile) {
+    if (!tile_fits(tile, T)) continue;
+    const ProjectCut t = project_cut(tile, T, out, steps, join, cus);
+    if (!any || t.us < c.us) c = t, p.tile = tile, any = true;
   }
-  if (p.splits == 1 && !join) p.full = (int)tiles;
+  p.full = (int)c.full;
+  p.splits = c.splits;
   // what it takes to fill the CUs: twice by itself, and what the parts leave beside them
-  const int64_t room = p.full ? 2 * cus : cus - rest * p.splits;
+  const int64_t room = p.full ? 2 * cus : cus - (tiles_of(p.tile, T, out) - p.full) * p.splits;
   p.u_splits = u_tiles ? (int)std::min<int64_t>(std::max<int64_t>(room / u_tiles, 1), std::min(kMaxUSplits, steps)) : 0;
   return p;
 }
@@ -80,17 +104,15 @@ inline size_t project_bytes(const ProjectPlan& p, int T, int out, int rank) {
 // What any call of up to T rows needs, whatever its format and its requests.
 inline size_t project_most_bytes(int T, int in, int out, int rank, int cus) {
   size_t most = 0;
-  auto see = [&](int t) {
-    for (int size : {1, 2})
-      for (int u_tiles : {0, rank ? 1 : 0})
-        most = std::max(most, project_part_floats(project_plan(t, (int64_t)in * size, out, u_tiles, cus), t, out) * 4);
-  };
-  see(std::min(T, 32));
-  see(std::min(T, 64));
-  // the cut is the same from one multiple of 128 rows to the next
-  for (int64_t t = 128; t < T; t += 128) see((int)t);
-  see(T);
-  return std::max<size_t>(((size_t)kMaxUSplits * T * rank * 4 + 255) / 256 * 256 + most, 256);
+  for (int tile = kTile32; tile <= kTile256; ++tile) {
+    const int rows = tile == kTile32 ? std::min(T, 64) : T;
+    if (tile != kTile32 && !tile_fits(tile, T)) continue;
+    const int64_t parts = std::min<int64_t>(most_parts(tile, cus), tiles_of(tile, rows, out) * steps_of((int64_t)in * 2));
+    most = std::max(most, (size_t)parts * kTiles[tile].rows * kTiles[tile].cols * 4);
+  }
+  // (the splits of u are as many as leave two workgroups a CU, and there is one for 32 rows)
+  const int64_t u_rows = std::max<int64_t>(T, std::min<int64_t>((int64_t)kMaxUSplits * T, (int64_t)64 * cus));
+  return std::max<size_t>(((size_t)u_rows * rank * 4 + 255) / 256 * 256 + most, 256);
 }
 
 }  // namespace fdm
