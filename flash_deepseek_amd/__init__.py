@@ -650,20 +650,23 @@ def add_rms_norm(x, add, norm_w, out, scale=None, sum=None, eps=1e-6, stream=Non
         _load_types()
     _on_device(fn, x, add, norm_w, out, scale, sum)
     xt = _elem(fn, "x", x.dtype)
+    ap = at = ast = sp = sst = wp = cp = cst = 0
+    if add is not None:
+        ap, at, ast = add.data_ptr(), _elem(fn, "add", add.dtype), _matrix(fn, "add", add, shape)
+    if sum is not None:
+        if sum.dtype is not x.dtype:
+            _refuse(fn, f"sum: x's type {x.dtype} is wanted, got {sum.dtype}")
+        sp, sst = sum.data_ptr(), _matrix(fn, "sum", sum, shape)
+    if norm_w is not None:
+        wp = _vector(fn, "norm_w", norm_w, d, _f32)
     if scale is None:
-        yt, ss = _elem(fn, "out", out.dtype), 0
+        yt = _elem(fn, "out", out.dtype)
     else:
         if out.dtype is not _e4m3 or scale.element_size() != 1:
             _refuse(fn, f"with scales out is float8_e4m3fn and scale bytes, got {out.dtype} and {scale.dtype}")
-        yt, ss = _lib.E4M3, _matrix(fn, "scale", scale, (T, (d + 127) // 128))
-    if sum is not None and sum.dtype is not x.dtype:
-        _refuse(fn, f"sum: x's type {x.dtype} is wanted, got {sum.dtype}")
-    call("fdm_add_rms_norm", x.data_ptr(), xt, _matrix(fn, "x", x, shape),
-         None if add is None else add.data_ptr(), 0 if add is None else _elem(fn, "add", add.dtype),
-         0 if add is None else _matrix(fn, "add", add, shape),
-         None if sum is None else sum.data_ptr(), 0 if sum is None else _matrix(fn, "sum", sum, shape),
-         None if norm_w is None else _vector(fn, "norm_w", norm_w, d, _f32), eps, out.data_ptr(), yt,
-         _matrix(fn, "out", out, shape), None if scale is None else scale.data_ptr(), ss, T, d, _call_stream(stream))
+        yt, cp, cst = _lib.E4M3, scale.data_ptr(), _matrix(fn, "scale", scale, (T, (d + 127) // 128))
+    call("fdm_add_rms_norm", x.data_ptr(), xt, _matrix(fn, "x", x, shape), ap or None, at, ast, sp or None, sst, wp or None, eps,
+         out.data_ptr(), yt, _matrix(fn, "out", out, shape), cp or None, cst, T, d, _call_stream(stream))
 
 
 class Adapters:

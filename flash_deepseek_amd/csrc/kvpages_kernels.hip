@@ -13,28 +13,38 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Exclusive sums over the workgroup's threads; *total gets the sum of all.
-template <typename T>
-__device__ __forceinline__ T scan(T mine, T* of_wave, T* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T upto = mine;
+// Exclusive sums over the workgroup's threads, N of them at a time; total gets the sums of all.
+template <int N, typename T>
+struct Scan {
+  T of_wave[kThreads / 64][N];
+  __device__ __forceinline__ void operator()(T (&v)[N], T (&total)[N]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    T upto[N];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T v = __shfl_up(upto, d);
-    if (lane >= d) upto += v;
-  }
-  if (lane == 63) of_wave[wave] = upto;
-  __syncthreads();
-  T before = 0, all = 0;
+    for (int n = 0; n < N; ++n) upto[n] = v[n];
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < wave) before += of_wave[w];
-    all += of_wave[w];
+    for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const T below = __shfl_up(upto[n], d);
+        if (lane >= d) upto[n] += below;
+      }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (lane == 63) of_wave[wave][n] = upto[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = upto[n] - v[n];
+      total[n] = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 64; ++w) {
+        if (w < wave) v[n] += of_wave[w][n];
+        total[n] += of_wave[w][n];
+      }
+    }
   }
-  __syncthreads();
-  *total = all;
-  return before + upto - mine;
-}
+};
 
 // The last b of start[0 .. B] (not falling) with start[b] <= i.
 __device__ __forceinline__ int owner(const int* start, int B, int i) {
@@ -68,74 +78,74 @@ __device__ __forceinline__ bool is_last(unsigned* turn, int* said) {
 // Every workgroup counts all sequences itself (B <= 4096, 16 a thread), so that one
 // launch needs no second one behind it; the last one to come to its end changes the
 // state that the others read.  A workgroup gives 1024 places at a time, four a
-// thread: a token's sequence is searched for in LDS, and the first token of a new
-// page names the page in the table.
+// thread: the first's sequence is searched for in LDS and its page read, the others
+// mostly share them; the first token of a new page names the page in the table.
+// Bound by latency, a chain of loads and scans: 64 sequences of up to four tokens 5.6 us of
+// kernel, 786,000 tokens of 512 sequences on pages of 16 FDM_GROW_US (their 6.3 MB take 1.2).
 __global__ __launch_bounds__(kThreads) void k_kv_grow(KvPagesArgs a, KvGrowArgs g) {
   __shared__ int start[kKvMaxSeqs + 1], first[kKvMaxSeqs], len[kKvMaxSeqs];
-  __shared__ int64_t wide[kThreads / 64];
-  __shared__ int narrow[kThreads / 64], said;
+  __shared__ Scan<2, int64_t> wide;
+  __shared__ Scan<3, int> narrow;
+  __shared__ int said;
   const int tid = threadIdx.x, per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(b0 + per, a.B);
   const int n_free = min(max(*a.n_free, 0), a.n_pages);
-  // what the sequences that have room ask for, up to each
-  int64_t pages = 0, tokens = 0, all64;
+  // what the sequences that have room ask for, up to each: pages, tokens
+  int64_t asked[2] = {0, 0}, all64[2];
   for (int b = b0; b < b1; ++b) {
     const int l = min(max(a.kv_len[b], 0), a.max_len), n = max(g.more[b], 0);
     const bool room = n <= a.max_len - l;
     len[b] = l;
     start[b] = room ? n : -1;
     first[b] = room ? pages_for(l + n, a.shift) - pages_for(l, a.shift) : 0;
-    pages += first[b];
-    tokens += room ? n : 0;
+    asked[0] += first[b];
+    asked[1] += room ? n : 0;
   }
-  pages = scan(pages, wide, &all64);
-  tokens = scan(tokens, wide, &all64);
-  // who is served
-  int n_sum = 0, need_sum = 0, refused = 0;
+  wide(asked, all64);
+  // who is served: tokens, pages, and those who are not
+  int got[3] = {0, 0, 0}, all[3];
   for (int b = b0; b < b1; ++b) {
     const int n = start[b], need = first[b];
-    pages += need;
-    tokens += max(n, 0);
-    const bool served = n >= 0 && (need == 0 || pages <= n_free) && tokens <= g.N;
-    refused += !served && n != 0;
+    asked[0] += need;
+    asked[1] += max(n, 0);
+    const bool served = n >= 0 && (need == 0 || asked[0] <= n_free) && asked[1] <= g.N;
+    got[2] += !served && n != 0;
     start[b] = served ? n : 0;
     first[b] = served ? need : 0;
-    n_sum += start[b];
-    need_sum += first[b];
+    got[0] += start[b];
+    got[1] += first[b];
   }
-  int total, taken, n_refused;
-  int at = scan(n_sum, narrow, &total), page_at = scan(need_sum, narrow, &taken);
-  scan(refused, narrow, &n_refused);
+  narrow(got, all);
+  const int total = all[0];
   for (int b = b0; b < b1; ++b) {
     const int n = start[b], need = first[b];
-    start[b] = at;
-    first[b] = page_at;
-    at += n;
-    page_at += need;
+    start[b] = got[0];
+    first[b] = got[1];
+    got[0] += n;
+    got[1] += need;
   }
   if (tid == 0) start[a.B] = total;
   __syncthreads();
   const int inside = (1 << a.shift) - 1;
   for (int64_t t0 = 4 * ((int64_t)blockIdx.x * kThreads + tid); t0 < g.N; t0 += (int64_t)4 * kThreads * gridDim.x) {
     int pos[4], slot[4];
-    int b = t0 < total ? owner(start, a.B, (int)t0) : 0;
+    int b = t0 < total ? owner(start, a.B, (int)t0) : 0, page = -1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int64_t t = t0 + k;
       pos[k] = 0;
       slot[k] = -1;
       if (t < total) {
-        while (start[b + 1] <= t) ++b;
+        bool same = k > 0;
+        while (start[b + 1] <= t) ++b, same = false;
         pos[k] = len[b] + (int)(t - start[b]);
-        const int p = pos[k] >> a.shift, have = pages_for(len[b], a.shift);
-        int* entry = a.pages + (int64_t)b * a.P + p;
-        int page;
-        if (p < have) {
-          page = *entry;
-        } else {
-          page = a.free[n_free - 1 - (first[b] + p - have)];
-          if ((pos[k] & inside) == 0) *entry = page;
+        const int at = pos[k] & inside;
+        if (!same || at == 0) {
+          const int p = pos[k] >> a.shift, have = pages_for(len[b], a.shift);
+          int* entry = a.pages + (int64_t)b * a.P + p;
+          page = p < have ? *entry : a.free[n_free - 1 - (first[b] + p - have)];
+          if (p >= have && at == 0) *entry = page;
         }
-        if (page >= 0 && page < a.n_pages) slot[k] = (page << a.shift) | (pos[k] & inside);
+        if (page >= 0 && page < a.n_pages) slot[k] = (page << a.shift) | at;
       }
     }
     if (g.vec && t0 + 4 <= g.N) {
@@ -157,30 +167,32 @@ __global__ __launch_bounds__(kThreads) void k_kv_grow(KvPagesArgs a, KvGrowArgs 
   }
   if (tid == 0) {
     g.q_start[a.B] = total;
-    *a.n_free = n_free - taken;
-    if (g.refused) *g.refused = n_refused;
+    *a.n_free = n_free - all[1];
+    if (g.refused) *g.refused = all[2];
   }
 }
 
 // The pages behind what each sequence keeps, onto the stack; one launch as above.
 __global__ __launch_bounds__(kThreads) void k_kv_trim(KvPagesArgs a, const int* keep) {
   __shared__ int before[kKvMaxSeqs + 1], stay[kKvMaxSeqs], len[kKvMaxSeqs];
-  __shared__ int narrow[kThreads / 64], said;
+  __shared__ Scan<1, int> scan;
+  __shared__ int said;
   const int tid = threadIdx.x, per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(b0 + per, a.B);
   const int n_free = min(max(*a.n_free, 0), a.n_pages);
-  int sum = 0, total;
+  int at[1] = {0}, all[1];
   for (int b = b0; b < b1; ++b) {
     const int l = min(max(a.kv_len[b], 0), a.max_len), k = keep[b] < 0 ? l : min(keep[b], l);
     len[b] = k;
     stay[b] = pages_for(k, a.shift);
     before[b] = pages_for(l, a.shift) - stay[b];
-    sum += before[b];
+    at[0] += before[b];
   }
-  int at = scan(sum, narrow, &total);
+  scan(at, all);
+  const int total = all[0];
   for (int b = b0; b < b1; ++b) {
     const int n = before[b];
-    before[b] = at;
-    at += n;
+    before[b] = at[0];
+    at[0] += n;
   }
   if (tid == 0) before[a.B] = total;
   __syncthreads();
@@ -194,15 +206,15 @@ __global__ __launch_bounds__(kThreads) void k_kv_trim(KvPagesArgs a, const int* 
   if (tid == 0) *a.n_free = (int)min((int64_t)n_free + total, (int64_t)a.n_pages);
 }
 
-// Workgroups: one for every 1024 places (tokens, or entries of the table, of which
-// a call seldom gives back many), a CU's worth at most.
+// Workgroups: one for every 1024 places (of the table, of which a call seldom gives back
+// much, entries), two a CU at most.
 hipError_t launch_kv_grow(const KvPagesArgs& a, const KvGrowArgs& g, hipStream_t s) {
-  const int wgs = (int)std::min<int64_t>(std::max<int64_t>(((int64_t)g.N + 1023) / 1024, 1), g_num_cus);
+  const int wgs = (int)std::min<int64_t>(std::max<int64_t>(((int64_t)g.N + 1023) / 1024, 1), 2 * g_num_cus);
   k_kv_grow<<<wgs, kThreads, 0, s>>>(a, g);
   return hipGetLastError();
 }
 hipError_t launch_kv_trim(const KvPagesArgs& a, const int* keep, hipStream_t s) {
-  const int wgs = (int)std::min<int64_t>(((int64_t)a.B * a.P + 8191) / 8192, g_num_cus);
+  const int wgs = (int)std::min<int64_t>(((int64_t)a.B * a.P + 4095) / 4096, g_num_cus);
   k_kv_trim<<<wgs, kThreads, 0, s>>>(a, keep);
   return hipGetLastError();
 }

@@ -129,8 +129,10 @@ template <typename TX, typename TA>
 hipError_t launch_of(const NormArgs& a, hipStream_t s) {
   const int chunks = (a.d + 7) / 8;
 #define FDM_NORM(NT, C) k_add_rms_norm<TX, TA, NT, C><<<a.T, NT, 0, s>>>(a)
+  // few rows: a value chunk a thread, the shortest chain; many: more loads a thread in flight
   if (chunks <= 64) FDM_NORM(64, 1);
   else if (chunks <= 256) FDM_NORM(256, 1);
+  else if (a.T <= g_num_cus && chunks <= 1024) FDM_NORM(1024, 1);
   else if (chunks <= 512) FDM_NORM(256, 2);
   else if (chunks <= 1024) FDM_NORM(256, 4);
   else if (chunks <= 2048) FDM_NORM(512, 4);

@@ -71,7 +71,7 @@ inline ProjectCut project_cut(int tile, int T, int out, int steps, bool join, in
   return c;
 }
 // u_tiles: workgroups that the adapters' first product takes at least, 0: no adapters.
-inline ProjectPlan project_plan(int T, int64_t row_bytes, int out, int u_tiles, int cus) {
+inline ProjectPlan project_plan(int T, int64_t row_bytes, int out, int u_tiles, int rank, int cus) {
   ProjectPlan p{};
   const int steps = steps_of(row_bytes);
   // few rows: the adapters' first product runs beside the matrix's, the joining launch has the second
@@ -85,9 +85,25 @@ inline ProjectPlan project_plan(int T, int64_t row_bytes, int out, int u_tiles, 
   }
   p.full = (int)c.full;
   p.splits = c.splits;
-  // what it takes to fill the CUs: twice by itself, and what the parts leave beside them
-  const int64_t room = p.full ? 2 * cus : cus - (tiles_of(p.tile, T, out) - p.full) * p.splits;
-  p.u_splits = u_tiles ? (int)std::min<int64_t>(std::max<int64_t>(room / u_tiles, 1), std::min(kMaxUSplits, steps)) : 0;
+  p.u_splits = 0;
+  // two workgroups a CU at most
+  const int most = u_tiles ? std::max(std::min(2 * cus / u_tiles, std::min(kMaxUSplits, steps)), 1) : 0;
+  if (u_tiles && p.full) {
+    p.u_splits = most;
+  } else if (u_tiles) {
+    // Beside the parts where there is room for both (a few too many do not matter), else before
+    // them.  6 us and, for a step of its eight waves, 0.3 and 0.035 a value of the rank: 512 rows of
+    // 7168 values of rank 64 43, 25, 16.4 and 12.3 in 1, 2, 4 and 8 splits, 256 rows of 16384 of
+    // rank 16 30.6, 18.0, 11.7 and 8.4.
+    const int64_t parts = (tiles_of(p.tile, T, out) - p.full) * p.splits, room = cus + cus / 20 - parts % cus;
+    const double main = ((steps + p.splits - 1) / p.splits) * kStepUs[p.tile] + 3;
+    double least = 0;
+    for (int s = 1; s <= most; ++s) {
+      const double u = 6 + (double)((steps + 8 * s - 1) / (8 * s)) * (0.3 + 0.035 * std::min(rank, kRankPart));
+      const double us = (int64_t)u_tiles * s <= room ? std::max(u, main) + 0.1 * u : u * ((u_tiles * s + cus - 1) / cus) + main;
+      if (s == 1 || us < least) least = us, p.u_splits = s;
+    }
+  }
   return p;
 }
 

@@ -16,7 +16,7 @@ int main() {
   int T, in, out, rank, B, n, size, cus;
   while (scanf("%d %d %d %d %d %d %d %d", &T, &in, &out, &rank, &B, &n, &size, &cus) == 8) {
     const int u = rank ? adapter_tiles(T, B, n) * rank_parts(rank) : 0;
-    const ProjectPlan p = project_plan(T, (int64_t)in * size, out, u, cus);
+    const ProjectPlan p = project_plan(T, (int64_t)in * size, out, u, rank, cus);
     printf("%d %d %d %d %lld %d %zu %zu %zu\n", p.tile, p.full, p.splits, p.u_splits, (long long)tiles_of(p.tile, T, out), steps_of((int64_t)in * size),
            project_bytes(p, T, out, rank), project_most_bytes(T, in, out, rank, cus), project_most_bytes(2 * T + 100, in, out, rank, cus));
   }
