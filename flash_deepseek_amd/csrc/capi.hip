@@ -2870,8 +2870,8 @@ int fdm_project(const fdm_projection* p, void* d_workspace, size_t workspace_byt
     return fail(FDM_E_INVAL, "y: rows of %d at stride %lld", p->out_dim, (long long)y_stride);
   if (fp8 && llabs(p->x_scale_stride) > FDM_PROJECT_MAX_STRIDE) return fail(FDM_E_INVAL, "scale stride %lld", (long long)p->x_scale_stride);
   if (int rc = check_ready()) return rc;
-  const int rank = adapters ? p->rank : 0, u_tiles = adapters ? adapter_tiles(p->T, p->B, p->n_adapters) * rank_parts(rank) : 0;
-  const ProjectPlan plan = project_plan(p->T, (int64_t)p->in_dim * size, p->out_dim, u_tiles, rank, g_num_cus);
+  const int rank = adapters ? p->rank : 0;
+  const ProjectPlan plan = project_plan(p->T, (int64_t)p->in_dim * size, p->out_dim, p->B, p->n_adapters, rank, g_num_cus);
   if (workspace_bytes < project_bytes(plan, p->T, p->out_dim, rank))
     return fail(FDM_E_INVAL, "workspace of %zu bytes: %zu are needed", workspace_bytes, project_bytes(plan, p->T, p->out_dim, rank));
   a.x = p->d_x;

@@ -136,31 +136,11 @@ __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int m, int id
   const int lane = threadIdx.x & 63, i0 = lane % kRows, g = lane / kRows;
   uint64_t left = __ballot(id >= 0);
   const float* u = a.u + (int64_t)m * a.rank;
-  const int64_t next = (int64_t)a.T * a.rank;  // part of the inner dimension
-  // F16 planes: the row's largest brought to [1, 2), so that none overflows and few are lost
-  float up = 1.0f, down = 1.0f;
-  if constexpr (FMT == kRowF16) {
-    float top = 0.0f;
-    if (id >= 0)
-      for (int j = 0; j < a.rank; ++j) {
-        float v = 0.0f;
-        for (int p = 0; p < a.u_splits; ++p) v += u[p * next + j];
-        top = fmaxf(top, fabsf(v));
-      }
-    const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 100);
-    up = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-    down = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
-  }
   while (left) {
     const int k = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
     const bool mine = id == k;
     left &= ~__ballot(mine);
     const T16* B = static_cast<const T16*>(a.b) + (int64_t)k * a.out * a.rank;
-    typename Block<FMT>::sum_t sum[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < Block<FMT>::kOf; ++i) sum[nb][i] = 0.0f;
     for (int j0 = 0; j0 < a.rank; j0 += kK) {
       const int j = j0 + 8 * g;
       float v[8];
@@ -172,24 +152,36 @@ __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int m, int id
 #pragma unroll
         for (int i = 0; i < 8; ++i) bv[nb][i] = (T16)0.0f;
       if (j < a.rank) {
-        if (mine)
-          for (int p = 0; p < a.u_splits; ++p) {
-            float part[8];
-            load8(u + p * next + j, true, part);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += part[i];
-          }
+        if (mine) load8(u + j, true, v);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const int n = min(n0 + matrix_row<FMT, NB>(i0, nb), a.out - 1);
           bv[nb] = *reinterpret_cast<const x8*>(B + (int64_t)n * a.rank + j);
         }
       }
+      // F16 numbers: the largest of these brought to [1, 2), so that none overflows and few are lost
+      float down = 1.0f;
+      if constexpr (FMT == kRowF16) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 100);
+        const float up = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+        down = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= up;
+      }
+      typename Block<FMT>::sum_t sum[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < Block<FMT>::kOf; ++i) sum[nb][i] = 0.0f;
       for (int p = 0; p < a.planes; ++p) {
         x8 w;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (p == 0) v[i] *= up;
           w[i] = (T16)v[i];
           const float rest = v[i] - (float)w[i];
           v[i] = fabsf(rest) < __builtin_inff() ? rest : 0.0f;  // an infinity has no rest
@@ -197,11 +189,11 @@ __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int m, int id
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) sum[nb] = mfma(bv[nb], w, sum[nb]);
       }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < Block<FMT>::kOf; ++i) acc[nb][i] = mine ? fmaf(sum[nb][i], down, acc[nb][i]) : acc[nb][i];
     }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int i = 0; i < Block<FMT>::kOf; ++i) acc[nb][i] = mine ? fmaf(sum[nb][i], down, acc[nb][i]) : acc[nb][i];
   }
 }
 

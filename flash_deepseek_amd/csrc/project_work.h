@@ -51,59 +51,72 @@ constexpr double kStepUs[] = {0.3, 0.42, 0.53, 1.6}, kPartUs[] = {0.015, 0.02, 0
 // Parts at most: two for every CU, one of the largest tiles (64 MB of sums).
 inline int most_parts(int tile, int cus) { return tile == kTile256 ? cus : 2 * cus; }
 // Tiles that are mostly rows past the end are not considered.
-inline bool tile_fits(int tile, int T) { return tile == kTile32 ? T <= 64 : T > kTiles[tile].rows / 2; }
+inline bool tile_fits(int tile, int T) { return tile == kTile32 ? T <= 32 : T > kTiles[tile].rows / 2; }
 
+// The adapters of a call: workgroups that their first product takes at least (0: none), rank,
+// how many there are, and requests.
+struct ProjectU {
+  int tiles, rank, n, B;
+};
 struct ProjectCut {
   int64_t full;
-  int splits;
+  int splits, u_splits;
   double us;
 };
-inline ProjectCut project_cut(int tile, int T, int out, int steps, bool join, int cus) {
+// The best number of splits of the adapters' first product, and what the launches up to the
+// join take with it: beside the `parts` of a cut where there is room for both (a few too many
+// do not matter), else before them.  Before whole tiles (parts 0) it has a launch of its own
+// and one split.
+// 4.5 us and, for a step of its eight waves, 0.3 and 0.035 a value of the rank: 512 rows of
+// 7168 values of rank 64 43, 25, 16.4 and 12.3 in 1, 2, 4 and 8 splits, 256 rows of 16384 of
+// rank 16 30.6, 18.0, 11.7 and 8.4.
+inline double with_u(ProjectU u, int steps, int64_t parts, double main, int cus, int* splits) {
+  *splits = 0;
+  if (!u.tiles) return main;
+  // two workgroups a CU at most
+  const int most = parts ? std::max(std::min(2 * cus / u.tiles, std::min(kMaxUSplits, steps)), 1) : 1;
+  const int64_t room = parts ? cus + cus / 20 - parts % cus : 0;
+  double least = 0;
+  for (int s = 1; s <= most; ++s) {
+    const double us = 4.5 + (double)((steps + 8 * s - 1) / (8 * s)) * (0.3 + 0.035 * std::min(u.rank, kRankPart));
+    const int64_t groups = (int64_t)u.tiles * s;
+    const double t = groups <= room ? std::max(us, main) + 0.1 * us : us * ((groups + cus - 1) / cus) + main;
+    if (s == 1 || t < least) least = t, *splits = s;
+  }
+  return least;
+}
+inline ProjectCut project_cut(int tile, int T, int out, int steps, ProjectU u, int cus) {
+  const int rows = kTiles[tile].rows;
   const int64_t tiles = tiles_of(tile, T, out), rest = tiles % cus;
   auto round = [&](int n) { return n * kStepUs[tile] + 3; };
   const double rounds = (double)(tiles / cus) * round(steps);
-  ProjectCut c{tiles - rest, 1, rounds + (rest ? round(steps) : 0) + (join ? rest * kPartUs[tile] : 0)};
-  for (int s = 2; s <= steps && rest * s <= most_parts(tile, cus); ++s) {
-    const double us = rounds + (double)((rest * s + cus - 1) / cus) * round((steps + s - 1) / s) + rest * s * kPartUs[tile] + (join ? 0 : 5);
-    if (us < c.us) c.us = us, c.splits = s;
+  // a tile's second products: 2 us, and 2 an adapter among its rows
+  const double second = u.tiles ? 2 + 2 * std::min<double>(std::min(u.n, rows), 1 + (double)u.B * std::min(rows, T) / T) : 0;
+  ProjectCut c{tiles, 1, 0, 0.0};
+  c.us = with_u(u, steps, 0, rounds + (rest ? round(steps) : 0) + (double)((tiles + cus - 1) / cus) * second, cus, &c.u_splits);
+  // (uncut tiles may be joined too, for the adapters' products in two launches of few rows)
+  for (int s = u.tiles && tiles < cus ? 1 : 2; s <= steps && rest * s <= most_parts(tile, cus) && rest; ++s) {
+    const double main = rounds + (double)(tiles / cus) * second + (double)((rest * s + cus - 1) / cus) * round((steps + s - 1) / s);
+    int u_splits;
+    const double us = with_u(u, steps, tiles < cus ? rest * s : 0, main, cus, &u_splits) + rest * s * kPartUs[tile] * std::min(1.0, (double)T / rows) + 5;
+    if (us < c.us) c = {tiles - rest, s, u_splits, us};
   }
-  if (c.splits == 1 && !join) c.full = tiles;
   return c;
 }
-// u_tiles: workgroups that the adapters' first product takes at least, 0: no adapters.
-inline ProjectPlan project_plan(int T, int64_t row_bytes, int out, int u_tiles, int rank, int cus) {
+// B requests of n adapters; rank 0: none.
+inline ProjectPlan project_plan(int T, int64_t row_bytes, int out, int B, int n, int rank, int cus) {
+  const ProjectU u{rank ? adapter_tiles(T, B, n) * rank_parts(rank) : 0, rank, n, B};
   ProjectPlan p{};
-  const int steps = steps_of(row_bytes);
-  // few rows: the adapters' first product runs beside the matrix's, the joining launch has the second
-  const bool join = u_tiles && T <= 64;
-  ProjectCut c{0, 1, 0.0};
+  ProjectCut c{};
   bool any = false;
   for (int tile = kTile32; tile <= kTile256; ++tile) {
     if (!tile_fits(tile, T)) continue;
-    const ProjectCut t = project_cut(tile, T, out, steps, join, cus);
+    const ProjectCut t = project_cut(tile, T, out, steps_of(row_bytes), u, cus);
     if (!any || t.us < c.us) c = t, p.tile = tile, any = true;
   }
   p.full = (int)c.full;
   p.splits = c.splits;
-  p.u_splits = 0;
-  // two workgroups a CU at most
-  const int most = u_tiles ? std::max(std::min(2 * cus / u_tiles, std::min(kMaxUSplits, steps)), 1) : 0;
-  if (u_tiles && p.full) {
-    p.u_splits = most;
-  } else if (u_tiles) {
-    // Beside the parts where there is room for both (a few too many do not matter), else before
-    // them.  6 us and, for a step of its eight waves, 0.3 and 0.035 a value of the rank: 512 rows of
-    // 7168 values of rank 64 43, 25, 16.4 and 12.3 in 1, 2, 4 and 8 splits, 256 rows of 16384 of
-    // rank 16 30.6, 18.0, 11.7 and 8.4.
-    const int64_t parts = (tiles_of(p.tile, T, out) - p.full) * p.splits, room = cus + cus / 20 - parts % cus;
-    const double main = ((steps + p.splits - 1) / p.splits) * kStepUs[p.tile] + 3;
-    double least = 0;
-    for (int s = 1; s <= most; ++s) {
-      const double u = 6 + (double)((steps + 8 * s - 1) / (8 * s)) * (0.3 + 0.035 * std::min(rank, kRankPart));
-      const double us = (int64_t)u_tiles * s <= room ? std::max(u, main) + 0.1 * u : u * ((u_tiles * s + cus - 1) / cus) + main;
-      if (s == 1 || us < least) least = us, p.u_splits = s;
-    }
-  }
+  p.u_splits = c.u_splits;
   return p;
 }
 
@@ -121,7 +134,7 @@ inline size_t project_bytes(const ProjectPlan& p, int T, int out, int rank) {
 inline size_t project_most_bytes(int T, int in, int out, int rank, int cus) {
   size_t most = 0;
   for (int tile = kTile32; tile <= kTile256; ++tile) {
-    const int rows = tile == kTile32 ? std::min(T, 64) : T;
+    const int rows = tile == kTile32 ? std::min(T, 32) : T;
     if (tile != kTile32 && !tile_fits(tile, T)) continue;
     const int64_t parts = std::min<int64_t>(most_parts(tile, cus), tiles_of(tile, rows, out) * steps_of((int64_t)in * 2));
     most = std::max(most, (size_t)parts * kTiles[tile].rows * kTiles[tile].cols * 4);

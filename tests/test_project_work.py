@@ -15,8 +15,7 @@ using namespace fdm;
 int main() {
   int T, in, out, rank, B, n, size, cus;
   while (scanf("%d %d %d %d %d %d %d %d", &T, &in, &out, &rank, &B, &n, &size, &cus) == 8) {
-    const int u = rank ? adapter_tiles(T, B, n) * rank_parts(rank) : 0;
-    const ProjectPlan p = project_plan(T, (int64_t)in * size, out, u, rank, cus);
+    const ProjectPlan p = project_plan(T, (int64_t)in * size, out, B, n, rank, cus);
     printf("%d %d %d %d %lld %d %zu %zu %zu\n", p.tile, p.full, p.splits, p.u_splits, (long long)tiles_of(p.tile, T, out), steps_of((int64_t)in * size),
            project_bytes(p, T, out, rank), project_most_bytes(T, in, out, rank, cus), project_most_bytes(2 * T + 100, in, out, rank, cus));
   }
@@ -57,8 +56,9 @@ def test_every_tile_is_done_once_and_fits(plans):
         assert full == tiles or full == tiles - tiles % cus, case  # whole rounds, or all
         assert 1 <= splits <= steps == -(-inner * size // 128), case
         assert splits == 1 or (tiles - full) * splits <= 2 * cus, case
-        assert full == tiles or splits > 1 or (rank and T <= 64), case
+        assert full == tiles or splits > 1 or rank, case
         assert (1 <= u <= min(8, steps)) if rank else u == 0, case
+        assert not (rank and full) or u == 1, case  # whole tiles read one sum
         assert need <= most <= more, case
         assert 256 <= most <= max(T, min(8 * T, 64 * cus)) * rank * 4 + 512 + 2 * cus * 128 * 128 * 4 + cus * 256 * 256 * 4, case
 
