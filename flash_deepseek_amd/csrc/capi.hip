@@ -2770,7 +2770,8 @@ int fdm_add_rms_norm(const void* d_x, int x_type, int64_t x_stride, const void* 
   const bool fp8 = y_type == FDM_E4M3;
   if (!fp8)
     if (int rc = elem_type(y_type, &a.y_type, "y")) return rc;
-  if (T < 0 || d < 1 || d > FDM_NORM_MAX_DIM) return fail(FDM_E_INVAL, "T=%d d=%d (1 .. %d)", T, d, FDM_NORM_MAX_DIM);
+  if (T < 0 || T > FDM_NORM_MAX_ROWS || d < 1 || d > FDM_NORM_MAX_DIM)
+    return fail(FDM_E_INVAL, "T=%d (0 .. %d) d=%d (1 .. %d)", T, FDM_NORM_MAX_ROWS, d, FDM_NORM_MAX_DIM);
   if (!(eps >= 0.0f) || !isfinite(eps)) return fail(FDM_E_INVAL, "eps %g", (double)eps);
   if (fp8 ? !d_scale && T > 0 : d_scale != nullptr) return fail(FDM_E_INVAL, "scale: E4M3 rows have one, the others none");
   if (T == 0) return check_ready();
@@ -2779,7 +2780,7 @@ int fdm_add_rms_norm(const void* d_x, int x_type, int64_t x_stride, const void* 
   if (!aligned(d_x, xs) || !aligned(d_add, as) || !aligned(d_sum, xs) || !aligned(d_y, ys) || !aligned(d_w, 4))
     return fail(FDM_E_INVAL, "misaligned pointer");
   for (int64_t s : {x_stride, add_stride, sum_stride, y_stride, scale_stride})
-    if (llabs(s) > INT64_MAX / 16) return fail(FDM_E_INVAL, "stride %lld", (long long)s);
+    if (s > INT64_MAX / 16 || s < -(INT64_MAX / 16)) return fail(FDM_E_INVAL, "stride %lld", (long long)s);
   const int groups = (d + 127) / 128;
   if (T > 1 && (llabs(y_stride) < d || (d_sum && llabs(sum_stride) < d) || (fp8 && llabs(scale_stride) < groups)))
     return fail(FDM_E_INVAL, "rows of y, sum or scale overlap");
@@ -2866,9 +2867,10 @@ int fdm_project(const fdm_projection* p, void* d_workspace, size_t workspace_byt
     if (s % (16 / size) || s < 0 || s > FDM_PROJECT_MAX_STRIDE)
       return fail(FDM_E_INVAL, "stride %lld: whole 16 bytes, up to %d elements", (long long)s, FDM_PROJECT_MAX_STRIDE);
   const int64_t y_stride = p->T > 1 ? p->y_stride : p->out_dim;
-  if (llabs(y_stride) < p->out_dim || llabs(y_stride) > FDM_PROJECT_MAX_STRIDE)
+  if ((y_stride > -p->out_dim && y_stride < p->out_dim) || y_stride > FDM_PROJECT_MAX_STRIDE || y_stride < -FDM_PROJECT_MAX_STRIDE)
     return fail(FDM_E_INVAL, "y: rows of %d at stride %lld", p->out_dim, (long long)y_stride);
-  if (fp8 && llabs(p->x_scale_stride) > FDM_PROJECT_MAX_STRIDE) return fail(FDM_E_INVAL, "scale stride %lld", (long long)p->x_scale_stride);
+  if (fp8 && (p->x_scale_stride > FDM_PROJECT_MAX_STRIDE || p->x_scale_stride < -FDM_PROJECT_MAX_STRIDE))
+     return fail(FDM_E_INVAL, "scale stride %lld", (long long)p->x_scale_stride);
   if (int rc = check_ready()) return rc;
   const int rank = adapters ? p->rank : 0;
   const ProjectPlan plan = project_plan(p->T, (int64_t)p->in_dim * size, p->out_dim, p->B, p->n_adapters, rank, g_num_cus);

@@ -261,7 +261,7 @@ __device__ __forceinline__ void adapter_in(const ProjectArgs& a, int split, int 
   if (tid < 32) l.list[tid] = -1;
   __syncthreads();
   for (int b = tid; b < a.B; b += kThreads) {
-    const int k = a.adapter[b], t0 = min(max(a.q_start[b], 0), a.T), n = min(a.q_start[b + 1], a.T) - t0;
+    const int k = a.adapter[b], t0 = min(max(a.q_start[b], 0), a.T), n = min(max(a.q_start[b + 1], 0), a.T) - t0;
     if (k >= 0 && k < a.n_adapters && n > 0) atomicAdd(&l.count[k], n);
   }
   __syncthreads();
@@ -301,7 +301,7 @@ __device__ __forceinline__ void adapter_in(const ProjectArgs& a, int split, int 
     int t0 = 0, n = 0;
     if (b < a.B && a.adapter[b] == k) {
       t0 = min(max(a.q_start[b], 0), a.T);
-      n = max(min(a.q_start[b + 1], a.T) - t0, 0);
+      n = max(min(max(a.q_start[b + 1], 0), a.T) - t0, 0);
     }
     int sum = n;
 #pragma unroll

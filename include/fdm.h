@@ -607,14 +607,15 @@ int fdm_kv_trim(const fdm_kv_pages *pages, const int32_t *d_keep, void *stream);
 /* ---- the residual's addition and its norm for several tokens (infer.m:369-374
  * and the additions of 1846-1850, 1922, without fdm_rms_norm's order of sums):
  *   s = x + add (d_add NULL: x),  y = s / sqrt(mean(s^2) + eps) * w (d_w fp32 [d], NULL: 1),
- * T rows of d values (1 .. FDM_NORM_MAX_DIM), strides in elements, in fp32, each
- * output rounded once: d_sum (may be NULL) receives s in x's type, d_y the norm of s
+ * T rows (up to FDM_NORM_MAX_ROWS) of d values (1 .. FDM_NORM_MAX_DIM), strides in
+ * elements, in fp32, each output rounded once: d_sum (may be NULL) receives s in x's type, d_y the norm of s
  * as it was before that rounding.  Types are FDM_GGML_F32, _F16, _BF16; y_type may
  * be FDM_E4M3: codes with a scale byte for every 128 values of a row, d_scale
  * [T][ceil(d / 128)], by the rule of FDM_KV_FP8 (zeros: 27, an infinity or NaN: 255).
  * d_sum may be d_x, d_y may be d_x or d_add (same size of elements and stride);
  * otherwise they must not overlap.  Rows of whole eights, 16-byte aligned, with add
  * in x's type or BF16, move by 16-byte accesses, any other value by value. */
+#define FDM_NORM_MAX_ROWS 2097152
 #define FDM_NORM_MAX_DIM 32768
 #define FDM_E4M3 100 /* 8-bit floats, no GGML type: an element type where it is named */
 int fdm_add_rms_norm(const void *d_x, int x_type, int64_t x_stride, const void *d_add, int add_type,
@@ -635,18 +636,22 @@ int fdm_add_rms_norm(const void *d_x, int x_type, int64_t x_stride, const void *
  *     255 makes its values NaN.
  * A [n][rank][in] and B [n][out][rank] are contiguous, F16 beside F16, else BF16;
  * d_times [n] fp32 (NULL: 1).  n_adapters 0: none, and the fields behind are not read.
- * y_type F32, F16 or BF16.  Strides in elements; x, W, A, B 16-byte aligned, rows of x
- * and W whole 16 bytes apart (strides of a single row are free).  in is a multiple of 8
- * (16 in E4M3), rank of 8; in, out <= FDM_PROJECT_MAX_DIM.  y must not overlap the inputs,
- * requests must not share rows.
+ * y_type F32, F16 or BF16.  Strides in elements, up to FDM_PROJECT_MAX_STRIDE; x, W, A, B
+ * 16-byte aligned, rows of x and W whole 16 bytes apart, not backwards (0: one row for
+ * all; strides of a single row are free).  in is a multiple of 8 (16 in E4M3), rank of 8;
+ * in, out <= FDM_PROJECT_MAX_DIM.  y must not overlap the inputs.  q_start does not fall,
+ * and is cut to 0 .. T.
  * Sums and A x are fp32, products exact but for E4M3 with a 16-bit y: there every eight
  * neighbouring products are added with what lies under 2^-13 of their largest cut off
- * (1e-4 of a result of 7168 normal values).  Where B (A x) runs on the matrix cores A x is
- * held as two numbers of the adapters' type (three for an fp32 y beside BF16), 2^-16 of itself
- * and less.  A row's result depends on its own values and adapter alone, whatever else is
- * in the call; its sums' order on T and the sizes.  The same arguments give the same bits.
+ * (1e-4 of a result of 7168 normal values).  An fp32 y, and A x, take the codes times
+ * their scale in BF16: exact for scale bytes of x and W from 10 to 246.  Where B (A x) runs
+ * on the matrix cores A x is held as two numbers of the adapters' type (three for an fp32 y
+ * beside BF16), off by 2^-16 of itself at most.  A row's result depends on its own values and
+ * adapter alone, whatever the others are; its sums' order on T and the sizes, B and
+ * n_adapters among them.  The same arguments give the same bits.
  * d_workspace: at least fdm_project_workspace(T, in, out, rank) bytes (rank 0: no
- * adapters), 256-byte aligned, used by the call alone until it has run on its
+ * adapters; T x rank fp32 numbers, some of them more than once, and up to 64 MB of
+ * sums; enough for fewer rows too), 256-byte aligned, used by the call alone until it has run on its
  * stream.  The call allocates nothing and may be captured. */
 #define FDM_PROJECT_MAX_ROWS 1048576
 #define FDM_PROJECT_MAX_DIM 262144

@@ -154,7 +154,7 @@ def projected(x, w, out_type, a=None, b=None, times=None, q_start=None, adapter=
             k = int(adapter[r])
             if not 0 <= k < a.shape[0]:
                 continue
-            t = slice(max(int(q_start[r]), 0), min(int(q_start[r + 1]), x.shape[0]))
+            t = slice(max(int(q_start[r]), 0), min(max(int(q_start[r + 1]), 0), x.shape[0]))
             c, A, B = (1.0 if times is None else float(times[k])), a[k].double(), b[k].double()
             u = x[t] @ A.T * c
             du = (x[t].abs() @ A.abs().T) * abs(c) * (n + 2) * 2.0 ** -23

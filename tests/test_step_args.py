@@ -94,3 +94,15 @@ def test_good_arguments_get_as_far_as_the_device():
     for bad in ((-1, 256, 64, 0), (4, 255, 64, 0), (4, 256, 0, 0), (4, 256, 64, 4), (4, 256, 64, 136)):
         assert _lib.lib.fdm_project_workspace(*bad, n) == INVAL
     assert _lib.lib.fdm_project_workspace(4, 256, 64, 16, None) == INVAL
+
+
+LEAST = -(1 << 63)
+
+
+def test_strides_and_rows_past_every_bound():
+    for k in ("xs", "as_", "ss", "ys", "cs"):
+        assert norm(**{k: LEAST}) == INVAL and norm(**{k: (1 << 63) - 1}) == INVAL, k
+    for k in ("x_stride", "w_stride", "y_stride"):
+        assert project(**{k: LEAST}) == INVAL and project(**{k: (1 << 63) - 16}) == INVAL, k
+    assert project(**{**FP8, "x_scale_stride": LEAST}) == INVAL
+    assert norm(T=(1 << 21) + 1) == INVAL
