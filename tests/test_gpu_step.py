@@ -311,3 +311,14 @@ def test_project_of_many_rows(fdm, fmt, T, out, counts):
     say(f"project {fmt} T={T} out={out}")
     run_project(fdm, s, y)
     C.check(y.cpu(), *want_of(s, y.dtype), "project")
+
+
+@pytest.mark.parametrize("fmt,ty", [("bf16", "bf16"), ("f16", "f32"), ("fp8", "bf16"), ("fp8", "f32")])
+@pytest.mark.parametrize("T", [20, 60, 128, 200])
+def test_project_to_many_columns(fdm, fmt, ty, T):
+    """Small tiles in whole rounds and a last one in parts, with adapters in both."""
+    s = project_case(rng(T), fmt, T, 512 if fmt == "fp8" else 256, 70000, 3, 24, [T // 4, 3, T - T // 4 - 3])
+    y = torch.empty(T, 70000, dtype=C.DTYPES[ty], device="cuda")
+    say(f"project {fmt}->{ty} T={T} out=70000")
+    run_project(fdm, s, y)
+    C.check(y.cpu(), *want_of(s, y.dtype), "project")
