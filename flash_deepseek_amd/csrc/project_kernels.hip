@@ -129,7 +129,7 @@ __device__ __forceinline__ int swap8(int row) {
 // each in BF16, 11 in F16), kept by the rows that are the adapter's own.  A row that
 // has another keeps its sum untouched, whatever B_a holds.
 template <int FMT, int NB>
-__device__ __forceinline__ void add_adapters(const ProjectArgs& a, int m, int id, int n0, typename Block<FMT>::sum_t* acc) {
+__device__ __forceinline__ void add_adapters(const ProjectArgs& a, int u_splits, int m, int id, int n0, typename Block<FMT>::sum_t* acc) {
   typedef typename Half<FMT>::T T16;
   typedef typename Half<FMT>::x8 x8;
   constexpr int kRows = Block<FMT>::kRows, kK = 8 * 64 / kRows;  // values of the rank that a product takes
@@ -153,6 +153,14 @@ __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int m, int id
         for (int i = 0; i < 8; ++i) bv[nb][i] = (T16)0.0f;
       if (j < a.rank) {
         if (mine) load8(u + j, true, v);
+        for (int p = 1; p < u_splits; ++p) {
+          float more[8];
+          if (mine) {
+            load8(u + (int64_t)p * a.T * a.rank + j, true, more);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += more[i];
+          }
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const int n = min(n0 + matrix_row<FMT, NB>(i0, nb), a.out - 1);
@@ -231,7 +239,7 @@ __device__ __forceinline__ void store_tile(const ProjectArgs& a, typename Block<
       if (m < a.T) store_columns<kCount>(part + (kRows * i + i0) * width, col, width, true, acc[i]);
       continue;
     }
-    if (a.n_adapters) add_adapters<FMT, NB>(a, m, ids[kRows * i + i0], n0, acc[i]);
+    if (a.n_adapters) add_adapters<FMT, NB>(a, 1, m, ids[kRows * i + i0], n0, acc[i]);
     if (m >= a.T) continue;
     char* y = static_cast<char*>(a.y) + (int64_t)m * a.y_bytes;
     if (a.y_type == ElemType::f32) store_columns<kCount>(reinterpret_cast<float*>(y), n0 + col, a.out, a.vec_y, acc[i]);
@@ -755,6 +763,63 @@ __global__ __launch_bounds__(256) void k_project_join(ProjectArgs a) {
   }
 }
 
+// The same on the matrix cores: a wave adds the parts of 16 rows by 32 columns and then B u of every
+// adapter among the rows.
+constexpr int kJoinCols = 128;  // of a workgroup
+template <int FMT, int BM, int BN>
+__global__ __launch_bounds__(256) void k_project_join_rows(ProjectArgs a) {
+  constexpr int NB = kJoinCols / 64;
+  __shared__ __attribute__((aligned(16))) float sums[16][kJoinCols + 4];
+  __shared__ int ids[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int m_tiles = (a.T + BM - 1) / BM, n_tiles = (a.out + BN - 1) / BN, rest = m_tiles * n_tiles - a.full;
+  const Place place = place_of(a.full + blockIdx.x, m_tiles, n_tiles);
+  const int row = 16 * ((int)blockIdx.y / (BN / kJoinCols)), col = kJoinCols * ((int)blockIdx.y % (BN / kJoinCols)) + 16 * NB * wave;
+  const int t0 = BM * place.m + row, n0 = BN * place.n + col, m = t0 + lane % 16;
+  if (t0 >= a.T) return;
+  const float* part = a.part + (int64_t)blockIdx.x * (BM * BN) + (row + lane % 16) * BN + col + lane / 16 * 4 * NB;
+  const int64_t next = (int64_t)rest * (BM * BN);
+  f32x4 acc[1][NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc[0][i] = *reinterpret_cast<const f32x4*>(part + 4 * i);
+  for (int p = 1; p < a.splits; ++p)
+#pragma unroll
+    for (int i = 0; i < NB; ++i) acc[0][i] += *reinterpret_cast<const f32x4*>(part + p * next + 4 * i);
+  if (tid < 16) ids[tid] = -1;
+  __syncthreads();
+  for (int b = tid; b < a.B; b += 256) {
+    const int k = a.adapter[b], from = max(a.q_start[b], t0), to = min(a.q_start[b + 1], min(t0 + 16, a.T));
+    if (k >= 0 && k < a.n_adapters)
+      for (int t = from; t < to; ++t) ids[t - t0] = k;
+  }
+  __syncthreads();
+  if (n0 < a.out) add_adapters<FMT, NB>(a, a.u_splits, m, ids[lane % 16], n0, acc[0]);
+  if (a.vec_y) {
+    if (m >= a.T) return;
+    char* y = static_cast<char*>(a.y) + (int64_t)m * a.y_bytes;
+    const int n = n0 + lane / 16 * 4 * NB;
+    if (a.y_type == ElemType::f32) store_columns<4 * NB>(reinterpret_cast<float*>(y), n, a.out, true, acc[0]);
+    else if (a.y_type == ElemType::f16) store_columns<4 * NB>(reinterpret_cast<_Float16*>(y), n, a.out, true, acc[0]);
+    else store_columns<4 * NB>(reinterpret_cast<__bf16*>(y), n, a.out, true, acc[0]);
+    return;
+  }
+  // value by value, in whole rows: 650 rows by 2111 of rank 64 in fp32 12.5 us, from the lanes 14.4
+#pragma unroll
+  for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4*>(&sums[lane % 16][16 * NB * wave + lane / 16 * 4 * NB + 4 * i]) = acc[0][i];
+  __syncthreads();
+  const int n = n0 - 16 * NB * wave + tid % kJoinCols;
+  if (n >= a.out) return;
+#pragma unroll
+  for (int i = tid / kJoinCols; i < 16; i += 256 / kJoinCols) {
+    if (t0 + i >= a.T) break;
+    const float v = sums[i][tid % kJoinCols];
+    char* to = static_cast<char*>(a.y) + (int64_t)(t0 + i) * a.y_bytes;
+    if (a.y_type == ElemType::f32) reinterpret_cast<float*>(to)[n] = v;
+    else if (a.y_type == ElemType::f16) reinterpret_cast<_Float16*>(to)[n] = (_Float16)v;
+    else reinterpret_cast<__bf16*>(to)[n] = (__bf16)v;
+  }
+}
+
 namespace {
 
 template <int FMT>
@@ -782,8 +847,16 @@ hipError_t launch_tiles(ProjectArgs a, const ProjectPlan& p, hipStream_t s) {
   // One chunk a workgroup, so that rows with adapters of their own do not wait for each other,
   // or where there are many, four: 64 rows by 2112 15.4 us a call against 19.2, 24 by
   // 24576 20.3 and 21.6, 500 by 2111 with two adapters 75 and 60, 256 by 7168 with 32 109 and 104.5.
+  // Many chunks on the matrix cores instead where 16 rows have two adapters at most, or B's rows
+  // are more than 64 bytes, so that a row a lane takes them apart.  650 rows by 2112 of 3, 80 and
+  // 650 requests with adapters of their own, rank 16: 7.1, 9.5 and 25 us on the matrix cores, 7.7,
+  // 8.5 and 12.7 without; rank 64: 12.5, 15.7 and 46, and 15.2, 27 and 124.  (256 rows by 7168
+  // with 32 adapters of rank 64 in turn are slower, 79 and 64.)
+  constexpr int kHalf = FMT == kRowF16 ? kRowF16 : kRowBf16;
   const int rows = std::min(BM, a.T), chunks = (rows * BN + 255) / 256;
-  if (rest * chunks <= 16 * g_num_cus) k_project_join<FMT, BM, BN, 1><<<dim3(rest, chunks), 256, 0, s>>>(a);
+  if ((int64_t)rest * chunks <= 16 * g_num_cus) k_project_join<FMT, BM, BN, 1><<<dim3(rest, chunks), 256, 0, s>>>(a);
+  else if (a.n_adapters && (a.rank > 32 || (int64_t)16 * a.B <= a.T))
+    k_project_join_rows<kHalf, BM, BN><<<dim3(rest, (rows + 15) / 16 * (BN / kJoinCols)), 256, 0, s>>>(a);
   else k_project_join<FMT, BM, BN, 4><<<dim3(rest, (chunks + 3) / 4), 256, 0, s>>>(a);
   return hipGetLastError();
 }
