@@ -11,12 +11,10 @@ namespace fdm {
 
 namespace {
 
-constexpr int kThreads = 256;
-
 // Exclusive sums over the workgroup's threads, N of them at a time; total gets the sums of all.
-template <int N, typename T>
+template <int NT, int N, typename T>
 struct Scan {
-  T of_wave[kThreads / 64][N];
+  T of_wave[NT / 64][N];
   __device__ __forceinline__ void operator()(T (&v)[N], T (&total)[N]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     T upto[N];
@@ -38,7 +36,7 @@ struct Scan {
       v[n] = upto[n] - v[n];
       total[n] = 0;
 #pragma unroll
-      for (int w = 0; w < kThreads / 64; ++w) {
+      for (int w = 0; w < NT / 64; ++w) {
         if (w < wave) v[n] += of_wave[w][n];
         total[n] += of_wave[w][n];
       }
@@ -75,19 +73,19 @@ __device__ __forceinline__ bool is_last(unsigned* turn, int* said) {
 
 }  // namespace
 
-// Every workgroup counts all sequences itself (B <= 4096, 16 a thread), so that one
+// Every workgroup counts all sequences itself (B <= 4096, four a thread at most), so that one
 // launch needs no second one behind it; the last one to come to its end changes the
-// state that the others read.  A workgroup gives 1024 places at a time, four a
-// thread: the first's sequence is searched for in LDS and its page read, the others
+// state that the others read.  A thread gives four places at a time: the first's sequence is searched for in LDS and its page read, the others
 // mostly share them; the first token of a new page names the page in the table.
-// Bound by latency, a chain of loads and scans: 64 sequences of up to four tokens 5.6 us of
-// kernel, 786,000 tokens of 512 sequences on pages of 16 FDM_GROW_US (their 6.3 MB take 1.2).
-__global__ __launch_bounds__(kThreads) void k_kv_grow(KvPagesArgs a, KvGrowArgs g) {
+// Bound by latency, a chain of loads and scans: 64 sequences of up to four tokens 5.0 us of
+// kernel, 786,000 tokens of 512 sequences on pages of 16 10.2 (their 6.3 MB take 1.2).
+template <int NT>
+__global__ __launch_bounds__(NT) void k_kv_grow(KvPagesArgs a, KvGrowArgs g) {
   __shared__ int start[kKvMaxSeqs + 1], first[kKvMaxSeqs], len[kKvMaxSeqs];
-  __shared__ Scan<2, int64_t> wide;
-  __shared__ Scan<3, int> narrow;
+  __shared__ Scan<NT, 2, int64_t> wide;
+  __shared__ Scan<NT, 3, int> narrow;
   __shared__ int said;
-  const int tid = threadIdx.x, per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(b0 + per, a.B);
+  const int tid = threadIdx.x, per = (a.B + NT - 1) / NT, b0 = tid * per, b1 = min(b0 + per, a.B);
   const int n_free = min(max(*a.n_free, 0), a.n_pages);
   // what the sequences that have room ask for, up to each: pages, tokens
   int64_t asked[2] = {0, 0}, all64[2];
@@ -126,7 +124,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_grow(KvPagesArgs a, KvGrowArgs 
   if (tid == 0) start[a.B] = total;
   __syncthreads();
   const int inside = (1 << a.shift) - 1;
-  for (int64_t t0 = 4 * ((int64_t)blockIdx.x * kThreads + tid); t0 < g.N; t0 += (int64_t)4 * kThreads * gridDim.x) {
+  for (int64_t t0 = 4 * ((int64_t)blockIdx.x * NT + tid); t0 < g.N; t0 += (int64_t)4 * NT * gridDim.x) {
     int pos[4], slot[4];
     int b = t0 < total ? owner(start, a.B, (int)t0) : 0, page = -1;
 #pragma unroll
@@ -173,11 +171,12 @@ __global__ __launch_bounds__(kThreads) void k_kv_grow(KvPagesArgs a, KvGrowArgs 
 }
 
 // The pages behind what each sequence keeps, onto the stack; one launch as above.
-__global__ __launch_bounds__(kThreads) void k_kv_trim(KvPagesArgs a, const int* keep) {
+template <int NT>
+__global__ __launch_bounds__(NT) void k_kv_trim(KvPagesArgs a, const int* keep) {
   __shared__ int before[kKvMaxSeqs + 1], stay[kKvMaxSeqs], len[kKvMaxSeqs];
-  __shared__ Scan<1, int> scan;
+  __shared__ Scan<NT, 1, int> scan;
   __shared__ int said;
-  const int tid = threadIdx.x, per = (a.B + kThreads - 1) / kThreads, b0 = tid * per, b1 = min(b0 + per, a.B);
+  const int tid = threadIdx.x, per = (a.B + NT - 1) / NT, b0 = tid * per, b1 = min(b0 + per, a.B);
   const int n_free = min(max(*a.n_free, 0), a.n_pages);
   int at[1] = {0}, all[1];
   for (int b = b0; b < b1; ++b) {
@@ -196,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void k_kv_trim(KvPagesArgs a, const int* 
   }
   if (tid == 0) before[a.B] = total;
   __syncthreads();
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + tid; i < total; i += (int64_t)kThreads * gridDim.x) {
+  for (int64_t i = (int64_t)blockIdx.x * NT + tid; i < total; i += (int64_t)NT * gridDim.x) {
     const int b = owner(before, a.B, (int)i);
     const int64_t to = (int64_t)n_free + total - 1 - i;
     if (to < a.n_pages) a.free[to] = a.pages[(int64_t)b * a.P + stay[b] + (i - before[b])];
@@ -206,16 +205,22 @@ __global__ __launch_bounds__(kThreads) void k_kv_trim(KvPagesArgs a, const int* 
   if (tid == 0) *a.n_free = (int)min((int64_t)n_free + total, (int64_t)a.n_pages);
 }
 
-// Workgroups: one for every 1024 places (of the table, of which a call seldom gives back
-// much, entries), two a CU at most.
+// Few sequences and places: workgroups of four waves, whose scans are the shorter (64 sequences of
+// up to four tokens: grow 5.0 us, with sixteen waves 6.4; trim 3.2 and 3.4); else of sixteen,
+// of which fewer follow each other at the last word (512 sequences, 786,000 tokens: 13.5 us and
+// 10.2; 140,000 pages of 16 given back 7.0 and 5.2).  A workgroup for every four places a thread (of the table, of
+// which a call seldom gives back much, four entries), one a CU at most.
 hipError_t launch_kv_grow(const KvPagesArgs& a, const KvGrowArgs& g, hipStream_t s) {
-  const int wgs = (int)std::min<int64_t>(std::max<int64_t>(((int64_t)g.N + 1023) / 1024, 1), 2 * g_num_cus);
-  k_kv_grow<<<wgs, kThreads, 0, s>>>(a, g);
+  const auto wgs = [&](int threads) { return (int)std::min<int64_t>(std::max<int64_t>(((int64_t)g.N + 4 * threads - 1) / (4 * threads), 1), g_num_cus); };
+  if (a.B <= 1024 && g.N <= 4096) k_kv_grow<256><<<wgs(256), 256, 0, s>>>(a, g);
+  else k_kv_grow<1024><<<wgs(1024), 1024, 0, s>>>(a, g);
   return hipGetLastError();
 }
 hipError_t launch_kv_trim(const KvPagesArgs& a, const int* keep, hipStream_t s) {
-  const int wgs = (int)std::min<int64_t>(((int64_t)a.B * a.P + 4095) / 4096, g_num_cus);
-  k_kv_trim<<<wgs, kThreads, 0, s>>>(a, keep);
+  const int64_t entries = (int64_t)a.B * a.P;
+  const auto wgs = [&](int per) { return (int)std::min<int64_t>((entries + per - 1) / per, g_num_cus); };
+  if (a.B <= 1024 && entries <= 16384) k_kv_trim<256><<<wgs(4096), 256, 0, s>>>(a, keep);
+  else k_kv_trim<1024><<<wgs(4096), 1024, 0, s>>>(a, keep);
   return hipGetLastError();
 }
 
