@@ -75,8 +75,9 @@ __device__ __forceinline__ bool is_last(unsigned* turn, int* said) {
 
 // Every workgroup counts all sequences itself (B <= 4096, four a thread at most), so that one
 // launch needs no second one behind it; the last one to come to its end changes the
-// state that the others read.  A thread gives four places at a time: the first's sequence is searched for in LDS and its page read, the others
-// mostly share them; the first token of a new page names the page in the table.
+// state that the others read.  A thread gives four places at a time: the first's sequence is
+// searched for in LDS and its page read, the others mostly share them; the first token of a
+// new page names the page in the table.
 // Bound by latency, a chain of loads and scans: 64 sequences of up to four tokens 5.0 us of
 // kernel, 786,000 tokens of 512 sequences on pages of 16 10.2 (their 6.3 MB take 1.2).
 template <int NT>
@@ -211,7 +212,9 @@ __global__ __launch_bounds__(NT) void k_kv_trim(KvPagesArgs a, const int* keep) 
 // 10.2; 140,000 pages of 16 given back 7.0 and 5.2).  A workgroup for every four places a thread (of the table, of
 // which a call seldom gives back much, four entries), one a CU at most.
 hipError_t launch_kv_grow(const KvPagesArgs& a, const KvGrowArgs& g, hipStream_t s) {
-  const auto wgs = [&](int threads) { return (int)std::min<int64_t>(std::max<int64_t>(((int64_t)g.N + 4 * threads - 1) / (4 * threads), 1), g_num_cus); };
+  const auto wgs = [&](int threads) {
+    return (int)std::min<int64_t>(std::max<int64_t>(((int64_t)g.N + 4 * threads - 1) / (4 * threads), 1), g_num_cus);
+  };
   if (a.B <= 1024 && g.N <= 4096) k_kv_grow<256><<<wgs(256), 256, 0, s>>>(a, g);
   else k_kv_grow<1024><<<wgs(1024), 1024, 0, s>>>(a, g);
   return hipGetLastError();

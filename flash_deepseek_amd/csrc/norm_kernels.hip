@@ -47,6 +47,11 @@ __device__ __forceinline__ void store_row(void* row, ElemType type, bool vec, in
 // C chunks held in registers between the sum and the result, so that every value is
 // read once.  TX, TA: the types of x and add where every row is 16-byte aligned and
 // whole eights, void for any other call.
+// Sums, the mean and the root are fp32; s is rounded where it is kept and where it is given,
+// not between.  A scale's 128 values are sixteen lanes' of one chunk, whose maximum they exchange.
+// Bound by memory: 16384 rows of 7168 BF16 values with an addition into codes 157 us, 5.24 TB/s (a
+// copy of 1 GiB: 5.09).  16 rows of 7168 fp32 values 4.4 us of kernel: one chain of load, sum and
+// store.
 template <typename TX, typename TA, int NT, int C>
 __global__ __launch_bounds__(NT) void k_add_rms_norm(NormArgs a) {
   constexpr bool kVec = !std::is_void_v<TX>;
@@ -129,7 +134,8 @@ template <typename TX, typename TA>
 hipError_t launch_of(const NormArgs& a, hipStream_t s) {
   const int chunks = (a.d + 7) / 8;
 #define FDM_NORM(NT, C) k_add_rms_norm<TX, TA, NT, C><<<a.T, NT, 0, s>>>(a)
-  // few rows: a value chunk a thread, the shortest chain; many: more loads a thread in flight
+  // few rows: a chunk a thread, the shortest chain (16 rows of 7168: 4.4 us, with four chunks 6.2);
+  // many: four a thread, more in flight where the workgroups fill the card anyway
   if (chunks <= 64) FDM_NORM(64, 1);
   else if (chunks <= 256) FDM_NORM(256, 1);
   else if (a.T <= g_num_cus && chunks <= 1024) FDM_NORM(1024, 1);

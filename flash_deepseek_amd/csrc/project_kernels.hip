@@ -28,7 +28,6 @@ struct Half {
   typedef std::conditional_t<FMT == kRowF16, _Float16, __bf16> T;
   typedef std::conditional_t<FMT == kRowF16, f16x8, bf16x8> x8;
 };
-__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -255,6 +254,10 @@ __device__ __forceinline__ void store_tile(const ProjectArgs& a, typename Block<
 // share the values of part `split` of `splits` of the inner dimension, 128 bytes of a
 // row of x at a time, the next ones on their way; their sums meet in LDS.  Ranks above 64
 // are two halves, tiles of their own (more sums and operands do not fit the registers).
+// Bound by what a CU brings of x from beyond its L2, some 25 bytes a ns: 5050 rows of 16384 BF16
+// values of rank 32 83 us on 162 CUs whatever is under way (one step a wave or four, eight waves or
+// sixteen, rows a power of two apart or not).  In three parts, on all CUs, 59, but then every
+// tile of the second product adds them up, which takes as much again.
 struct AdapterLds {
   int count[kMaxAdapters];
   int list[32], chosen[2], of_wave[8];
@@ -455,6 +458,11 @@ __device__ __forceinline__ Place place_of(int tile, int m_tiles, int n_tiles) {
 // before.  Without turns all read, then multiply.
 // The first a.u_groups workgroups do the adapters' first product, the next a.full a tile
 // each, the others a part of one.
+// Measured (a launch; the library's BF16 product of 8192^3 reaches 1.38 PFLOP/s, its e4m3 one
+// 2.65): 5050 rows of 16384 BF16 values by 7168 in tiles of 256 x 256 1020 us with the adapters' second
+// product, 1.16 PFLOP/s, 10276 of 7168 codes by 18432 1200 us, 2.26; there the power bounds it: the
+// matrix cores are busy 61 and 56 % of the cycles, and the clock falls from 2.4 to 1.7 GHz.  256 rows of 16384 by 7168 91 us, 2.9 TB/s; 24 of 1536 F16 by
+// 24576 14.5, 5.5 TB/s; one row of 7168 by 1536 7.1, two launches' latencies with the join.
 template <int FMT, int BM, int BN, int WM, int WN, int RING, int TURN>
 __global__ __launch_bounds__(64 * WM * WN) void k_project(ProjectArgs a) {
   constexpr bool kCodes = FMT == kRowFp8 || FMT == kRowFp8Wide;
@@ -674,7 +682,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_project(ProjectArgs a) {
 // CHUNKS times 256 neighbouring values of a tile's parts a workgroup, 256 / BN rows each, a
 // value a thread and chunk.  All of a thread's parts are requested before the rows' adapters
 // are looked up; where there is one chunk the four waves share them, four values a lane.  B's row
-// of an adapter is read once for the neighbouring rows that have it.
+// of an adapter is read once for the neighbouring rows that have it.  Bound by latency: 64 rows by
+// 2112 in eight parts, rank 16, 4.9 us; 256 by 7168 in two 5.1, with an adapter a row 11.7.
 template <int FMT, int BM, int BN, int CHUNKS>
 __global__ __launch_bounds__(256) void k_project_join(ProjectArgs a) {
   typedef typename Half<FMT>::T T16;
