@@ -631,9 +631,11 @@ def kv_trim(pages, keep, stream=None):
 
 def _matrix(fn, name, t, shape):
     """The row stride of a tensor of `shape` whose rows are contiguous."""
-    if t.shape != shape or (t.stride(1) != 1 and shape[1] > 1):
-        _refuse(fn, f"{name}: {tuple(shape)} with contiguous rows is wanted, got {tuple(t.shape)} of strides {t.stride()}")
-    return t.stride(0)
+    if t.shape == shape:
+        rows, inner = t.stride()
+        if inner == 1 or shape[1] <= 1:
+            return rows
+    _refuse(fn, f"{name}: {tuple(shape)} with contiguous rows is wanted, got {tuple(t.shape)} of strides {t.stride()}")
 
 
 def add_rms_norm(x, add, norm_w, out, scale=None, sum=None, eps=1e-6, stream=None):
