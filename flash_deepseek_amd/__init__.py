@@ -583,6 +583,8 @@ class KvPages:
             _refuse(fn, f"page_size {page_size}: a power of two")
         self.pages, self.kv_len, self.free, self.n_free, self.page_size = pages, kv_len, free, n_free, page_size
         self._turn = torch.zeros(1, dtype=torch.int32, device=pages.device)
+        if pages.is_cuda and not torch.cuda.is_current_stream_capturing():  # there for calls on any stream
+            torch.cuda.current_stream(pages.device).synchronize()
         self.desc = _lib.KvPagesDesc(*at, self._turn.data_ptr(), B, P, n, page_size)
         self.device = pages.get_device()
 

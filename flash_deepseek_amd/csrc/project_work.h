@@ -77,8 +77,10 @@ inline double with_u(ProjectU u, int steps, int64_t parts, double main, int cus,
   const int most = parts ? std::max(std::min(2 * cus / u.tiles, std::min(kMaxUSplits, steps)), 1) : 1;
   const int64_t room = parts ? cus + cus / 20 - parts % cus : 0;
   double least = 0;
-  for (int s = 1; s <= most; ++s) {
-    const double us = 4.5 + (double)((steps + 8 * s - 1) / (8 * s)) * (0.3 + 0.035 * std::min(u.rank, kRankPart));
+  for (int s = 1, each = 0; s <= most; ++s) {
+    if ((steps + 8 * s - 1) / (8 * s) == each) continue;  // more splits, no fewer steps
+    each = (steps + 8 * s - 1) / (8 * s);
+    const double us = 4.5 + (double)each * (0.3 + 0.035 * std::min(u.rank, kRankPart));
     const int64_t groups = (int64_t)u.tiles * s;
     const double t = groups <= room ? std::max(us, main) + 0.1 * us : us * ((groups + cus - 1) / cus) + main;
     if (s == 1 || t < least) least = t, *splits = s;
@@ -97,8 +99,10 @@ inline ProjectCut project_cut(int tile, int T, int out, int steps, ProjectU u, i
   // (uncut tiles may be joined too, for the adapters' products in two launches of few rows)
   for (int s = u.tiles && tiles < cus ? 1 : 2; s <= steps && rest * s <= most_parts(tile, cus) && rest; ++s) {
     const double main = rounds + (double)(tiles / cus) * second + (double)((rest * s + cus - 1) / cus) * round((steps + s - 1) / s);
+    const double join = rest * s * kPartUs[tile] * std::min(1.0, (double)T / rows) + 5;
+    if (main + join >= c.us) continue;  // (the adapters take nothing away)
     int u_splits;
-    const double us = with_u(u, steps, tiles < cus ? rest * s : 0, main, cus, &u_splits) + rest * s * kPartUs[tile] * std::min(1.0, (double)T / rows) + 5;
+    const double us = with_u(u, steps, tiles < cus ? rest * s : 0, main, cus, &u_splits) + join;
     if (us < c.us) c = {tiles - rest, s, u_splits, us};
   }
   return c;

@@ -296,3 +296,40 @@ def test_books_of_two_caches_at_once(fdm):
             want = b.grow(n, N)
         assert [v.tolist() for v in o] == list(want[:3])
         same(p, b)
+
+
+def test_books_made_beside_other_work(fdm):
+    """A handle that is made while its stream is busy serves another stream at once."""
+    b = books(rng(5), 3, 40, 200, 16, 300)
+    tensors = ints(b.pages), ints(b.kv_len), ints(b.free), ints([b.n_free])
+    new, q, pos, slots = ints([5, 0, 70]), *(torch.empty(k, dtype=torch.int32, device="cuda") for k in (4, 80, 80))
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    x = torch.randn(4096, 4096, device="cuda")
+    for _ in range(20):
+        x = x @ x * 1e-2
+    p = fdm.KvPages(*tensors, 16)
+    fdm.kv_grow(p, new, q, pos, slots, stream=other)
+    other.synchronize()
+    want = b.grow([5, 0, 70], 80)
+    assert [q.tolist(), pos.tolist(), slots.tolist()] == list(want[:3])
+    same(p, b)
+
+
+@pytest.mark.parametrize("fmt,ty", [("f16", torch.bfloat16), ("bf16", torch.float16), ("fp8", torch.float16)])
+@pytest.mark.parametrize("T,out", [(3, 300), (50, 520), (300, 2100), (2100, 4200)])
+def test_rows_in_one_type_results_in_another(fdm, fmt, ty, T, out):
+    s = project_case(rng(T), fmt, T, 176, out, 3, 40, [T // 2, 1, T - T // 2 - 1])
+    y = run_project(fdm, s, torch.empty(T, out, dtype=ty, device="cuda"))
+    C.check(y.cpu(), *want_of(s, ty), "project")
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16", "fp8"])
+@pytest.mark.parametrize("ty", [torch.float32, torch.float16])
+@pytest.mark.parametrize("T,out,rank,counts", [(500, 2111, 64, [250, 250]), (500, 2112, 16, [3, 497]), (700, 2113, 128, [1] * 700), (700, 2120, 8, [7] * 100),
+                                               (300, 7200, 40, [1] * 300), (2100, 7001, 24, [900, 1200])])
+def test_joins_of_many_chunks(fdm, fmt, ty, T, out, rank, counts):
+    """Parts joined on the matrix cores and value by value, long and short ranks, odd columns."""
+    s = project_case(rng(T + rank), fmt, T, 1552, out, 9, rank, counts)
+    y = run_project(fdm, s, torch.empty(T, out, dtype=ty, device="cuda"))
+    C.check(y.cpu(), *want_of(s, ty), "project")
