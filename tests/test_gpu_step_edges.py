@@ -333,3 +333,68 @@ def test_joins_of_many_chunks(fdm, fmt, ty, T, out, rank, counts):
     s = project_case(rng(T + rank), fmt, T, 1552, out, 9, rank, counts)
     y = run_project(fdm, s, torch.empty(T, out, dtype=ty, device="cuda"))
     C.check(y.cpu(), *want_of(s, ty), "project")
+
+
+# ---- the largest -----------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt,T,inner,out,rank", [("bf16", 1 << 20, 16, 24, 8), ("fp8", 2, 16, 1 << 18, 8), ("bf16", 3, 1 << 18, 5, 16), ("fp8", 40, 1 << 18, 130, 128),
+                                                 ("f16", 1000, 1 << 16, 260, 24)])
+def test_projections_of_the_largest_sizes(fdm, fmt, T, inner, out, rank):
+    s = project_case(rng(T), fmt, T, inner, out, 2, rank, [T - 2, 1, 1])
+    say(f"project {fmt} T={T} in={inner} out={out}")
+    y = run_project(fdm, s, torch.empty(T, out, device="cuda"))
+    C.check(y.cpu(), *want_of(s, y.dtype), "project")
+
+
+def test_norm_of_the_most_rows(fdm):
+    x = normal(rng(1), 1 << 21, 8)
+    y = torch.empty(1 << 21, 8, device="cuda")
+    fdm.add_rms_norm(x.cuda(), None, None, y)
+    want = C.normed(x, None, None, 1e-6)[1]
+    C.check(y.cpu(), want, want.abs() * (C.NORM_TOL + 2.0 ** -24), "norm")
+
+
+def test_books_of_the_most_places(fdm):
+    """2^25 places in one call, and slots just below 2^31."""
+    n, page = 1 << 23, 1 << 15
+    p = fdm.kv_pages(4, 300, 65535, page)
+    p.free.copy_(torch.arange(65535, dtype=torch.int32))  # the last pages first
+    q, pos, slots = (torch.empty(k, dtype=torch.int32, device="cuda") for k in (5, 4 * n, 4 * n))
+    fdm.kv_grow(p, ints([5, 0, 7, 0]), q, pos, slots)
+    assert slots[:5].tolist() == [65534 * page + i for i in range(5)] and slots[5:12].tolist() == [65533 * page + i for i in range(7)]
+    assert (slots[12:] == -1).all() and (pos[12:] == 0).all()
+    fdm.kv_grow(p, ints([n] * 4), q, pos, slots)
+    assert q.tolist() == [k * n for k in range(5)] and p.kv_len.tolist() == [n + 5, n, n + 7, n]
+    for b, at in enumerate((5, 0, 7, 0)):
+        want = torch.arange(at, at + n, device="cuda")
+        assert torch.equal(pos[b * n:(b + 1) * n].long(), want)
+        assert torch.equal(slots[b * n:(b + 1) * n].long(), p.pages[b].long()[want // page] * page + want % page)
+    used = torch.cat([p.pages[b][:-(-m // page)] for b, m in enumerate(p.kv_len.tolist())])
+    assert used.unique().numel() == used.numel() == 65535 - p.n_free.item()
+    fdm.kv_trim(p, ints([0, 0, 0, 0]))
+    assert p.n_free.item() == 65535 and p.free.unique().numel() == 65535 and p.kv_len.sum() == 0
+
+
+def test_calls_of_two_threads(fdm):
+    """Two threads with a stream and a workspace each."""
+    import threading
+    jobs, failed = [], []
+    for k, (T, out) in enumerate(((70, 700), (300, 2100))):
+        s = {n: v.cuda() if isinstance(v, torch.Tensor) else v for n, v in project_case(rng(k), "bf16", T, 528, out, 3, 32, [T // 2, T - T // 2]).items()}
+        want = run_project(fdm, s, torch.empty(T, out, dtype=torch.bfloat16, device="cuda"))
+        jobs.append((s, want, fdm.project_workspace(T, 528, out, 32), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+
+    def work(s, want, ws, stream):
+        outs = [torch.empty_like(want) for _ in range(20)]
+        stream.wait_stream(torch.cuda.current_stream())
+        for y in outs:
+            run_project(fdm, s, y, workspace=ws, stream=stream)
+        stream.synchronize()
+        failed.extend(i for i, y in enumerate(outs) if not torch.equal(y, want))
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
