@@ -166,7 +166,8 @@ __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int u_splits,
           bv[nb] = *reinterpret_cast<const x8*>(B + (int64_t)n * a.rank + j);
         }
       }
-      // F16 numbers: the largest of these brought to [1, 2), so that none overflows and few are lost
+      // F16 numbers: the largest of these brought to [1, 2) (below 4 where 2^-127 would be its
+      // factor), so that none overflows and few are lost
       float down = 1.0f;
       if constexpr (FMT == kRowF16) {
         float top = 0.0f;
@@ -174,7 +175,7 @@ __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int u_splits,
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -100), 100);
+        const int e = min(max((int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127, -126), 126);
         const float up = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
         down = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
 #pragma unroll
