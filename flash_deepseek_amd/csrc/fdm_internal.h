@@ -484,7 +484,7 @@ struct ProjectArgs {
   int n_adapters, rank;       // 0: none
   const int *q_start, *adapter;  // [B + 1], [B]
   int B;
-  int planes;                 // 16-bit numbers that stand for one of u on the matrix cores
+  int planes;                 // BF16 numbers that stand for one of u on the matrix cores
   float* u;                   // workspace [u_splits][T][rank]
   float* part;                // workspace [splits][tiles - full][rows][cols]
   int full, splits, u_splits;

@@ -124,8 +124,8 @@ __device__ __forceinline__ int swap8(int row) {
 }
 
 // The adapters' second product on a wave's sums: for every adapter among the rows of a
-// block, B_a u on the matrix cores, u as sums of 16-bit numbers (a.planes of them: 8 bits
-// each in BF16, 11 in F16), kept by the rows that are the adapter's own.  A row that
+// block, B_a u on the matrix cores, u as sums of 16-bit numbers (a.planes of 8 bits each in
+// BF16, two of 11 in F16), kept by the rows that are the adapter's own.  A row that
 // has another keeps its sum untouched, whatever B_a holds.
 template <int FMT, int NB>
 __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int u_splits, int m, int id, int n0, typename Block<FMT>::sum_t* acc) {
@@ -186,16 +186,36 @@ __device__ __forceinline__ void add_adapters(const ProjectArgs& a, int u_splits,
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int i = 0; i < Block<FMT>::kOf; ++i) sum[nb][i] = 0.0f;
-      for (int p = 0; p < a.planes; ++p) {
+      // v as 16-bit numbers, each the rest of those before it (an infinity has none)
+      auto next = [&]() {
         x8 w;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           w[i] = (T16)v[i];
           const float rest = v[i] - (float)w[i];
-          v[i] = fabsf(rest) < __builtin_inff() ? rest : 0.0f;  // an infinity has no rest
+          v[i] = fabsf(rest) < __builtin_inff() ? rest : 0.0f;
         }
+        return w;
+      };
+      if constexpr (FMT == kRowF16) {
+        // The rest, at most 2^-10, times 2^24 and its product first: beside values near 1 it
+        // would lie below F16's steps of 2^-24 from 2^-14 on.  So a value is off by 2^-22 of itself,
+        // or 2^-36 of the largest.
+        const x8 first = next();
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) sum[nb] = mfma(bv[nb], w, sum[nb]);
+        for (int i = 0; i < 8; ++i) v[i] *= 0x1p24f;
+        const x8 second = next();
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          sum[nb] = mfma(bv[nb], second, sum[nb]);
+          sum[nb] = mfma(bv[nb], first, sum[nb] * 0x1p-24f);
+        }
+      } else {
+        for (int p = 0; p < a.planes; ++p) {
+          const x8 w = next();
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) sum[nb] = mfma(bv[nb], w, sum[nb]);
+        }
       }
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)

@@ -646,7 +646,8 @@ int fdm_add_rms_norm(const void *d_x, int x_type, int64_t x_stride, const void *
  * (1e-4 of a result of 7168 normal values).  An fp32 y, and A x, take the codes times
  * their scale in BF16: exact for scale bytes of x and W from 10 to 246.  Where B (A x) runs
  * on the matrix cores A x is held as two numbers of the adapters' type (three for an fp32 y
- * beside BF16), off by 2^-16 of itself at most.  A row's result depends on its own values and
+ * beside BF16), off by 2^-16 of itself at most, in F16 by 2^-22 or by 2^-36 of the largest
+ * of 32 neighbours of the rank.  A row's result depends on its own values and
  * adapter alone, whatever the others are; its sums' order on T and the sizes, B and
  * n_adapters among them.  The same arguments give the same bits.
  * d_workspace: at least fdm_project_workspace(T, in, out, rank) bytes (rank 0: no

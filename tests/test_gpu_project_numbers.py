@@ -1,7 +1,5 @@
 """Numbers of a projection's adapters far apart from each other and near the ends of
 their range, and what the products of e4m3 rows cut off, against float64."""
-import math
-
 import pytest
 import torch
 
@@ -28,3 +26,27 @@ def test_adapters_at_the_ends_of_fp32(fdm, fmt, T, out, rank):
     say(f"project {fmt} T={T} out={out} rank={rank}, the ends of fp32")
     y = run_project(fdm, s, torch.empty(T, out, device="cuda"))
     C.check(y.cpu(), *want_of(s, y.dtype), "project")
+
+
+@pytest.mark.parametrize("T,out,rank", SIZES)
+def test_adapters_of_values_far_apart(fdm, T, out, rank):
+    """A x spread over 2^-18 of its largest and B the other way round, so that every value of the
+    rank counts the same.  In F16: each off by 2^-16 of itself, or 2^-36 of the largest, at most."""
+    g = rng(T + rank)
+    s = project_case(g, "f16", T, 64, out, 2, rank, [T // 2, T - T // 2])
+    s["adapter"], s["times"] = torch.tensor([0, 1], dtype=torch.int32), None
+    s["w"] = (normal(g, out, 64) * 2.0 ** -8).half()
+    down = torch.exp2(-18.0 * torch.randperm(rank, generator=g) / (rank - 1)).round(decimals=9)
+    s["a"] = (normal(g, 2, rank, 64) * 2.0 ** 5 * down[None, :, None]).half()
+    s["b"] = (normal(g, 2, out, rank) * 2.0 ** -10 / down).half()
+    x, w, a, b = (s[k].cuda().double() for k in ("x", "w", "a", "b"))
+    n = 64 / 8 + 24
+    want, tol = x @ w.T, (x.abs() @ w.abs().T) * n * 2.0 ** -23
+    for k, t in ((0, slice(0, T // 2)), (1, slice(T // 2, T))):
+        u = x[t] @ a[k].T
+        du = (x[t].abs() @ a[k].abs().T) * (n + 2) * 2.0 ** -23 + torch.maximum(u.abs() * 2.0 ** -16, u.abs().amax(-1, keepdim=True) * 2.0 ** -36)
+        want[t] += u @ b[k].T
+        tol[t] += du @ b[k].abs().T + (u.abs() @ b[k].abs().T) * (rank / 8 + 24) * 2.0 ** -23
+    say(f"project f16 T={T} out={out} rank={rank}, far apart")
+    y = run_project(fdm, s, torch.empty(T, out, device="cuda"))
+    C.check(y, want, tol + want.abs() * 2.0 ** -24, "project")
