@@ -562,11 +562,21 @@ def mla_attend(cache, q_lat, q_rope, q_start, kv_len, pages, scale, out, mask=No
 
 
 # ---- what stands between the attention of one layer and of the next ---------------------
+def _outside_captures(fn, device):
+    """What is filled during a capture holds nothing until the graph's first replay, and is filled again by each."""
+    import torch
+    if device.type == "cuda":
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                _refuse(fn, "made while the stream is captured")
+
+
 class KvPages:
     """The books of a paged cache (int32 tensors of the caller, kept alive here and
     changed in place): pages [B, P] the page numbers of each sequence, kv_len [B]
     its cached positions, free [n_pages] a stack of free pages, n_free [1] how
-    many.  No two sequences have a page in common."""
+    many.  No two sequences have a page in common.  It is made before a capture
+    whose calls use it, not inside."""
 
     def __init__(self, pages, kv_len, free, n_free, page_size):
         import torch
@@ -581,9 +591,10 @@ class KvPages:
                                                                ("n_free", n_free, 1))]
         if page_size < 1 or page_size & (page_size - 1):
             _refuse(fn, f"page_size {page_size}: a power of two")
+        _outside_captures(fn, pages.device)
         self.pages, self.kv_len, self.free, self.n_free, self.page_size = pages, kv_len, free, n_free, page_size
         self._turn = torch.zeros(1, dtype=torch.int32, device=pages.device)
-        if pages.is_cuda and not torch.cuda.is_current_stream_capturing():  # there for calls on any stream
+        if pages.is_cuda:  # there for calls on any stream
             torch.cuda.current_stream(pages.device).synchronize()
         self.desc = _lib.KvPagesDesc(*at, self._turn.data_ptr(), B, P, n, page_size)
         self.device = pages.get_device()
@@ -594,6 +605,7 @@ def kv_pages(B, pages_per_seq, n_pages, page_size=64):
     cache of n_pages, all of them free."""
     import torch
     dev = torch.device("cuda", torch.cuda.current_device() if _device is None else _device)
+    _outside_captures("kv_pages", dev)
     return KvPages(torch.full((B, pages_per_seq), -1, dtype=torch.int32, device=dev), torch.zeros(B, dtype=torch.int32, device=dev),
                    torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev),
                    torch.full((1,), n_pages, dtype=torch.int32, device=dev), page_size)
