@@ -27,6 +27,7 @@ current stream; all compute is the library's own HIP kernels).  Every call
 is asynchronous on torch's current stream unless noted.
 """
 import ctypes
+import threading
 
 from . import _lib
 from ._lib import (DENSE_FFN, EXPERT_Q4K_BYTES, EXPERT_Q6K_BYTES, HIDDEN, MAX_K, MAX_LAYERS, MAX_TOKENS,
@@ -571,6 +572,26 @@ def _outside_captures(fn, device):
                 _refuse(fn, "made while the stream is captured")
 
 
+_words = {}  # device -> the zeroed words of which handles still get some, and how many did
+_all_words = []
+_words_lock = threading.Lock()
+
+
+def _zero_word(device):
+    """A zeroed word that nobody else ever gets: launches that are queued, and graphs that captured
+    some, count on it when its handle is gone.  Four bytes of each handle stay."""
+    import torch
+    with _words_lock:
+        words, used = _words.get(device, (None, 0))
+        if words is None or used == words.numel():
+            words, used = torch.zeros(1024, dtype=torch.int32, device=device), 0
+            if words.is_cuda:
+                torch.cuda.current_stream(device).synchronize()
+            _all_words.append(words)
+        _words[device] = words, used + 1
+        return words[used:used + 1]
+
+
 class KvPages:
     """The books of a paged cache (int32 tensors of the caller, kept alive here and
     changed in place): pages [B, P] the page numbers of each sequence, kv_len [B]
@@ -593,7 +614,7 @@ class KvPages:
             _refuse(fn, f"page_size {page_size}: a power of two")
         _outside_captures(fn, pages.device)
         self.pages, self.kv_len, self.free, self.n_free, self.page_size = pages, kv_len, free, n_free, page_size
-        self._turn = torch.zeros(1, dtype=torch.int32, device=pages.device)
+        self._turn = _zero_word(pages.device)
         if pages.is_cuda:  # there for calls on any stream
             torch.cuda.current_stream(pages.device).synchronize()
         self.desc = _lib.KvPagesDesc(*at, self._turn.data_ptr(), B, P, n, page_size)

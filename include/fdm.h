@@ -572,7 +572,8 @@ int fdm_mla_attend(const fdm_kv_cache *cache, const fdm_mla_batch *batch, const 
  * first *d_n_free entries; sequence b has the pages d_pages[b][0 ..
  * ceil(kv_len[b] / page_size) - 1], which no other sequence has.  All of it is
  * the caller's device memory and changes in place; d_turn is a word of the
- * library's, zero at first.  kv_len is cut to 0 .. pages_stride * page_size (and
+ * library's, zero before the first call, and as long as any call, a captured one's replay
+ * too, may come.  kv_len is cut to 0 .. pages_stride * page_size (and
  * 2^31 - 4097), *d_n_free to 0 .. n_pages, as they are read.  Calls on the same
  * pages follow each other on one stream; they may be captured.
  *
