@@ -874,20 +874,13 @@ hipError_t launch_tiles(ProjectArgs a, const ProjectPlan& p, hipStream_t s) {
   k_project<FMT, BM, BN, WM, WN, RING, TURN><<<a.u_groups + a.full + rest * a.splits, 64 * WM * WN, 0, s>>>(a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !rest) return e;
-  // One chunk a workgroup, so that rows with adapters of their own do not wait for each other,
-  // or where there are many, four: 64 rows by 2112 15.4 us a call against 19.2, 24 by
-  // 24576 20.3 and 21.6, 500 by 2111 with two adapters 75 and 60, 256 by 7168 with 32 109 and 104.5.
-  // Many chunks on the matrix cores instead where 16 rows have two adapters at most, or B's rows
-  // are more than 64 bytes, so that a row a lane takes them apart.  650 rows by 2112 of 3, 80 and
-  // 650 requests with adapters of their own, rank 16: 7.1, 9.5 and 25 us on the matrix cores, 7.7,
-  // 8.5 and 12.7 without; rank 64: 12.5, 15.7 and 46, and 15.2, 27 and 124.  (256 rows by 7168
-  // with 32 adapters of rank 64 in turn are slower, 79 and 64.)
   constexpr int kHalf = FMT == kRowF16 ? kRowF16 : kRowBf16;
-  const int rows = std::min(BM, a.T), chunks = (rows * BN + 255) / 256;
-  if ((int64_t)rest * chunks <= 16 * g_num_cus) k_project_join<FMT, BM, BN, 1><<<dim3(rest, chunks), 256, 0, s>>>(a);
-  else if (a.n_adapters && (a.rank > 32 || (int64_t)16 * a.B <= a.T))
-    k_project_join_rows<kHalf, BM, BN><<<dim3(rest, (rows + 15) / 16 * (BN / kJoinCols)), 256, 0, s>>>(a);
-  else k_project_join<FMT, BM, BN, 4><<<dim3(rest, (chunks + 3) / 4), 256, 0, s>>>(a);
+  const int rows = std::min(BM, a.T), chunks = join_chunks(p.tile, a.T);
+  switch (project_join(p, a.T, a.out, a.B, a.rank, g_num_cus)) {
+    case kJoinOne: k_project_join<FMT, BM, BN, 1><<<dim3(rest, chunks), 256, 0, s>>>(a); break;
+    case kJoinRows: k_project_join_rows<kHalf, BM, BN><<<dim3(rest, (rows + 15) / 16 * (BN / kJoinCols)), 256, 0, s>>>(a); break;
+    default: k_project_join<FMT, BM, BN, 4><<<dim3(rest, (chunks + 3) / 4), 256, 0, s>>>(a); break;
+  }
   return hipGetLastError();
 }
 

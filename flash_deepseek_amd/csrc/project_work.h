@@ -124,6 +124,24 @@ inline ProjectPlan project_plan(int T, int64_t row_bytes, int out, int B, int n,
   return p;
 }
 
+// How the parts are joined (kJoinNone: every tile is whole).  One chunk of 256 values a workgroup, so
+// that rows with adapters of their own do not wait for each other, or where there are many,
+// four: 64 rows by 2112 15.4 us a call against 19.2, 24 by 24576 20.3 and 21.6, 500 by 2111
+// with two adapters 75 and 60, 256 by 7168 with 32 109 and 104.5.
+// Many chunks on the matrix cores instead where 16 rows have two adapters at most, or B's rows
+// are more than 64 bytes, so that a row a lane takes them apart.  650 rows by 2112 of 3, 80 and
+// 650 requests with adapters of their own, rank 16: 7.1, 9.5 and 25 us on the matrix cores, 7.7,
+// 8.5 and 12.7 without; rank 64: 12.5, 15.7 and 46, and 15.2, 27 and 124.  (256 rows by 7168
+// with 32 adapters of rank 64 in turn are slower, 79 and 64.)
+enum ProjectJoin { kJoinNone, kJoinOne, kJoinFour, kJoinRows };
+inline int join_chunks(int tile, int T) { return (std::min(kTiles[tile].rows, T) * kTiles[tile].cols + 255) / 256; }
+inline ProjectJoin project_join(const ProjectPlan& p, int T, int out, int B, int rank, int cus) {
+  const int64_t rest = tiles_of(p.tile, T, out) - p.full;
+  if (!rest) return kJoinNone;
+  if (rest * join_chunks(p.tile, T) <= 16 * cus) return kJoinOne;
+  return rank && (rank > 32 || (int64_t)16 * B <= T) ? kJoinRows : kJoinFour;
+}
+
 // fp32 values of the parts [splits][tiles][rows][cols] and of the adapters' first product
 // [u_splits][T][rank]
 inline size_t project_part_floats(const ProjectPlan& p, int T, int out) {
