@@ -16,11 +16,12 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // How rows and matrix are read: as they are, or e4m3 as one product of 64 codes (kRowFp8) or
-// widened to BF16 (kRowFp8Wide).  The fp8 products of gfx950 add eight neighbours before
-// they go into the fp32 sum, and what lies 2^-14 and more under the largest of the eight is
-// cut off there (measured; 2^-24 in BF16 and F16).  Of a row of 7168 normal values that
-// is 1e-4 of the result, a tenth of a 16-bit result's own rounding, but a thousand times an
-// fp32 one's: fp32 results take the BF16 products, in which codes and scales are exact.
+// widened to BF16 (kRowFp8Wide).  The fp8 products of gfx950 add eight neighbours in steps
+// of 2^-13 of the largest one's power of two before they go into the fp32 sum (measured; 2^-23
+// in BF16 and F16).  Of a row of 7168 normal values that is 1.5e-5 of the result, a
+// hundredth of a BF16 result's own rounding and a fourteenth of an F16 one's, but 130 times
+// what an fp32 one is off by: fp32 results take the BF16 products, in which codes and scales
+// are exact.
 constexpr int kRowF16 = 0, kRowBf16 = 1, kRowFp8 = 2, kRowFp8Wide = 3;
 
 template <int FMT>

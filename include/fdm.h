@@ -572,8 +572,8 @@ int fdm_mla_attend(const fdm_kv_cache *cache, const fdm_mla_batch *batch, const 
  * first *d_n_free entries; sequence b has the pages d_pages[b][0 ..
  * ceil(kv_len[b] / page_size) - 1], which no other sequence has.  All of it is
  * the caller's device memory and changes in place; d_turn is a word of the
- * library's, zero before the first call, and as long as any call, a captured one's replay
- * too, may come.  kv_len is cut to 0 .. pages_stride * page_size (and
+ * library's, zero before the first call and kept as long as one may run, a captured call's
+ * replay among them.  kv_len is cut to 0 .. pages_stride * page_size (and
  * 2^31 - 4097), *d_n_free to 0 .. n_pages, as they are read.  Calls on the same
  * pages follow each other on one stream; they may be captured.
  *
@@ -643,8 +643,8 @@ int fdm_add_rms_norm(const void *d_x, int x_type, int64_t x_stride, const void *
  * in, out <= FDM_PROJECT_MAX_DIM.  y must not overlap the inputs.  q_start does not fall,
  * and is cut to 0 .. T.
  * Sums and A x are fp32, products exact but for E4M3 with a 16-bit y: there every eight
- * neighbouring products are added with what lies under 2^-13 of their largest cut off
- * (1e-4 of a result of 7168 normal values).  An fp32 y, and A x, take the codes times
+ * neighbouring products are added in steps of 2^-13 of the power of two of their largest
+ * (off by 1.5e-5 of a result of 7168 normal values; an F16 result's own rounding is 2e-4).  An fp32 y, and A x, take the codes times
  * their scale in BF16: exact for scale bytes of x and W from 10 to 246.  Where B (A x) runs
  * on the matrix cores A x is held as two numbers of the adapters' type (three for an fp32 y
  * beside BF16), off by 2^-16 of itself at most, in F16 by 2^-22 or by 2^-36 of the largest

@@ -50,3 +50,40 @@ def test_adapters_of_values_far_apart(fdm, T, out, rank):
     say(f"project f16 T={T} out={out} rank={rank}, far apart")
     y = run_project(fdm, s, torch.empty(T, out, device="cuda"))
     C.check(y, want, tol + want.abs() * 2.0 ** -24, "project")
+
+
+@pytest.mark.parametrize("ty", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T", [5, 40, 100, 140])
+def test_where_e4m3_products_end(fdm, T, ty):
+    """1 + 2^-j - 1, the first two among eight neighbours: kept to 2^-13, and off by less than that below; all of it in fp32."""
+    out, j = 200, 6 + torch.arange(200) // 2 % 10
+    sign = 1.0 - 2.0 * (torch.arange(200) % 2)
+    x, w = torch.zeros(T, 64), torch.zeros(out, 64)
+    x[:, 1] = 2.0 ** -6
+    x[:, 0] = x[:, 16] = w[:, 0] = 1.0
+    w[:, 16] = -1.0
+    w[:, 1] = sign * torch.exp2(6.0 - j)
+    F8 = torch.float8_e4m3fn
+    s = {"x": x.to(F8), "w": w.to(F8), "x_scale": torch.full((T, 1), 127, dtype=torch.uint8), "w_scale": torch.full((2, 1), 127, dtype=torch.uint8)}
+    y = run_project(fdm, s, torch.empty(T, out, dtype=ty, device="cuda")).double().cpu()
+    want = (sign * torch.exp2(-j.double())).expand(T, out)
+    kept = (j <= 13) | (ty is torch.float32)
+    assert torch.equal(y[:, kept], want[:, kept])
+    assert ((y - want).abs() < 2.0 ** -13).all()
+
+
+@pytest.mark.parametrize("ty", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,out", [(20, 2112), (64, 2112), (256, 2112), (2048, 4200)])
+def test_what_e4m3_products_lose(fdm, T, out, ty):
+    """Of 7168 normal values, with steps of 2^-13 of the power of two of the largest of eight: 2.0e-5 of
+    the results' rms where each product is cut to them, 1.5e-5 where it is rounded (a model of the eight
+    in float64; cut downwards it would be 2.2e-4).  Beside the rounding of the results themselves, and
+    sqrt(7168 / 32) roundings of 2^-24 of sums of that size in fp32."""
+    g = rng(T)
+    x, w = torch.randn(T, 7168, generator=g), torch.randn(out, 7168, generator=g) * 7168 ** -0.5
+    (xc, xs), (wc, ws) = C.quantised_rows(x), C.quantised_matrix(w)
+    y = run_project(fdm, {"x": xc, "w": wc, "x_scale": xs, "w_scale": ws}, torch.empty(T, out, dtype=ty, device="cuda"))
+    want = C.widened_rows(xc.cuda(), xs.cuda()) @ C.widened_matrix(wc.cuda(), ws.cuda()).T
+    own = (want.to(ty).double() - want).square().mean()
+    lost = 2.5e-5 if ty is not torch.float32 else 15 * 2.0 ** -24
+    assert (y.double() - want).square().mean() <= own + (lost * want.square().mean().sqrt()) ** 2
