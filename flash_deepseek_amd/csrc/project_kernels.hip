@@ -482,8 +482,9 @@ __device__ __forceinline__ Place place_of(int tile, int m_tiles, int n_tiles) {
 // each, the others a part of one.
 // Measured (a launch; the library's BF16 product of 8192^3 reaches 1.38 PFLOP/s, its e4m3 one
 // 2.65): 5050 rows of 16384 BF16 values by 7168 in tiles of 256 x 256 1020 us with the adapters' second
-// product, 1.16 PFLOP/s, 10276 of 7168 codes by 18432 1200 us, 2.26; there the power bounds it: the
-// matrix cores are busy 61 and 56 % of the cycles, and the clock falls from 2.4 to 1.7 GHz.  256 rows of 16384 by 7168 91 us, 2.9 TB/s; 24 of 1536 F16 by
+// product, 1.16 PFLOP/s, 10276 of 7168 codes by 18432 1200 us, 2.26: the matrix cores are busy 61 and
+// 56 % of the cycles, at 1.7 GHz of 2.4, which the products' power leaves (the library reaches 1.34 on
+// the first matrix and 3.20 on 8192 rows by the second, with one scale an operand).  256 rows of 16384 by 7168 91 us, 2.9 TB/s; 24 of 1536 F16 by
 // 24576 14.5, 5.5 TB/s; one row of 7168 by 1536 7.1, two launches' latencies with the join.
 template <int FMT, int BM, int BN, int WM, int WN, int RING, int TURN>
 __global__ __launch_bounds__(64 * WM * WN) void k_project(ProjectArgs a) {

@@ -45,8 +45,12 @@ inline int rank_parts(int rank) { return (rank + kRankPart - 1) / kRankPart; }
 //   a step of 128 bytes in a workgroup  0.3, 0.42, 0.53, 1.6 by tile; 3 a round for its two ends
 //   a part                              0.015, 0.02, 0.03, 0.13; 5 for the joining launch
 // (500 rows of 16384 BF16 values by 7168: tiles of 128 rows 137 us, of 256 in four parts 138;
-// 1000 rows 276 and, in two parts, 238; 256 rows 79 and 93; 128 rows of 7168 by 576 in tiles
-// of 64 rows 11.9, of 128 15.1; of 1536 by 24576 23.7 and 17.2.)
+// 1000 rows 276 and, in two parts, 238; 256 rows 79 and 93; 128 rows of 1536 by 24576 in tiles
+// of 64 rows 23.7, of 128 17.2.)
+// It takes tiles of 128 rows too soon where 128 to 256 rows meet few columns: 128 rows of 7168
+// BF16 values by 576 and 2112 19 and 14 parts of them (at their best 15.1 and 18.0 us) where 20 and
+// 7 of 64 rows take 11.9 and 15.9; 256 rows by 576 16.4 and 13.8, of codes by 2112 21.8 and 18.9;
+// and leaves 1000 rows by 2112 whole, 59.7, in three parts 54.8.
 constexpr double kStepUs[] = {0.3, 0.42, 0.53, 1.6}, kPartUs[] = {0.015, 0.02, 0.03, 0.13};
 // Parts at most: two for every CU, one of the largest tiles (64 MB of sums).
 inline int most_parts(int tile, int cus) { return tile == kTile256 ? cus : 2 * cus; }

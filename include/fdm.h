@@ -609,8 +609,9 @@ int fdm_kv_trim(const fdm_kv_pages *pages, const int32_t *d_keep, void *stream);
  * and the additions of 1846-1850, 1922, without fdm_rms_norm's order of sums):
  *   s = x + add (d_add NULL: x),  y = s / sqrt(mean(s^2) + eps) * w (d_w fp32 [d], NULL: 1),
  * T rows (up to FDM_NORM_MAX_ROWS) of d values (1 .. FDM_NORM_MAX_DIM), strides in
- * elements, in fp32, each output rounded once: d_sum (may be NULL) receives s in x's type, d_y the norm of s
- * as it was before that rounding.  Types are FDM_GGML_F32, _F16, _BF16; y_type may
+ * elements, in fp32 (a row whose squares' sum is past it gives zeros), each output rounded
+ * once: d_sum (may be NULL) receives s in x's type, d_y the norm of s as it was before that
+ * rounding.  Types are FDM_GGML_F32, _F16, _BF16; y_type may
  * be FDM_E4M3: codes with a scale byte for every 128 values of a row, d_scale
  * [T][ceil(d / 128)], by the rule of FDM_KV_FP8 (zeros: 27, an infinity or NaN: 255).
  * d_sum may be d_x, d_y may be d_x or d_add (same size of elements and stride);
@@ -648,7 +649,8 @@ int fdm_add_rms_norm(const void *d_x, int x_type, int64_t x_stride, const void *
  * their scale in BF16: exact for scale bytes of x and W from 10 to 246.  Where B (A x) runs
  * on the matrix cores A x is held as two numbers of the adapters' type (three for an fp32 y
  * beside BF16), off by 2^-16 of itself at most, in F16 by 2^-22 or by 2^-36 of the largest
- * of 32 neighbours of the rank.  A row's result depends on its own values and
+ * of 32 neighbours of the rank; an infinity in A or B, or past fp32 in A x, may leave its
+ * adapter's rows NaN where the formula has an infinity.  A row's result depends on its own values and
  * adapter alone, whatever the others are; its sums' order on T and the sizes, B and
  * n_adapters among them.  The same arguments give the same bits.
  * d_workspace: at least fdm_project_workspace(T, in, out, rank) bytes (rank 0: no
